@@ -72,10 +72,12 @@ def build_torch_ops(verbose: bool = False) -> Path:
     cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
     incs = [f"-I{p}" for p in include_paths()] + [f"-I{Path(nvcc_path()).resolve().parent.parent / 'include'}",
                                                    f"-I{INCLUDE}"]
+    # libstdc++.so.6 is named so that it is the one torch has loaded: a toolchain without it links libstdc++.a into the
+    # operator layer, and a second copy's locale facets crash where an error message formats a number
     tmp = TORCH_OPS.with_suffix(".so.tmp")
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *incs,
            str(CSRC / TORCH_OPS_SOURCE), "-o", str(tmp), f"-L{PKG}", "-lqf_b200", f"-L{tdir / 'lib'}", "-lc10",
-           "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-Wl,-rpath,$ORIGIN"]
+           "-lc10_cuda", "-l:libstdc++.so.6", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
