@@ -197,6 +197,53 @@ int qf_w8a16_gemm_rmsnorm(const void* x, int64_t ldx, const void* residual, int6
 int qf_quantize_rows_int8(const void* w, int64_t ldw, int V, int H, int8_t* q, int64_t ldq, float* scale,
                           void* stream);
 
+/* ---- block-scaled fp8 layers ------------------------------------------------------------------------------------
+ * For checkpoints whose linear weights are e4m3 with one fp32 scale for each block of 128 x 128 and whose activations
+ * are quantized at run time in groups of 128 along k (the reference plugin serves the int8 form of the same layers
+ * only, plugin/qwen_fastpath/w8a16.py).  Neither call needs a workspace.
+ *
+ * qf_fp8_quantize: x bf16 [M, K] (row stride ldx elements), or with silu_mul != 0 [M, 2K] holding the merged gate
+ * (columns [0, K)) and up ([K, 2K)).  Per token row and group of 128 consecutive k (the last may be shorter):
+ *   v = x, or silu(gate) * up in fp32;  a = max(max|v|, 448 * 2^-60);  scale = a / 448;
+ *   q = e4m3(v * (448 / a)), round to nearest even.
+ * A NaN makes its group's scale and values NaN.  q: e4m3 [M, K] (row stride ldq bytes; bytes past K are not written),
+ * scale: fp32 [M, ceil(K / 128)] (row stride lds).  x 2-byte aligned; 16-byte accesses where the rows allow them.
+ * K <= QF_FP8_MAX_K. */
+#define QF_FP8_MAX_K 1048576
+int qf_fp8_quantize(const void* x, int64_t ldx, int M, int K, int silu_mul, void* q, int64_t ldq, float* scale,
+                    int64_t lds, unsigned flags, void* stream);
+
+/* y[m, n] = out( sum_g sa[m, g] * sw[n / 128, g] * sum_{k in group g} a[m, k] * w[n, k]  (+ bias[n]) ), exact e4m3
+ * products, fp32 sums, one rounding to the output type.  a: e4m3 [M, K] (row stride lda bytes); a_scale fp32 element
+ * (m, g) at m * sa_m + g * sa_g; w: e4m3 [N, K] row-major (row stride ldw bytes); w_scale fp32 element (n / 128, g) at
+ * (n / 128) * sw_n + g * sw_g; bias bf16 [N] or NULL (added in fp32 before the rounding); y bf16 or fp32 (y_dtype),
+ * row stride ldy elements.  Any M, N, K >= 1 (M == 0 or N == 0 is a no-op).  a and w 16-byte aligned with lda and ldw
+ * multiples of 16. */
+int qf_fp8_block_gemm(const void* a, int64_t lda, const float* a_scale, int64_t sa_m, int64_t sa_g, const void* w,
+                      int64_t ldw, const float* w_scale, int64_t sw_n, int64_t sw_g, const void* bias, void* y,
+                      int64_t ldy, int y_dtype, int M, int N, int K, unsigned flags, void* stream);
+
+/* ---- residual update with the norms on both sides of a block -----------------------------------------------------
+ * One pass over a token row of H elements, fp32 inside (the reference plugin leaves norms to vLLM):
+ *   u = x, or x * rsqrt(mean(x^2) + eps) * (post_weight + weight_offset) where post_weight is given;
+ *   v = u, or u * act(gate) where gate is given (gate_act: none = the gate itself, sigmoid, silu);
+ *   r' = residual + residual_scale * v (residual NULL: zero), stored to residual_out in the residual's type;
+ *   h = r' * rsqrt(mean(r'^2) + eps) * (pre_weight + weight_offset), from the unrounded r', stored to out as bf16, or,
+ *   where out_scale is given, quantized as qf_fp8_quantize does (out e4m3, row stride ldo bytes).
+ * x, gate, weights bf16; residual and residual_out both bf16 or both fp32 (residual_dtype).  gate element (m, h) at
+ * m * gate_sm + h * gate_sh with gate_sh 0 or 1 (gate_sm 0: one row for all tokens).  pre_weight and out are given
+ * together or both NULL; residual_out may be NULL.  residual_out may be residual itself, and out may be x; other
+ * overlaps are not allowed.  1 <= H <= QF_NORM_MAX_H. */
+#define QF_NORM_MAX_H 16384
+#define QF_GATE_NONE 0
+#define QF_GATE_SIGMOID 1
+#define QF_GATE_SILU 2
+int qf_residual_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, int residual_dtype,
+                     const void* gate, int64_t gate_sm, int64_t gate_sh, int gate_act, const void* post_weight,
+                     const void* pre_weight, float weight_offset, float residual_scale, float eps,
+                     void* residual_out, int64_t ldro, void* out, int64_t ldo, float* out_scale, int64_t lds, int M,
+                     int H, unsigned flags, void* stream);
+
 /* Reads and clears the workspace's sticky device error flag (synchronises `stream`).  *status receives
  * QF_OK or QF_ERR_TIMEOUT.  Not for the hot path. */
 int qf_workspace_status(void* ws, void* stream, int* status);

@@ -21,6 +21,11 @@ QF_NOALLOC_MAX_N = 262144
 QF_AR_MAX_RANKS = 8
 QF_AR_MAX_CHUNKS = 256
 QF_IPC_HANDLE_BYTES = 64
+QF_FP8_MAX_K = 1048576
+QF_NORM_MAX_H = 16384
+QF_GATE_NONE = 0
+QF_GATE_SIGMOID = 1
+QF_GATE_SILU = 2
 ABI_VERSION = 1
 
 # (name, restype, argtypes) -- one entry per function declared in include/qf_b200.h
@@ -62,6 +67,16 @@ SIGNATURES = [
       _c.c_void_p]),
     ("qf_quantize_rows_int8", _c.c_int,
      [_c.c_void_p, _c.c_int64, _c.c_int, _c.c_int, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p]),
+    ("qf_fp8_quantize", _c.c_int,
+     [_c.c_void_p, _c.c_int64, _c.c_int, _c.c_int, _c.c_int, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_uint,
+      _c.c_void_p]),
+    ("qf_fp8_block_gemm", _c.c_int,
+     [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64,
+      _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_uint, _c.c_void_p]),
+    ("qf_residual_norm", _c.c_int,
+     [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int,
+      _c.c_void_p, _c.c_void_p, _c.c_float, _c.c_float, _c.c_float, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64,
+      _c.c_void_p, _c.c_int64, _c.c_int, _c.c_int, _c.c_uint, _c.c_void_p]),
     ("qf_allreduce_buffer_bytes", _c.c_size_t, [_c.c_int]),
     ("qf_symm_alloc", _c.c_int, [_c.c_size_t, _c.POINTER(_c.c_void_p)]),
     ("qf_symm_free", _c.c_int, [_c.c_void_p]),
@@ -119,8 +134,8 @@ _torch_ops_loaded = False
 
 
 def load_torch_ops():
-    """Registers ``torch.ops.qf_b200.int8_linear`` (the PyTorch operator over this C ABI, csrc/qf_torch_ops.cpp);
-    raises if it is not built.  Returns the op."""
+    """Registers ``torch.ops.qf_b200.*`` (the PyTorch operators over this C ABI, csrc/qf_torch_ops.cpp); raises if they
+    are not built.  Returns the ``int8_linear`` op."""
     global _torch_ops_loaded
     import torch
     if not _torch_ops_loaded:

@@ -4,7 +4,7 @@
 ``qwen_a100_fastpath_b200/libqf_b200.so`` with the CUDA runtime linked statically, so the library needs no
 toolkit at run time and loads on a machine without a GPU (no CUDA call happens at load).  It then compiles
 ``csrc/qf_torch_ops.cpp`` with the host C++ compiler against the installed PyTorch into ``_qf_torch_ops.so``
-(``torch.ops.qf_b200.int8_linear``), linked to ``libqf_b200.so`` next to it.
+(``torch.ops.qf_b200.*``), linked to ``libqf_b200.so`` next to it.
 """
 from __future__ import annotations
 
@@ -20,7 +20,8 @@ INCLUDE = PKG.parent / "include"
 LIB = PKG / "libqf_b200.so"
 TORCH_OPS = PKG / "_qf_torch_ops.so"
 TORCH_OPS_SOURCE = "qf_torch_ops.cpp"
-SOURCES = ["qf_w8a16.cu", "qf_allreduce.cu", "qf_quant.cu", "qf_w8a8.cu", "qf_spec_attn.cu"]
+SOURCES = ["qf_w8a16.cu", "qf_allreduce.cu", "qf_quant.cu", "qf_w8a8.cu", "qf_spec_attn.cu", "qf_fp8_quant.cu",
+           "qf_fp8_gemm.cu", "qf_norm.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

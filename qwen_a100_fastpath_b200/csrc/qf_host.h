@@ -5,4 +5,8 @@
 namespace qf {
 // Records the message of a failing entry point (returned by qf_last_error_detail on this thread) and returns code.
 int fail(int code, const std::string& msg);
+
+// Checks that the current device is a B200 (sm_100a) and returns its index and SM count (either may be null).  The
+// answer is kept per device; QF_OK or the code recorded by fail().
+int require_b200(int* dev, int* sms);
 }  // namespace qf

@@ -8,7 +8,13 @@
 // of Python-level checks and a ctypes call.  Workspaces come from the PyTorch caching allocator, one per
 // (device, stream) and kind, zero-filled when allocated (the kernels leave their counters at zero).  The caller
 // decides eligibility (bf16 activations, a weight the tensor maps can take); anything else raises.
+//
+// torch.ops.qf_b200.fp8_quantize / fp8_block_mm / fp8_block_linear / residual_norm are the operators of block-scaled fp8
+// layers (fp8.py and norms.py document them).  They need no workspace: what they make comes from the caching allocator,
+// so calls on several streams, and captured graphs, share nothing.  They refuse a call with a ValueError before anything
+// is launched, and inputs that require a gradient too: none of them has a backward.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -98,10 +104,303 @@ at::Tensor int8_linear_meta(const at::Tensor& x, const at::Tensor& w_q, const at
   return at::empty(out_shape, x.options());
 }
 
+// ---------------------------------------------------------------------------------------- block-scaled fp8 layers
+#define QF_REFUSE_UNLESS(cond, ...) TORCH_CHECK_VALUE(cond, __VA_ARGS__)
+
+using OptTensor = c10::optional<at::Tensor>;
+
+constexpr int64_t kBlock = 128;
+int64_t blocks(int64_t v) { return (v + kBlock - 1) / kBlock; }
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+void check_input(const char* op, const char* name, const at::Tensor& t, at::ScalarType type, const at::Device& dev) {
+  QF_REFUSE_UNLESS(t.is_cuda(), op, ": ", name, " must be a CUDA tensor (there is no CPU path)");
+  QF_REFUSE_UNLESS(t.device() == dev, op, ": ", name, " is on ", t.device(), ", the first input on ", dev);
+  QF_REFUSE_UNLESS(t.scalar_type() == type, op, ": ", name, " must be ", type, ", got ", t.scalar_type());
+  QF_REFUSE_UNLESS(!(at::GradMode::is_enabled() && t.requires_grad()), op, ": ", name,
+                   " requires a gradient and the operator has no backward (call it under torch.no_grad())");
+}
+
+cudaStream_t stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+int as_int(const char* op, int64_t v) {
+  QF_REFUSE_UNLESS(v <= INT32_MAX, op, ": a size of ", v, " is too large");
+  return static_cast<int>(v);
+}
+
+// [..., K] as rows of unit column stride, without a copy where the strides allow it.
+at::Tensor as_rows(const at::Tensor& x) {
+  at::Tensor r = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  if (r.size(1) > 1 && r.stride(1) != 1) r = r.contiguous();
+  if (r.size(0) > 1 && r.stride(0) < r.size(1)) r = r.contiguous();  // broadcast or overlapping rows
+  return r;
+}
+
+// The rows of a result with x's leading dimensions (a view).
+at::Tensor with_leading(const at::Tensor& rows, const at::Tensor& x) {
+  if (x.dim() == 2) return rows;
+  return x.dim() == 1 ? rows.select(0, 0) : rows.unflatten(0, x.sizes().slice(0, x.dim() - 1));
+}
+
+// e4m3 rows of 16-byte stride, as the product's tensor maps take them.
+at::Tensor empty_rows(int64_t M, int64_t K, const at::Tensor& like) {
+  at::Tensor q = at::empty({M, (K + 15) / 16 * 16}, like.options().dtype(at::kFloat8_e4m3fn));
+  return K % 16 ? q.narrow(1, 0, K) : q;
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_rows(const char* op, const at::Tensor& x2, bool silu_mul) {
+  const int64_t M = x2.size(0), K = silu_mul ? x2.size(1) / 2 : x2.size(1);
+  at::Tensor q = empty_rows(M, K, x2);
+  at::Tensor s = at::empty({M, blocks(K)}, x2.options().dtype(at::kFloat));
+  if (M && K)
+    check(qf_fp8_quantize(x2.data_ptr(), x2.stride(0), as_int(op, M), as_int(op, K), silu_mul, q.data_ptr(), q.stride(0),
+                          s.data_ptr<float>(), s.stride(0), QF_FLAG_PDL, stream_of(x2)),
+          "qf_fp8_quantize");
+  return {q, s};
+}
+
+std::tuple<at::Tensor, at::Tensor> fp8_quantize(const at::Tensor& x, bool silu_mul) {
+  QF_REFUSE_UNLESS(x.dim() >= 1, "fp8_quantize: x must have at least one dimension");
+  QF_REFUSE_UNLESS(!silu_mul || x.size(-1) % 2 == 0, "fp8_quantize: silu_mul needs gate and up halves of one width");
+  const int64_t K = silu_mul ? x.size(-1) / 2 : x.size(-1);
+  QF_REFUSE_UNLESS(K >= 1 && K <= QF_FP8_MAX_K, "fp8_quantize: 1 to ", QF_FP8_MAX_K, " values per row, got ", K);
+  check_input("fp8_quantize", "x", x, at::kBFloat16, x.device());
+  c10::cuda::CUDAGuard guard(x.device());
+  auto [q, s] = quantize_rows("fp8_quantize", as_rows(x), silu_mul);
+  return {with_leading(q, x), with_leading(s, x)};
+}
+
+void check_weight(const char* op, const at::Tensor& w_t, const at::Tensor& w_scale, const OptTensor& bias, int64_t K,
+                  const at::Device& dev) {
+  check_input(op, "w_t", w_t, at::kFloat8_e4m3fn, dev);
+  QF_REFUSE_UNLESS(w_t.dim() == 2 && w_t.size(0) == K, op, ": w_t must be [K, N] with K = ", K, ", got ", w_t.sizes());
+  const int64_t N = w_t.size(1);
+  QF_REFUSE_UNLESS(K >= 1 && K <= QF_FP8_MAX_K && N <= QF_MAX_N, op, ": K must be 1 to ", QF_FP8_MAX_K,
+                   " and N at most ", QF_MAX_N);
+  QF_REFUSE_UNLESS((K == 1 || w_t.stride(0) == 1) && (N <= 1 || (w_t.stride(1) >= K && w_t.stride(1) % 16 == 0)) &&
+                       reinterpret_cast<uintptr_t>(w_t.data_ptr()) % 16 == 0,
+                   op, ": w_t must be the [K, N] view of 16-byte aligned rows of a weight (stride (1, ldw), ldw a multiple "
+                   "of 16)");
+  check_input(op, "w_scale", w_scale, at::kFloat, dev);
+  QF_REFUSE_UNLESS(w_scale.dim() == 2 && w_scale.size(0) == blocks(N) && w_scale.size(1) == blocks(K), op,
+                   ": w_scale must be [", blocks(N), ", ", blocks(K), "], got ", w_scale.sizes());
+  if (given(bias)) {
+    check_input(op, "bias", *bias, at::kBFloat16, dev);
+    QF_REFUSE_UNLESS(bias->numel() == N, op, ": bias must hold ", N, " values");
+  }
+}
+
+void run_mm(const char* op, const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t,
+            const at::Tensor& w_scale, const OptTensor& bias, at::Tensor& y) {
+  const int64_t M = a.size(0), K = a.size(1), N = w_t.size(1);
+  if (M == 0 || N == 0) return;
+  at::Tensor b;
+  if (given(bias)) b = bias->reshape({-1}).contiguous();
+  check(qf_fp8_block_gemm(a.data_ptr(), a.stride(0), a_scale.data_ptr<float>(), a_scale.stride(0), a_scale.stride(1),
+                          w_t.data_ptr(), N > 1 ? w_t.stride(1) : K, w_scale.data_ptr<float>(), w_scale.stride(0),
+                          w_scale.stride(1), b.defined() ? b.data_ptr() : nullptr, y.data_ptr(), y.stride(0),
+                          y.scalar_type() == at::kFloat ? QF_DTYPE_F32 : QF_DTYPE_BF16, as_int(op, M), as_int(op, N),
+                          as_int(op, K), QF_FLAG_PDL, stream_of(a)),
+        "qf_fp8_block_gemm");
+}
+
+at::Tensor checked_a(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t, const at::Tensor& w_scale,
+                     const OptTensor& bias) {
+  const char* op = "fp8_block_mm";
+  QF_REFUSE_UNLESS(a.dim() == 2, op, ": a must be [M, K]");
+  check_input(op, "a", a, at::kFloat8_e4m3fn, a.device());
+  const int64_t M = a.size(0), K = a.size(1);
+  check_weight(op, w_t, w_scale, bias, K, a.device());
+  check_input(op, "a_scale", a_scale, at::kFloat, a.device());
+  QF_REFUSE_UNLESS(a_scale.dim() == 2 && a_scale.size(0) == M && a_scale.size(1) == blocks(K), op, ": a_scale must be [",
+                   M, ", ", blocks(K), "], got ", a_scale.sizes());
+  const bool fits = (K == 1 || a.stride(1) == 1) && (M <= 1 || (a.stride(0) >= K && a.stride(0) % 16 == 0)) &&
+                    reinterpret_cast<uintptr_t>(a.data_ptr()) % 16 == 0;
+  if (fits || M == 0) return a;
+  at::Tensor r = empty_rows(M, K, a);
+  r.copy_(a);
+  return r;
+}
+
+at::Tensor fp8_block_mm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t,
+                        const at::Tensor& w_scale, const OptTensor& bias, bool out_f32) {
+  c10::cuda::OptionalCUDAGuard guard(a.is_cuda() ? c10::optional<c10::Device>(a.device()) : c10::nullopt);
+  const at::Tensor r = checked_a(a, a_scale, w_t, w_scale, bias);
+  at::Tensor y = at::empty({a.size(0), w_t.size(1)}, a.options().dtype(out_f32 ? at::kFloat : at::kBFloat16));
+  run_mm("fp8_block_mm", r, a_scale, w_t, w_scale, bias, y);
+  return y;
+}
+
+void fp8_block_mm_out(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t, const at::Tensor& w_scale,
+                      const OptTensor& bias, at::Tensor out) {
+  const char* op = "fp8_block_mm";
+  c10::cuda::OptionalCUDAGuard guard(a.is_cuda() ? c10::optional<c10::Device>(a.device()) : c10::nullopt);
+  const at::Tensor r = checked_a(a, a_scale, w_t, w_scale, bias);
+  const int64_t M = a.size(0), N = w_t.size(1);
+  QF_REFUSE_UNLESS(out.device() == a.device() && out.dim() == 2 && out.size(0) == M && out.size(1) == N &&
+                       (out.scalar_type() == at::kFloat || out.scalar_type() == at::kBFloat16) &&
+                       (N == 1 || out.stride(1) == 1) && (M <= 1 || out.stride(0) >= N),
+                   op, ": out must be bf16 or fp32 [", M, ", ", N, "] on a's device with unit column stride");
+  for (const at::Tensor& t : {a, a_scale, w_t, w_scale}) at::assert_no_overlap(out, t);
+  if (given(bias)) at::assert_no_overlap(out, *bias);
+  run_mm(op, r, a_scale, w_t, w_scale, bias, out);
+}
+
+at::Tensor fp8_block_linear(const at::Tensor& x, const at::Tensor& w_t, const at::Tensor& w_scale, const OptTensor& bias) {
+  const char* op = "fp8_block_linear";
+  QF_REFUSE_UNLESS(x.dim() >= 1, op, ": x must have at least one dimension");
+  check_input(op, "x", x, at::kBFloat16, x.device());
+  check_weight(op, w_t, w_scale, bias, x.size(-1), x.device());
+  c10::cuda::CUDAGuard guard(x.device());
+  const at::Tensor x2 = as_rows(x);
+  at::Tensor y = at::empty({x2.size(0), w_t.size(1)}, x.options());
+  if (x2.size(0) && w_t.size(1)) {
+    auto [q, s] = quantize_rows(op, x2, false);
+    run_mm(op, q, s, w_t, w_scale, bias, y);
+  }
+  return with_leading(y, x);
+}
+
+// What residual_norm and residual_norm_out share; `r_out` is where the new residual goes.  Returns (h, scale), each
+// undefined where it is not asked for.
+std::tuple<at::Tensor, at::Tensor> run_norm(const at::Tensor& x, const OptTensor& residual, const OptTensor& pre_weight,
+                                            const OptTensor& post_weight, const OptTensor& gate, int64_t gate_act,
+                                            double residual_scale, double weight_offset, double eps, bool quantize,
+                                            at::Tensor& r_out) {
+  const char* op = "residual_norm";
+  const int64_t H = x.size(-1);
+  const at::Tensor x2 = as_rows(x);
+  const int64_t M = x2.size(0);
+  at::Tensor r2, g2, post, pre, h, s;
+  if (given(residual)) r2 = as_rows(*residual);
+  int64_t gm = 0, gh = 0;
+  if (given(gate)) {
+    // broadcast to the rows; the kernel takes a column stride of zero or one and any row stride
+    g2 = gate->dim() == 2 && x.dim() == 2 ? gate->expand({M, H}) : gate->expand(x.sizes()).reshape({M, H});
+    if (H > 1 && g2.stride(1) != 0 && g2.stride(1) != 1) g2 = g2.contiguous();
+    gm = M > 1 ? g2.stride(0) : 0;
+    gh = H > 1 ? g2.stride(1) : 0;
+  }
+  if (given(post_weight)) post = post_weight->contiguous();
+  const bool want_h = given(pre_weight);
+  if (want_h) {
+    pre = pre_weight->contiguous();
+    h = quantize ? empty_rows(M, H, x) : at::empty({M, H}, x.options());
+    if (quantize) s = at::empty({M, blocks(H)}, x.options().dtype(at::kFloat));
+  }
+  at::Tensor ro2 = r_out.dim() == 2 ? r_out : r_out.view({M, H});
+  if (M) {
+    auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    auto ld = [](const at::Tensor& t) { return t.defined() ? t.stride(0) : 0; };
+    check(qf_residual_norm(ptr(x2), ld(x2), ptr(r2), ld(r2), r_out.scalar_type() == at::kFloat ? QF_DTYPE_F32 : QF_DTYPE_BF16,
+                           ptr(g2), gm, gh, static_cast<int>(gate_act), ptr(post), ptr(pre),
+                           static_cast<float>(weight_offset), static_cast<float>(residual_scale), static_cast<float>(eps),
+                           ro2.data_ptr(), ro2.stride(0), ptr(h), ld(h), s.defined() ? s.data_ptr<float>() : nullptr, ld(s),
+                           as_int(op, M), as_int(op, H), QF_FLAG_PDL, stream_of(x)),
+          "qf_residual_norm");
+  }
+  if (h.defined()) h = with_leading(h, x);
+  if (s.defined()) s = with_leading(s, x);
+  return {h, s};
+}
+
+void check_norm(const at::Tensor& x, const OptTensor& residual, const OptTensor& pre_weight, const OptTensor& post_weight,
+                const OptTensor& gate, int64_t gate_act, double eps, bool quantize) {
+  const char* op = "residual_norm";
+  QF_REFUSE_UNLESS(x.dim() >= 1, op, ": x must have at least one dimension");
+  check_input(op, "x", x, at::kBFloat16, x.device());
+  const int64_t H = x.size(-1);
+  QF_REFUSE_UNLESS(H >= 1 && H <= QF_NORM_MAX_H, op, ": rows of 1 to ", QF_NORM_MAX_H, " values, got ", H);
+  if (given(residual)) {
+    QF_REFUSE_UNLESS(residual->scalar_type() == at::kBFloat16 || residual->scalar_type() == at::kFloat, op,
+                     ": residual must be bf16 or fp32");
+    check_input(op, "residual", *residual, residual->scalar_type(), x.device());
+    QF_REFUSE_UNLESS(residual->sizes() == x.sizes(), op, ": residual must have x's shape ", x.sizes(), ", got ",
+                     residual->sizes());
+  }
+  for (const auto& [name, w] : {std::make_pair("pre_weight", &pre_weight), std::make_pair("post_weight", &post_weight)})
+    if (given(*w)) {
+      check_input(op, name, **w, at::kBFloat16, x.device());
+      QF_REFUSE_UNLESS((*w)->dim() == 1 && (*w)->size(0) == H, op, ": ", name, " must be [", H, "]");
+    }
+  QF_REFUSE_UNLESS(!quantize || given(pre_weight), op, ": quantize needs pre_weight");
+  QF_REFUSE_UNLESS(gate_act >= QF_GATE_NONE && gate_act <= QF_GATE_SILU, op, ": unknown gate activation");
+  if (given(gate)) {
+    check_input(op, "gate", *gate, at::kBFloat16, x.device());
+    QF_REFUSE_UNLESS(gate->dim() <= x.dim(), op, ": gate has more dimensions than x");
+    for (int64_t i = 1; i <= gate->dim(); ++i)
+      QF_REFUSE_UNLESS(gate->size(-i) == 1 || gate->size(-i) == x.size(-i), op, ": gate ", gate->sizes(),
+                       " does not broadcast to ", x.sizes());
+  } else {
+    QF_REFUSE_UNLESS(gate_act == QF_GATE_NONE, op, ": a gate activation without a gate");
+  }
+  QF_REFUSE_UNLESS(eps >= 0 && eps <= 3.4e38, op, ": eps must be finite and >= 0");
+}
+
+std::tuple<OptTensor, OptTensor, at::Tensor> residual_norm(const at::Tensor& x, const OptTensor& residual,
+                                                           const OptTensor& pre_weight, const OptTensor& post_weight,
+                                                           const OptTensor& gate, int64_t gate_act, double residual_scale,
+                                                           double weight_offset, double eps, bool quantize) {
+  check_norm(x, residual, pre_weight, post_weight, gate, gate_act, eps, quantize);
+  c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor r_out = at::empty(x.sizes(), given(residual) ? residual->options() : x.options());
+  auto [h, s] = run_norm(x, residual, pre_weight, post_weight, gate, gate_act, residual_scale, weight_offset, eps, quantize,
+                         r_out);
+  return {h.defined() ? OptTensor(h) : c10::nullopt, s.defined() ? OptTensor(s) : c10::nullopt, r_out};
+}
+
+std::tuple<OptTensor, OptTensor> residual_norm_out(const at::Tensor& x, const OptTensor& residual,
+                                                   const OptTensor& pre_weight, const OptTensor& post_weight,
+                                                   const OptTensor& gate, int64_t gate_act, double residual_scale,
+                                                   double weight_offset, double eps, bool quantize,
+                                                   at::Tensor residual_out) {
+  const char* op = "residual_norm";
+  check_norm(x, residual, pre_weight, post_weight, gate, gate_act, eps, quantize);
+  const at::ScalarType type = given(residual) ? residual->scalar_type() : at::kBFloat16;
+  check_input(op, "residual_out", residual_out, type, x.device());
+  QF_REFUSE_UNLESS(residual_out.sizes() == x.sizes(), op, ": residual_out must have x's shape ", x.sizes());
+  const int64_t H = x.size(-1);
+  QF_REFUSE_UNLESS((H == 1 || residual_out.stride(-1) == 1) && (residual_out.dim() == 2 || residual_out.is_contiguous()) &&
+                       (residual_out.dim() != 2 || residual_out.size(0) <= 1 || residual_out.stride(0) >= H),
+                   op, ": residual_out must have unit column stride and rows that do not overlap (and be contiguous "
+                   "unless it is 2-D)");
+  if (given(residual)) {
+    // the residual itself is updated in place; any other overlap would be read after it is written
+    if (residual->data_ptr() != residual_out.data_ptr() || residual->strides() != residual_out.strides())
+      at::assert_no_overlap(residual_out, *residual);
+  }
+  at::assert_no_overlap(residual_out, x);
+  for (const OptTensor* t : {&pre_weight, &post_weight, &gate})
+    if (given(*t)) at::assert_no_overlap(residual_out, **t);
+  c10::cuda::CUDAGuard guard(x.device());
+  auto [h, s] = run_norm(x, residual, pre_weight, post_weight, gate, gate_act, residual_scale, weight_offset, eps, quantize,
+                         residual_out);
+  return {h.defined() ? OptTensor(h) : c10::nullopt, s.defined() ? OptTensor(s) : c10::nullopt};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(qf_b200, m) {
   m.def("int8_linear(Tensor x, Tensor w_q, Tensor w_s, Tensor? bias) -> Tensor");
+  m.def("fp8_quantize(Tensor x, bool silu_mul) -> (Tensor, Tensor)");
+  m.def("fp8_block_mm(Tensor a, Tensor a_scale, Tensor w_t, Tensor w_scale, Tensor? bias, bool out_f32) -> Tensor");
+  m.def("fp8_block_mm_out(Tensor a, Tensor a_scale, Tensor w_t, Tensor w_scale, Tensor? bias, Tensor(a!) out) -> ()");
+  m.def("fp8_block_linear(Tensor x, Tensor w_t, Tensor w_scale, Tensor? bias) -> Tensor");
+  m.def("residual_norm(Tensor x, Tensor? residual, Tensor? pre_weight, Tensor? post_weight, Tensor? gate, int gate_act, "
+        "float residual_scale, float weight_offset, float eps, bool quantize) -> (Tensor?, Tensor?, Tensor)");
+  m.def("residual_norm_out(Tensor x, Tensor? residual, Tensor? pre_weight, Tensor? post_weight, Tensor? gate, int gate_act, "
+        "float residual_scale, float weight_offset, float eps, bool quantize, Tensor(a!) residual_out) -> "
+        "(Tensor?, Tensor?)");
+}
+// CompositeExplicitAutograd: CPU tensors reach the operators' own refusals instead of the dispatcher's.
+TORCH_LIBRARY_IMPL(qf_b200, CompositeExplicitAutograd, m) {
+  m.impl("fp8_quantize", fp8_quantize);
+  m.impl("fp8_block_mm", fp8_block_mm);
+  m.impl("fp8_block_mm_out", fp8_block_mm_out);
+  m.impl("fp8_block_linear", fp8_block_linear);
+  m.impl("residual_norm", residual_norm);
+  m.impl("residual_norm_out", residual_norm_out);
 }
 TORCH_LIBRARY_IMPL(qf_b200, CUDA, m) { m.impl("int8_linear", int8_linear); }
 TORCH_LIBRARY_IMPL(qf_b200, Meta, m) { m.impl("int8_linear", int8_linear_meta); }
