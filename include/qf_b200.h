@@ -223,6 +223,11 @@ int qf_fp8_block_gemm(const void* a, int64_t lda, const float* a_scale, int64_t 
                       int64_t ldw, const float* w_scale, int64_t sw_n, int64_t sw_g, const void* bias, void* y,
                       int64_t ldy, int y_dtype, int M, int N, int K, unsigned flags, void* stream);
 
+/* Reads and clears the current device's sticky error flag of qf_fp8_block_gemm (synchronises `stream`): every wait inside
+ * a launch is bounded (about 4 s), and one that expires leaves QF_ERR_TIMEOUT here and a result that is not valid.
+ * Not for the hot path. */
+int qf_fp8_status(void* stream, int* status);
+
 /* ---- residual update with the norms on both sides of a block -----------------------------------------------------
  * One pass over a token row of H elements, fp32 inside (the reference plugin leaves norms to vLLM):
  *   u = x, or x * rsqrt(mean(x^2) + eps) * (post_weight + weight_offset) where post_weight is given;

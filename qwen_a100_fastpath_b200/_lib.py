@@ -73,6 +73,7 @@ SIGNATURES = [
     ("qf_fp8_block_gemm", _c.c_int,
      [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64,
       _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_uint, _c.c_void_p]),
+    ("qf_fp8_status", _c.c_int, [_c.c_void_p, _c.POINTER(_c.c_int)]),
     ("qf_residual_norm", _c.c_int,
      [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int,
       _c.c_void_p, _c.c_void_p, _c.c_float, _c.c_float, _c.c_float, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64,

@@ -5,11 +5,20 @@
 // a[m, k] * w[n, k].  Products of e4m3 values are exact in fp32; each P_g is summed by the tensor cores in fp32 and
 // folded into fp32 sums with one multiply-add per group and output.
 //
-// fp8_rows_kernel: a CTA of eight warps takes 16 weight rows and 8 * NT tokens, warp w the groups w, w + 8, ...; the
+// fp8_tile_kernel (more than 16 token rows): 128 token rows x BN channels on tcgen05 kind::f8f6f4, one tensor-memory
+// accumulator per k group; two producer and two issuing warps feed it from a ring of TMA stages (128-byte rows, 128-byte
+// swizzle), eight warps add each finished accumulator, times its scales, to fp32 sums in registers while the next
+// groups are multiplied.  With fewer tiles than SMs a cluster shares a tile's groups and adds its parts over distributed
+// shared memory, in rank order.  What bounds it: shared memory's 128 bytes a clock, which a group's copies and operand
+// reads take twice (2 x (16 KiB + BN * 128)).
+//
+// fp8_rows_kernel (up to 16): a CTA of eight warps takes 16 weight rows and 8 * NT tokens, warp w the groups w, w + 8, ...; the
 // weights go from global memory straight into the registers of mma.sync m16n8k32 (weights as the 16-row operand), the
 // warps' sums are added in shared memory in warp order.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>
 
 #include <cstdint>
 #include <mutex>
@@ -121,8 +130,558 @@ __global__ void __launch_bounds__(kRowWarps * 32) fp8_rows_kernel(const Fp8Param
   }
 }
 
+// ---------------------------------------------------------------------------------------------- tcgen05 tiles
+constexpr int kTileM = 128;
+constexpr long long kFp8WaitClocks = 8000000000ll;  // about 4 s; the global timer would cost each poll its read
+
+__device__ int g_fp8_err;  // sticky: QF_ERR_TIMEOUT once a bounded wait expired (read by qf_fp8_status)
+
+// Scales of kScaleK groups at a time, kScaleBufs chunks in flight, in shared memory.
+constexpr int kScaleK = 8, kScaleBufs = 3;
+
+constexpr int kMaxStages = 12;
+
+template <int BN, int EW, bool SPLIT> struct TileGeo {
+  static constexpr int kThreads = 128 + 32 * EW;
+  static constexpr int kBBytes = BN * kFp8Block;
+  // a stage: the weight tile, then the token rows of the tile (fewer than 128 where the call has fewer)
+  static constexpr int kRing = 196 * 1024;
+  static constexpr int kTmemCols = 512;
+  static constexpr int kAccs = kTmemCols / BN;    // one k group each
+  static constexpr int kCols = BN * 4 / EW;       // columns per epilogue thread
+  static constexpr int kChunks = kCols / 32;
+  static constexpr int kOffBar = kRing;
+  static constexpr int kNumBars = 2 * kMaxStages + 2 * kAccs + 1;
+  static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+  static constexpr int kOffScale = kOffMisc + 24;
+  // a chunk: [group][epilogue thread], then per epilogue warp [group][one of its two weight blocks]
+  static constexpr int kScaleBuf = kScaleK * (32 * EW + 2 * EW);
+  static constexpr int kSmemBytes = kOffScale + kScaleBufs * kScaleBuf * 4 + 1024;
+  static_assert(EW == 4 || EW == 8, "one or two warps per tensor-memory quarter");
+  static_assert(kCols % 32 == 0 && kCols <= 128, "columns per epilogue thread");
+  static_assert(kRing / (kBBytes + kTileM * kFp8Block) >= 4 && kSmemBytes <= 227 * 1024, "shared memory");
+  static_assert(!SPLIT || kTileM * BN * 4 <= kRing, "the partial tile reuses the ring");
+};
+
+__device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (true) {
+    if (*abort_flag) return false;
+    if (mbar_try_wait(bar, parity)) return true;
+    if (clock64() - t0 > kFp8WaitClocks) {
+      atomicExch(&g_fp8_err, QF_ERR_TIMEOUT);
+      *abort_flag = 1;
+      return false;
+    }
+  }
+}
+
+struct TileParams {
+  Fp8Params p;
+  int mtiles, ntiles, splits;
+  int box_rows;  // token rows copied per tile
+  int stages;    // of the ring: weight tile and token rows
+  int vec_out;
+};
+
+// First output row and column of tile t.  Tiles run down the token rows first (bands of 32 tiles, 4096 rows), so that
+// the CTAs of a wave share weight tiles through L2 and a band of activations stays there.
+__device__ __forceinline__ void tile_origin(const TileParams& tp, int t, int bn, int* m0, int* n0) {
+  if (tp.mtiles == 1) {
+    *m0 = 0;
+    *n0 = t * bn;
+    return;
+  }
+  const int band = tp.mtiles > 32 ? t / (32 * tp.ntiles) : 0;
+  const int rows = min(32, tp.mtiles - 32 * band);
+  const int in = t - band * 32 * tp.ntiles;
+  *m0 = (32 * band + in % rows) * kTileM;
+  *n0 = in / rows * bn;
+}
+
+__device__ __forceinline__ void store8(const TileParams& tp, int m, int n, const float (&v)[8]) {
+  const Fp8Params& p = tp.p;
+  float o[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = v[j] + ((p.bias && n + j < p.N) ? __bfloat162float(p.bias[n + j]) : 0.f);
+  const int64_t at = static_cast<int64_t>(m) * p.ldy + n;
+  if (p.y_f32) {
+    float* y = static_cast<float*>(p.y) + at;
+    if (tp.vec_out && n + 8 <= p.N) {
+      reinterpret_cast<float4*>(y)[0] = make_float4(o[0], o[1], o[2], o[3]);
+      reinterpret_cast<float4*>(y)[1] = make_float4(o[4], o[5], o[6], o[7]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n + j < p.N) y[j] = o[j];
+    }
+  } else {
+    __nv_bfloat16* y = static_cast<__nv_bfloat16*>(p.y) + at;
+    if (tp.vec_out && n + 8 <= p.N) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * j], o[2 * j + 1]);
+        w[j] = reinterpret_cast<const uint32_t&>(h);
+      }
+      *reinterpret_cast<uint4*>(y) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n + j < p.N) y[j] = __float2bfloat16_rn(o[j]);
+    }
+  }
+}
+
+template <int BN, int EW, bool SPLIT>
+__global__ void __launch_bounds__(128 + 32 * EW, 1)
+    fp8_tile_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
+                    const __grid_constant__ TileParams tp) {
+  using C = TileGeo<BN, EW, SPLIT>;
+  constexpr int A = C::kAccs;
+  const int S = tp.stages;
+  const uint32_t stage_bytes = C::kBBytes + static_cast<uint32_t>(tp.box_rows) * kFp8Block;
+  const Fp8Params& p = tp.p;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* acc_full = empty + kMaxStages;
+  uint64_t* acc_empty = acc_full + A;
+  uint64_t* mma_done = acc_empty + A;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int ntotal = tp.mtiles * tp.ntiles;
+  // with SPLIT the cluster's CTAs take one tile and a share of its k groups each
+  const int rank = SPLIT ? static_cast<int>(cluster_rank()) : 0;
+  const int first = SPLIT ? static_cast<int>(blockIdx.x) / tp.splits : static_cast<int>(blockIdx.x);
+  const int step = SPLIT ? ntotal : static_cast<int>(gridDim.x);
+  const int k0 = SPLIT ? static_cast<int>(static_cast<int64_t>(p.kb) * rank / tp.splits) : 0;
+  const int k1 = SPLIT ? static_cast<int>(static_cast<int64_t>(p.kb) * (rank + 1) / tp.splits) : p.kb;
+
+  const uint64_t pol_w = policy_evict_normal();
+  const uint64_t pol_a = policy_evict_last();
+  auto copy_group = [&](int s, int kb, int m0, int n0) {
+    uint8_t* dst = smem + s * stage_bytes;
+    mbar_arrive_expect_tx(&full[s], stage_bytes);
+    tma_load_2d(dst, &tmap_w, &full[s], kb * kFp8Block, n0, pol_w);
+    tma_load_2d(dst + C::kBBytes, &tmap_a, &full[s], kb * kFp8Block, m0, pol_a);
+  };
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tmap_a);
+    prefetch_tensormap(&tmap_w);
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < A; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], EW);  // one arrival per epilogue warp
+    }
+    mbar_init(mma_done, 2);
+    *s_abort = 0;
+    fence_mbar_init();
+    // the first group is on its way before the CTA meets
+    pdl_wait();
+    int m0, n0;
+    tile_origin(tp, first, BN, &m0, &n0);
+    copy_group(0, k0, m0, n0);
+  }
+  if (warp == 2) tmem_alloc(s_tmem, C::kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  pdl_launch_dependents();  // after the tensor memory is held: a dependent's CTA could otherwise take it and wait for us
+  pdl_wait();
+
+  // where an epilogue thread holds more than 64 sums: 168 registers a thread at launch, and the three warpgroups'
+  // 56 + 224 + 224 use what the block has
+  if (warp < 4) {
+    if (C::kCols > 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    // A barrier wait takes a producing or issuing lane some 200 clocks even where the barrier is complete, as long as the
+    // matrix instructions of a group: two warps take turns in both roles.
+    if (warp < 2) {
+      if (lane == 0) {
+        int it = 0;
+        int s = warp;          // stage and phase of this warp's next turn
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int t = first; t < ntotal && ok; t += step) {
+          int m0, n0;
+          tile_origin(tp, t, BN, &m0, &n0);
+          for (int kb = k0; kb < k1; ++kb, ++it) {
+            if ((it & 1) != warp) continue;
+            if (it > 0) {  // the first group is under way
+              if (!fp8_wait(&empty[s], phase ^ 1, s_abort)) {
+                ok = false;
+                break;
+              }
+              copy_group(s, kb, m0, n0);
+            }
+            s += 2;
+            if (s >= S) s -= S, phase ^= 1;
+          }
+        }
+        // every copy issued must land before the shared memory is released
+        for (int i = it > S ? it - S : 0; i < it; ++i) {
+          if ((i & 1) != warp) continue;
+          const long long t0 = clock64();
+          while (!mbar_try_wait(&full[i % S], static_cast<uint32_t>(i / S) & 1u)) {
+            if (clock64() - t0 > kFp8WaitClocks) {
+              atomicExch(&g_fp8_err, QF_ERR_TIMEOUT);
+              *s_abort = 1;
+              break;
+            }
+          }
+        }
+      }
+      __syncwarp();
+    } else {
+      if (lane == 0) {
+        constexpr uint32_t idesc = idesc_e4m3(kTileM, BN);
+        const uint32_t smem_base = smem_u32(smem);
+        int it = 0;
+        int s = warp - 2;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int t = first; t < ntotal && ok; t += step) {
+          for (int kb = k0; kb < k1; ++kb, ++it) {
+            if ((it & 1) != warp - 2) continue;
+            const int b = it % A;
+            if (!fp8_wait(&acc_empty[b], ((it / A) & 1) ^ 1, s_abort)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();  // after the epilogue's loads (the copies' own barriers need no fence)
+            if (!fp8_wait(&full[s], phase, s_abort)) {
+              ok = false;
+              break;
+            }
+            const uint32_t w_addr = smem_base + s * stage_bytes;
+            // rows of the tile past box_rows are whatever lies behind them in the ring: their results are not used
+            const uint64_t a_desc = smem_desc_k128_sw128(w_addr + C::kBBytes);
+            const uint64_t b_desc = smem_desc_k128_sw128(w_addr);
+            const uint32_t d = tmem + static_cast<uint32_t>(b * BN);
+#pragma unroll
+            for (int k = 0; k < kFp8Block / 32; ++k) mma_e4m3(d, a_desc + 2 * k, b_desc + 2 * k, idesc, k != 0);
+            mma_commit(&empty[s]);
+            mma_commit(&acc_full[b]);
+            s += 2;
+            if (s >= S) s -= S, phase ^= 1;
+          }
+        }
+        // all issued MMAs complete before the tensor memory can be freed
+        mma_commit(mma_done);
+        const long long t0 = clock64();
+        while (!mbar_try_wait(mma_done, 0)) {
+          if (clock64() - t0 > kFp8WaitClocks) {
+            atomicExch(&g_fp8_err, QF_ERR_TIMEOUT);
+            break;
+          }
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    if (C::kCols > 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int q = warp & 3;                        // tensor-memory lane quarter this warp may read
+    const int col0 = (warp - 4) / 4 * C::kCols;    // its columns of the tile
+    const int row = 32 * q + lane;
+    const int et = threadIdx.x - 128;
+    float* s_scale = reinterpret_cast<float*>(smem + C::kOffScale);
+    const int nb_last = (p.N - 1) / kFp8Block;
+
+    // Scales: each thread copies its row's, and the warp its two weight blocks', a chunk of groups at a time and two
+    // chunks ahead (a cache miss per group would stall every one of them); the copies run on across tiles.
+    int lt = first, lk = k0, lch = 0;
+    const float* l_sa = nullptr;
+    const float* l_sw = nullptr;
+    auto load_chunk_of_scales = [&]() {
+      if (lt < ntotal) {
+        if (lk == k0) {
+          int m0, n0;
+          tile_origin(tp, lt, BN, &m0, &n0);
+          l_sa = p.sa + static_cast<int64_t>(min(m0 + row, p.M - 1)) * p.sa_m;
+          const int nb = (n0 + col0 + ((lane & 1) ? C::kCols - 1 : 0)) / kFp8Block;
+          l_sw = p.sw + static_cast<int64_t>(min(nb, nb_last)) * p.sw_n;
+        }
+        const uint32_t dst = smem_u32(s_scale + lch % kScaleBufs * C::kScaleBuf);
+#pragma unroll
+        for (int i = 0; i < kScaleK; ++i) {
+          const int64_t g = min(lk + i, p.kb - 1);
+          cp_async4(dst + 4 * (i * 32 * EW + et), l_sa + g * p.sa_g);
+        }
+        if (lane < 2 * kScaleK) {
+          const int64_t g = min(lk + lane / 2, p.kb - 1);
+          cp_async4(dst + 4 * (kScaleK * 32 * EW + (warp - 4) * 2 * kScaleK + lane), l_sw + g * p.sw_g);
+        }
+        lk += kScaleK;
+        if (lk >= k1) lk = k0, lt += step;
+      }
+      cp_async_commit();
+      ++lch;
+    };
+    load_chunk_of_scales();
+    load_chunk_of_scales();
+
+    int it = 0, ch = 0;
+    bool ok = true;
+    for (int t = first; t < ntotal && ok; t += step) {
+      int m0, n0;
+      tile_origin(tp, t, BN, &m0, &n0);
+      const int m = m0 + row;
+      // the thread's columns lie in at most two scale blocks; 32 of them in one (n0 and col0 are multiples of 32)
+      const int split_col = kFp8Block - (n0 + col0) % kFp8Block;
+      uint64_t acc[C::kCols / 2];
+#pragma unroll
+      for (int j = 0; j < C::kCols / 2; ++j) acc[j] = 0;
+      for (int kc = k0; kc < k1 && ok; kc += kScaleK, ++ch) {
+        __syncwarp();  // the buffer of the chunk before last is free in every lane
+        load_chunk_of_scales();
+        cp_async_wait<2>();
+        __syncwarp();
+        const float* sc = s_scale + ch % kScaleBufs * C::kScaleBuf;
+        const float* scw = sc + kScaleK * 32 * EW + (warp - 4) * 2 * kScaleK;
+        const int kn = min(kScaleK, k1 - kc);
+        for (int i = 0; i < kn; ++i, ++it) {
+          const int b = it % A;
+          const float sa = sc[i * 32 * EW + et];
+          const float s0 = sa * scw[2 * i], s1 = sa * scw[2 * i + 1];
+          // the warp goes on together (tcgen05.ld needs it whole): at once, or with lane 0's bounded wait
+          if (!__all_sync(0xffffffffu, mbar_try_wait(&acc_full[b], (it / A) & 1))) {
+            int have = 0;
+            if (lane == 0) have = fp8_wait(&acc_full[b], (it / A) & 1, s_abort) ? 1 : 0;
+            if (!__shfl_sync(0xffffffffu, have, 0)) {
+              ok = false;
+              break;
+            }
+          }
+          tc_fence_after();
+          const uint32_t src = tmem + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(b * BN + col0);
+          // the next 32 columns are on their way while these are added
+          uint32_t r[2][32];
+          tmem_ld_32x32b_x32_async(src, r[0]);
+#pragma unroll
+          for (int c = 0; c < C::kChunks; ++c) {
+            tmem_ld_wait(r[c & 1]);
+            if (c + 1 < C::kChunks) {
+              tmem_ld_32x32b_x32_async(src + 32 * (c + 1), r[(c + 1) & 1]);
+            } else {
+              tc_fence_before();
+              if (lane == 0) mbar_arrive(&acc_empty[b]);
+            }
+            const float s = 32 * c < split_col ? s0 : s1;
+            const uint64_t s2 = pack_f32x2(s, s);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              fma_f32x2(acc[16 * c + j],
+                        pack_f32x2(__uint_as_float(r[c & 1][2 * j]), __uint_as_float(r[c & 1][2 * j + 1])), s2);
+          }
+        }
+      }
+      if (!ok) break;
+      if (SPLIT) {
+        // the ring is idle (every accumulator was read, so every MMA and copy is done): it takes the partial tile,
+        // column by column
+        float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int j = 0; j < C::kCols / 2; ++j) {
+          const float2 v = unpack_f32x2(acc[j]);
+          part[(col0 + 2 * j) * kTileM + row] = v.x;
+          part[(col0 + 2 * j + 1) * kTileM + row] = v.y;
+        }
+      } else if (m < p.M) {
+#pragma unroll
+        for (int j = 0; j < C::kCols / 8; ++j) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack_f32x2(acc[4 * j + i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+          }
+          store8(tp, m, n0 + col0 + 8 * j, v);
+        }
+      }
+    }
+    cp_async_wait<0>();
+  }
+  tc_fence_before();
+  if (SPLIT) {
+    cluster_sync();
+    // each CTA adds an equal part of the tile over the cluster, in rank order, and stores it
+    int m0, n0;
+    tile_origin(tp, first, BN, &m0, &n0);
+    const int rows = min(kTileM, p.M - m0), pieces = BN / 8;
+    const uint32_t part = smem_u32(smem);
+    if (!*s_abort) {
+      for (int e = rank * C::kThreads + threadIdx.x; e < rows * pieces; e += tp.splits * C::kThreads) {
+        const int row = e % rows, c = e / rows * 8;
+        if (n0 + c >= p.N) continue;
+        float v[8] = {};
+        for (int r = 0; r < tp.splits; ++r) {
+          const uint32_t src = map_to_rank(part + static_cast<uint32_t>((c * kTileM + row) * 4), r);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] += ld_cluster_f32(src + j * kTileM * 4);
+        }
+        store8(tp, m0 + row, n0 + c, v);
+      }
+    }
+    cluster_sync();  // no CTA leaves while another reads its part
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc(tmem, C::kTmemCols);
+}
+
 std::mutex g_dev_mu;
 int g_dev_sms[64] = {};
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+
+int encode_rows(CUtensorMap* map, const void* base, int K, int rows, int64_t row_bytes, int box_rows) {
+  {
+    std::lock_guard<std::mutex> lk(g_dev_mu);
+    if (!g_encode) {
+      cudaDriverEntryPointQueryResult qres;
+      void* fn = nullptr;
+      const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres);
+      if (e != cudaSuccess || qres != cudaDriverEntryPointSuccess || !fn)
+        return fail(QF_ERR_DRIVER, "cuTensorMapEncodeTiled entry point not found");
+      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }
+  }
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(kFp8Block), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(QF_ERR_DRIVER, "cuTensorMapEncodeTiled rejected the tensor (error " + std::to_string(r) + ")");
+  return QF_OK;
+}
+
+template <int BN, int EW, bool SPLIT>
+int launch_tiles(TileParams tp, int dev, int sms, int splits, unsigned flags, cudaStream_t st) {
+  using C = TileGeo<BN, EW, SPLIT>;
+  static bool attr_set[64] = {};
+  {
+    std::lock_guard<std::mutex> lk(g_dev_mu);
+    if (!attr_set[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(fp8_tile_kernel<BN, EW, SPLIT>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+      if (e != cudaSuccess) return fail(QF_ERR_LAUNCH, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+      attr_set[dev] = true;
+    }
+  }
+  const Fp8Params& p = tp.p;
+  tp.mtiles = (p.M + kTileM - 1) / kTileM;
+  tp.ntiles = (p.N + BN - 1) / BN;
+  tp.splits = splits;
+  CUtensorMap ta, tw;
+  // one row has no stride of its own: any multiple of 16 not below the row does
+  const int64_t one = (static_cast<int64_t>(p.K) + 15) / 16 * 16;
+  // whole swizzle atoms of eight rows
+  tp.box_rows = p.M < kTileM ? (p.M + 7) / 8 * 8 : kTileM;
+  tp.stages = C::kRing / (C::kBBytes + tp.box_rows * kFp8Block);
+  if (tp.stages > kMaxStages) tp.stages = kMaxStages;
+  // the last stage's MMA reads 128 rows from its token rows on: they have to lie in the ring
+  while (tp.stages * (C::kBBytes + tp.box_rows * kFp8Block) + (kTileM - tp.box_rows) * kFp8Block > C::kRing) --tp.stages;
+  int rc = encode_rows(&ta, p.a, p.K, p.M, p.M > 1 ? p.lda : one, tp.box_rows);
+  if (rc) return rc;
+  rc = encode_rows(&tw, p.w, p.K, p.N, p.N > 1 ? p.ldw : one, BN);
+  if (rc) return rc;
+  const int total = tp.mtiles * tp.ntiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(SPLIT ? total * splits : (total < sms ? total : sms)));
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int na = 0;
+  if (flags & QF_FLAG_PDL) {
+    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[na++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (SPLIT) {
+    attr[na].id = cudaLaunchAttributeClusterDimension;
+    attr[na].val.clusterDim.x = static_cast<unsigned>(splits);
+    attr[na].val.clusterDim.y = 1;
+    attr[na++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = static_cast<unsigned>(na);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_tile_kernel<BN, EW, SPLIT>, ta, tw, tp);
+  return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
+}
+
+// Clusters of `split` CTAs (one per SM) that the device runs at once: a cluster stays within one group of SMs, so this is
+// less than SMs / split for some sizes.  Asked once per device.
+int resident_clusters(int dev, int sms, int split) {
+  if (split == 1) return sms;
+  static int known[64][9] = {};
+  std::lock_guard<std::mutex> lk(g_dev_mu);
+  if (known[dev][split] == 0) {
+    using C = TileGeo<128, 8, true>;
+    int n = 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(split * sms));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaFuncSetAttribute(fp8_tile_kernel<128, 8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         C::kSmemBytes);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, fp8_tile_kernel<128, 8, true>, &cfg);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+    known[dev][split] = n > 0 ? n : -1;
+  }
+  return known[dev][split];
+}
+
+// Tile width and k split.  Time of a choice in microseconds: whole waves of CTAs, each a start and its groups at the
+// measured rate of one CTA (a group of 64 / 128 / 256 channels takes 0.30 / 0.38 / 0.52 us, shared memory's bandwidth),
+// and for a split the join of the parts.
+int tiles_any(const TileParams& tp, int dev, int sms, unsigned flags, cudaStream_t st) {
+  const Fp8Params& p = tp.p;
+  const int mt = (p.M + kTileM - 1) / kTileM;
+  int best_bn = 0, best_split = 1;
+  double best = 1e30;
+  for (int bn = 64; bn <= 256; bn *= 2) {
+    const double group = bn == 64 ? 0.30 : bn == 128 ? 0.38 : 0.52;
+    const long long tiles = static_cast<long long>(mt) * ((p.N + bn - 1) / bn);
+    for (int split = 1; split <= 8 && split <= p.kb; ++split) {
+      if (split > 1 && tiles * split > sms) break;  // a split is for the SMs that would idle
+      const int at_once = resident_clusters(dev, sms, split);
+      if (at_once <= 0) continue;
+      const double waves = static_cast<double>((tiles + at_once - 1) / at_once);
+      const double t = waves * (((p.kb + split - 1) / split) * group + 0.8) + (split > 1 ? 1.2 + 0.004 * bn : 0.0);
+      if (t < best) best = t, best_bn = bn, best_split = split;
+    }
+  }
+  if (best_split > 1) {
+    if (best_bn == 64) return launch_tiles<64, 8, true>(tp, dev, sms, best_split, flags, st);
+    if (best_bn == 128) return launch_tiles<128, 8, true>(tp, dev, sms, best_split, flags, st);
+    return launch_tiles<256, 8, true>(tp, dev, sms, best_split, flags, st);
+  }
+  if (best_bn == 64) return launch_tiles<64, 8, false>(tp, dev, sms, 1, flags, st);
+  if (best_bn == 128) return launch_tiles<128, 8, false>(tp, dev, sms, 1, flags, st);
+  return launch_tiles<256, 8, false>(tp, dev, sms, 1, flags, st);
+}
 
 }  // namespace
 
@@ -170,7 +729,8 @@ extern "C" int qf_fp8_block_gemm(const void* a, int64_t lda, const float* a_scal
   if (reinterpret_cast<uintptr_t>(a_scale) % 4 || reinterpret_cast<uintptr_t>(w_scale) % 4 ||
       reinterpret_cast<uintptr_t>(bias) % 2 || reinterpret_cast<uintptr_t>(y) % yb)
     return fail(QF_ERR_ALIGN, "scales, bias and y must be aligned to their element");
-  const int rc = require_b200(nullptr, nullptr);
+  int dev = 0, sms = 0;
+  const int rc = require_b200(&dev, &sms);
   if (rc) return rc;
   Fp8Params p = {};
   p.a = static_cast<const uint8_t*>(a);
@@ -191,6 +751,13 @@ extern "C" int qf_fp8_block_gemm(const void* a, int64_t lda, const float* a_scal
   p.N = N;
   p.K = K;
   p.kb = (K + kFp8Block - 1) / kFp8Block;
+  if (M > 16) {
+    TileParams tp = {};
+    tp.p = p;
+    tp.vec_out = reinterpret_cast<uintptr_t>(y) % 16 == 0 && (M == 1 || ldy * yb % 16 == 0);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return tiles_any(tp, dev, sms, flags, st);
+  }
   const int nt = M <= 8 ? 1 : 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((N + 15) / 16), static_cast<unsigned>((M + 8 * nt - 1) / (8 * nt)));
@@ -204,4 +771,20 @@ extern "C" int qf_fp8_block_gemm(const void* a, int64_t lda, const float* a_scal
   const cudaError_t e = nt == 1 ? cudaLaunchKernelEx(&cfg, fp8_rows_kernel<1>, p)
                                 : cudaLaunchKernelEx(&cfg, fp8_rows_kernel<2>, p);
   return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
+}
+
+extern "C" int qf_fp8_status(void* stream, int* status) {
+  if (!status) return fail(QF_ERR_INVALID, "null status");
+  const int rc = require_b200(nullptr, nullptr);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int v = 0;
+  const int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_fp8_err, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && v != 0) e = cudaMemcpyToSymbolAsync(g_fp8_err, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+  if (e == cudaSuccess && v != 0) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return fail(QF_ERR_LAUNCH, cudaGetErrorString(e));
+  *status = v;
+  return QF_OK;
 }

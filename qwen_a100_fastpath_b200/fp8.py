@@ -16,9 +16,11 @@ anything is launched; there is no CPU path, no backward and no fallback.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
-from ._lib import load_torch_ops
+from ._lib import LIB, check, load_torch_ops
 
 load_torch_ops()
 _quantize = torch.ops.qf_b200.fp8_quantize.default
@@ -59,3 +61,12 @@ def fp8_block_linear(x: torch.Tensor, w_t: torch.Tensor, w_scale: torch.Tensor,
     """The linear layer of a block-scaled fp8 checkpoint on bf16 ``x [..., K]``: ``fp8_block_mm(*fp8_quantize(x), w_t,
     w_scale, bias)`` with the leading dimensions kept, bf16 ``[..., N]``."""
     return _linear(x, w_t, w_scale, bias)
+
+
+def fp8_status(device=None) -> int:
+    """Read and clear the device's sticky error flag of the block-scaled product (``QF_OK`` or ``QF_ERR_TIMEOUT``, after a
+    bounded wait inside a launch expired); synchronises the device's current stream."""
+    with torch.cuda.device(torch.cuda.current_device() if device is None else device):
+        st = ctypes.c_int(0)
+        check("qf_fp8_status", LIB.qf_fp8_status(torch.cuda.current_stream().cuda_stream, ctypes.byref(st)))
+        return st.value

@@ -115,6 +115,10 @@ def test_norm_argument_validation(kw, code):
     assert len(LIB.qf_last_error_detail()) > 0
 
 
+def test_status_needs_a_place():
+    assert LIB.qf_fp8_status(None, None) == -1
+
+
 def test_empty_calls_make_no_cuda_call():
     assert quantize(M=0) == 0 and quantize(K=0, ldx=0) == 0
     assert gemm(M=0) == 0 and gemm(N=0) == 0

@@ -331,3 +331,9 @@ def test_refusals(dev):
     with pytest.raises(RuntimeError, match="single memory location"):
         fp8_block_mm(a, sa2, w, sw, out=big[:1024].view(4, 256))
     torch.cuda.synchronize(dev)
+
+
+def test_no_wait_expired(dev):
+    """None of the launches above (the same process) left a timeout behind."""
+    from qwen_a100_fastpath_b200.fp8 import fp8_status
+    assert fp8_status(dev) == 0
