@@ -12,8 +12,10 @@
 // shared memory, in rank order.  What bounds it: shared memory's 128 bytes a clock, which a group's copies and operand
 // reads take twice (2 x (16 KiB + BN * 128)).
 //
-// fp8_rows_kernel (up to 16): a CTA of eight warps takes 16 weight rows and 8 * NT tokens, warp w the groups w, w + 8, ...; the
-// weights go from global memory straight into the registers of mma.sync m16n8k32 (weights as the 16-row operand), the
+// fp8_rows_kernel (up to 16): bound by the weights' bytes.  A CTA takes tiles of 16 weight rows, a producer copies eight k groups of
+// them and of the token rows per stage into a ring (one TMA copy each: a copy costs its issuer and the TMA unit the same
+// whatever it moves), and warp w of eight multiplies the stage's k group w with
+// mma.sync m16n8k32 (weights as the 16-row operand, so that 8 token columns are not padded to a tcgen05 tile); the
 // warps' sums are added in shared memory in warp order.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -32,7 +34,7 @@
 namespace qf {
 namespace {
 
-constexpr int kRowWarps = 8;
+constexpr int kRowWarps = 4;
 
 struct Fp8Params {
   const uint8_t* a;
@@ -50,6 +52,49 @@ struct Fp8Params {
   int M, N, K, kb;
 };
 
+constexpr long long kFp8WaitClocks = 8000000000ll;  // about 4 s; the global timer would cost each poll its read
+
+__device__ int g_fp8_err;  // sticky: QF_ERR_TIMEOUT once a bounded wait expired (read by qf_fp8_status)
+
+__device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (true) {
+    if (*abort_flag) return false;
+    if (mbar_try_wait(bar, parity)) return true;
+    if (clock64() - t0 > kFp8WaitClocks) {
+      atomicExch(&g_fp8_err, QF_ERR_TIMEOUT);
+      *abort_flag = 1;
+      return false;
+    }
+  }
+}
+
+// The same by a whole warp, which goes on together: at once, or with lane 0's bounded wait.
+__device__ __forceinline__ bool fp8_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  int have = 0;
+  if ((threadIdx.x & 31) == 0) have = fp8_wait(bar, parity, abort_flag) ? 1 : 0;
+  return __shfl_sync(0xffffffffu, have, 0) != 0;
+}
+
+// ---------------------------------------------------------------------------------------------- few token rows
+constexpr int kRowPerSm = 3;
+
+// A tile of 16 * MT weight rows and 8 * NT tokens; a stage holds G k groups for each warp: [group][weight rows]
+// [128 bytes], then [group][token rows][128 bytes].
+template <int NT, int MT, int G> struct RowGeo {
+  static constexpr int kRows = 16 * MT;
+  static constexpr int kGroups = kRowWarps * G;
+  static constexpr int kWBytes = kGroups * kRows * kFp8Block;
+  static constexpr int kABytes = kGroups * 8 * NT * kFp8Block;
+  static constexpr int kStage = kWBytes + kABytes;
+  static constexpr int kSum = kRowWarps * NT * MT * 128;     // floats of the warps' sums
+  static constexpr int kStages = (224 * 1024 / kRowPerSm - 2048 - kSum * 4) / kStage;
+  static constexpr int kSmemBytes = kStages * kStage + kSum * 4 + 1024;
+  static_assert(kStages >= 2 && kSmemBytes <= 227 * 1024 / kRowPerSm - 1024, "shared memory");
+};
+
 // 16 bytes of an operand row from column k; bytes past K read as zero and are not touched.
 __device__ __forceinline__ uint4 load_chunk(const uint8_t* row, int k, int K) {
   if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
@@ -60,82 +105,219 @@ __device__ __forceinline__ uint4 load_chunk(const uint8_t* row, int k, int K) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int NT>
-__global__ void __launch_bounds__(kRowWarps * 32) fp8_rows_kernel(const Fp8Params p) {
-  __shared__ float red[kRowWarps][NT][32][4];
-  pdl_launch_dependents();
-  pdl_wait();
+// Scales of a warp's k group: the weight block's, tokens' 2t and 2t + 1 of each 8.
+template <int NT> struct RowScales {
+  float sw, sa[NT][2];
+};
+
+// One finished output, with its bias.
+__device__ __forceinline__ void store_row_sum(const Fp8Params& p, int n, int m, float v) {
+  if (n >= p.N || m >= p.M) return;
+  if (p.bias) v += __bfloat162float(p.bias[n]);
+  const int64_t at = static_cast<int64_t>(m) * p.ldy + n;
+  if (p.y_f32)
+    static_cast<float*>(p.y)[at] = v;
+  else
+    static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
+}
+
+template <int NT, int MT, int G>
+__global__ void __launch_bounds__(kRowWarps * 32 + 32, kRowPerSm)
+    fp8_rows_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
+                    const Fp8Params p, int ntiles) {
+  using C = RowGeo<NT, MT, G>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[C::kStages], empty[C::kStages];
+  __shared__ volatile int abort_flag;
+  float* red = reinterpret_cast<float*>(ring + C::kStages * C::kStage);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int gid = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (8 * NT);
-  // rows past the end repeat the last one: their products are computed and not stored
-  const uint8_t* w_lo = p.w + static_cast<int64_t>(min(n0 + gid, p.N - 1)) * p.ldw;
-  const uint8_t* w_hi = p.w + static_cast<int64_t>(min(n0 + gid + 8, p.N - 1)) * p.ldw;
-  const uint8_t* a_row[NT];
-  const float* sa_row[NT][2];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    a_row[j] = p.a + static_cast<int64_t>(min(m0 + 8 * j + gid, p.M - 1)) * p.lda;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) sa_row[j][i] = p.sa + static_cast<int64_t>(min(m0 + 8 * j + 2 * t + i, p.M - 1)) * p.sa_m;
-  }
-  const float* sw_row = p.sw + static_cast<int64_t>(n0 / kFp8Block) * p.sw_n;
-  float acc[NT][4] = {};
-  for (int g = warp; g < p.kb; g += kRowWarps) {
-    const int k = g * kFp8Block + 16 * t;
-    uint4 lo[2], hi[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      lo[c] = load_chunk(w_lo, k + 64 * c, p.K);
-      hi[c] = load_chunk(w_hi, k + 64 * c, p.K);
+  const int m0 = blockIdx.y * (8 * NT);
+  const int kfull = p.K / kFp8Block;  // groups that are copied; a shorter last one is read where it is used
+  const int nst = (kfull + C::kGroups - 1) / C::kGroups;
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tmap_w);
+    prefetch_tensormap(&tmap_a);
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kRowWarps);
     }
-    const float sw = __ldg(sw_row + g * p.sw_g);
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      float d[4] = {};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint4 b = load_chunk(a_row[j], k + 64 * c, p.K);
-        // the thread's 16 bytes stand for the instruction's k slots of two steps, the same ones in both operands
-        mma_e4m3_m16n8k32(d, lo[c].x, hi[c].x, lo[c].y, hi[c].y, b.x, b.y);
-        mma_e4m3_m16n8k32(d, lo[c].z, hi[c].z, lo[c].w, hi[c].w, b.z, b.w);
-      }
-      const float s0 = sw * __ldg(sa_row[j][0] + g * p.sa_g), s1 = sw * __ldg(sa_row[j][1] + g * p.sa_g);
-      acc[j][0] = fmaf(d[0], s0, acc[j][0]);
-      acc[j][1] = fmaf(d[1], s1, acc[j][1]);
-      acc[j][2] = fmaf(d[2], s0, acc[j][2]);
-      acc[j][3] = fmaf(d[3], s1, acc[j][3]);
-    }
+    abort_flag = 0;
+    fence_mbar_init();
   }
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) red[warp][j][lane][i] = acc[j][i];
   __syncthreads();
-  for (int e = threadIdx.x; e < NT * 128; e += kRowWarps * 32) {
-    const int r = e % 16, tok = e / 16;
-    const int src = (r % 8) * 4 + (tok % 8) / 2, reg = (r / 8) * 2 + (tok & 1);
-    float s = 0.f;
+  pdl_launch_dependents();
+  if (warp == kRowWarps) {
+    if (lane == 0) {
+      const uint64_t pol_w = policy_evict_first();
+      const uint64_t pol_a = policy_evict_last();
+      // the first stages' weights into L2 while the kernel before this one ends (no value is read before the wait)
+      for (int st = 0; st < min(C::kStages, nst); ++st)
+        tma_prefetch_3d(&tmap_w, 0, static_cast<int>(blockIdx.x) * C::kRows, st * C::kGroups);
+      pdl_wait();
+      int issued = 0, s = 0;
+      uint32_t phase = 1;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x) {
+        for (int st = 0; st < nst; ++st, ++issued) {
+          if (!fp8_wait(&empty[s], phase, &abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = ring + s * C::kStage;
+          mbar_arrive_expect_tx(&full[s], C::kStage);
+          tma_load_3d(dst, &tmap_w, &full[s], 0, tile * C::kRows, st * C::kGroups, pol_w);
+          tma_load_3d(dst + C::kWBytes, &tmap_a, &full[s], 0, m0, st * C::kGroups, pol_a);
+          if (++s == C::kStages) s = 0, phase ^= 1;
+        }
+      }
+      // every copy issued lands before the shared memory is given up
+      for (int i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&full[i % C::kStages], (i / C::kStages) & 1)) {
+          if (clock64() - t0 > kFp8WaitClocks) {
+            atomicExch(&g_fp8_err, QF_ERR_TIMEOUT);
+            abort_flag = 1;
+            break;
+          }
+        }
+      }
+    }
+  } else {
+    pdl_wait();
+    const int gid = lane >> 2, t = lane & 3;
+    // tokens past the end repeat the last one: their products are computed and not stored
+    const float* sa_row[NT][2];
 #pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) s += red[w][tok / 8][src][reg];
-    const int n = n0 + r, m = m0 + tok;
-    if (n < p.N && m < p.M) {
-      if (p.bias) s += __bfloat162float(p.bias[n]);
-      const int64_t at = static_cast<int64_t>(m) * p.ldy + n;
-      if (p.y_f32)
-        static_cast<float*>(p.y)[at] = s;
-      else
-        static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(s);
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        sa_row[j][i] = p.sa + static_cast<int64_t>(min(m0 + 8 * j + 2 * t + i, p.M - 1)) * p.sa_m;
+    // Thread t of a row takes the 16-byte pieces 2t and 2t + 1 of its 128 bytes, at their places under the 128-byte
+    // swizzle (piece ^ row % 8): the rows of a quarter warp then fall on different banks.
+    const uint32_t base = smem_u32(ring) + static_cast<uint32_t>(gid * 128);
+    const uint32_t piece[2] = {static_cast<uint32_t>(((2 * t) ^ gid) * 16), static_cast<uint32_t>(((2 * t + 1) ^ gid) * 16)};
+    int s = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x) {
+      const int n0 = tile * C::kRows;
+      const float* sw_row = p.sw + static_cast<int64_t>(n0 / kFp8Block) * p.sw_n;
+      auto load_scales = [&](RowScales<NT>& r, int g) {
+        if (g >= p.kb) return;
+        r.sw = __ldg(sw_row + g * p.sw_g);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) r.sa[j][i] = __ldg(sa_row[j][i] + g * p.sa_g);
+      };
+      float acc[NT][MT][4] = {};
+      auto add = [&](const uint4 (&lo)[MT][2], const uint4 (&hi)[MT][2], const uint4 (&b)[NT][2], const RowScales<NT>& r) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float s0 = r.sw * r.sa[j][0], s1 = r.sw * r.sa[j][1];
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            float d[2][4] = {};  // two chains of instructions
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              // the thread's 16 bytes stand for the instruction's k slots of two steps, the same ones in both operands
+              mma_e4m3_m16n8k32(d[c], lo[i][c].x, hi[i][c].x, lo[i][c].y, hi[i][c].y, b[j][c].x, b[j][c].y);
+              mma_e4m3_m16n8k32(d[c], lo[i][c].z, hi[i][c].z, lo[i][c].w, hi[i][c].w, b[j][c].z, b[j][c].w);
+            }
+            acc[j][i][0] = fmaf(d[0][0] + d[1][0], s0, acc[j][i][0]);
+            acc[j][i][1] = fmaf(d[0][1] + d[1][1], s1, acc[j][i][1]);
+            acc[j][i][2] = fmaf(d[0][2] + d[1][2], s0, acc[j][i][2]);
+            acc[j][i][3] = fmaf(d[0][3] + d[1][3], s1, acc[j][i][3]);
+          }
+        }
+      };
+      // group i of the warp's G in stage st
+      auto group_of = [&](int st, int i) { return st * C::kGroups + i * kRowWarps + warp; };
+      auto stage = [&](int st, RowScales<NT> (&r)[G]) {
+        if (!fp8_wait_warp(&full[s], phase, &abort_flag)) {
+          ok = false;
+          return;
+        }
+        uint4 lo[G][MT][2], hi[G][MT][2], b[G][NT][2];
+#pragma unroll
+        for (int u = 0; u < G; ++u) {
+          const uint32_t w_at = base + static_cast<uint32_t>(s * C::kStage + (u * kRowWarps + warp) * (C::kRows * kFp8Block));
+          const uint32_t a_at =
+              base + static_cast<uint32_t>(s * C::kStage + C::kWBytes + (u * kRowWarps + warp) * (8 * NT * kFp8Block));
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              lo[u][i][c] = lds128(w_at + 16 * i * kFp8Block + piece[c]);
+              hi[u][i][c] = lds128(w_at + (16 * i + 8) * kFp8Block + piece[c]);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) b[u][j][c] = lds128(a_at + 8 * j * kFp8Block + piece[c]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+        if (++s == C::kStages) s = 0, phase ^= 1;
+#pragma unroll
+        for (int u = 0; u < G; ++u) {
+          if (group_of(st, u) < kfull) add(lo[u], hi[u], b[u], r[u]);
+          load_scales(r[u], group_of(st + 2, u));  // two stages ahead
+        }
+      };
+      RowScales<NT> r0[G] = {}, r1[G] = {};
+#pragma unroll
+      for (int u = 0; u < G; ++u) {
+        load_scales(r0[u], group_of(0, u));
+        load_scales(r1[u], group_of(1, u));
+      }
+      for (int st = 0; st < nst && ok; st += 2) {
+        stage(st, r0);
+        if (st + 1 < nst && ok) stage(st + 1, r1);
+      }
+      if (kfull < p.kb && kfull % kRowWarps == warp) {  // the shorter last group
+        const int k = kfull * kFp8Block + 32 * t;
+        uint4 lo[MT][2], hi[MT][2], b[NT][2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            lo[i][c] = load_chunk(p.w + static_cast<int64_t>(min(n0 + 16 * i + gid, p.N - 1)) * p.ldw, k + 16 * c, p.K);
+            hi[i][c] = load_chunk(p.w + static_cast<int64_t>(min(n0 + 16 * i + gid + 8, p.N - 1)) * p.ldw, k + 16 * c, p.K);
+          }
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            b[j][c] = load_chunk(p.a + static_cast<int64_t>(min(m0 + 8 * j + gid, p.M - 1)) * p.lda, k + 16 * c, p.K);
+        }
+        load_scales(r0[0], kfull);
+        add(lo, hi, b, r0[0]);
+      }
+      // the warps' sums in warp order
+      named_bar_sync(1, kRowWarps * 32);  // the tile before is read
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) red[(((warp * NT + j) * MT + i) * 4 + e) * 32 + lane] = acc[j][i][e];
+      named_bar_sync(1, kRowWarps * 32);
+      // an abort that one warp saw before this barrier, all see here: they leave with the same barriers behind them
+      ok = !abort_flag;
+      for (int e = threadIdx.x; e < NT * MT * 128 && ok; e += kRowWarps * 32) {
+        const int r = e % C::kRows, tk = e / C::kRows;
+        const int src = (r % 8) * 4 + (tk % 8) / 2, reg = (r % 16 / 8) * 2 + (tk & 1);
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) v += red[(((w * NT + tk / 8) * MT + r / 16) * 4 + reg) * 32 + src];
+        store_row_sum(p, n0 + r, m0 + tk, v);
+      }
     }
   }
+  __syncthreads();
 }
 
 // ---------------------------------------------------------------------------------------------- tcgen05 tiles
 constexpr int kTileM = 128;
-constexpr long long kFp8WaitClocks = 8000000000ll;  // about 4 s; the global timer would cost each poll its read
-
-__device__ int g_fp8_err;  // sticky: QF_ERR_TIMEOUT once a bounded wait expired (read by qf_fp8_status)
-
 // Scales of kScaleK groups at a time, kScaleBufs chunks in flight, in shared memory.
 constexpr int kScaleK = 8, kScaleBufs = 3;
 
@@ -162,20 +344,6 @@ template <int BN, int EW, bool SPLIT> struct TileGeo {
   static_assert(kRing / (kBBytes + kTileM * kFp8Block) >= 4 && kSmemBytes <= 227 * 1024, "shared memory");
   static_assert(!SPLIT || kTileM * BN * 4 <= kRing, "the partial tile reuses the ring");
 };
-
-__device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (true) {
-    if (*abort_flag) return false;
-    if (mbar_try_wait(bar, parity)) return true;
-    if (clock64() - t0 > kFp8WaitClocks) {
-      atomicExch(&g_fp8_err, QF_ERR_TIMEOUT);
-      *abort_flag = 1;
-      return false;
-    }
-  }
-}
 
 struct TileParams {
   Fp8Params p;
@@ -452,14 +620,9 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1)
           const int b = it % A;
           const float sa = sc[i * 32 * EW + et];
           const float s0 = sa * scw[2 * i], s1 = sa * scw[2 * i + 1];
-          // the warp goes on together (tcgen05.ld needs it whole): at once, or with lane 0's bounded wait
-          if (!__all_sync(0xffffffffu, mbar_try_wait(&acc_full[b], (it / A) & 1))) {
-            int have = 0;
-            if (lane == 0) have = fp8_wait(&acc_full[b], (it / A) & 1, s_abort) ? 1 : 0;
-            if (!__shfl_sync(0xffffffffu, have, 0)) {
-              ok = false;
-              break;
-            }
+          if (!fp8_wait_warp(&acc_full[b], (it / A) & 1, s_abort)) {  // tcgen05.ld needs the warp whole
+            ok = false;
+            break;
           }
           tc_fence_after();
           const uint32_t src = tmem + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(b * BN + col0);
@@ -543,18 +706,22 @@ std::mutex g_dev_mu;
 int g_dev_sms[64] = {};
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 
+int find_encode() {
+  std::lock_guard<std::mutex> lk(g_dev_mu);
+  if (g_encode) return QF_OK;
+  cudaDriverEntryPointQueryResult qres;
+  void* fn = nullptr;
+  const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres);
+  if (e != cudaSuccess || qres != cudaDriverEntryPointSuccess || !fn)
+    return fail(QF_ERR_DRIVER, "cuTensorMapEncodeTiled entry point not found");
+  g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  return QF_OK;
+}
+
+// Operand rows, in boxes of one k group.
 int encode_rows(CUtensorMap* map, const void* base, int K, int rows, int64_t row_bytes, int box_rows) {
-  {
-    std::lock_guard<std::mutex> lk(g_dev_mu);
-    if (!g_encode) {
-      cudaDriverEntryPointQueryResult qres;
-      void* fn = nullptr;
-      const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres);
-      if (e != cudaSuccess || qres != cudaDriverEntryPointSuccess || !fn)
-        return fail(QF_ERR_DRIVER, "cuTensorMapEncodeTiled entry point not found");
-      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }
-  }
+  const int rc = find_encode();
+  if (rc) return rc;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
   cuuint32_t box[2] = {static_cast<cuuint32_t>(kFp8Block), static_cast<cuuint32_t>(box_rows)};
@@ -619,6 +786,69 @@ int launch_tiles(TileParams tp, int dev, int sms, int splits, unsigned flags, cu
   cfg.numAttrs = static_cast<unsigned>(na);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_tile_kernel<BN, EW, SPLIT>, ta, tw, tp);
   return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
+}
+
+// The whole k groups of operand rows as [group][row][128 bytes].
+int encode_groups(CUtensorMap* map, const void* base, int K, int rows, int64_t row_bytes, int box_rows, int box_groups) {
+  const int rc = find_encode();
+  if (rc) return rc;
+  cuuint64_t dims[3] = {kFp8Block, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(K / kFp8Block)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_bytes), kFp8Block};
+  cuuint32_t box[3] = {kFp8Block, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(box_groups)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(QF_ERR_DRIVER, "cuTensorMapEncodeTiled rejected the tensor (error " + std::to_string(r) + ")");
+  return QF_OK;
+}
+
+template <int NT, int MT, int G> int launch_rows(const Fp8Params& p, int dev, int sms, unsigned flags, cudaStream_t st) {
+  using C = RowGeo<NT, MT, G>;
+  static bool attr_set[64] = {};
+  {
+    std::lock_guard<std::mutex> lk(g_dev_mu);
+    if (!attr_set[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(fp8_rows_kernel<NT, MT, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+      if (e != cudaSuccess) return fail(QF_ERR_LAUNCH, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+      attr_set[dev] = true;
+    }
+  }
+  CUtensorMap ta = {}, tw = {};
+  if (p.K >= kFp8Block) {
+    // one row has no stride of its own: any multiple of 16 not below the row does
+    const int64_t one = (static_cast<int64_t>(p.K) + 15) / 16 * 16;
+    int rc = encode_groups(&ta, p.a, p.K, p.M, p.M > 1 ? p.lda : one, 8 * NT, C::kGroups);
+    if (rc == QF_OK) rc = encode_groups(&tw, p.w, p.K, p.N, p.N > 1 ? p.ldw : one, C::kRows, C::kGroups);
+    if (rc) return rc;
+  }
+  cudaLaunchConfig_t cfg = {};
+  // as few CTAs as finish in the same number of rounds: all of them run at once and share the memory evenly, so an SM
+  // with one more costs nothing, but a last round for a few would
+  const int ntiles = (p.N + C::kRows - 1) / C::kRows;
+  const int rounds = (ntiles + sms * kRowPerSm - 1) / (sms * kRowPerSm);
+  cfg.gridDim = dim3(static_cast<unsigned>((ntiles + rounds - 1) / rounds), static_cast<unsigned>((p.M + 8 * NT - 1) / (8 * NT)));
+  cfg.blockDim = dim3(kRowWarps * 32 + 32);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = (flags & QF_FLAG_PDL) ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_rows_kernel<NT, MT, G>, ta, tw, p, ntiles);
+  return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
+}
+
+// Tiles of 32 weight rows halve the token rows copied per weight row and the waits per byte, where there are enough of
+// them for two CTAs on every SM (10240 x 5120, 5 tokens: 10.6 us against 12.4; 34816 x 5120: 28.4 against 29.0); fewer
+// rows are better spread thin (5120 x 17408, one token: 16 rows 19.1 us, 32 rows 25.5).  With 16 rows a warp takes two
+// k groups per stage up to 8 tokens (19.1 us against 20.4); above, a stage of that size would leave a ring of two.
+int rows_any(const Fp8Params& p, int dev, int sms, unsigned flags, cudaStream_t st) {
+  const bool wide = (p.N + 31) / 32 >= 2 * sms;
+  if (p.M <= 8) return wide ? launch_rows<1, 2, 1>(p, dev, sms, flags, st) : launch_rows<1, 1, 2>(p, dev, sms, flags, st);
+  return wide ? launch_rows<2, 2, 1>(p, dev, sms, flags, st) : launch_rows<2, 1, 1>(p, dev, sms, flags, st);
 }
 
 // Clusters of `split` CTAs (one per SM) that the device runs at once: a cluster stays within one group of SMs, so this is
@@ -758,19 +988,7 @@ extern "C" int qf_fp8_block_gemm(const void* a, int64_t lda, const float* a_scal
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return tiles_any(tp, dev, sms, flags, st);
   }
-  const int nt = M <= 8 ? 1 : 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((N + 15) / 16), static_cast<unsigned>((M + 8 * nt - 1) / (8 * nt)));
-  cfg.blockDim = dim3(kRowWarps * 32);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = (flags & QF_FLAG_PDL) ? 1 : 0;
-  const cudaError_t e = nt == 1 ? cudaLaunchKernelEx(&cfg, fp8_rows_kernel<1>, p)
-                                : cudaLaunchKernelEx(&cfg, fp8_rows_kernel<2>, p);
-  return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
+  return rows_any(p, dev, sms, flags, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int qf_fp8_status(void* stream, int* status) {

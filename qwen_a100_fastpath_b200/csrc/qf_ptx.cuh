@@ -1,7 +1,7 @@
 // qf_ptx.cuh -- thin inline-PTX wrappers used by the sm_100a kernels of libqf_b200.
 //
 // Only documented PTX ISA forms are used: mbarrier (arrive / expect_tx / try_wait.parity), the tiled TMA
-// loads cp.async.bulk.tensor.2d / .4d (no multicast), createpolicy for L2 eviction hints, griddepcontrol for
+// loads cp.async.bulk.tensor.2d / .3d / .4d (no multicast) and the 3-D prefetch into L2, createpolicy for L2 eviction hints, griddepcontrol for
 // programmatic dependent launch, bar.sync on named barriers, ldmatrix (.trans), ex2.approx, mma.sync m16n8k16
 // bf16 / f16, and the tcgen05 forms listed further down.
 #pragma once
@@ -81,6 +81,22 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)), "l"(policy)
       : "memory");
+}
+
+// Three-dimensional tiled load, and the hint that brings its box into L2 without reading a value.
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
 }
 
 // Brings a kernel-parameter tensor map into the TMA unit's descriptor cache before its first copy.
