@@ -10,12 +10,13 @@
 //
 // Bound by memory for many rows and by two block-wide sums for one.  A CTA takes a row, a thread C pieces of eight
 // consecutive elements, everything stays in registers between the loads and the stores, and each sum is one
-// shuffle tree and one barrier.  CTAs walk the rows with the weights kept in registers (packed bf16), which saves
-// reading them from L2 once per row.  Sixteen threads hold a group of 128, so the quantizer's maximum is four shuffles.
+// shuffle tree and one barrier.  Where there are many rows, CTAs walk over them with the weights kept in registers (packed
+// bf16, which saves reading them from L2 once per row) and the next rows arriving in shared memory.  Sixteen threads hold a group of 128, so the quantizer's maximum is four shuffles.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <mutex>
 #include <string>
 
 #include "../../include/qf_b200.h"
@@ -44,6 +45,7 @@ struct NormParams {
   float alpha, eps, offset;
   int act;
   int M, H;
+  int stages;  // rows ahead (kAhead)
 };
 
 // Sum over the CTA, the same order on every thread: shuffle tree, then the warps' sums one after the other.
@@ -124,14 +126,59 @@ __device__ __forceinline__ float activate(float g, int act) {
   return act == QF_GATE_SIGMOID ? s : g * s;
 }
 
-// VEC: H and every row stride a multiple of eight elements and every pointer 16-byte aligned, so that a piece is whole
-// or absent and moves in 16-byte accesses.  R32: the residual is fp32.  QUANT: h leaves as e4m3 groups.
-template <int C, bool VEC, bool R32, bool QUANT>
+// How a kernel reads its rows.
+//   kAny: element by element, for any sizes, strides and alignments;
+//   kWide: 16-byte loads (H and every row stride a multiple of eight elements, every pointer 16-byte aligned);
+//   kAhead: the same rows by bulk copies into shared memory, `stages` rows ahead, where a CTA walks over several rows:
+//     what a thread could hold of the next row in registers is too little in flight (8192 x 5120 with fp32 residual and
+//     gate: 157 us with the next row in registers).
+enum RowMode { kAny, kWide, kAhead };
+
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = bf16_lo(w[i]);
+    v[2 * i + 1] = bf16_hi(w[i]);
+  }
+}
+
+constexpr long long kRowWaitClocks = 8000000000ll;  // about 4 s
+constexpr int kMaxRowStages = 4;
+constexpr long long kNormRing = 216 * 1024;  // shared memory of an SM for the rows ahead
+
+// R32: the residual is fp32.  QUANT: h leaves as e4m3 groups.
+template <int C, int MODE, bool R32, bool QUANT>
 __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) {
+  constexpr bool VEC = MODE != kAny;
   __shared__ float red[2][2][32];
+  __shared__ uint64_t full[kMaxRowStages];
+  extern __shared__ __align__(128) uint8_t ring[];
   pdl_launch_dependents();
-  pdl_wait();
   const int T = blockDim.x;
+  const bool gate_row = p.gate && p.gate_sh;  // a gate value for each element, not one for the row
+  const int off_r = 2 * p.H, off_g = off_r + (p.residual ? (R32 ? 4 : 2) * p.H : 0);
+  const int stage_bytes = off_g + (gate_row ? 2 * p.H : 0);
+  if (MODE == kAhead) {
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+      fence_mbar_init();
+    }
+    __syncthreads();
+  }
+  pdl_wait();
+  auto copy_row = [&](int m, int s) {  // by one thread
+    uint8_t* dst = ring + s * stage_bytes;
+    mbar_arrive_expect_tx(&full[s], stage_bytes);
+    bulk_load(dst, p.x + static_cast<int64_t>(m) * p.ldx, 2 * p.H, &full[s]);
+    if (p.residual)
+      bulk_load(dst + off_r, static_cast<const uint8_t*>(p.residual) + static_cast<int64_t>(m) * p.ldr * (R32 ? 4 : 2),
+                off_g - off_r, &full[s]);
+    if (gate_row) bulk_load(dst + off_g, p.gate + static_cast<int64_t>(m) * p.gate_sm, 2 * p.H, &full[s]);
+  };
+  if (MODE == kAhead && threadIdx.x == 0)
+    for (int s = 0; s < p.stages; ++s)
+      if (blockIdx.x + static_cast<long long>(s) * gridDim.x < p.M) copy_row(blockIdx.x + s * gridDim.x, s);
   uint32_t wpost[C][4], wpre[C][4];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -145,16 +192,43 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
     for (int i = 0; i < 4; ++i) wpre[c][i] = pack_bf16(t[2 * i], t[2 * i + 1]);
   }
   const float inv_h = 1.f / static_cast<float>(p.H);
-  int parity = 0;
+  int parity = 0, stage = 0;
+  uint32_t phase = 0;
   for (int m = blockIdx.x; m < p.M; m += gridDim.x, parity ^= 1) {
-    float v[C][8];
+    // where this row's operands are: in the ring, or, always otherwise and after a copy that did not arrive in time, in
+    // global memory
+    const __nv_bfloat16* x = p.x + static_cast<int64_t>(m) * p.ldx;
+    const uint8_t* res = static_cast<const uint8_t*>(p.residual) + (p.residual ? static_cast<int64_t>(m) * p.ldr * (R32 ? 4 : 2) : 0);
+    const __nv_bfloat16* gate = p.gate + (p.gate ? static_cast<int64_t>(m) * p.gate_sm : 0);
+    if (MODE == kAhead) {
+      bool have = mbar_try_wait(&full[stage], phase);
+      for (const long long t0 = clock64(); !have && clock64() - t0 < kRowWaitClocks;) have = mbar_try_wait(&full[stage], phase);
+      if (have) {
+        const uint8_t* src = ring + stage * stage_bytes;
+        x = reinterpret_cast<const __nv_bfloat16*>(src);
+        res = src + off_r;
+        if (gate_row) gate = reinterpret_cast<const __nv_bfloat16*>(src + off_g);
+      }
+    }
+    float v[C][8], r[C][8];
+    uint4 g4[C];
     float s = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int e = (c * T + static_cast<int>(threadIdx.x)) * 8;
-      load8_bf16<VEC>(p.x + static_cast<int64_t>(m) * p.ldx + e, p.H - e, v[c]);
+      load8_bf16<VEC>(x + e, p.H - e, v[c]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s = fmaf(v[c][i], v[c][i], s);
+      for (int i = 0; i < 8; ++i) s = fmaf(v[c][i], v[c][i], s), r[c][i] = 0.f;
+      if (MODE == kWide) {  // everything of the row on its way at once
+        if (p.residual) {
+          if (R32)
+            load8_f32<true>(reinterpret_cast<const float*>(res) + e, p.H - e, r[c]);
+          else
+            load8_bf16<true>(reinterpret_cast<const __nv_bfloat16*>(res) + e, p.H - e, r[c]);
+        }
+        g4[c] = make_uint4(0, 0, 0, 0);
+        if (gate_row && e < p.H) g4[c] = *reinterpret_cast<const uint4*>(gate + e);
+      }
     }
     if (p.post) {
       const float n = rsqrtf(fmaf(cta_sum(s, red[parity][0]), inv_h, p.eps));
@@ -167,33 +241,31 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
         }
     }
     s = 0.f;
+    const float row_gate = p.gate && !p.gate_sh ? activate(__bfloat162float(*gate), p.act) : 1.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int e = (c * T + static_cast<int>(threadIdx.x)) * 8;
-      if (p.gate) {
+      if (gate_row) {
         float g[8];
-        const __nv_bfloat16* src = p.gate + static_cast<int64_t>(m) * p.gate_sm;
-        if (p.gate_sh) {
-          load8_bf16<VEC>(src + e, p.H - e, g);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[c][i] *= activate(g[i], p.act);
-        } else {
-          const float a = activate(__bfloat162float(*src), p.act);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[c][i] *= a;
-        }
-      }
-      float r[8] = {};
-      if (p.residual) {
-        if (R32)
-          load8_f32<VEC>(static_cast<const float*>(p.residual) + static_cast<int64_t>(m) * p.ldr + e, p.H - e, r);
+        if (MODE == kWide)
+          unpack8(g4[c], g);
         else
-          load8_bf16<VEC>(static_cast<const __nv_bfloat16*>(p.residual) + static_cast<int64_t>(m) * p.ldr + e, p.H - e,
-                          r);
+          load8_bf16<VEC>(gate + e, p.H - e, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c][i] *= activate(g[i], p.act);
+      } else if (p.gate) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c][i] *= row_gate;
+      }
+      if (MODE != kWide && p.residual) {
+        if (R32)
+          load8_f32<VEC>(reinterpret_cast<const float*>(res) + e, p.H - e, r[c]);
+        else
+          load8_bf16<VEC>(reinterpret_cast<const __nv_bfloat16*>(res) + e, p.H - e, r[c]);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[c][i] = fmaf(p.alpha, v[c][i], r[i]);
+        v[c][i] = fmaf(p.alpha, v[c][i], r[c][i]);
         // elements past the row must not enter the sum (a gate of infinity there would not be zero times x)
         if (e + i >= p.H) v[c][i] = 0.f;
         s = fmaf(v[c][i], v[c][i], s);
@@ -206,8 +278,18 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
                            v[c]);
       }
     }
+    float n = 0.f;
+    if (p.pre)
+      n = rsqrtf(fmaf(cta_sum(s, red[parity][1]), inv_h, p.eps));
+    else if (MODE == kAhead)
+      __syncthreads();
+    if (MODE == kAhead) {
+      // behind that barrier every thread has read the stage
+      const long long next = m + static_cast<long long>(p.stages) * gridDim.x;
+      if (threadIdx.x == 0 && next < p.M) copy_row(static_cast<int>(next), stage);
+      if (++stage == p.stages) stage = 0, phase ^= 1;
+    }
     if (!p.pre) continue;
-    const float n = rsqrtf(fmaf(cta_sum(s, red[parity][1]), inv_h, p.eps));
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int e = (c * T + static_cast<int>(threadIdx.x)) * 8;
@@ -242,11 +324,58 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
   }
 }
 
-template <int C, bool VEC> cudaError_t launch_norm(const cudaLaunchConfig_t& cfg, const NormParams& p, bool r32, bool quant) {
-  if (r32) return quant ? cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, VEC, true, true>, p)
-                        : cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, VEC, true, false>, p);
-  return quant ? cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, VEC, false, true>, p)
-               : cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, VEC, false, false>, p);
+// Launches one instance: with several rows to a CTA and rows that bulk copies take, as kAhead.
+template <int C, bool R32, bool QUANT>
+cudaError_t launch_norm(NormParams p, bool vec, int threads, int dev, int sms, bool pdl, cudaStream_t st) {
+  // resident CTAs per SM by registers, asked once per CTA size
+  static std::mutex mu;
+  static int resident[64][17] = {};
+  int per_sm;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    int& known = resident[dev][threads / 32];
+    if (known == 0) {
+      cudaError_t e = cudaFuncSetAttribute(residual_norm_kernel<C, kAhead, R32, QUANT>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, kNormRing);
+      if (e == cudaSuccess)
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&known, residual_norm_kernel<C, kAhead, R32, QUANT>, threads, 0);
+      if (e != cudaSuccess) {
+        known = 0;
+        return e;
+      }
+      if (known > 16) known = 16;
+      if (known < 1) known = 1;
+    }
+    per_sm = known;
+  }
+  const long long bytes = static_cast<long long>(p.H) * (2 + (p.residual ? (R32 ? 4 : 2) : 0) + (p.gate && p.gate_sh ? 2 : 0));
+  while (per_sm > 1 && kNormRing / per_sm / bytes < 2) --per_sm;
+  p.stages = static_cast<int>(kNormRing / per_sm / bytes);
+  if (p.stages > kMaxRowStages) p.stages = kMaxRowStages;
+  const bool ahead = vec && p.stages >= 2 && p.M > 2 * sms * per_sm;
+  const long long grid = static_cast<long long>(sms) * per_sm;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.M < grid || !ahead ? p.M : grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = ahead ? static_cast<size_t>(p.stages * bytes) : 0;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  if (ahead) return cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, kAhead, R32, QUANT>, p);
+  return vec ? cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, kWide, R32, QUANT>, p)
+             : cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, kAny, R32, QUANT>, p);
+}
+
+template <int C>
+cudaError_t launch_norm(const NormParams& p, bool r32, bool quant, bool vec, int threads, int dev, int sms, bool pdl,
+                        cudaStream_t st) {
+  if (r32) return quant ? launch_norm<C, true, true>(p, vec, threads, dev, sms, pdl, st)
+                        : launch_norm<C, true, false>(p, vec, threads, dev, sms, pdl, st);
+  return quant ? launch_norm<C, false, true>(p, vec, threads, dev, sms, pdl, st)
+               : launch_norm<C, false, false>(p, vec, threads, dev, sms, pdl, st);
 }
 
 bool aligned(const void* ptr, size_t n) { return reinterpret_cast<uintptr_t>(ptr) % n == 0; }
@@ -281,8 +410,8 @@ extern "C" int qf_residual_norm(const void* x, int64_t ldx, const void* residual
   if (!aligned(x, 2) || !aligned(residual, rb) || !aligned(residual_out, rb) || !aligned(gate, 2) ||
       !aligned(post_weight, 2) || !aligned(pre_weight, 2) || (!quant && !aligned(out, 2)) || !aligned(out_scale, 4))
     return fail(QF_ERR_ALIGN, "pointers must be aligned to their element");
-  int sms = 0;
-  int rc = require_b200(nullptr, &sms);
+  int dev = 0, sms = 0;
+  int rc = require_b200(&dev, &sms);
   if (rc) return rc;
   NormParams p = {};
   p.x = static_cast<const __nv_bfloat16*>(x);
@@ -314,23 +443,10 @@ extern "C" int qf_residual_norm(const void* x, int64_t ldx, const void* residual
   const int pieces = (H + 7) / 8;
   const int C = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : 4;
   const int threads = ((pieces + C - 1) / C + 31) / 32 * 32;
-  const int per_sm = 2048 / threads < 1 ? 1 : (2048 / threads > 8 ? 8 : 2048 / threads);
-  const long long grid = static_cast<long long>(sms) * per_sm;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(M < grid ? M : grid));
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = (flags & QF_FLAG_PDL) ? 1 : 0;
-  cudaError_t e;
-  if (vec)
-    e = C == 1 ? launch_norm<1, true>(cfg, p, r32, quant) : C == 2 ? launch_norm<2, true>(cfg, p, r32, quant)
-                                                                    : launch_norm<4, true>(cfg, p, r32, quant);
-  else
-    e = C == 1 ? launch_norm<1, false>(cfg, p, r32, quant) : C == 2 ? launch_norm<2, false>(cfg, p, r32, quant)
-                                                                    : launch_norm<4, false>(cfg, p, r32, quant);
+  const bool pdl = (flags & QF_FLAG_PDL) != 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = C == 1   ? launch_norm<1>(p, r32, quant, vec, threads, dev, sms, pdl, st)
+                        : C == 2 ? launch_norm<2>(p, r32, quant, vec, threads, dev, sms, pdl, st)
+                                 : launch_norm<4>(p, r32, quant, vec, threads, dev, sms, pdl, st);
   return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
 }
