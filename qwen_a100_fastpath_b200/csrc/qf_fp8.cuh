@@ -5,6 +5,8 @@
 
 #include <cstdint>
 
+#include "qf_ptx.cuh"
+
 namespace qf {
 
 constexpr int kFp8Block = 128;                   // one scale for this many elements along k (and channels of a weight)
@@ -16,6 +18,41 @@ constexpr float kFp8AmaxFloor = kE4m3Max * kFp8ScaleFloor;
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 1 / (1 + e^-x) of two values: e^-x = 2^t * 2^c with t = -x * log2(e) rounded and c what the rounding left, 2^t by the
+// special-function unit (2 ulp) and 2^c = 1 + c * ln(2), then the unit's reciprocal (1 ulp): good to 8 * 2^-24, at some
+// eight instructions a value (packed fp32 pairs) where expf and an IEEE quotient take some thirty.  Beyond |x| = 88.5,
+// where the result is 1 or under 2^-127, x counts as that bound, which makes the latter zero; a NaN stays one.
+__device__ __forceinline__ float2 sigmoid2(float a, float b) {
+  const uint64_t kL = pack_f32x2(-1.44269502f, -1.44269502f);              // log2(e) = 1.44269502 + 1.92596303e-8
+  const uint64_t kLLow = pack_f32x2(-1.92596303e-8f, -1.92596303e-8f);
+  const uint64_t kLn2 = pack_f32x2(0.693147182f, 0.693147182f);
+  const uint64_t kOne = pack_f32x2(1.f, 1.f);
+  const uint64_t x = pack_f32x2(min_nan(max_nan(a, -88.5f), 88.5f), min_nan(max_nan(b, -88.5f), 88.5f));
+  const uint64_t t = mul_f32x2(x, kL);
+  const float2 tf = unpack_f32x2(t);
+  uint64_t c = pack_f32x2(-tf.x, -tf.y);
+  fma_f32x2(c, x, kL);     // exact
+  fma_f32x2(c, x, kLLow);
+  uint64_t f = kOne;
+  fma_f32x2(f, c, kLn2);
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(tf.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(tf.y));
+  uint64_t d = kOne;
+  fma_f32x2(d, pack_f32x2(e.x, e.y), f);
+  const float2 df = unpack_f32x2(d);
+  float2 r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(df.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(df.y));
   return r;
 }
 

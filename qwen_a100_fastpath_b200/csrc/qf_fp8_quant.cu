@@ -60,7 +60,7 @@ __device__ __forceinline__ void load16(const __nv_bfloat16* row, int k, int K, b
 }
 
 template <bool SILU>
-__global__ void __launch_bounds__(256) fp8_quantize_kernel(const QtParams p) {
+__global__ void __launch_bounds__(256, SILU ? 6 : 8) fp8_quantize_kernel(const QtParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t group = blockIdx.x * (blockDim.x / kQtLanes) + threadIdx.x / kQtLanes;
@@ -76,7 +76,11 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const QtParams p) {
     float u[kQtPer];
     load16(row + p.K, k, live ? p.K : 0, p.vec_in, u);
 #pragma unroll
-    for (int i = 0; i < kQtPer; ++i) v[i] = __fdiv_rn(v[i], 1.f + expf(-v[i])) * u[i];
+    for (int i = 0; i < kQtPer; i += 2) {
+      const float2 s = sigmoid2(v[i], v[i + 1]);
+      v[i] = v[i] * s.x * u[i];
+      v[i + 1] = v[i + 1] * s.y * u[i + 1];
+    }
   }
   float a = kFp8AmaxFloor;
 #pragma unroll

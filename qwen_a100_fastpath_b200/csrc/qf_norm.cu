@@ -120,10 +120,10 @@ template <bool VEC> __device__ __forceinline__ void store8_f32(float* dst, int n
   }
 }
 
-__device__ __forceinline__ float activate(float g, int act) {
-  if (act == QF_GATE_NONE) return g;
-  const float s = __fdiv_rn(1.f, 1.f + expf(-g));
-  return act == QF_GATE_SIGMOID ? s : g * s;
+__device__ __forceinline__ float2 activate2(float a, float b, int act) {
+  if (act == QF_GATE_NONE) return make_float2(a, b);
+  const float2 s = sigmoid2(a, b);
+  return act == QF_GATE_SIGMOID ? s : make_float2(a * s.x, b * s.y);
 }
 
 // How a kernel reads its rows.
@@ -148,8 +148,8 @@ constexpr int kMaxRowStages = 4;
 constexpr long long kNormRing = 216 * 1024;  // shared memory of an SM for the rows ahead
 
 // R32: the residual is fp32.  QUANT: h leaves as e4m3 groups.
-template <int C, int MODE, bool R32, bool QUANT>
-__global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) {
+template <int C, int MAX_T, int MODE, bool R32, bool QUANT>
+__global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) residual_norm_kernel(const NormParams p) {
   constexpr bool VEC = MODE != kAny;
   __shared__ float red[2][2][32];
   __shared__ uint64_t full[kMaxRowStages];
@@ -241,7 +241,11 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
         }
     }
     s = 0.f;
-    const float row_gate = p.gate && !p.gate_sh ? activate(__bfloat162float(*gate), p.act) : 1.f;
+    float row_gate = 1.f;
+    if (p.gate && !p.gate_sh) {
+      const float g = __bfloat162float(*gate);
+      row_gate = activate2(g, g, p.act).x;
+    }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int e = (c * T + static_cast<int>(threadIdx.x)) * 8;
@@ -252,7 +256,11 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
         else
           load8_bf16<VEC>(gate + e, p.H - e, g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[c][i] *= activate(g[i], p.act);
+        for (int i = 0; i < 8; i += 2) {
+          const float2 a = activate2(g[i], g[i + 1], p.act);
+          v[c][i] *= a.x;
+          v[c][i + 1] *= a.y;
+        }
       } else if (p.gate) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[c][i] *= row_gate;
@@ -325,7 +333,7 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
 }
 
 // Launches one instance: with several rows to a CTA and rows that bulk copies take, as kAhead.
-template <int C, bool R32, bool QUANT>
+template <int C, int MAX_T, bool R32, bool QUANT>
 cudaError_t launch_norm(NormParams p, bool vec, int threads, int dev, int sms, bool pdl, cudaStream_t st) {
   // resident CTAs per SM by registers, asked once per CTA size
   static std::mutex mu;
@@ -335,10 +343,10 @@ cudaError_t launch_norm(NormParams p, bool vec, int threads, int dev, int sms, b
     std::lock_guard<std::mutex> lk(mu);
     int& known = resident[dev][threads / 32];
     if (known == 0) {
-      cudaError_t e = cudaFuncSetAttribute(residual_norm_kernel<C, kAhead, R32, QUANT>,
+      cudaError_t e = cudaFuncSetAttribute(residual_norm_kernel<C, MAX_T, kAhead, R32, QUANT>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize, kNormRing);
       if (e == cudaSuccess)
-        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&known, residual_norm_kernel<C, kAhead, R32, QUANT>, threads, 0);
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&known, residual_norm_kernel<C, MAX_T, kAhead, R32, QUANT>, threads, 0);
       if (e != cudaSuccess) {
         known = 0;
         return e;
@@ -364,18 +372,18 @@ cudaError_t launch_norm(NormParams p, bool vec, int threads, int dev, int sms, b
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  if (ahead) return cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, kAhead, R32, QUANT>, p);
-  return vec ? cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, kWide, R32, QUANT>, p)
-             : cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, kAny, R32, QUANT>, p);
+  if (ahead) return cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, MAX_T, kAhead, R32, QUANT>, p);
+  return vec ? cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, MAX_T, kWide, R32, QUANT>, p)
+             : cudaLaunchKernelEx(&cfg, residual_norm_kernel<C, MAX_T, kAny, R32, QUANT>, p);
 }
 
-template <int C>
+template <int C, int MAX_T>
 cudaError_t launch_norm(const NormParams& p, bool r32, bool quant, bool vec, int threads, int dev, int sms, bool pdl,
                         cudaStream_t st) {
-  if (r32) return quant ? launch_norm<C, true, true>(p, vec, threads, dev, sms, pdl, st)
-                        : launch_norm<C, true, false>(p, vec, threads, dev, sms, pdl, st);
-  return quant ? launch_norm<C, false, true>(p, vec, threads, dev, sms, pdl, st)
-               : launch_norm<C, false, false>(p, vec, threads, dev, sms, pdl, st);
+  if (r32) return quant ? launch_norm<C, MAX_T, true, true>(p, vec, threads, dev, sms, pdl, st)
+                        : launch_norm<C, MAX_T, true, false>(p, vec, threads, dev, sms, pdl, st);
+  return quant ? launch_norm<C, MAX_T, false, true>(p, vec, threads, dev, sms, pdl, st)
+               : launch_norm<C, MAX_T, false, false>(p, vec, threads, dev, sms, pdl, st);
 }
 
 bool aligned(const void* ptr, size_t n) { return reinterpret_cast<uintptr_t>(ptr) % n == 0; }
@@ -439,14 +447,21 @@ extern "C" int qf_residual_norm(const void* x, int64_t ldx, const void* residual
   const bool vec = H % 8 == 0 && rows16(x, ldx) && rows16(residual, ldr) && rows16(residual_out, ldro) &&
                    rows16(out, ldo) && (!gate || gate_sh == 0 || rows16(gate, gate_sm)) && aligned(post_weight, 16) &&
                    aligned(pre_weight, 16);
-  // pieces per thread: the fewest that keep the CTA at 512 threads
+  // pieces per thread: the fewest that keep the CTA at 320 threads, so that two are resident and one works while the other
+  // is at a barrier; wider rows, of which shared memory holds too few for two CTAs anyway, take up to 512 threads
+  // (4096 x 8192, fp32 residual and gate: 84 us with two pieces on 512 threads, 116 with four on 256)
   const int pieces = (H + 7) / 8;
-  const int C = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : 4;
+  const int C = pieces <= 320 ? 1 : pieces <= 1024 ? 2 : 4;
   const int threads = ((pieces + C - 1) / C + 31) / 32 * 32;
   const bool pdl = (flags & QF_FLAG_PDL) != 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = C == 1   ? launch_norm<1>(p, r32, quant, vec, threads, dev, sms, pdl, st)
-                        : C == 2 ? launch_norm<2>(p, r32, quant, vec, threads, dev, sms, pdl, st)
-                                 : launch_norm<4>(p, r32, quant, vec, threads, dev, sms, pdl, st);
+  cudaError_t e;
+  if (C == 1)
+    e = launch_norm<1, 320>(p, r32, quant, vec, threads, dev, sms, pdl, st);
+  else if (C == 2)
+    e = threads <= 320 ? launch_norm<2, 320>(p, r32, quant, vec, threads, dev, sms, pdl, st)
+                       : launch_norm<2, 512>(p, r32, quant, vec, threads, dev, sms, pdl, st);
+  else
+    e = launch_norm<4, 512>(p, r32, quant, vec, threads, dev, sms, pdl, st);
   return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
 }
