@@ -15,6 +15,7 @@
 // is launched, and inputs that require a gradient too: none of them has a backward.
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -143,16 +144,21 @@ at::Tensor with_leading(const at::Tensor& rows, const at::Tensor& x) {
   return x.dim() == 1 ? rows.select(0, 0) : rows.unflatten(0, x.sizes().slice(0, x.dim() - 1));
 }
 
+// A new tensor of the caching allocator, without the dispatcher's share of a small call's time.
+at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt));
+}
+
 // e4m3 rows of 16-byte stride, as the product's tensor maps take them.
 at::Tensor empty_rows(int64_t M, int64_t K, const at::Tensor& like) {
-  at::Tensor q = at::empty({M, (K + 15) / 16 * 16}, like.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor q = empty_on(like, {M, (K + 15) / 16 * 16}, at::kFloat8_e4m3fn);
   return K % 16 ? q.narrow(1, 0, K) : q;
 }
 
 std::tuple<at::Tensor, at::Tensor> quantize_rows(const char* op, const at::Tensor& x2, bool silu_mul) {
   const int64_t M = x2.size(0), K = silu_mul ? x2.size(1) / 2 : x2.size(1);
   at::Tensor q = empty_rows(M, K, x2);
-  at::Tensor s = at::empty({M, blocks(K)}, x2.options().dtype(at::kFloat));
+  at::Tensor s = empty_on(x2, {M, blocks(K)}, at::kFloat);
   if (M && K)
     check(qf_fp8_quantize(x2.data_ptr(), x2.stride(0), as_int(op, M), as_int(op, K), silu_mul, q.data_ptr(), q.stride(0),
                           s.data_ptr<float>(), s.stride(0), QF_FLAG_PDL, stream_of(x2)),
@@ -227,7 +233,7 @@ at::Tensor fp8_block_mm(const at::Tensor& a, const at::Tensor& a_scale, const at
                         const at::Tensor& w_scale, const OptTensor& bias, bool out_f32) {
   c10::cuda::OptionalCUDAGuard guard(a.is_cuda() ? c10::optional<c10::Device>(a.device()) : c10::nullopt);
   const at::Tensor r = checked_a(a, a_scale, w_t, w_scale, bias);
-  at::Tensor y = at::empty({a.size(0), w_t.size(1)}, a.options().dtype(out_f32 ? at::kFloat : at::kBFloat16));
+  at::Tensor y = empty_on(a, {a.size(0), w_t.size(1)}, out_f32 ? at::kFloat : at::kBFloat16);
   run_mm("fp8_block_mm", r, a_scale, w_t, w_scale, bias, y);
   return y;
 }
@@ -254,7 +260,7 @@ at::Tensor fp8_block_linear(const at::Tensor& x, const at::Tensor& w_t, const at
   check_weight(op, w_t, w_scale, bias, x.size(-1), x.device());
   c10::cuda::CUDAGuard guard(x.device());
   const at::Tensor x2 = as_rows(x);
-  at::Tensor y = at::empty({x2.size(0), w_t.size(1)}, x.options());
+  at::Tensor y = empty_on(x, {x2.size(0), w_t.size(1)}, at::kBFloat16);
   if (x2.size(0) && w_t.size(1)) {
     auto [q, s] = quantize_rows(op, x2, false);
     run_mm(op, q, s, w_t, w_scale, bias, y);
@@ -286,8 +292,8 @@ std::tuple<at::Tensor, at::Tensor> run_norm(const at::Tensor& x, const OptTensor
   const bool want_h = given(pre_weight);
   if (want_h) {
     pre = pre_weight->contiguous();
-    h = quantize ? empty_rows(M, H, x) : at::empty({M, H}, x.options());
-    if (quantize) s = at::empty({M, blocks(H)}, x.options().dtype(at::kFloat));
+    h = quantize ? empty_rows(M, H, x) : empty_on(x, {M, H}, at::kBFloat16);
+    if (quantize) s = empty_on(x, {M, blocks(H)}, at::kFloat);
   }
   at::Tensor ro2 = r_out.dim() == 2 ? r_out : r_out.view({M, H});
   if (M) {
@@ -344,7 +350,7 @@ std::tuple<OptTensor, OptTensor, at::Tensor> residual_norm(const at::Tensor& x, 
                                                            double weight_offset, double eps, bool quantize) {
   check_norm(x, residual, pre_weight, post_weight, gate, gate_act, eps, quantize);
   c10::cuda::CUDAGuard guard(x.device());
-  at::Tensor r_out = at::empty(x.sizes(), given(residual) ? residual->options() : x.options());
+  at::Tensor r_out = empty_on(x, x.sizes(), given(residual) ? residual->scalar_type() : at::kBFloat16);
   auto [h, s] = run_norm(x, residual, pre_weight, post_weight, gate, gate_act, residual_scale, weight_offset, eps, quantize,
                          r_out);
   return {h.defined() ? OptTensor(h) : c10::nullopt, s.defined() ? OptTensor(s) : c10::nullopt, r_out};
@@ -379,6 +385,47 @@ std::tuple<OptTensor, OptTensor> residual_norm_out(const at::Tensor& x, const Op
   return {h.defined() ? OptTensor(h) : c10::nullopt, s.defined() ? OptTensor(s) : c10::nullopt};
 }
 
+// Shapes and types only, for tracing: the same leading dimensions, e4m3 rows of 16-byte stride.
+at::Tensor meta_rows(const at::Tensor& x, int64_t K) {
+  std::vector<int64_t> s(x.sizes().begin(), x.sizes().end());
+  s.back() = (K + 15) / 16 * 16;
+  at::Tensor q = at::empty(s, x.options().dtype(at::kFloat8_e4m3fn));
+  return K % 16 ? q.narrow(-1, 0, K) : q;
+}
+at::Tensor meta_like(const at::Tensor& x, int64_t last, at::ScalarType type) {
+  std::vector<int64_t> s(x.sizes().begin(), x.sizes().end());
+  s.back() = last;
+  return at::empty(s, x.options().dtype(type));
+}
+std::tuple<at::Tensor, at::Tensor> fp8_quantize_meta(const at::Tensor& x, bool silu_mul) {
+  const int64_t K = silu_mul ? x.size(-1) / 2 : x.size(-1);
+  return {meta_rows(x, K), meta_like(x, blocks(K), at::kFloat)};
+}
+at::Tensor fp8_block_mm_meta(const at::Tensor& a, const at::Tensor&, const at::Tensor& w_t, const at::Tensor&,
+                             const OptTensor&, bool out_f32) {
+  return meta_like(a, w_t.size(1), out_f32 ? at::kFloat : at::kBFloat16);
+}
+void fp8_block_mm_out_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
+                           at::Tensor) {}
+at::Tensor fp8_block_linear_meta(const at::Tensor& x, const at::Tensor& w_t, const at::Tensor&, const OptTensor&) {
+  return meta_like(x, w_t.size(1), at::kBFloat16);
+}
+std::tuple<OptTensor, OptTensor> residual_norm_out_meta(const at::Tensor& x, const OptTensor&, const OptTensor& pre_weight,
+                                                        const OptTensor&, const OptTensor&, int64_t, double, double, double,
+                                                        bool quantize, at::Tensor) {
+  if (!given(pre_weight)) return {c10::nullopt, c10::nullopt};
+  if (!quantize) return {meta_like(x, x.size(-1), at::kBFloat16), c10::nullopt};
+  return {meta_rows(x, x.size(-1)), meta_like(x, blocks(x.size(-1)), at::kFloat)};
+}
+std::tuple<OptTensor, OptTensor, at::Tensor> residual_norm_meta(const at::Tensor& x, const OptTensor& residual,
+                                                                const OptTensor& pre_weight, const OptTensor& post_weight,
+                                                                const OptTensor& gate, int64_t act, double scale, double offset,
+                                                                double eps, bool quantize) {
+  at::Tensor r = meta_like(x, x.size(-1), given(residual) ? residual->scalar_type() : at::kBFloat16);
+  auto [h, s] = residual_norm_out_meta(x, residual, pre_weight, post_weight, gate, act, scale, offset, eps, quantize, r);
+  return {h, s, r};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(qf_b200, m) {
@@ -403,4 +450,12 @@ TORCH_LIBRARY_IMPL(qf_b200, CompositeExplicitAutograd, m) {
   m.impl("residual_norm_out", residual_norm_out);
 }
 TORCH_LIBRARY_IMPL(qf_b200, CUDA, m) { m.impl("int8_linear", int8_linear); }
-TORCH_LIBRARY_IMPL(qf_b200, Meta, m) { m.impl("int8_linear", int8_linear_meta); }
+TORCH_LIBRARY_IMPL(qf_b200, Meta, m) {
+  m.impl("int8_linear", int8_linear_meta);
+  m.impl("fp8_quantize", fp8_quantize_meta);
+  m.impl("fp8_block_mm", fp8_block_mm_meta);
+  m.impl("fp8_block_mm_out", fp8_block_mm_out_meta);
+  m.impl("fp8_block_linear", fp8_block_linear_meta);
+  m.impl("residual_norm", residual_norm_meta);
+  m.impl("residual_norm_out", residual_norm_out_meta);
+}

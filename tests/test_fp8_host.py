@@ -150,3 +150,25 @@ def test_operators_refuse_cpu_tensors_and_bad_names():
         norms.residual_norm(x, x, x[0])
     with pytest.raises(ValueError, match="gate_act"):
         norms.residual_norm(x, x, x[0], gate=x, gate_act="relu")
+
+
+def test_meta_shapes():
+    """Under tracing the operators answer with the shapes, types and row strides of the real call."""
+    from qwen_a100_fastpath_b200 import fp8, norms
+    x = torch.empty(3, 4, 1000, dtype=torch.bfloat16, device="meta")
+    q, s = fp8.fp8_quantize(x)
+    assert q.shape == x.shape and q.dtype == torch.float8_e4m3fn and q.stride(-2) == 1008 and s.shape == (3, 4, 8)
+    q, s = fp8.fp8_quantize(x, silu_mul=True)
+    assert q.shape == (3, 4, 500) and s.shape == (3, 4, 4)
+    w = torch.empty(640, 1008, dtype=torch.float8_e4m3fn, device="meta")[:, :1000].t()
+    sw = torch.empty(5, 8, device="meta")
+    y = fp8.fp8_block_linear(x, w, sw)
+    assert y.shape == (3, 4, 640) and y.dtype == torch.bfloat16
+    a, sa = fp8.fp8_quantize(x.view(12, 1000))
+    assert fp8.fp8_block_mm(a, sa, w, sw, out_dtype=torch.float32).dtype == torch.float32
+    r = torch.empty(3, 4, 1000, device="meta")
+    (q, s), ro = norms.residual_norm(x, r, x[0, 0], quantize=True)
+    assert q.shape == x.shape and s.shape == (3, 4, 8) and ro.dtype == torch.float32
+    h, ro = norms.residual_norm(x, None, x[0, 0], residual_out=torch.empty_like(x))
+    assert h.shape == x.shape and h.dtype == torch.bfloat16
+    assert norms.residual_norm(x, r, None)[0] is None
