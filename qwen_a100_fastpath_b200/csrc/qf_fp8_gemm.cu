@@ -129,15 +129,17 @@ __global__ void __launch_bounds__(kRowWarps * 32 + 32, kRowPerSm)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[C::kStages], empty[C::kStages];
-  __shared__ volatile int abort_flag;
+  __shared__ volatile int abort_flag, leave;
   float* red = reinterpret_cast<float*>(ring + C::kStages * C::kStage);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m0 = blockIdx.y * (8 * NT);
   const int kfull = p.K / kFp8Block;  // groups that are copied; a shorter last one is read where it is used
   const int nst = (kfull + C::kGroups - 1) / C::kGroups;
   if (threadIdx.x == 0) {
-    prefetch_tensormap(&tmap_w);
-    prefetch_tensormap(&tmap_a);
+    if (nst > 0) {  // without a whole k group there are no maps
+      prefetch_tensormap(&tmap_w);
+      prefetch_tensormap(&tmap_a);
+    }
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], kRowWarps);
@@ -300,9 +302,10 @@ __global__ void __launch_bounds__(kRowWarps * 32 + 32, kRowPerSm)
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) red[(((warp * NT + j) * MT + i) * 4 + e) * 32 + lane] = acc[j][i][e];
+      if (threadIdx.x == 0) leave = abort_flag;
       named_bar_sync(1, kRowWarps * 32);
-      // an abort that one warp saw before this barrier, all see here: they leave with the same barriers behind them
-      ok = !abort_flag;
+      // one reading of the flag for all warps: they leave, or go on, with the same barriers behind them
+      ok = !leave;
       for (int e = threadIdx.x; e < NT * MT * 128 && ok; e += kRowWarps * 32) {
         const int r = e % C::kRows, tk = e / C::kRows;
         const int src = (r % 8) * 4 + (tk % 8) / 2, reg = (r % 16 / 8) * 2 + (tk & 1);

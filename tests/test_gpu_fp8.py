@@ -138,6 +138,7 @@ SHAPES = [
     (16, 1024, 5120), (17, 1000, 200), (31, 64, 384), (33, 640, 520), (64, 2048, 1024), (72, 1280, 5120), (127, 257, 129),
     (128, 256, 256), (129, 384, 1000), (200, 4352, 4096), (333, 2600, 1160), (512, 512, 2176), (700, 130, 77), (1000, 1, 300),
     (256, 2304, 128), (1030, 3000, 1024),
+    (40, 96, 1), (100, 1, 16), (16, 9500, 130), (7, 9480, 300), (6, 5000, 1023), (90, 512, 20000), (4500, 136, 256),
 ]
 
 
@@ -274,6 +275,37 @@ def test_block_linear(dev, M, N, K, ld, off, bias):
     q, s = orc.quantize(f64(x))                        # bit-identical to the layer's own quantization
     ref, mag = orc.block_mm(q, s, wv, f64(sw), f64(b) if bias else None)
     check_mm(y, ref, mag, K)
+
+
+def test_first_call_in_a_capture():
+    """A process whose first calls are captured ones (nothing that a call sets up once needs an eager call before)."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+from qwen_a100_fastpath_b200.fp8 import fp8_block_linear, fp8_status
+from qwen_a100_fastpath_b200.norms import residual_norm
+dev = torch.device('cuda', 0)
+g = torch.Generator(device=dev).manual_seed(1)
+w = torch.randn(512, 640, device=dev, generator=g).to(torch.float8_e4m3fn).t()
+sw = torch.rand(4, 5, device=dev, generator=g)
+n = torch.ones(640, device=dev, dtype=torch.bfloat16)
+xs = [torch.randn(m, 640, device=dev, generator=g).to(torch.bfloat16) for m in (3, 12, 50, 4000)]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = [fp8_block_linear(residual_norm(x, x, n)[0], w, sw) for x in xs]
+graph.replay()
+torch.cuda.synchronize()
+for x, y in zip(xs, out):
+    assert torch.equal(fp8_block_linear(residual_norm(x, x, n)[0], w, sw), y)
+assert fp8_status() == 0
+print('captured first')
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       cwd=Path(__file__).resolve().parent.parent)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
 
 
 def test_block_linear_shapes_and_not_finite(dev):

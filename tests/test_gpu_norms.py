@@ -89,7 +89,7 @@ def test_options(dev, residual, quantize, post, gate, act):
 
 @pytest.mark.parametrize("quantize", [False, True])
 @pytest.mark.parametrize("M,H", [(1, 1), (1, 7), (2, 8), (1, 128), (3, 129), (4, 255), (1, 5120), (2, 4096), (3, 4104), (2, 8192),
-                                 (2, 8200), (1, 16384), (3, 16383), (3000, 136), (1201, 5120)])
+                                 (2, 8200), (1, 16384), (3, 16383), (3000, 136), (1201, 5120), (5000, 8), (2500, 2568), (900, 8192), (700, 16384)])
 def test_sizes(dev, M, H, quantize):
     from qwen_a100_fastpath_b200.norms import residual_norm
     x, r, g, pre, pw = make(dev, M, H, "full", "f32", seed=M + H)
@@ -133,6 +133,32 @@ def test_strides_in_place_and_optional_parts(dev, H):
         check(hb, rb2, x, r, pre, pw, gb, "sigmoid", 0.5, 0.0, False)
     h0, r0 = residual_norm(x[:0], r[:0], pre, quantize=True)
     assert h0[0].shape == (0, H) and r0.shape == (0, H)
+
+
+@pytest.mark.parametrize("residual", ["bf16", "f32"])
+@pytest.mark.parametrize("gate", ["none", "full", "channel", "token"])
+def test_many_rows_in_place(dev, residual, gate):
+    """Several rows to a CTA (they arrive ahead in shared memory): every kind of gate, the residual updated in place with
+    neighbours left as they were, the same bits as calls of a few rows."""
+    import torch
+    from qwen_a100_fastpath_b200.norms import residual_norm
+    M, H = 2600, 1024
+    x, r, g, pre, pw = make(dev, M, H, gate, residual, seed=11)
+    kw = dict(eps=EPS, post_weight=pw, gate_act="sigmoid" if gate != "none" else "none", residual_scale=0.7)
+    parts = [slice(0, 7), slice(1300, 1310), slice(M - 5, M)]
+    few = [residual_norm(x[p], r[p], pre, gate=g[p] if gate in ("full", "token") else g, **kw) for p in parts]
+    buf = torch.full((M + 2, H + 8), 9.0, dtype=r.dtype, device=dev)
+    r2 = buf[1:M + 1, :H]
+    r2.copy_(r)
+    h, ro = residual_norm(x, r2, pre, gate=g, residual_out=r2, **kw)
+    assert ro is r2
+    for p, (hf, rf) in zip(parts, few):
+        assert torch.equal(h[p], hf) and torch.equal(r2[p], rf)
+    check(h, r2, x, r, pre, pw, g, kw["gate_act"], 0.7, 0.0, False)
+    assert residual_norm(x, r, None, gate=g, **kw)[0] is None
+    assert torch.equal(residual_norm(x, r, None, gate=g, **kw)[1], r2)
+    r2.fill_(9.0)
+    assert (buf == 9.0).all()
 
 
 @pytest.mark.parametrize("quantize", [False, True])
