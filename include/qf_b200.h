@@ -200,7 +200,9 @@ int qf_quantize_rows_int8(const void* w, int64_t ldw, int V, int H, int8_t* q, i
 /* ---- block-scaled fp8 layers ------------------------------------------------------------------------------------
  * For checkpoints whose linear weights are e4m3 with one fp32 scale for each block of 128 x 128 and whose activations
  * are quantized at run time in groups of 128 along k (the reference plugin serves the int8 form of the same layers
- * only, plugin/qwen_fastpath/w8a16.py).  Neither call needs a workspace.
+ * only, plugin/qwen_fastpath/w8a16.py).  Neither call needs a workspace.  With QF_FLAG_PDL these calls and
+ * qf_residual_norm read nothing before the previous kernel on the stream has completed (some weights may be brought into
+ * L2 before): the weights too may have been written by it.
  *
  * qf_fp8_quantize: x bf16 [M, K] (row stride ldx elements), or with silu_mul != 0 [M, 2K] holding the merged gate
  * (columns [0, K)) and up ([K, 2K)).  Per token row and group of 128 consecutive k (the last may be shorter):
