@@ -28,8 +28,8 @@ __device__ __forceinline__ float min_nan(float a, float b) {
 }
 
 // 1 / (1 + e^-x) of two values: e^-x = 2^t * 2^c with t = -x * log2(e) rounded and c what the rounding left, 2^t by the
-// special-function unit (2 ulp) and 2^c = 1 + c * ln(2), then the unit's reciprocal (1 ulp): good to 8 * 2^-24, at some
-// eight instructions a value (packed fp32 pairs) where expf and an IEEE quotient take some thirty.  Beyond |x| = 88.5,
+// special-function unit (2 ulp) and 2^c = 1 + c * ln(2), then the unit's reciprocal with one Newton step: good to
+// 8 * 2^-24, at some ten instructions a value (packed fp32 pairs) where expf and an IEEE quotient take some thirty.  Beyond |x| = 88.5,
 // where the result is 1 or under 2^-127, x counts as that bound, which makes the latter zero; a NaN stays one.
 __device__ __forceinline__ float2 sigmoid2(float a, float b) {
   const uint64_t kL = pack_f32x2(-1.44269502f, -1.44269502f);              // log2(e) = 1.44269502 + 1.92596303e-8
@@ -53,7 +53,10 @@ __device__ __forceinline__ float2 sigmoid2(float a, float b) {
   float2 r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(df.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(df.y));
-  return r;
+  uint64_t rest = kOne, q = pack_f32x2(r.x, r.y);
+  fma_f32x2(rest, pack_f32x2(-df.x, -df.y), q);  // 1 - d * r, exact
+  fma_f32x2(q, q, rest);
+  return unpack_f32x2(q);
 }
 
 // Two fp32 -> two e4m3 bytes (lo in bits 0-7), round to nearest even, saturated to +-448, NaN kept.

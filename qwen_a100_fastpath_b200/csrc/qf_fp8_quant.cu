@@ -10,7 +10,7 @@
 // Eight threads share a group (16 elements, 32 contiguous bytes each), its maximum is three shuffles, nothing
 // crosses a warp, and the groups of all rows form one flat index, so one row fills as many SMs as it has work for.  Eight
 // CTAs per SM (six with the gate, whose arithmetic needs the registers) keep enough loads in flight: 4096 x 17408 takes
-// 34 us (6.2 TB/s), with the gate 72 us (5.0 TB/s; five CTAs 76, eight 88 with spills); one row of 5120 1.5 us.
+// 34 us (6.2 TB/s), with the gate 75 us (4.8 TB/s; fewer or more CTAs 4 to 16 us longer); one row of 5120 1.5 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
