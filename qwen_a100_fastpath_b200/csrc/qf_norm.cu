@@ -12,7 +12,7 @@
 // consecutive elements, everything stays in registers between the loads and the stores, and each sum is one
 // shuffle tree and one barrier.  Where there are many rows, CTAs walk over them with the weights kept in registers (packed
 // bf16, which saves reading them from L2 once per row) and the next rows arriving in shared memory.  Sixteen threads hold a group of 128, so the quantizer's maximum is four shuffles.
-// Measured (B200): 8192 x 5120 with fp32 residual, full gate and both norms 95 us (6.2 TB/s); with bf16 residual and
+// Measured (B200): 8192 x 5120 with fp32 residual, full gate and both norms 95..105 us (5.6..6.2 TB/s); with bf16 residual and
 // quantized output alone 66 us (4.4 TB/s, bound by the barriers of a row); one row 3.5 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
