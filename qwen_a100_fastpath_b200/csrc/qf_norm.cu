@@ -172,18 +172,18 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
     __syncthreads();
   }
   pdl_wait();
-  auto copy_row = [&](int m, int s) {  // by one thread
+  auto copy_row = [&](long long m, int s) {  // by one thread
     uint8_t* dst = ring + s * stage_bytes;
     mbar_arrive_expect_tx(&full[s], stage_bytes);
-    bulk_load(dst, p.x + static_cast<int64_t>(m) * p.ldx, 2 * p.H, &full[s]);
+    bulk_load(dst, p.x + m * p.ldx, 2 * p.H, &full[s]);
     if (p.residual)
-      bulk_load(dst + off_r, static_cast<const uint8_t*>(p.residual) + static_cast<int64_t>(m) * p.ldr * (R32 ? 4 : 2),
+      bulk_load(dst + off_r, static_cast<const uint8_t*>(p.residual) + m * p.ldr * (R32 ? 4 : 2),
                 off_g - off_r, &full[s]);
-    if (gate_row) bulk_load(dst + off_g, p.gate + static_cast<int64_t>(m) * p.gate_sm, 2 * p.H, &full[s]);
+    if (gate_row) bulk_load(dst + off_g, p.gate + m * p.gate_sm, 2 * p.H, &full[s]);
   };
   if (MODE == kAhead && threadIdx.x == 0)
     for (int s = 0; s < p.stages; ++s)
-      if (blockIdx.x + static_cast<long long>(s) * gridDim.x < p.M) copy_row(blockIdx.x + s * gridDim.x, s);
+      if (blockIdx.x + static_cast<long long>(s) * gridDim.x < p.M) copy_row(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
   uint32_t wpost[C][4], wpre[C][4];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -199,12 +199,13 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
   const float inv_h = 1.f / static_cast<float>(p.H);
   int parity = 0, stage = 0;
   uint32_t phase = 0;
-  for (int m = blockIdx.x; m < p.M; m += gridDim.x, parity ^= 1) {
+  // 64 bits: with as many CTAs as rows, the step past the last row leaves 32 bits from 2^30 rows on
+  for (long long m = blockIdx.x; m < p.M; m += gridDim.x, parity ^= 1) {
     // where this row's operands are: in the ring, or, always otherwise and after a copy that did not arrive in time, in
     // global memory
-    const __nv_bfloat16* x = p.x + static_cast<int64_t>(m) * p.ldx;
-    const uint8_t* res = static_cast<const uint8_t*>(p.residual) + (p.residual ? static_cast<int64_t>(m) * p.ldr * (R32 ? 4 : 2) : 0);
-    const __nv_bfloat16* gate = p.gate + (p.gate ? static_cast<int64_t>(m) * p.gate_sm : 0);
+    const __nv_bfloat16* x = p.x + m * p.ldx;
+    const uint8_t* res = static_cast<const uint8_t*>(p.residual) + (p.residual ? m * p.ldr * (R32 ? 4 : 2) : 0);
+    const __nv_bfloat16* gate = p.gate + (p.gate ? m * p.gate_sm : 0);
     if (MODE == kAhead) {
       bool have = mbar_try_wait(&full[stage], phase);
       for (const long long t0 = clock64(); !have && clock64() - t0 < kRowWaitClocks;) have = mbar_try_wait(&full[stage], phase);
@@ -285,10 +286,9 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
       }
       if (p.residual_out) {
         if (R32)
-          store8_f32<VEC>(static_cast<float*>(p.residual_out) + static_cast<int64_t>(m) * p.ldro + e, p.H - e, v[c]);
+          store8_f32<VEC>(static_cast<float*>(p.residual_out) + m * p.ldro + e, p.H - e, v[c]);
         else
-          store8_bf16<VEC>(static_cast<__nv_bfloat16*>(p.residual_out) + static_cast<int64_t>(m) * p.ldro + e, p.H - e,
-                           v[c]);
+          store8_bf16<VEC>(static_cast<__nv_bfloat16*>(p.residual_out) + m * p.ldro + e, p.H - e, v[c]);
       }
     }
     float n = 0.f;
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
     if (MODE == kAhead) {
       // behind that barrier every thread has read the stage
       const long long next = m + static_cast<long long>(p.stages) * gridDim.x;
-      if (threadIdx.x == 0 && next < p.M) copy_row(static_cast<int>(next), stage);
+      if (threadIdx.x == 0 && next < p.M) copy_row(next, stage);
       if (++stage == p.stages) stage = 0, phase ^= 1;
     }
     if (!p.pre) continue;
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
         v[c][2 * i + 1] *= n * (bf16_hi(wpre[c][i]) + p.offset);
       }
       if (!QUANT) {
-        store8_bf16<VEC>(static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(m) * p.ldo + e, p.H - e, v[c]);
+        store8_bf16<VEC>(static_cast<__nv_bfloat16*>(p.out) + m * p.ldo + e, p.H - e, v[c]);
         continue;
       }
       float a = kFp8AmaxFloor;
@@ -322,10 +322,10 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
       for (int off = 1; off < kFp8Block / 8; off <<= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, off));
       const float inv = __fdiv_rn(kE4m3Max, a);
       if (e < p.H && e % kFp8Block == 0)
-        p.scale[static_cast<int64_t>(m) * p.lds + e / kFp8Block] = __fdiv_rn(a, kE4m3Max);
+        p.scale[m * p.lds + e / kFp8Block] = __fdiv_rn(a, kE4m3Max);
       const uint32_t lo = f32x4_to_e4m3x4(v[c][0] * inv, v[c][1] * inv, v[c][2] * inv, v[c][3] * inv);
       const uint32_t hi = f32x4_to_e4m3x4(v[c][4] * inv, v[c][5] * inv, v[c][6] * inv, v[c][7] * inv);
-      uint8_t* dst = static_cast<uint8_t*>(p.out) + static_cast<int64_t>(m) * p.ldo + e;
+      uint8_t* dst = static_cast<uint8_t*>(p.out) + m * p.ldo + e;
       if (VEC) {
         if (e + 8 <= p.H) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
       } else {
