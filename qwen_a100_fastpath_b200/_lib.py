@@ -78,6 +78,7 @@ SIGNATURES = [
      [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int,
       _c.c_void_p, _c.c_void_p, _c.c_float, _c.c_float, _c.c_float, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64,
       _c.c_void_p, _c.c_int64, _c.c_int, _c.c_int, _c.c_uint, _c.c_void_p]),
+    ("qf_residual_norm_status", _c.c_int, [_c.c_void_p, _c.POINTER(_c.c_int)]),
     ("qf_allreduce_buffer_bytes", _c.c_size_t, [_c.c_int]),
     ("qf_symm_alloc", _c.c_int, [_c.c_size_t, _c.POINTER(_c.c_void_p)]),
     ("qf_symm_free", _c.c_int, [_c.c_void_p]),

@@ -941,6 +941,22 @@ int require_b200(int* dev_out, int* sms) {
   return QF_OK;
 }
 
+int read_error_word(const void* symbol, void* stream, int* status) {
+  if (!status) return fail(QF_ERR_INVALID, "null status");
+  const int rc = require_b200(nullptr, nullptr);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int v = 0;
+  const int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, symbol, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && v != 0) e = cudaMemcpyToSymbolAsync(symbol, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+  if (e == cudaSuccess && v != 0) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return fail(QF_ERR_LAUNCH, cudaGetErrorString(e));
+  *status = v;
+  return QF_OK;
+}
+
 }  // namespace qf
 
 using namespace qf;
@@ -997,18 +1013,4 @@ extern "C" int qf_fp8_block_gemm(const void* a, int64_t lda, const float* a_scal
   return rows_any(p, dev, sms, flags, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int qf_fp8_status(void* stream, int* status) {
-  if (!status) return fail(QF_ERR_INVALID, "null status");
-  const int rc = require_b200(nullptr, nullptr);
-  if (rc) return rc;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int v = 0;
-  const int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_fp8_err, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  if (e == cudaSuccess && v != 0) e = cudaMemcpyToSymbolAsync(g_fp8_err, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
-  if (e == cudaSuccess && v != 0) e = cudaStreamSynchronize(st);
-  if (e != cudaSuccess) return fail(QF_ERR_LAUNCH, cudaGetErrorString(e));
-  *status = v;
-  return QF_OK;
-}
+extern "C" int qf_fp8_status(void* stream, int* status) { return read_error_word(&g_fp8_err, stream, status); }

@@ -18,6 +18,8 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <cstdlib>
+#include <cstring>
 #include <mutex>
 #include <string>
 
@@ -48,7 +50,10 @@ struct NormParams {
   int act;
   int M, H;
   int stages;  // rows ahead (kAhead)
+  long long wait_clocks;  // limit of a thread's wait for a row ahead
 };
+
+__device__ int g_norm_err;  // sticky: QF_ERR_TIMEOUT once such a wait ran out (read by qf_residual_norm_status)
 
 // Sum over the CTA, the same order on every thread: shuffle tree, then the warps' sums one after the other.
 __device__ __forceinline__ float cta_sum(float s, float* red) {
@@ -158,6 +163,7 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
   constexpr bool VEC = MODE != kAny;
   __shared__ float red[2][2][32];
   __shared__ uint64_t full[kMaxRowStages];
+  __shared__ volatile int ring_off;  // kAhead: a thread's wait for a row ran out
   extern __shared__ __align__(128) uint8_t ring[];
   pdl_launch_dependents();
   const int T = blockDim.x;
@@ -167,6 +173,7 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
   if (MODE == kAhead) {
     if (threadIdx.x == 0) {
       for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+      ring_off = 0;
       fence_mbar_init();
     }
     __syncthreads();
@@ -199,21 +206,31 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
   const float inv_h = 1.f / static_cast<float>(p.H);
   int parity = 0, stage = 0;
   uint32_t phase = 0;
+  long long left_at = -1;  // kAhead: the row at which this thread left the ring
   // 64 bits: with as many CTAs as rows, the step past the last row leaves 32 bits from 2^30 rows on
   for (long long m = blockIdx.x; m < p.M; m += gridDim.x, parity ^= 1) {
-    // where this row's operands are: in the ring, or, always otherwise and after a copy that did not arrive in time, in
-    // global memory
+    // where this row's operands are: in the ring, or in global memory
     const __nv_bfloat16* x = p.x + m * p.ldx;
     const uint8_t* res = static_cast<const uint8_t*>(p.residual) + (p.residual ? m * p.ldr * (R32 ? 4 : 2) : 0);
     const __nv_bfloat16* gate = p.gate + (p.gate ? m * p.gate_sm : 0);
-    if (MODE == kAhead) {
-      bool have = mbar_try_wait(&full[stage], phase);
-      for (const long long t0 = clock64(); !have && clock64() - t0 < kRowWaitClocks;) have = mbar_try_wait(&full[stage], phase);
+    if (MODE == kAhead && left_at < 0) {
+      // A thread whose wait runs out, or that waits when another's has, leaves the ring for good and reads this and
+      // all later rows from global memory (no thread but itself writes the elements it reads): the phases of a barrier that
+      // it has not seen complete would no longer tell it anything.  The others go on: a stage is only filled again by thread
+      // 0, after it saw the stage's last copy arrive, so what they wait for is that copy or one that is never issued.
+      bool have = mbar_test_wait(&full[stage], phase);
+      if (!have)
+        for (const long long t0 = clock64(); !have && !ring_off && clock64() - t0 < p.wait_clocks;)
+          have = mbar_try_wait(&full[stage], phase);
       if (have) {
         const uint8_t* src = ring + stage * stage_bytes;
         x = reinterpret_cast<const __nv_bfloat16*>(src);
         res = src + off_r;
         if (gate_row) gate = reinterpret_cast<const __nv_bfloat16*>(src + off_g);
+      } else {
+        left_at = m;
+        ring_off = 1;
+        atomicExch(&g_norm_err, QF_ERR_TIMEOUT);
       }
     }
     float v[C][8], r[C][8];
@@ -296,7 +313,7 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
       n = rsqrtf(fmaf(cta_sum(s, red[parity][1]), inv_h, p.eps));
     else if (MODE == kAhead)
       __syncthreads();
-    if (MODE == kAhead) {
+    if (MODE == kAhead && left_at < 0) {
       // behind that barrier every thread has read the stage
       const long long next = m + static_cast<long long>(p.stages) * gridDim.x;
       if (threadIdx.x == 0 && next < p.M) copy_row(next, stage);
@@ -333,6 +350,16 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
         for (int i = 0; i < 8; ++i)
           if (e + i < p.H) dst[i] = static_cast<uint8_t>((i < 4 ? lo : hi) >> (8 * (i % 4)));
       }
+    }
+  }
+  if (MODE == kAhead && threadIdx.x == 0 && left_at >= 0) {
+    // the copies still under way land before the shared memory is given up: those of the rows from left_at on for which there
+    // was a stage
+    for (int s = 0; s < p.stages && left_at + static_cast<long long>(s) * gridDim.x < p.M; ++s) {
+      const long long t0 = clock64();
+      while (!mbar_try_wait(&full[stage], phase) && clock64() - t0 < kRowWaitClocks) {
+      }
+      if (++stage == p.stages) stage = 0, phase ^= 1;
     }
   }
 }
@@ -389,6 +416,17 @@ cudaError_t launch_norm(const NormParams& p, bool r32, bool quant, bool vec, int
                         : launch_norm<C, MAX_T, true, false>(p, vec, threads, dev, sms, pdl, st);
   return quant ? launch_norm<C, MAX_T, false, true>(p, vec, threads, dev, sms, pdl, st)
                : launch_norm<C, MAX_T, false, false>(p, vec, threads, dev, sms, pdl, st);
+}
+
+// Limit of a wait for a row ahead.  QF_NORM_WAIT_CLOCKS (read only with QF_TEST_OVERRIDES=1, once per process) replaces
+// it: with 0 the tests run the path of a wait that ran out.
+long long row_wait_clocks() {
+  static const long long v = [] {
+    const char* t = std::getenv("QF_TEST_OVERRIDES");
+    const char* e = std::getenv("QF_NORM_WAIT_CLOCKS");
+    return t && std::strcmp(t, "1") == 0 && e ? std::atoll(e) : kRowWaitClocks;
+  }();
+  return v;
 }
 
 bool aligned(const void* ptr, size_t n) { return reinterpret_cast<uintptr_t>(ptr) % n == 0; }
@@ -448,6 +486,7 @@ extern "C" int qf_residual_norm(const void* x, int64_t ldx, const void* residual
   p.act = gate_act;
   p.M = M;
   p.H = H;
+  p.wait_clocks = row_wait_clocks();
   auto rows16 = [&](const void* ptr, int64_t ld) { return !ptr || (aligned(ptr, 16) && (M == 1 || ld % 8 == 0)); };
   const bool vec = H % 8 == 0 && rows16(x, ldx) && rows16(residual, ldr) && rows16(residual_out, ldro) &&
                    rows16(out, ldo) && (!gate || gate_sh == 0 || rows16(gate, gate_sm)) && aligned(post_weight, 16) &&
@@ -470,3 +509,5 @@ extern "C" int qf_residual_norm(const void* x, int64_t ldx, const void* residual
     e = launch_norm<4, 512>(p, r32, quant, vec, threads, dev, sms, pdl, st);
   return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
 }
+
+extern "C" int qf_residual_norm_status(void* stream, int* status) { return read_error_word(&g_norm_err, stream, status); }

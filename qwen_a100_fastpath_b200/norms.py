@@ -7,10 +7,12 @@ block-scaled fp8 product its quantized activations directly.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
-from ._lib import load_torch_ops
+from ._lib import LIB, check, load_torch_ops
 
 load_torch_ops()
 _norm = torch.ops.qf_b200.residual_norm.default
@@ -46,3 +48,13 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, pre_weight: to
                          residual_out)
         r = residual_out
     return ((h, s) if quantize else h), r
+
+
+def residual_norm_status(device=None) -> int:
+    """Read and clear the device's sticky error flag of ``residual_norm`` (``QF_OK``, or ``QF_ERR_TIMEOUT`` after a bounded
+    wait for a row inside a launch expired; the rows were then read another way and the results are valid); synchronises the
+    device's current stream."""
+    with torch.cuda.device(torch.cuda.current_device() if device is None else device):
+        st = ctypes.c_int(0)
+        check("qf_residual_norm_status", LIB.qf_residual_norm_status(torch.cuda.current_stream().cuda_stream, ctypes.byref(st)))
+        return st.value

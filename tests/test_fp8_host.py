@@ -172,3 +172,7 @@ def test_meta_shapes():
     h, ro = norms.residual_norm(x, None, x[0, 0], residual_out=torch.empty_like(x))
     assert h.shape == x.shape and h.dtype == torch.bfloat16
     assert norms.residual_norm(x, r, None)[0] is None
+
+
+def test_norm_status_needs_a_place():
+    assert LIB.qf_residual_norm_status(None, None) == -1
