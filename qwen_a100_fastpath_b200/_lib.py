@@ -109,6 +109,16 @@ class QFError(RuntimeError):
         super().__init__(f"{fn}: {LIB.qf_strerror(code).decode()} ({code}): {detail}")
 
 
+class QFOverlapError(ValueError, RuntimeError):
+    """An output of an operator shares memory with an input: an argument refused like any other (``ValueError``), and the
+    ``RuntimeError`` that torch's own operators raise for such a call."""
+
+
+def refused_out(e: ValueError) -> ValueError:
+    """What an operator called with an output raises for its own refusal ``e``."""
+    return QFOverlapError(*e.args) if "single memory location" in str(e) else e
+
+
 def _load() -> ctypes.CDLL:
     if not LIB_PATH.exists():
         raise ImportError(f"{LIB_PATH.name} is not built; run `python -m qwen_a100_fastpath_b200.build` "

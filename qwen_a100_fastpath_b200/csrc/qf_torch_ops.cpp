@@ -14,7 +14,6 @@
 // so calls on several streams, and captured graphs, share nothing.  They refuse a call with a ValueError before anything
 // is launched, and inputs that require a gradient too: none of them has a backward.
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -128,6 +127,62 @@ cudaStream_t stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDASt
 int as_int(const char* op, int64_t v) {
   QF_REFUSE_UNLESS(v <= INT32_MAX, op, ": a size of ", v, " is too large");
   return static_cast<int>(v);
+}
+
+// The bytes of a tensor as `rows` intervals of `width` bytes, `step` bytes apart.  Exact for rows of adjacent elements; what
+// lies between the elements of other tensors counts as theirs.
+struct Intervals {
+  int64_t begin, width, step, rows;
+  int64_t end() const { return begin + (rows - 1) * step + width; }
+};
+
+Intervals intervals_of(const at::Tensor& t) {
+  // the dimension of the largest stride gives the rows, the others' span their width
+  int64_t rows = 1, step = 0, span = 1;
+  int outer = -1;
+  for (int i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) > step) step = t.stride(i), rows = t.size(i), outer = i;
+  for (int i = 0; i < t.dim(); ++i)
+    if (i != outer && t.size(i) > 1) span += (t.size(i) - 1) * t.stride(i);
+  const int64_t es = static_cast<int64_t>(t.element_size());
+  Intervals v = {static_cast<int64_t>(reinterpret_cast<uintptr_t>(t.data_ptr())), span * es, step * es, rows};
+  if (v.width >= v.step) v = {v.begin, (v.rows - 1) * v.step + v.width, 0, 1};  // adjacent or overlapping rows: one interval
+  return v;
+}
+
+bool overlap(const at::Tensor& ta, const at::Tensor& tb) {
+  if (ta.numel() == 0 || tb.numel() == 0) return false;
+  Intervals a = intervals_of(ta), b = intervals_of(tb);
+  if (a.end() <= b.begin || b.end() <= a.begin) return false;
+  if (a.rows > 1 && b.rows > 1 && a.step == b.step) {
+    // columns of one larger tensor: the rows' places within a step decide
+    const int64_t at = ((b.begin - a.begin) % a.step + a.step) % a.step;
+    if (at >= a.width && at + b.width <= a.step) return false;
+  }
+  // walk both upwards, always on with the row that ends first
+  int64_t i = 0, j = 0;
+  if (a.step && b.begin > a.begin + a.width) i = (b.begin - a.begin - a.width) / a.step;  // rows that end before the other begins
+  if (b.step && a.begin > b.begin + b.width) j = (a.begin - b.begin - b.width) / b.step;
+  while (i < a.rows && j < b.rows) {
+    const int64_t pa = a.begin + i * a.step, pb = b.begin + j * b.step;
+    if (pa < pb + b.width && pb < pa + a.width) return true;
+    if (pa + a.width <= pb) ++i; else ++j;
+  }
+  return false;
+}
+
+// Whether two tensors of one shape and type hold the same elements at the same places.
+bool same_elements(const at::Tensor& a, const at::Tensor& b) {
+  if (a.data_ptr() != b.data_ptr()) return false;
+  for (int i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+
+// "single memory location" is what torch's own operators say of such a call.
+void check_no_overlap(const char* op, const char* out_name, const at::Tensor& out, const char* name, const at::Tensor& t) {
+  QF_REFUSE_UNLESS(!overlap(out, t), op, ": ", out_name, " shares memory with ", name,
+                   ": elements of the two refer to a single memory location");
 }
 
 // [..., K] as rows of unit column stride, without a copy where the strides allow it.
@@ -248,8 +303,11 @@ void fp8_block_mm_out(const at::Tensor& a, const at::Tensor& a_scale, const at::
                        (out.scalar_type() == at::kFloat || out.scalar_type() == at::kBFloat16) &&
                        (N == 1 || out.stride(1) == 1) && (M <= 1 || out.stride(0) >= N),
                    op, ": out must be bf16 or fp32 [", M, ", ", N, "] on a's device with unit column stride");
-  for (const at::Tensor& t : {a, a_scale, w_t, w_scale}) at::assert_no_overlap(out, t);
-  if (given(bias)) at::assert_no_overlap(out, *bias);
+  check_no_overlap(op, "out", out, "a", a);
+  check_no_overlap(op, "out", out, "a_scale", a_scale);
+  check_no_overlap(op, "out", out, "w_t", w_t);
+  check_no_overlap(op, "out", out, "w_scale", w_scale);
+  if (given(bias)) check_no_overlap(op, "out", out, "bias", *bias);
   run_mm(op, r, a_scale, w_t, w_scale, bias, out);
 }
 
@@ -371,14 +429,13 @@ std::tuple<OptTensor, OptTensor> residual_norm_out(const at::Tensor& x, const Op
                        (residual_out.dim() != 2 || residual_out.size(0) <= 1 || residual_out.stride(0) >= H),
                    op, ": residual_out must have unit column stride and rows that do not overlap (and be contiguous "
                    "unless it is 2-D)");
-  if (given(residual)) {
-    // the residual itself is updated in place; any other overlap would be read after it is written
-    if (residual->data_ptr() != residual_out.data_ptr() || residual->strides() != residual_out.strides())
-      at::assert_no_overlap(residual_out, *residual);
-  }
-  at::assert_no_overlap(residual_out, x);
-  for (const OptTensor* t : {&pre_weight, &post_weight, &gate})
-    if (given(*t)) at::assert_no_overlap(residual_out, **t);
+  // the residual itself is updated in place; any other overlap would be read after it is written
+  if (given(residual) && !same_elements(*residual, residual_out))
+    check_no_overlap(op, "residual_out", residual_out, "residual", *residual);
+  check_no_overlap(op, "residual_out", residual_out, "x", x);
+  if (given(pre_weight)) check_no_overlap(op, "residual_out", residual_out, "pre_weight", *pre_weight);
+  if (given(post_weight)) check_no_overlap(op, "residual_out", residual_out, "post_weight", *post_weight);
+  if (given(gate)) check_no_overlap(op, "residual_out", residual_out, "gate", *gate);
   c10::cuda::CUDAGuard guard(x.device());
   auto [h, s] = run_norm(x, residual, pre_weight, post_weight, gate, gate_act, residual_scale, weight_offset, eps, quantize,
                          residual_out);

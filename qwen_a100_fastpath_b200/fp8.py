@@ -20,7 +20,7 @@ import ctypes
 
 import torch
 
-from ._lib import LIB, check, load_torch_ops
+from ._lib import LIB, check, load_torch_ops, refused_out
 
 load_torch_ops()
 _quantize = torch.ops.qf_b200.fp8_quantize.default
@@ -47,9 +47,14 @@ def fp8_block_mm(a: torch.Tensor, a_scale: torch.Tensor, w_t: torch.Tensor, w_sc
     products, fp32 sums, one rounding to ``out_dtype`` (bf16 or fp32).  ``a`` e4m3 ``[M, K]`` with fp32 ``a_scale
     [M, ceil(K / 128)]`` (any strides) as ``fp8_quantize`` returns them; ``w_t`` e4m3 ``[K, N]`` with stride ``(1, ldw)``,
     16-byte aligned, ``ldw % 16 == 0``; ``bias`` bf16 ``[N]``, added in fp32.  Rows of ``a`` that are not 16-byte aligned
-    are copied first.  ``out`` may supply the result (it decides the type then); it must not overlap an input."""
+    are copied first.  ``out`` may supply the result (it decides the type then); it must not share memory with an input
+    (refused as ``_lib.QFOverlapError``, a ``ValueError``; bytes between the elements of an input that is not rows of adjacent
+    elements count as its own)."""
     if out is not None:
-        _mm_out(a, a_scale, w_t, w_scale, bias, out)
+        try:
+            _mm_out(a, a_scale, w_t, w_scale, bias, out)
+        except ValueError as e:
+            raise refused_out(e) from None
         return out
     if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
         raise ValueError("out_dtype must be torch.bfloat16 or torch.float32")

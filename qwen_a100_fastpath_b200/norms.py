@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import LIB, check, load_torch_ops
+from ._lib import LIB, check, load_torch_ops, refused_out
 
 load_torch_ops()
 _norm = torch.ops.qf_b200.residual_norm.default
@@ -36,16 +36,19 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, pre_weight: to
       with ``quantize`` the pair ``(q, scale)`` that ``fp8.fp8_quantize`` would make of the unrounded ``h``; ``None`` where
       ``pre_weight`` is ``None``.
 
-    ``residual_out`` receives ``r``; it may be ``residual`` itself (updated in place) and must not overlap the other
-    inputs.  The same rules on devices, streams and errors as in ``fp8``."""
+    ``residual_out`` receives ``r``; it may be ``residual`` itself (updated in place) and must share no other memory with an
+    input (refused as ``fp8.fp8_block_mm`` does).  The same rules on devices, streams and errors as in ``fp8``."""
     act = GATE_ACTS.get(gate_act)
     if act is None:
         raise ValueError(f"gate_act must be one of {tuple(GATE_ACTS)}, got {gate_act!r}")
     if residual_out is None:
         h, s, r = _norm(x, residual, pre_weight, post_weight, gate, act, residual_scale, weight_offset, eps, quantize)
     else:
-        h, s = _norm_out(x, residual, pre_weight, post_weight, gate, act, residual_scale, weight_offset, eps, quantize,
-                         residual_out)
+        try:
+            h, s = _norm_out(x, residual, pre_weight, post_weight, gate, act, residual_scale, weight_offset, eps, quantize,
+                             residual_out)
+        except ValueError as e:
+            raise refused_out(e) from None
         r = residual_out
     return ((h, s) if quantize else h), r
 
