@@ -210,7 +210,7 @@ int qf_quantize_rows_int8(const void* w, int64_t ldw, int V, int H, int8_t* q, i
  *   q = e4m3(v * (448 / a)), round to nearest even.
  * A NaN makes its group's scale and values NaN.  q: e4m3 [M, K] (row stride ldq bytes; bytes past K are not written),
  * scale: fp32 [M, ceil(K / 128)] (row stride lds).  x 2-byte aligned; 16-byte accesses where the rows allow them.
- * K <= QF_FP8_MAX_K. */
+ * K <= QF_FP8_MAX_K, M * ceil(K / 128) < 2^31. */
 #define QF_FP8_MAX_K 1048576
 int qf_fp8_quantize(const void* x, int64_t ldx, int M, int K, int silu_mul, void* q, int64_t ldq, float* scale,
                     int64_t lds, unsigned flags, void* stream);
@@ -219,8 +219,9 @@ int qf_fp8_quantize(const void* x, int64_t ldx, int M, int K, int silu_mul, void
  * products, fp32 sums, one rounding to the output type.  a: e4m3 [M, K] (row stride lda bytes); a_scale fp32 element
  * (m, g) at m * sa_m + g * sa_g; w: e4m3 [N, K] row-major (row stride ldw bytes); w_scale fp32 element (n / 128, g) at
  * (n / 128) * sw_n + g * sw_g; bias bf16 [N] or NULL (added in fp32 before the rounding); y bf16 or fp32 (y_dtype),
- * row stride ldy elements.  Any M, N, K >= 1 (M == 0 or N == 0 is a no-op).  a and w 16-byte aligned with lda and ldw
- * multiples of 16. */
+ * row stride ldy elements.  1 <= M <= QF_FP8_MAX_M, 1 <= N <= QF_MAX_N, 1 <= K <= QF_FP8_MAX_K (M == 0 or N == 0 is a
+ * no-op), and ceil(M / 128) * ceil(N / 64) below 2^31 - 4096.  a and w 16-byte aligned with lda and ldw multiples of 16. */
+#define QF_FP8_MAX_M 2147483520 /* 2^31 - 128: the rows of the last tile have 32-bit numbers */
 int qf_fp8_block_gemm(const void* a, int64_t lda, const float* a_scale, int64_t sa_m, int64_t sa_g, const void* w,
                       int64_t ldw, const float* w_scale, int64_t sw_n, int64_t sw_g, const void* bias, void* y,
                       int64_t ldy, int y_dtype, int M, int N, int K, unsigned flags, void* stream);

@@ -22,6 +22,7 @@ QF_AR_MAX_RANKS = 8
 QF_AR_MAX_CHUNKS = 256
 QF_IPC_HANDLE_BYTES = 64
 QF_FP8_MAX_K = 1048576
+QF_FP8_MAX_M = 2147483520
 QF_NORM_MAX_H = 16384
 QF_GATE_NONE = 0
 QF_GATE_SIGMOID = 1

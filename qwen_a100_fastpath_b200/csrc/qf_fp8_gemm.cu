@@ -969,7 +969,10 @@ extern "C" int qf_fp8_block_gemm(const void* a, int64_t lda, const float* a_scal
   if (y_dtype != QF_DTYPE_BF16 && y_dtype != QF_DTYPE_F32) return fail(QF_ERR_DTYPE, "y must be bf16 or fp32");
   if (M == 0 || N == 0) return QF_OK;
   if (K == 0) return fail(QF_ERR_SHAPE, "K must be >= 1");
-  if (K > QF_FP8_MAX_K || N > QF_MAX_N || M > QF_MAX_N) return fail(QF_ERR_SHAPE, "M, N or K too large");
+  // tile numbers, and the step of a grid past the last, have 32 bits
+  if (K > QF_FP8_MAX_K || N > QF_MAX_N || M > QF_FP8_MAX_M ||
+      static_cast<int64_t>((M + kTileM - 1) / kTileM) * ((N + 63) / 64) >= INT32_MAX - 4095)
+    return fail(QF_ERR_SHAPE, "M, N or K too large");
   if (!a || !a_scale || !w || !w_scale || !y) return fail(QF_ERR_INVALID, "null pointer");
   if ((M > 1 && lda < K) || (N > 1 && ldw < K) || (M > 1 && ldy < N))
     return fail(QF_ERR_STRIDE, "leading dimension too small");

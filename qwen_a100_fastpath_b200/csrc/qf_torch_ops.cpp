@@ -124,9 +124,18 @@ void check_input(const char* op, const char* name, const at::Tensor& t, at::Scal
 
 cudaStream_t stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
-int as_int(const char* op, int64_t v) {
-  QF_REFUSE_UNLESS(v <= INT32_MAX, op, ": a size of ", v, " is too large");
-  return static_cast<int>(v);
+// Rows of [..., K], K >= 1.
+int64_t rows_of(const at::Tensor& x) { return x.dim() == 2 ? x.size(0) : x.numel() / x.size(-1); }
+
+void check_groups(const char* op, int64_t M, int64_t K) {
+  QF_REFUSE_UNLESS(M <= INT32_MAX && M * blocks(K) <= INT32_MAX, op, ": ", M, " rows of ", blocks(K),
+                   " groups are more than 2^31 - 1 groups");
+}
+
+// What the product takes (the last limit is the one on its tiles).
+void check_rows(const char* op, int64_t M, int64_t N) {
+  QF_REFUSE_UNLESS(M <= QF_FP8_MAX_M && (M + 127) / 128 * ((N + 63) / 64) < INT32_MAX - 4095, op, ": ", M, " rows of ", N,
+                   " results are too many");
 }
 
 // The bytes of a tensor as `rows` intervals of `width` bytes, `step` bytes apart.  Exact for rows of adjacent elements; what
@@ -210,12 +219,12 @@ at::Tensor empty_rows(int64_t M, int64_t K, const at::Tensor& like) {
   return K % 16 ? q.narrow(1, 0, K) : q;
 }
 
-std::tuple<at::Tensor, at::Tensor> quantize_rows(const char* op, const at::Tensor& x2, bool silu_mul) {
+std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x2, bool silu_mul) {
   const int64_t M = x2.size(0), K = silu_mul ? x2.size(1) / 2 : x2.size(1);
   at::Tensor q = empty_rows(M, K, x2);
   at::Tensor s = empty_on(x2, {M, blocks(K)}, at::kFloat);
   if (M && K)
-    check(qf_fp8_quantize(x2.data_ptr(), x2.stride(0), as_int(op, M), as_int(op, K), silu_mul, q.data_ptr(), q.stride(0),
+    check(qf_fp8_quantize(x2.data_ptr(), x2.stride(0), static_cast<int>(M), static_cast<int>(K), silu_mul, q.data_ptr(), q.stride(0),
                           s.data_ptr<float>(), s.stride(0), QF_FLAG_PDL, stream_of(x2)),
           "qf_fp8_quantize");
   return {q, s};
@@ -227,8 +236,9 @@ std::tuple<at::Tensor, at::Tensor> fp8_quantize(const at::Tensor& x, bool silu_m
   const int64_t K = silu_mul ? x.size(-1) / 2 : x.size(-1);
   QF_REFUSE_UNLESS(K >= 1 && K <= QF_FP8_MAX_K, "fp8_quantize: 1 to ", QF_FP8_MAX_K, " values per row, got ", K);
   check_input("fp8_quantize", "x", x, at::kBFloat16, x.device());
+  check_groups("fp8_quantize", rows_of(x), K);
   c10::cuda::CUDAGuard guard(x.device());
-  auto [q, s] = quantize_rows("fp8_quantize", as_rows(x), silu_mul);
+  auto [q, s] = quantize_rows(as_rows(x), silu_mul);
   return {with_leading(q, x), with_leading(s, x)};
 }
 
@@ -252,7 +262,7 @@ void check_weight(const char* op, const at::Tensor& w_t, const at::Tensor& w_sca
   }
 }
 
-void run_mm(const char* op, const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t,
+void run_mm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t,
             const at::Tensor& w_scale, const OptTensor& bias, at::Tensor& y) {
   const int64_t M = a.size(0), K = a.size(1), N = w_t.size(1);
   if (M == 0 || N == 0) return;
@@ -261,14 +271,13 @@ void run_mm(const char* op, const at::Tensor& a, const at::Tensor& a_scale, cons
   check(qf_fp8_block_gemm(a.data_ptr(), a.stride(0), a_scale.data_ptr<float>(), a_scale.stride(0), a_scale.stride(1),
                           w_t.data_ptr(), N > 1 ? w_t.stride(1) : K, w_scale.data_ptr<float>(), w_scale.stride(0),
                           w_scale.stride(1), b.defined() ? b.data_ptr() : nullptr, y.data_ptr(), y.stride(0),
-                          y.scalar_type() == at::kFloat ? QF_DTYPE_F32 : QF_DTYPE_BF16, as_int(op, M), as_int(op, N),
-                          as_int(op, K), QF_FLAG_PDL, stream_of(a)),
+                          y.scalar_type() == at::kFloat ? QF_DTYPE_F32 : QF_DTYPE_BF16, static_cast<int>(M),
+                          static_cast<int>(N), static_cast<int>(K), QF_FLAG_PDL, stream_of(a)),
         "qf_fp8_block_gemm");
 }
 
-at::Tensor checked_a(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t, const at::Tensor& w_scale,
-                     const OptTensor& bias) {
-  const char* op = "fp8_block_mm";
+void check_mm(const char* op, const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t, const at::Tensor& w_scale,
+              const OptTensor& bias) {
   QF_REFUSE_UNLESS(a.dim() == 2, op, ": a must be [M, K]");
   check_input(op, "a", a, at::kFloat8_e4m3fn, a.device());
   const int64_t M = a.size(0), K = a.size(1);
@@ -276,6 +285,12 @@ at::Tensor checked_a(const at::Tensor& a, const at::Tensor& a_scale, const at::T
   check_input(op, "a_scale", a_scale, at::kFloat, a.device());
   QF_REFUSE_UNLESS(a_scale.dim() == 2 && a_scale.size(0) == M && a_scale.size(1) == blocks(K), op, ": a_scale must be [",
                    M, ", ", blocks(K), "], got ", a_scale.sizes());
+  check_rows(op, M, w_t.size(1));
+}
+
+// a with rows that the product's tensor maps take, copied where they are not.
+at::Tensor aligned_rows(const at::Tensor& a) {
+  const int64_t M = a.size(0), K = a.size(1);
   const bool fits = (K == 1 || a.stride(1) == 1) && (M <= 1 || (a.stride(0) >= K && a.stride(0) % 16 == 0)) &&
                     reinterpret_cast<uintptr_t>(a.data_ptr()) % 16 == 0;
   if (fits || M == 0) return a;
@@ -287,9 +302,10 @@ at::Tensor checked_a(const at::Tensor& a, const at::Tensor& a_scale, const at::T
 at::Tensor fp8_block_mm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t,
                         const at::Tensor& w_scale, const OptTensor& bias, bool out_f32) {
   c10::cuda::OptionalCUDAGuard guard(a.is_cuda() ? c10::optional<c10::Device>(a.device()) : c10::nullopt);
-  const at::Tensor r = checked_a(a, a_scale, w_t, w_scale, bias);
+  check_mm("fp8_block_mm", a, a_scale, w_t, w_scale, bias);
+  const at::Tensor r = aligned_rows(a);
   at::Tensor y = empty_on(a, {a.size(0), w_t.size(1)}, out_f32 ? at::kFloat : at::kBFloat16);
-  run_mm("fp8_block_mm", r, a_scale, w_t, w_scale, bias, y);
+  run_mm(r, a_scale, w_t, w_scale, bias, y);
   return y;
 }
 
@@ -297,7 +313,7 @@ void fp8_block_mm_out(const at::Tensor& a, const at::Tensor& a_scale, const at::
                       const OptTensor& bias, at::Tensor out) {
   const char* op = "fp8_block_mm";
   c10::cuda::OptionalCUDAGuard guard(a.is_cuda() ? c10::optional<c10::Device>(a.device()) : c10::nullopt);
-  const at::Tensor r = checked_a(a, a_scale, w_t, w_scale, bias);
+  check_mm(op, a, a_scale, w_t, w_scale, bias);
   const int64_t M = a.size(0), N = w_t.size(1);
   QF_REFUSE_UNLESS(out.device() == a.device() && out.dim() == 2 && out.size(0) == M && out.size(1) == N &&
                        (out.scalar_type() == at::kFloat || out.scalar_type() == at::kBFloat16) &&
@@ -308,7 +324,7 @@ void fp8_block_mm_out(const at::Tensor& a, const at::Tensor& a_scale, const at::
   check_no_overlap(op, "out", out, "w_t", w_t);
   check_no_overlap(op, "out", out, "w_scale", w_scale);
   if (given(bias)) check_no_overlap(op, "out", out, "bias", *bias);
-  run_mm(op, r, a_scale, w_t, w_scale, bias, out);
+  run_mm(aligned_rows(a), a_scale, w_t, w_scale, bias, out);
 }
 
 at::Tensor fp8_block_linear(const at::Tensor& x, const at::Tensor& w_t, const at::Tensor& w_scale, const OptTensor& bias) {
@@ -316,12 +332,14 @@ at::Tensor fp8_block_linear(const at::Tensor& x, const at::Tensor& w_t, const at
   QF_REFUSE_UNLESS(x.dim() >= 1, op, ": x must have at least one dimension");
   check_input(op, "x", x, at::kBFloat16, x.device());
   check_weight(op, w_t, w_scale, bias, x.size(-1), x.device());
+  check_groups(op, rows_of(x), x.size(-1));
+  check_rows(op, rows_of(x), w_t.size(1));
   c10::cuda::CUDAGuard guard(x.device());
   const at::Tensor x2 = as_rows(x);
   at::Tensor y = empty_on(x, {x2.size(0), w_t.size(1)}, at::kBFloat16);
   if (x2.size(0) && w_t.size(1)) {
-    auto [q, s] = quantize_rows(op, x2, false);
-    run_mm(op, q, s, w_t, w_scale, bias, y);
+    auto [q, s] = quantize_rows(x2, false);
+    run_mm(q, s, w_t, w_scale, bias, y);
   }
   return with_leading(y, x);
 }
@@ -332,7 +350,6 @@ std::tuple<at::Tensor, at::Tensor> run_norm(const at::Tensor& x, const OptTensor
                                             const OptTensor& post_weight, const OptTensor& gate, int64_t gate_act,
                                             double residual_scale, double weight_offset, double eps, bool quantize,
                                             at::Tensor& r_out) {
-  const char* op = "residual_norm";
   const int64_t H = x.size(-1);
   const at::Tensor x2 = as_rows(x);
   const int64_t M = x2.size(0);
@@ -361,7 +378,7 @@ std::tuple<at::Tensor, at::Tensor> run_norm(const at::Tensor& x, const OptTensor
                            ptr(g2), gm, gh, static_cast<int>(gate_act), ptr(post), ptr(pre),
                            static_cast<float>(weight_offset), static_cast<float>(residual_scale), static_cast<float>(eps),
                            ro2.data_ptr(), ro2.stride(0), ptr(h), ld(h), s.defined() ? s.data_ptr<float>() : nullptr, ld(s),
-                           as_int(op, M), as_int(op, H), QF_FLAG_PDL, stream_of(x)),
+                           static_cast<int>(M), static_cast<int>(H), QF_FLAG_PDL, stream_of(x)),
           "qf_residual_norm");
   }
   if (h.defined()) h = with_leading(h, x);
@@ -376,6 +393,7 @@ void check_norm(const at::Tensor& x, const OptTensor& residual, const OptTensor&
   check_input(op, "x", x, at::kBFloat16, x.device());
   const int64_t H = x.size(-1);
   QF_REFUSE_UNLESS(H >= 1 && H <= QF_NORM_MAX_H, op, ": rows of 1 to ", QF_NORM_MAX_H, " values, got ", H);
+  QF_REFUSE_UNLESS(rows_of(x) <= INT32_MAX, op, ": ", rows_of(x), " rows are too many");
   if (given(residual)) {
     QF_REFUSE_UNLESS(residual->scalar_type() == at::kBFloat16 || residual->scalar_type() == at::kFloat, op,
                      ": residual must be bf16 or fp32");

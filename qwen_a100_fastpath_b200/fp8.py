@@ -36,7 +36,7 @@ def fp8_quantize(x: torch.Tensor, silu_mul: bool = False):
     ``a = max(max|v|, 448 * 2^-60)``, ``scale = a / 448`` (fp32 ``[..., ceil(K / 128)]``), ``q = e4m3(v * (448 / a))``
     rounded to nearest even (``float8_e4m3fn [..., K]``, rows 16 bytes aligned).  ``v`` is ``x``, or with ``silu_mul``
     ``silu(x[..., :K]) * x[..., K:]`` in fp32 for ``x [..., 2 K]`` (the merged gate_up output).  A NaN makes its group's
-    scale and values NaN."""
+    scale and values NaN.  K <= 2^20, fewer than 2^31 groups in all."""
     return _quantize(x, silu_mul)
 
 
@@ -46,7 +46,7 @@ def fp8_block_mm(a: torch.Tensor, a_scale: torch.Tensor, w_t: torch.Tensor, w_sc
     """``y[m, n] = sum_g a_scale[m, g] * w_scale[n // 128, g] * sum_{k in g} a[m, k] * w[n, k] (+ bias[n])``: exact e4m3
     products, fp32 sums, one rounding to ``out_dtype`` (bf16 or fp32).  ``a`` e4m3 ``[M, K]`` with fp32 ``a_scale
     [M, ceil(K / 128)]`` (any strides) as ``fp8_quantize`` returns them; ``w_t`` e4m3 ``[K, N]`` with stride ``(1, ldw)``,
-    16-byte aligned, ``ldw % 16 == 0``; ``bias`` bf16 ``[N]``, added in fp32.  Rows of ``a`` that are not 16-byte aligned
+    16-byte aligned, ``ldw % 16 == 0``, K and N up to 2^20, M up to 2^31 - 128; ``bias`` bf16 ``[N]``, added in fp32.  Rows of ``a`` that are not 16-byte aligned
     are copied first.  ``out`` may supply the result (it decides the type then); it must not share memory with an input
     (refused as ``_lib.QFOverlapError``, a ``ValueError``; bytes between the elements of an input that is not rows of adjacent
     elements count as its own)."""

@@ -25,7 +25,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, pre_weight: to
                   post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, gate_act: str = "none",
                   residual_scale: float = 1.0, weight_offset: float = 0.0, quantize: bool = False,
                   residual_out: torch.Tensor | None = None):
-    """``(h, r)`` for the block output ``x`` bf16 ``[..., H]`` (H <= 16384), in fp32 inside:
+    """``(h, r)`` for the block output ``x`` bf16 ``[..., H]`` (H <= 16384, fewer than 2^31 rows), in fp32 inside:
 
     * ``u = x``, or with ``post_weight`` bf16 ``[H]`` ``u = x * rsqrt(mean(x^2) + eps) * (post_weight + weight_offset)``;
     * ``v = u``, or with ``gate`` (bf16, broadcast to x's shape) ``v = u * act(gate)``, ``gate_act`` one of "none" (the

@@ -176,3 +176,12 @@ def test_meta_shapes():
 
 def test_norm_status_needs_a_place():
     assert LIB.qf_residual_norm_status(None, None) == -1
+
+
+@pytest.mark.parametrize("kw", [
+    dict(M=_lib.QF_FP8_MAX_M + 1, K=16, lda=16, N=16, ldw=16, ldy=16),     # the last tile's rows pass 2^31
+    dict(M=2 ** 31 - 1, K=16, lda=16, N=16, ldw=16, ldy=16),
+    dict(M=_lib.QF_FP8_MAX_M, K=16, lda=16, N=_lib.QF_MAX_N, ldw=16, ldy=_lib.QF_MAX_N),   # more tiles than 2^31
+])
+def test_gemm_refuses_more_tiles_than_it_can_number(kw):
+    assert gemm(**kw) == -2 and b"too large" in LIB.qf_last_error_detail()
