@@ -27,36 +27,47 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 
-// 1 / (1 + e^-x) of two values: e^-x = 2^t * 2^c with t = -x * log2(e) rounded and c what the rounding left, 2^t by the
-// special-function unit (2 ulp) and 2^c = 1 + c * ln(2), then the unit's reciprocal with one Newton step: good to
-// 8 * 2^-24, at some ten instructions a value (packed fp32 pairs) where expf and an IEEE quotient take some thirty.  Beyond |x| = 88.5,
-// where the result is 1 or under 2^-127, x counts as that bound, which makes the latter zero; a NaN stays one.
+// 1 / (1 + e^-x) of two values.  e^-x = 2^n * 2^f with n = -x * log2(e) rounded to a whole number and f the rest (log2(e) in two
+// parts); 2^f = 1 + f * g(f), g the polynomial of degree 5 through its values at the six Chebyshev nodes of [-1/2, 1/2]
+// (2^f is then 0.16 * 2^-24 off with the coefficients rounded).  The sum is formed as 2^-64 + 2^(n-64) * 2^f, in one
+// rounding, so that neither it nor its reciprocal leaves the normal range before the last product; the reciprocal is the
+// special-function unit's with one Newton step.  Over all bf16 x, which is what the gates are: within 2 * 2^-24 of the value
+// where that is a normal number (1 / (1 + expf(-x)) 2.3 * 2^-24), within half a step where it is subnormal (expf's form is zero
+// from x = -88.7 on, this one from -104).  Above 40 the result is 1; a NaN stays one.  Some 11 instructions a value (packed
+// fp32 pairs), where expf and an IEEE quotient take some thirty (4096 x 17408 with the gate: 76.7 us against 99.6).
 __device__ __forceinline__ float2 sigmoid2(float a, float b) {
-  const uint64_t kL = pack_f32x2(-1.44269502f, -1.44269502f);              // log2(e) = 1.44269502 + 1.92596303e-8
-  const uint64_t kLLow = pack_f32x2(-1.92596303e-8f, -1.92596303e-8f);
-  const uint64_t kLn2 = pack_f32x2(0.693147182f, 0.693147182f);
-  const uint64_t kOne = pack_f32x2(1.f, 1.f);
-  const uint64_t x = pack_f32x2(min_nan(max_nan(a, -88.5f), 88.5f), min_nan(max_nan(b, -88.5f), 88.5f));
-  const uint64_t t = mul_f32x2(x, kL);
+  auto both = [](float v) { return pack_f32x2(v, v); };
+  const uint64_t x = pack_f32x2(min_nan(max_nan(a, -105.f), 40.f), min_nan(max_nan(b, -105.f), 40.f));
+  // 1.5 * 2^23 rounds a sum to whole numbers; 63 = 127 - 64 makes its low bits the exponent of 2^(n-64), n from -58 to 151
+  constexpr float kMagic = 12582912.f + 63.f;
+  uint64_t t = both(kMagic);
+  fma_f32x2(t, x, both(-1.44269502f));      // log2(e) = 1.44269502 + 1.92596303e-8
+  uint64_t f = both(kMagic);
+  fma_f32x2(f, t, both(-1.f));              // -n, exact
+  fma_f32x2(f, x, both(-1.44269502f));
+  fma_f32x2(f, x, both(-1.92596303e-8f));
+  constexpr float kG[6] = {0.6931471824645996f,   0.24022650718688965f,  0.055503569543361664f,
+                           0.009618083015084267f, 0.0013390863314270973f, 0.00015453163359779865f};
+  uint64_t g = both(kG[5]);
+#pragma unroll
+  for (int i = 4; i >= 0; --i) {
+    uint64_t next = both(kG[i]);
+    fma_f32x2(next, g, f);
+    g = next;
+  }
+  uint64_t p = both(1.f);
+  fma_f32x2(p, g, f);
   const float2 tf = unpack_f32x2(t);
-  uint64_t c = pack_f32x2(-tf.x, -tf.y);
-  fma_f32x2(c, x, kL);     // exact
-  fma_f32x2(c, x, kLLow);
-  uint64_t f = kOne;
-  fma_f32x2(f, c, kLn2);
-  float2 e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(tf.x));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(tf.y));
-  uint64_t d = kOne;
-  fma_f32x2(d, pack_f32x2(e.x, e.y), f);
+  uint64_t d = both(0x1p-64f);
+  fma_f32x2(d, p, pack_f32x2(__uint_as_float(__float_as_uint(tf.x) << 23), __uint_as_float(__float_as_uint(tf.y) << 23)));
   const float2 df = unpack_f32x2(d);
-  float2 r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(df.x));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(df.y));
-  uint64_t rest = kOne, q = pack_f32x2(r.x, r.y);
-  fma_f32x2(rest, pack_f32x2(-df.x, -df.y), q);  // 1 - d * r, exact
+  float2 r;  // negative, which saves negating d
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(-df.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(-df.y));
+  uint64_t rest = both(1.f), q = pack_f32x2(r.x, r.y);
+  fma_f32x2(rest, d, q);
   fma_f32x2(q, q, rest);
-  return unpack_f32x2(q);
+  return unpack_f32x2(mul_f32x2(q, both(-0x1p-64f)));
 }
 
 // Two fp32 -> two e4m3 bytes (lo in bits 0-7), round to nearest even, saturated to +-448, NaN kept.

@@ -9,8 +9,9 @@
 // Bound by memory: 2 (4 with the gate) bytes read and 1 written per element, so one pass with everything in registers.
 // Eight threads share a group (16 elements, 32 contiguous bytes each), its maximum is three shuffles, nothing
 // crosses a warp, and the groups of all rows form one flat index, so one row fills as many SMs as it has work for.  Eight
-// CTAs per SM (six with the gate, whose arithmetic needs the registers) keep enough loads in flight: 4096 x 17408 takes
-// 34 us (6.2 TB/s), with the gate 75 us (4.8 TB/s; fewer or more CTAs 4 to 16 us longer); one row of 5120 1.5 us.
+// CTAs per SM (six with the gate, whose arithmetic needs the registers; what a thread has loaded stays packed until it is used,
+// which keeps it at 40) keep enough loads in flight: 4096 x 17408 takes 34 us (6.2 TB/s), with the gate 77 us through the call
+// (4.7 TB/s; five CTAs 82; unpacked at once 98); one row of 5120 1.5 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -41,23 +42,26 @@ struct QtParams {
   int vec_in, vec_out;
 };
 
-// 16 bf16 of a row from column k: two 16-byte loads where the whole piece lies in the row, else one by one (zeros
+// 16 bf16 of a row from column k, packed: two 16-byte loads where the whole piece lies in the row, else one by one (zeros
 // past the end, which leave the group's maximum as it is).
-__device__ __forceinline__ void load16(const __nv_bfloat16* row, int k, int K, bool vec, float (&v)[kQtPer]) {
+struct Piece {
+  uint32_t w[kQtPer / 2];
+};
+
+__device__ __forceinline__ void load16(const __nv_bfloat16* row, int k, int K, bool vec, Piece& v) {
   if (vec && k + kQtPer <= K) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + k) + j);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[8 * j + 2 * i] = bf16_lo(w[i]);
-        v[8 * j + 2 * i + 1] = bf16_hi(w[i]);
-      }
+      v.w[4 * j] = u.x, v.w[4 * j + 1] = u.y, v.w[4 * j + 2] = u.z, v.w[4 * j + 3] = u.w;
     }
   } else {
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(row);
 #pragma unroll
-    for (int i = 0; i < kQtPer; ++i) v[i] = k + i < K ? __bfloat162float(row[k + i]) : 0.f;
+    for (int i = 0; i < kQtPer; ++i) {
+      const uint32_t h = k + i < K ? src[k + i] : 0u;
+      v.w[i / 2] = i % 2 ? v.w[i / 2] | (h << 16) : h;
+    }
   }
 }
 
@@ -72,16 +76,18 @@ __global__ void __launch_bounds__(256, SILU ? 6 : 8) fp8_quantize_kernel(const Q
   const uint32_t g = live ? group - m * p.kb : 0;
   const int k = static_cast<int>(g) * kFp8Block + static_cast<int>(threadIdx.x % kQtLanes) * kQtPer;
   const __nv_bfloat16* row = p.x + static_cast<int64_t>(m) * p.ldx;
+  Piece x, up;
+  load16(row, k, live ? p.K : 0, p.vec_in, x);
+  if (SILU) load16(row + p.K, k, live ? p.K : 0, p.vec_in, up);
   float v[kQtPer];
-  load16(row, k, live ? p.K : 0, p.vec_in, v);
-  if (SILU) {
-    float u[kQtPer];
-    load16(row + p.K, k, live ? p.K : 0, p.vec_in, u);
 #pragma unroll
-    for (int i = 0; i < kQtPer; i += 2) {
+  for (int i = 0; i < kQtPer; i += 2) {
+    v[i] = bf16_lo(x.w[i / 2]);
+    v[i + 1] = bf16_hi(x.w[i / 2]);
+    if (SILU) {
       const float2 s = sigmoid2(v[i], v[i + 1]);
-      v[i] = v[i] * s.x * u[i];
-      v[i + 1] = v[i + 1] * s.y * u[i + 1];
+      v[i] = v[i] * s.x * bf16_lo(up.w[i / 2]);
+      v[i + 1] = v[i + 1] * s.y * bf16_hi(up.w[i / 2]);
     }
   }
   float a = kFp8AmaxFloor;
