@@ -296,9 +296,9 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         v[c][i] = fmaf(p.alpha, v[c][i], r[c][i]);
-        // elements past the row must not enter the sum (a gate of infinity there would not be zero times x)
-        if (e + i >= p.H) v[c][i] = 0.f;
-        s = fmaf(v[c][i], v[c][i], s);
+        // elements past the row must not enter the sum (a gate of infinity there would not be zero times x); with wide
+        // loads a piece is in the row or not as a whole
+        if ((VEC ? e : e + i) < p.H) s = fmaf(v[c][i], v[c][i], s);
       }
       if (p.residual_out) {
         if (R32)
@@ -333,7 +333,8 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
       }
       float a = kFp8AmaxFloor;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a = max_nan(a, e + i < p.H ? fabsf(v[c][i]) : 0.f);
+      for (int i = 0; i < 8; ++i)
+        if ((VEC ? e : e + i) < p.H) a = max_nan(a, fabsf(v[c][i]));
 #pragma unroll
       for (int off = 1; off < kFp8Block / 8; off <<= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, off));
       const float inv = __fdiv_rn(kE4m3Max, a);
