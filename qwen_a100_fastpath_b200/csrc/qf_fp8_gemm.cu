@@ -100,11 +100,11 @@ template <int NT, int MT, int G> struct RowGeo {
 
 // 16 bytes of an operand row from column k; bytes past K read as zero and are not touched.
 __device__ __forceinline__ uint4 load_chunk(const uint8_t* row, int k, int K) {
-  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  if (k + 16 <= K) return *reinterpret_cast<const uint4*>(row + k);
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    if (k + i < K) w[i / 4] |= static_cast<uint32_t>(__ldg(row + k + i)) << (8 * (i % 4));
+    if (k + i < K) w[i / 4] |= static_cast<uint32_t>(row[k + i]) << (8 * (i % 4));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -210,17 +210,16 @@ __global__ void __launch_bounds__(kRowWarps * 32 + 32, kRowPerSm)
       const float* sw_row = p.sw + static_cast<int64_t>(n0 / kFp8Block) * p.sw_n;
       auto load_scales = [&](RowScales<NT>& r, int g) {
         if (g >= p.kb) return;
-        r.sw = __ldg(sw_row + g * p.sw_g);
+        r.sw = sw_row[g * p.sw_g];
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) r.sa[j][i] = __ldg(sa_row[j][i] + g * p.sa_g);
+          for (int i = 0; i < 2; ++i) r.sa[j][i] = sa_row[j][i][g * p.sa_g];
       };
       float acc[NT][MT][4] = {};
-      auto add = [&](const uint4 (&lo)[MT][2], const uint4 (&hi)[MT][2], const uint4 (&b)[NT][2], const RowScales<NT>& r) {
+      auto add = [&](const uint4 (&lo)[MT][2], const uint4 (&hi)[MT][2], const uint4 (&b)[NT][2], const float (&sc)[NT][2]) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const float s0 = r.sw * r.sa[j][0], s1 = r.sw * r.sa[j][1];
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
             float d[2][4] = {};  // two chains of instructions
@@ -230,16 +229,27 @@ __global__ void __launch_bounds__(kRowWarps * 32 + 32, kRowPerSm)
               mma_e4m3_m16n8k32(d[c], lo[i][c].x, hi[i][c].x, lo[i][c].y, hi[i][c].y, b[j][c].x, b[j][c].y);
               mma_e4m3_m16n8k32(d[c], lo[i][c].z, hi[i][c].z, lo[i][c].w, hi[i][c].w, b[j][c].z, b[j][c].w);
             }
-            acc[j][i][0] = fmaf(d[0][0] + d[1][0], s0, acc[j][i][0]);
-            acc[j][i][1] = fmaf(d[0][1] + d[1][1], s1, acc[j][i][1]);
-            acc[j][i][2] = fmaf(d[0][2] + d[1][2], s0, acc[j][i][2]);
-            acc[j][i][3] = fmaf(d[0][3] + d[1][3], s1, acc[j][i][3]);
+            acc[j][i][0] = fmaf(d[0][0] + d[1][0], sc[j][0], acc[j][i][0]);
+            acc[j][i][1] = fmaf(d[0][1] + d[1][1], sc[j][1], acc[j][i][1]);
+            acc[j][i][2] = fmaf(d[0][2] + d[1][2], sc[j][0], acc[j][i][2]);
+            acc[j][i][3] = fmaf(d[0][3] + d[1][3], sc[j][1], acc[j][i][3]);
           }
         }
       };
       // group i of the warp's G in stage st
       auto group_of = [&](int st, int i) { return st * C::kGroups + i * kRowWarps + warp; };
+      auto product = [](const RowScales<NT>& r, float (&sc)[NT][2]) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sc[j][0] = r.sw * r.sa[j][0], sc[j][1] = r.sw * r.sa[j][1];
+      };
       auto stage = [&](int st, RowScales<NT> (&r)[G]) {
+        // the scales of two stages ahead are on their way before the wait (16 x 10240 x 5120 16.9 us; behind the products 18.4)
+        float sc[G][NT][2];
+#pragma unroll
+        for (int u = 0; u < G; ++u) {
+          product(r[u], sc[u]);
+          load_scales(r[u], group_of(st + 2, u));
+        }
         if (!fp8_wait_warp(&full[s], phase, &abort_flag)) {
           ok = false;
           return;
@@ -265,10 +275,8 @@ __global__ void __launch_bounds__(kRowWarps * 32 + 32, kRowPerSm)
         if (lane == 0) mbar_arrive(&empty[s]);
         if (++s == C::kStages) s = 0, phase ^= 1;
 #pragma unroll
-        for (int u = 0; u < G; ++u) {
-          if (group_of(st, u) < kfull) add(lo[u], hi[u], b[u], r[u]);
-          load_scales(r[u], group_of(st + 2, u));  // two stages ahead
-        }
+        for (int u = 0; u < G; ++u)
+          if (group_of(st, u) < kfull) add(lo[u], hi[u], b[u], sc[u]);
       };
       RowScales<NT> r0[G] = {}, r1[G] = {};
 #pragma unroll
@@ -295,7 +303,9 @@ __global__ void __launch_bounds__(kRowWarps * 32 + 32, kRowPerSm)
             b[j][c] = load_chunk(p.a + static_cast<int64_t>(min(m0 + 8 * j + gid, p.M - 1)) * p.lda, k + 16 * c, p.K);
         }
         load_scales(r0[0], kfull);
-        add(lo, hi, b, r0[0]);
+        float sc[NT][2];
+        product(r0[0], sc);
+        add(lo, hi, b, sc);
       }
       // the warps' sums in warp order
       named_bar_sync(1, kRowWarps * 32);  // the tile before is read

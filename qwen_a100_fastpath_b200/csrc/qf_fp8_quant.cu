@@ -52,7 +52,7 @@ __device__ __forceinline__ void load16(const __nv_bfloat16* row, int k, int K, b
   if (vec && k + kQtPer <= K) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + k) + j);
+      const uint4 u = reinterpret_cast<const uint4*>(row + k)[j];
       v.w[4 * j] = u.x, v.w[4 * j + 1] = u.y, v.w[4 * j + 2] = u.z, v.w[4 * j + 3] = u.w;
     }
   } else {

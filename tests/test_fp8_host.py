@@ -185,3 +185,13 @@ def test_norm_status_needs_a_place():
 ])
 def test_gemm_refuses_more_tiles_than_it_can_number(kw):
     assert gemm(**kw) == -2 and b"too large" in LIB.qf_last_error_detail()
+
+
+def test_operands_are_read_by_ordinary_loads():
+    """The kernels start under the tail of the kernel before them, which may still write their operands: loads that the
+    hardware and the compiler may take for invariant (ld.global.nc, __ldg) are not for them."""
+    from pathlib import Path
+    csrc = Path(_lib.__file__).resolve().parent / "csrc"
+    for name in ("qf_fp8.cuh", "qf_fp8_gemm.cu", "qf_fp8_quant.cu", "qf_norm.cu"):
+        text = (csrc / name).read_text()
+        assert "__ldg" not in text and "global.nc" not in text and "__restrict__" not in text, name

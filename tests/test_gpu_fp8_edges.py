@@ -52,3 +52,47 @@ def test_too_many_rows_are_refused_first(dev):
     assert torch.cuda.max_memory_allocated(dev) == base
     del rows
     assert torch.cuda.memory_allocated(dev) == before
+
+
+@pytest.mark.parametrize("M", [3, 16, 200])
+def test_operands_written_by_the_kernel_before(dev, M):
+    """Chains in which each launch, begun under the tail of the one before, reads what that one wrote over older values:
+    activations, scales, bias, residual and gate.  The bits of the same calls with the device idle in between."""
+    import torch
+    from qwen_a100_fastpath_b200.fp8 import fp8_block_mm, fp8_quantize
+    from qwen_a100_fastpath_b200.norms import residual_norm
+    N, K = 512, 640
+    gen = torch.Generator(device=dev).manual_seed(M)
+
+    def e4m3(*shape):
+        return torch.randn(*shape, device=dev, generator=gen).to(torch.float8_e4m3fn)
+
+    w, w2 = e4m3(N, K).t(), e4m3(K, N).t()
+    sw, sw2 = torch.rand(4, 5, device=dev, generator=gen) * 0.01, torch.rand(5, 4, device=dev, generator=gen) * 0.01
+    x0 = torch.randn(M, K, device=dev, generator=gen).to(torch.bfloat16)
+
+    def chain(pause):
+        def done():
+            if pause:
+                torch.cuda.synchronize(dev)
+
+        r, y, z = x0.clone(), torch.zeros(M, N, device=dev), torch.zeros(M, K, device=dev, dtype=torch.bfloat16)
+        kept = []
+        done()
+        for _ in range(12):
+            h, _ = residual_norm(z, r, x0[0], gate=r, gate_act="sigmoid", residual_out=torch.empty_like(r))
+            done()
+            residual_norm(h, r, None, gate=h, gate_act="sigmoid", residual_out=r)   # the residual over itself
+            done()
+            a, s = fp8_quantize(r)                                                  # of what was just written
+            done()
+            fp8_block_mm(a, s, w, sw, bias=r[0, :N], out=y)                         # y over the last round's
+            done()
+            fp8_block_mm(a[:, :N], y[:, :4], w2, sw2, out=z)                        # y as scales, z over the last round's
+            done()
+            kept += [h, r.clone(), y.clone(), z.clone()]
+        return kept
+
+    want, got = chain(True), chain(False)
+    for a, b in zip(got, want):
+        assert torch.equal(a.nan_to_num(), b.nan_to_num()) and torch.isfinite(b).any()
