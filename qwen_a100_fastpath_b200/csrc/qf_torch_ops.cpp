@@ -99,27 +99,133 @@ at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& w_q, const at::Ten
 
 at::Tensor int8_linear_meta(const at::Tensor& x, const at::Tensor& w_q, const at::Tensor& w_s,
                             const c10::optional<at::Tensor>& bias) {
-  std::vector<int64_t> out_shape(x.sizes().begin(), x.sizes().end());
-  out_shape.back() = w_q.size(1);
-  return at::empty(out_shape, x.options());
+  std::vector<c10::SymInt> out_shape = x.sym_sizes().vec();
+  out_shape.back() = w_q.sym_size(1);
+  return at::empty_symint(out_shape, x.options());
 }
 
 // ---------------------------------------------------------------------------------------- block-scaled fp8 layers
 #define QF_REFUSE_UNLESS(cond, ...) TORCH_CHECK_VALUE(cond, __VA_ARGS__)
+// Equality of sizes that may be symbolic: tracing goes on with it as a fact and fixes neither side.
+bool same_size(const c10::SymInt& a, const c10::SymInt& b) {
+  if (C10_LIKELY(!a.is_heap_allocated() && !b.is_heap_allocated())) return a.as_int_unchecked() == b.as_int_unchecked();
+  return a.sym_eq(b).expect_true(__FILE__, __LINE__);
+}
+#define QF_REFUSE_UNLESS_EQ(a, b, ...) TORCH_CHECK_VALUE(same_size(a, b), __VA_ARGS__)
 
 using OptTensor = c10::optional<at::Tensor>;
 
 constexpr int64_t kBlock = 128;
 int64_t blocks(int64_t v) { return (v + kBlock - 1) / kBlock; }
+c10::SymInt blocks(const c10::SymInt& v) { return (v + (kBlock - 1)) / kBlock; }
 
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 
-void check_input(const char* op, const char* name, const at::Tensor& t, at::ScalarType type, const at::Device& dev) {
+void check_type(const char* op, const char* name, const at::Tensor& t, at::ScalarType type) {
+  QF_REFUSE_UNLESS(t.scalar_type() == type, op, ": ", name, " must be ", type, ", got ", t.scalar_type());
+}
+
+void check_input(const char* op, const char* name, const at::Tensor& t, const at::Device& dev) {
   QF_REFUSE_UNLESS(t.is_cuda(), op, ": ", name, " must be a CUDA tensor (there is no CPU path)");
   QF_REFUSE_UNLESS(t.device() == dev, op, ": ", name, " is on ", t.device(), ", the first input on ", dev);
-  QF_REFUSE_UNLESS(t.scalar_type() == type, op, ": ", name, " must be ", type, ", got ", t.scalar_type());
   QF_REFUSE_UNLESS(!(at::GradMode::is_enabled() && t.requires_grad()), op, ": ", name,
                    " requires a gradient and the operator has no backward (call it under torch.no_grad())");
+}
+
+// ---- types and shapes, of real calls and of traced ones (whose sizes may be symbolic) ----
+void check_quantize_shapes(const at::Tensor& x, bool silu_mul) {
+  const char* op = "fp8_quantize";
+  QF_REFUSE_UNLESS(x.dim() >= 1, op, ": x must have at least one dimension");
+  check_type(op, "x", x, at::kBFloat16);
+  if (silu_mul)
+    QF_REFUSE_UNLESS_EQ(x.sym_size(-1) % 2, 0, op, ": silu_mul needs gate and up halves of one width");
+}
+
+void check_weight_shapes(const char* op, const at::Tensor& w_t, const at::Tensor& w_scale, const OptTensor& bias,
+                         const c10::SymInt& K) {
+  check_type(op, "w_t", w_t, at::kFloat8_e4m3fn);
+  QF_REFUSE_UNLESS(w_t.dim() == 2, op, ": w_t must be [K, N], got ", w_t.sym_sizes());
+  QF_REFUSE_UNLESS_EQ(w_t.sym_size(0), K, op, ": w_t must be [K, N] with K = ", K, ", got ", w_t.sym_sizes());
+  const c10::SymInt N = w_t.sym_size(1);
+  check_type(op, "w_scale", w_scale, at::kFloat);
+  QF_REFUSE_UNLESS(w_scale.dim() == 2, op, ": w_scale must have two dimensions");
+  for (int i = 0; i < 2; ++i)
+    QF_REFUSE_UNLESS_EQ(w_scale.sym_size(i), blocks(i ? K : N), op, ": w_scale must be [", blocks(N), ", ", blocks(K),
+                        "], got ", w_scale.sym_sizes());
+  if (given(bias)) {
+    check_type(op, "bias", *bias, at::kBFloat16);
+    QF_REFUSE_UNLESS_EQ(bias->sym_numel(), N, op, ": bias must hold ", N, " values");
+  }
+}
+
+void check_mm_shapes(const char* op, const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t,
+                     const at::Tensor& w_scale, const OptTensor& bias) {
+  QF_REFUSE_UNLESS(a.dim() == 2, op, ": a must be [M, K]");
+  check_type(op, "a", a, at::kFloat8_e4m3fn);
+  const c10::SymInt M = a.sym_size(0), K = a.sym_size(1);
+  check_weight_shapes(op, w_t, w_scale, bias, K);
+  check_type(op, "a_scale", a_scale, at::kFloat);
+  QF_REFUSE_UNLESS(a_scale.dim() == 2, op, ": a_scale must have two dimensions");
+  for (int i = 0; i < 2; ++i)
+    QF_REFUSE_UNLESS_EQ(a_scale.sym_size(i), i ? blocks(K) : M, op, ": a_scale must be [", M, ", ", blocks(K), "], got ",
+                        a_scale.sym_sizes());
+}
+
+void check_out_shapes(const char* op, const at::Tensor& out, const at::Tensor& a, const at::Tensor& w_t) {
+  const c10::SymInt M = a.sym_size(0), N = w_t.sym_size(1);
+  QF_REFUSE_UNLESS(out.dim() == 2 && (out.scalar_type() == at::kFloat || out.scalar_type() == at::kBFloat16), op,
+                   ": out must be bf16 or fp32 [", M, ", ", N, "]");
+  for (int i = 0; i < 2; ++i)
+    QF_REFUSE_UNLESS_EQ(out.sym_size(i), i ? N : M, op, ": out must be bf16 or fp32 [", M, ", ", N, "], got ",
+                        out.sym_sizes());
+}
+
+void check_linear_shapes(const char* op, const at::Tensor& x, const at::Tensor& w_t, const at::Tensor& w_scale,
+                         const OptTensor& bias) {
+  QF_REFUSE_UNLESS(x.dim() >= 1, op, ": x must have at least one dimension");
+  check_type(op, "x", x, at::kBFloat16);
+  check_weight_shapes(op, w_t, w_scale, bias, x.sym_size(-1));
+}
+
+void check_same_sizes(const char* op, const char* name, const at::Tensor& t, const at::Tensor& x) {
+  QF_REFUSE_UNLESS(t.dim() == x.dim(), op, ": ", name, " must have x's shape ", x.sym_sizes(), ", got ", t.sym_sizes());
+  // (an equality at a time, so that a symbolic one is taken as a fact)
+  for (int64_t i = 0; i < x.dim(); ++i)
+    QF_REFUSE_UNLESS_EQ(t.sym_size(i), x.sym_size(i), op, ": ", name, " must have x's shape ", x.sym_sizes(), ", got ",
+                        t.sym_sizes());
+}
+
+void check_norm_shapes(const at::Tensor& x, const OptTensor& residual, const OptTensor& pre_weight,
+                       const OptTensor& post_weight, const OptTensor& gate, int64_t gate_act, double eps, bool quantize) {
+  const char* op = "residual_norm";
+  QF_REFUSE_UNLESS(x.dim() >= 1, op, ": x must have at least one dimension");
+  check_type(op, "x", x, at::kBFloat16);
+  if (given(residual)) {
+    QF_REFUSE_UNLESS(residual->scalar_type() == at::kBFloat16 || residual->scalar_type() == at::kFloat, op,
+                     ": residual must be bf16 or fp32");
+    check_same_sizes(op, "residual", *residual, x);
+  }
+  for (const auto& [name, w] : {std::make_pair("pre_weight", &pre_weight), std::make_pair("post_weight", &post_weight)})
+    if (given(*w)) {
+      check_type(op, name, **w, at::kBFloat16);
+      QF_REFUSE_UNLESS((*w)->dim() == 1, op, ": ", name, " must be [", x.sym_size(-1), "]");
+      QF_REFUSE_UNLESS_EQ((*w)->sym_size(0), x.sym_size(-1), op, ": ", name, " must be [", x.sym_size(-1), "]");
+    }
+  QF_REFUSE_UNLESS(!quantize || given(pre_weight), op, ": quantize needs pre_weight");
+  QF_REFUSE_UNLESS(gate_act >= QF_GATE_NONE && gate_act <= QF_GATE_SILU, op, ": unknown gate activation");
+  if (given(gate)) {
+    check_type(op, "gate", *gate, at::kBFloat16);
+    QF_REFUSE_UNLESS(gate->dim() <= x.dim(), op, ": gate has more dimensions than x");
+    for (int64_t i = 1; i <= gate->dim(); ++i) {
+      const std::optional<int64_t> g = gate->sym_size(-i).maybe_as_int();
+      if (!g || *g != 1)
+        QF_REFUSE_UNLESS_EQ(gate->sym_size(-i), x.sym_size(-i), op, ": gate ", gate->sym_sizes(), " does not broadcast to ",
+                            x.sym_sizes());
+    }
+  } else {
+    QF_REFUSE_UNLESS(gate_act == QF_GATE_NONE, op, ": a gate activation without a gate");
+  }
+  QF_REFUSE_UNLESS(eps >= 0 && eps <= 3.4e38, op, ": eps must be finite and >= 0");
 }
 
 cudaStream_t stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
@@ -231,35 +337,28 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x2, bool silu
 }
 
 std::tuple<at::Tensor, at::Tensor> fp8_quantize(const at::Tensor& x, bool silu_mul) {
-  QF_REFUSE_UNLESS(x.dim() >= 1, "fp8_quantize: x must have at least one dimension");
-  QF_REFUSE_UNLESS(!silu_mul || x.size(-1) % 2 == 0, "fp8_quantize: silu_mul needs gate and up halves of one width");
+  check_quantize_shapes(x, silu_mul);
   const int64_t K = silu_mul ? x.size(-1) / 2 : x.size(-1);
   QF_REFUSE_UNLESS(K >= 1 && K <= QF_FP8_MAX_K, "fp8_quantize: 1 to ", QF_FP8_MAX_K, " values per row, got ", K);
-  check_input("fp8_quantize", "x", x, at::kBFloat16, x.device());
+  check_input("fp8_quantize", "x", x, x.device());
   check_groups("fp8_quantize", rows_of(x), K);
   c10::cuda::CUDAGuard guard(x.device());
   auto [q, s] = quantize_rows(as_rows(x), silu_mul);
   return {with_leading(q, x), with_leading(s, x)};
 }
 
-void check_weight(const char* op, const at::Tensor& w_t, const at::Tensor& w_scale, const OptTensor& bias, int64_t K,
+void check_weight(const char* op, const at::Tensor& w_t, const at::Tensor& w_scale, const OptTensor& bias,
                   const at::Device& dev) {
-  check_input(op, "w_t", w_t, at::kFloat8_e4m3fn, dev);
-  QF_REFUSE_UNLESS(w_t.dim() == 2 && w_t.size(0) == K, op, ": w_t must be [K, N] with K = ", K, ", got ", w_t.sizes());
-  const int64_t N = w_t.size(1);
+  check_input(op, "w_t", w_t, dev);
+  const int64_t K = w_t.size(0), N = w_t.size(1);
   QF_REFUSE_UNLESS(K >= 1 && K <= QF_FP8_MAX_K && N <= QF_MAX_N, op, ": K must be 1 to ", QF_FP8_MAX_K,
                    " and N at most ", QF_MAX_N);
   QF_REFUSE_UNLESS((K == 1 || w_t.stride(0) == 1) && (N <= 1 || (w_t.stride(1) >= K && w_t.stride(1) % 16 == 0)) &&
                        reinterpret_cast<uintptr_t>(w_t.data_ptr()) % 16 == 0,
                    op, ": w_t must be the [K, N] view of 16-byte aligned rows of a weight (stride (1, ldw), ldw a multiple "
                    "of 16)");
-  check_input(op, "w_scale", w_scale, at::kFloat, dev);
-  QF_REFUSE_UNLESS(w_scale.dim() == 2 && w_scale.size(0) == blocks(N) && w_scale.size(1) == blocks(K), op,
-                   ": w_scale must be [", blocks(N), ", ", blocks(K), "], got ", w_scale.sizes());
-  if (given(bias)) {
-    check_input(op, "bias", *bias, at::kBFloat16, dev);
-    QF_REFUSE_UNLESS(bias->numel() == N, op, ": bias must hold ", N, " values");
-  }
+  check_input(op, "w_scale", w_scale, dev);
+  if (given(bias)) check_input(op, "bias", *bias, dev);
 }
 
 void run_mm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t,
@@ -278,14 +377,11 @@ void run_mm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_
 
 void check_mm(const char* op, const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t, const at::Tensor& w_scale,
               const OptTensor& bias) {
-  QF_REFUSE_UNLESS(a.dim() == 2, op, ": a must be [M, K]");
-  check_input(op, "a", a, at::kFloat8_e4m3fn, a.device());
-  const int64_t M = a.size(0), K = a.size(1);
-  check_weight(op, w_t, w_scale, bias, K, a.device());
-  check_input(op, "a_scale", a_scale, at::kFloat, a.device());
-  QF_REFUSE_UNLESS(a_scale.dim() == 2 && a_scale.size(0) == M && a_scale.size(1) == blocks(K), op, ": a_scale must be [",
-                   M, ", ", blocks(K), "], got ", a_scale.sizes());
-  check_rows(op, M, w_t.size(1));
+  check_mm_shapes(op, a, a_scale, w_t, w_scale, bias);
+  check_input(op, "a", a, a.device());
+  check_weight(op, w_t, w_scale, bias, a.device());
+  check_input(op, "a_scale", a_scale, a.device());
+  check_rows(op, a.size(0), w_t.size(1));
 }
 
 // a with rows that the product's tensor maps take, copied where they are not.
@@ -314,11 +410,10 @@ void fp8_block_mm_out(const at::Tensor& a, const at::Tensor& a_scale, const at::
   const char* op = "fp8_block_mm";
   c10::cuda::OptionalCUDAGuard guard(a.is_cuda() ? c10::optional<c10::Device>(a.device()) : c10::nullopt);
   check_mm(op, a, a_scale, w_t, w_scale, bias);
+  check_out_shapes(op, out, a, w_t);
   const int64_t M = a.size(0), N = w_t.size(1);
-  QF_REFUSE_UNLESS(out.device() == a.device() && out.dim() == 2 && out.size(0) == M && out.size(1) == N &&
-                       (out.scalar_type() == at::kFloat || out.scalar_type() == at::kBFloat16) &&
-                       (N == 1 || out.stride(1) == 1) && (M <= 1 || out.stride(0) >= N),
-                   op, ": out must be bf16 or fp32 [", M, ", ", N, "] on a's device with unit column stride");
+  QF_REFUSE_UNLESS(out.device() == a.device() && (N == 1 || out.stride(1) == 1) && (M <= 1 || out.stride(0) >= N), op,
+                   ": out must be on a's device with unit column stride and rows that do not overlap");
   check_no_overlap(op, "out", out, "a", a);
   check_no_overlap(op, "out", out, "a_scale", a_scale);
   check_no_overlap(op, "out", out, "w_t", w_t);
@@ -329,9 +424,9 @@ void fp8_block_mm_out(const at::Tensor& a, const at::Tensor& a_scale, const at::
 
 at::Tensor fp8_block_linear(const at::Tensor& x, const at::Tensor& w_t, const at::Tensor& w_scale, const OptTensor& bias) {
   const char* op = "fp8_block_linear";
-  QF_REFUSE_UNLESS(x.dim() >= 1, op, ": x must have at least one dimension");
-  check_input(op, "x", x, at::kBFloat16, x.device());
-  check_weight(op, w_t, w_scale, bias, x.size(-1), x.device());
+  check_linear_shapes(op, x, w_t, w_scale, bias);
+  check_input(op, "x", x, x.device());
+  check_weight(op, w_t, w_scale, bias, x.device());
   check_groups(op, rows_of(x), x.size(-1));
   check_rows(op, rows_of(x), w_t.size(1));
   c10::cuda::CUDAGuard guard(x.device());
@@ -389,35 +484,15 @@ std::tuple<at::Tensor, at::Tensor> run_norm(const at::Tensor& x, const OptTensor
 void check_norm(const at::Tensor& x, const OptTensor& residual, const OptTensor& pre_weight, const OptTensor& post_weight,
                 const OptTensor& gate, int64_t gate_act, double eps, bool quantize) {
   const char* op = "residual_norm";
-  QF_REFUSE_UNLESS(x.dim() >= 1, op, ": x must have at least one dimension");
-  check_input(op, "x", x, at::kBFloat16, x.device());
+  check_norm_shapes(x, residual, pre_weight, post_weight, gate, gate_act, eps, quantize);
+  check_input(op, "x", x, x.device());
   const int64_t H = x.size(-1);
   QF_REFUSE_UNLESS(H >= 1 && H <= QF_NORM_MAX_H, op, ": rows of 1 to ", QF_NORM_MAX_H, " values, got ", H);
   QF_REFUSE_UNLESS(rows_of(x) <= INT32_MAX, op, ": ", rows_of(x), " rows are too many");
-  if (given(residual)) {
-    QF_REFUSE_UNLESS(residual->scalar_type() == at::kBFloat16 || residual->scalar_type() == at::kFloat, op,
-                     ": residual must be bf16 or fp32");
-    check_input(op, "residual", *residual, residual->scalar_type(), x.device());
-    QF_REFUSE_UNLESS(residual->sizes() == x.sizes(), op, ": residual must have x's shape ", x.sizes(), ", got ",
-                     residual->sizes());
-  }
-  for (const auto& [name, w] : {std::make_pair("pre_weight", &pre_weight), std::make_pair("post_weight", &post_weight)})
-    if (given(*w)) {
-      check_input(op, name, **w, at::kBFloat16, x.device());
-      QF_REFUSE_UNLESS((*w)->dim() == 1 && (*w)->size(0) == H, op, ": ", name, " must be [", H, "]");
-    }
-  QF_REFUSE_UNLESS(!quantize || given(pre_weight), op, ": quantize needs pre_weight");
-  QF_REFUSE_UNLESS(gate_act >= QF_GATE_NONE && gate_act <= QF_GATE_SILU, op, ": unknown gate activation");
-  if (given(gate)) {
-    check_input(op, "gate", *gate, at::kBFloat16, x.device());
-    QF_REFUSE_UNLESS(gate->dim() <= x.dim(), op, ": gate has more dimensions than x");
-    for (int64_t i = 1; i <= gate->dim(); ++i)
-      QF_REFUSE_UNLESS(gate->size(-i) == 1 || gate->size(-i) == x.size(-i), op, ": gate ", gate->sizes(),
-                       " does not broadcast to ", x.sizes());
-  } else {
-    QF_REFUSE_UNLESS(gate_act == QF_GATE_NONE, op, ": a gate activation without a gate");
-  }
-  QF_REFUSE_UNLESS(eps >= 0 && eps <= 3.4e38, op, ": eps must be finite and >= 0");
+  if (given(residual)) check_input(op, "residual", *residual, x.device());
+  if (given(pre_weight)) check_input(op, "pre_weight", *pre_weight, x.device());
+  if (given(post_weight)) check_input(op, "post_weight", *post_weight, x.device());
+  if (given(gate)) check_input(op, "gate", *gate, x.device());
 }
 
 std::tuple<OptTensor, OptTensor, at::Tensor> residual_norm(const at::Tensor& x, const OptTensor& residual,
@@ -440,8 +515,9 @@ std::tuple<OptTensor, OptTensor> residual_norm_out(const at::Tensor& x, const Op
   const char* op = "residual_norm";
   check_norm(x, residual, pre_weight, post_weight, gate, gate_act, eps, quantize);
   const at::ScalarType type = given(residual) ? residual->scalar_type() : at::kBFloat16;
-  check_input(op, "residual_out", residual_out, type, x.device());
-  QF_REFUSE_UNLESS(residual_out.sizes() == x.sizes(), op, ": residual_out must have x's shape ", x.sizes());
+  check_type(op, "residual_out", residual_out, type);
+  check_input(op, "residual_out", residual_out, x.device());
+  check_same_sizes(op, "residual_out", residual_out, x);
   const int64_t H = x.size(-1);
   QF_REFUSE_UNLESS((H == 1 || residual_out.stride(-1) == 1) && (residual_out.dim() == 2 || residual_out.is_contiguous()) &&
                        (residual_out.dim() != 2 || residual_out.size(0) <= 1 || residual_out.stride(0) >= H),
@@ -460,45 +536,61 @@ std::tuple<OptTensor, OptTensor> residual_norm_out(const at::Tensor& x, const Op
   return {h.defined() ? OptTensor(h) : c10::nullopt, s.defined() ? OptTensor(s) : c10::nullopt};
 }
 
-// Shapes and types only, for tracing: the same leading dimensions, e4m3 rows of 16-byte stride.
-at::Tensor meta_rows(const at::Tensor& x, int64_t K) {
-  std::vector<int64_t> s(x.sizes().begin(), x.sizes().end());
+// Types and shapes only, for tracing: the same refusals of them, the same leading dimensions (which may be symbolic), e4m3
+// rows of 16-byte stride.
+at::Tensor meta_rows(const at::Tensor& x, const c10::SymInt& K) {
+  std::vector<c10::SymInt> s = x.sym_sizes().vec();
   s.back() = (K + 15) / 16 * 16;
-  at::Tensor q = at::empty(s, x.options().dtype(at::kFloat8_e4m3fn));
-  return K % 16 ? q.narrow(-1, 0, K) : q;
+  at::Tensor q = at::empty_symint(s, x.options().dtype(at::kFloat8_e4m3fn));
+  const std::optional<int64_t> k = K.maybe_as_int();
+  return k && *k % 16 == 0 ? q : q.narrow_symint(-1, 0, K);
 }
-at::Tensor meta_like(const at::Tensor& x, int64_t last, at::ScalarType type) {
-  std::vector<int64_t> s(x.sizes().begin(), x.sizes().end());
+at::Tensor meta_like(const at::Tensor& x, const c10::SymInt& last, at::ScalarType type) {
+  std::vector<c10::SymInt> s = x.sym_sizes().vec();
   s.back() = last;
-  return at::empty(s, x.options().dtype(type));
+  return at::empty_symint(s, x.options().dtype(type));
 }
 std::tuple<at::Tensor, at::Tensor> fp8_quantize_meta(const at::Tensor& x, bool silu_mul) {
-  const int64_t K = silu_mul ? x.size(-1) / 2 : x.size(-1);
+  check_quantize_shapes(x, silu_mul);
+  const c10::SymInt K = silu_mul ? x.sym_size(-1) / 2 : x.sym_size(-1);
   return {meta_rows(x, K), meta_like(x, blocks(K), at::kFloat)};
 }
-at::Tensor fp8_block_mm_meta(const at::Tensor& a, const at::Tensor&, const at::Tensor& w_t, const at::Tensor&,
-                             const OptTensor&, bool out_f32) {
-  return meta_like(a, w_t.size(1), out_f32 ? at::kFloat : at::kBFloat16);
+at::Tensor fp8_block_mm_meta(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t, const at::Tensor& w_scale,
+                             const OptTensor& bias, bool out_f32) {
+  check_mm_shapes("fp8_block_mm", a, a_scale, w_t, w_scale, bias);
+  return meta_like(a, w_t.sym_size(1), out_f32 ? at::kFloat : at::kBFloat16);
 }
-void fp8_block_mm_out_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
-                           at::Tensor) {}
-at::Tensor fp8_block_linear_meta(const at::Tensor& x, const at::Tensor& w_t, const at::Tensor&, const OptTensor&) {
-  return meta_like(x, w_t.size(1), at::kBFloat16);
+void fp8_block_mm_out_meta(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t, const at::Tensor& w_scale,
+                           const OptTensor& bias, at::Tensor out) {
+  check_mm_shapes("fp8_block_mm", a, a_scale, w_t, w_scale, bias);
+  check_out_shapes("fp8_block_mm", out, a, w_t);
 }
-std::tuple<OptTensor, OptTensor> residual_norm_out_meta(const at::Tensor& x, const OptTensor&, const OptTensor& pre_weight,
-                                                        const OptTensor&, const OptTensor&, int64_t, double, double, double,
-                                                        bool quantize, at::Tensor) {
+at::Tensor fp8_block_linear_meta(const at::Tensor& x, const at::Tensor& w_t, const at::Tensor& w_scale, const OptTensor& bias) {
+  check_linear_shapes("fp8_block_linear", x, w_t, w_scale, bias);
+  return meta_like(x, w_t.sym_size(1), at::kBFloat16);
+}
+// (h, scale) of a call without refusals left.
+std::tuple<OptTensor, OptTensor> meta_h(const at::Tensor& x, const OptTensor& pre_weight, bool quantize) {
   if (!given(pre_weight)) return {c10::nullopt, c10::nullopt};
-  if (!quantize) return {meta_like(x, x.size(-1), at::kBFloat16), c10::nullopt};
-  return {meta_rows(x, x.size(-1)), meta_like(x, blocks(x.size(-1)), at::kFloat)};
+  if (!quantize) return {meta_like(x, x.sym_size(-1), at::kBFloat16), c10::nullopt};
+  return {meta_rows(x, x.sym_size(-1)), meta_like(x, blocks(x.sym_size(-1)), at::kFloat)};
+}
+std::tuple<OptTensor, OptTensor> residual_norm_out_meta(const at::Tensor& x, const OptTensor& residual,
+                                                        const OptTensor& pre_weight, const OptTensor& post_weight,
+                                                        const OptTensor& gate, int64_t gate_act, double, double, double eps,
+                                                        bool quantize, at::Tensor residual_out) {
+  check_norm_shapes(x, residual, pre_weight, post_weight, gate, gate_act, eps, quantize);
+  check_type("residual_norm", "residual_out", residual_out, given(residual) ? residual->scalar_type() : at::kBFloat16);
+  check_same_sizes("residual_norm", "residual_out", residual_out, x);
+  return meta_h(x, pre_weight, quantize);
 }
 std::tuple<OptTensor, OptTensor, at::Tensor> residual_norm_meta(const at::Tensor& x, const OptTensor& residual,
                                                                 const OptTensor& pre_weight, const OptTensor& post_weight,
-                                                                const OptTensor& gate, int64_t act, double scale, double offset,
+                                                                const OptTensor& gate, int64_t gate_act, double, double,
                                                                 double eps, bool quantize) {
-  at::Tensor r = meta_like(x, x.size(-1), given(residual) ? residual->scalar_type() : at::kBFloat16);
-  auto [h, s] = residual_norm_out_meta(x, residual, pre_weight, post_weight, gate, act, scale, offset, eps, quantize, r);
-  return {h, s, r};
+  check_norm_shapes(x, residual, pre_weight, post_weight, gate, gate_act, eps, quantize);
+  auto [h, s] = meta_h(x, pre_weight, quantize);
+  return {h, s, meta_like(x, x.sym_size(-1), given(residual) ? residual->scalar_type() : at::kBFloat16)};
 }
 
 }  // namespace
