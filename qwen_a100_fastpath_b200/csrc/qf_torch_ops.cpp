@@ -12,9 +12,10 @@
 // torch.ops.qf_b200.fp8_quantize / fp8_block_mm / fp8_block_linear / residual_norm are the operators of block-scaled fp8
 // layers (fp8.py and norms.py document them).  They need no workspace: what they make comes from the caching allocator,
 // so calls on several streams, and captured graphs, share nothing.  They refuse a call with a ValueError before anything
-// is launched, and inputs that require a gradient too: none of them has a backward.
+// is launched, and tensors that require a gradient or carry a tangent too: none of them has a derivative.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -128,8 +129,30 @@ void check_type(const char* op, const char* name, const at::Tensor& t, at::Scala
 void check_input(const char* op, const char* name, const at::Tensor& t, const at::Device& dev) {
   QF_REFUSE_UNLESS(t.is_cuda(), op, ": ", name, " must be a CUDA tensor (there is no CPU path)");
   QF_REFUSE_UNLESS(t.device() == dev, op, ": ", name, " is on ", t.device(), ", the first input on ", dev);
-  QF_REFUSE_UNLESS(!(at::GradMode::is_enabled() && t.requires_grad()), op, ": ", name,
-                   " requires a gradient and the operator has no backward (call it under torch.no_grad())");
+}
+
+// In the place of torch's fallback for operators without a backward: refuses tensors that want a derivative, outputs among
+// them, and goes on to the operator.  Here the derivatives of torch.func's transformations can be seen too.
+void refuse_derivatives(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+  const bool backward = at::GradMode::is_enabled();
+  const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  const size_t n = op.schema().arguments().size();
+  for (size_t i = 0; i < n; ++i) {
+    const c10::IValue& v = (*stack)[stack->size() - n + i];
+    if (!v.isTensor()) continue;
+    const at::Tensor& t = v.toTensor();
+    if (!t.defined()) continue;
+    QF_REFUSE_UNLESS(!(backward && t.requires_grad()), op.schema().name(), ": ", op.schema().arguments()[i].name(),
+                     " requires a gradient and the operator has no backward (call it under torch.no_grad())");
+    QF_REFUSE_UNLESS(!(forward && t._fw_grad(0).defined()), op.schema().name(), ": ", op.schema().arguments()[i].name(),
+                     " has a forward-mode tangent and the operator has no derivative");
+  }
+  op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
+}
+
+// A tensor was written: autograd tells by its version where a value it kept is no longer there.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 // ---- types and shapes, of real calls and of traced ones (whose sizes may be symbolic) ----
@@ -420,6 +443,7 @@ void fp8_block_mm_out(const at::Tensor& a, const at::Tensor& a_scale, const at::
   check_no_overlap(op, "out", out, "w_scale", w_scale);
   if (given(bias)) check_no_overlap(op, "out", out, "bias", *bias);
   run_mm(aligned_rows(a), a_scale, w_t, w_scale, bias, out);
+  written(out);
 }
 
 at::Tensor fp8_block_linear(const at::Tensor& x, const at::Tensor& w_t, const at::Tensor& w_scale, const OptTensor& bias) {
@@ -533,6 +557,7 @@ std::tuple<OptTensor, OptTensor> residual_norm_out(const at::Tensor& x, const Op
   c10::cuda::CUDAGuard guard(x.device());
   auto [h, s] = run_norm(x, residual, pre_weight, post_weight, gate, gate_act, residual_scale, weight_offset, eps, quantize,
                          residual_out);
+  written(residual_out);
   return {h.defined() ? OptTensor(h) : c10::nullopt, s.defined() ? OptTensor(s) : c10::nullopt};
 }
 
@@ -564,6 +589,7 @@ void fp8_block_mm_out_meta(const at::Tensor& a, const at::Tensor& a_scale, const
                            const OptTensor& bias, at::Tensor out) {
   check_mm_shapes("fp8_block_mm", a, a_scale, w_t, w_scale, bias);
   check_out_shapes("fp8_block_mm", out, a, w_t);
+  written(out);
 }
 at::Tensor fp8_block_linear_meta(const at::Tensor& x, const at::Tensor& w_t, const at::Tensor& w_scale, const OptTensor& bias) {
   check_linear_shapes("fp8_block_linear", x, w_t, w_scale, bias);
@@ -582,6 +608,7 @@ std::tuple<OptTensor, OptTensor> residual_norm_out_meta(const at::Tensor& x, con
   check_norm_shapes(x, residual, pre_weight, post_weight, gate, gate_act, eps, quantize);
   check_type("residual_norm", "residual_out", residual_out, given(residual) ? residual->scalar_type() : at::kBFloat16);
   check_same_sizes("residual_norm", "residual_out", residual_out, x);
+  written(residual_out);
   return meta_h(x, pre_weight, quantize);
 }
 std::tuple<OptTensor, OptTensor, at::Tensor> residual_norm_meta(const at::Tensor& x, const OptTensor& residual,
@@ -615,6 +642,11 @@ TORCH_LIBRARY_IMPL(qf_b200, CompositeExplicitAutograd, m) {
   m.impl("fp8_block_linear", fp8_block_linear);
   m.impl("residual_norm", residual_norm);
   m.impl("residual_norm_out", residual_norm_out);
+}
+TORCH_LIBRARY_IMPL(qf_b200, Autograd, m) {
+  for (const char* op : {"fp8_quantize", "fp8_block_mm", "fp8_block_mm_out", "fp8_block_linear", "residual_norm",
+                         "residual_norm_out"})
+    m.impl(op, torch::CppFunction::makeFromBoxedFunction<&refuse_derivatives>());
 }
 TORCH_LIBRARY_IMPL(qf_b200, CUDA, m) { m.impl("int8_linear", int8_linear); }
 TORCH_LIBRARY_IMPL(qf_b200, Meta, m) {

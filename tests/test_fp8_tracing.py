@@ -105,3 +105,47 @@ def test_refusals_of_types_and_shapes():
         with pytest.raises(ValueError):
             f()
             pytest.fail(f"case {i} was taken")
+
+
+def test_written_outputs_raise_their_version():
+    m = "meta"
+    x, r = torch.empty(4, 256, dtype=BF16, device=m), torch.empty(4, 256, device=m)
+    norms.residual_norm(x, r, None, residual_out=r)
+    assert r._version == 1 and r[:2]._version == 1
+    a, sa = fp8.fp8_quantize(x)
+    out = torch.empty(8, 300, device=m)
+    fp8.fp8_block_mm(a, sa, torch.empty(300, 256, dtype=E4M3, device=m).t(), torch.empty(3, 2, device=m), out=out[2:6])
+    assert out._version == 1 and a._version == 0 and x._version == 0
+
+
+def test_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwd
+    m = "meta"
+    x, n = torch.empty(4, 256, dtype=BF16, device=m), torch.empty(256, dtype=BF16, device=m)
+    r = torch.empty(4, 256, device=m)
+    a, sa = fp8.fp8_quantize(x)
+    w, sw = torch.empty(300, 256, dtype=E4M3, device=m).t(), torch.empty(3, 2, device=m)
+    leaf = n.clone().requires_grad_()
+    out = torch.empty(4, 300, device=m, requires_grad=True)
+    with pytest.raises(ValueError, match="requires a gradient"):
+        norms.residual_norm(x, r, leaf)
+    for t in (out, out * 1):
+        with pytest.raises(ValueError, match="out requires a gradient"):
+            fp8.fp8_block_mm(a, sa, w, sw, out=t)
+    with torch.no_grad():
+        norms.residual_norm(x, r, leaf)
+        fp8.fp8_block_mm(a, sa, w, sw, out=out)
+    with torch.inference_mode():
+        norms.residual_norm(x, r, leaf, residual_out=torch.empty(4, 256, device=m))
+    kept = torch.inference_mode()(lambda: torch.empty(4, 256, device=m))()
+    norms.residual_norm(x, r, n, residual_out=kept)              # an inference tensor has no version
+    with fwd.dual_level():
+        with pytest.raises(ValueError, match="tangent"):
+            fp8.fp8_quantize(fwd.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(ValueError, match="tangent"):
+            norms.residual_norm(x, fwd.make_dual(r, torch.ones_like(r)), n)
+    f = lambda t: fp8.fp8_quantize(t)[1].sum()  # noqa: E731
+    with pytest.raises(ValueError, match="tangent"):
+        torch.func.jvp(f, (x,), (torch.ones_like(x),))
+    with pytest.raises(ValueError, match="requires a gradient"):
+        torch.func.grad(f)(x)

@@ -96,3 +96,26 @@ def test_operands_written_by_the_kernel_before(dev, M):
     want, got = chain(True), chain(False)
     for a, b in zip(got, want):
         assert torch.equal(a.nan_to_num(), b.nan_to_num()) and torch.isfinite(b).any()
+
+
+def test_autograd_notices_written_outputs(dev):
+    """A value that autograd kept for a backward pass and that an operator then overwrites is noticed, as with torch's own
+    in-place operators."""
+    import torch
+    from qwen_a100_fastpath_b200.fp8 import fp8_block_mm, fp8_quantize
+    from qwen_a100_fastpath_b200.norms import residual_norm
+    leaf = torch.ones(4, 256, device=dev, requires_grad=True)
+    x = torch.ones(4, 256, device=dev, dtype=torch.bfloat16)
+    a, sa = fp8_quantize(x)
+    w = torch.ones(256, 256, device=dev).to(torch.float8_e4m3fn).t()
+    for write in (lambda r: residual_norm(x, r, x[0], residual_out=r),
+                  lambda r: fp8_block_mm(a, sa, w, torch.ones(2, 2, device=dev), out=r)):
+        kept = leaf.exp()                              # its backward needs the value itself
+        write(kept.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            kept.sum().backward()
+        with pytest.raises(ValueError, match="requires a gradient"):
+            write(leaf.exp())
+        with pytest.raises(ValueError, match="requires a gradient"):
+            write(leaf)
+    assert (leaf == 1).all()
