@@ -339,7 +339,10 @@ constexpr int kScaleK = 8, kScaleBufs = 3;
 
 constexpr int kMaxStages = 12;
 
-template <int BN, int EW, bool SPLIT> struct TileGeo {
+constexpr int kEpiWarps = 8;  // two for each tensor-memory quarter
+
+template <int BN, bool SPLIT> struct TileGeo {
+  static constexpr int EW = kEpiWarps;
   static constexpr int kThreads = 128 + 32 * EW;
   static constexpr int kBBytes = BN * kFp8Block;
   // a stage: the weight tile, then the token rows of the tile (fewer than 128 where the call has fewer)
@@ -355,7 +358,6 @@ template <int BN, int EW, bool SPLIT> struct TileGeo {
   // a chunk: [group][epilogue thread], then per epilogue warp [group][one of its two weight blocks]
   static constexpr int kScaleBuf = kScaleK * (32 * EW + 2 * EW);
   static constexpr int kSmemBytes = kOffScale + kScaleBufs * kScaleBuf * 4 + 1024;
-  static_assert(EW == 4 || EW == 8, "one or two warps per tensor-memory quarter");
   static_assert(kCols % 32 == 0 && kCols <= 128, "columns per epilogue thread");
   static_assert(kRing / (kBBytes + kTileM * kFp8Block) >= 4 && kSmemBytes <= 227 * 1024, "shared memory");
   static_assert(!SPLIT || kTileM * BN * 4 <= kRing, "the partial tile reuses the ring");
@@ -418,12 +420,12 @@ __device__ __forceinline__ void store8(const TileParams& tp, int m, int n, const
   }
 }
 
-template <int BN, int EW, bool SPLIT>
-__global__ void __launch_bounds__(128 + 32 * EW, 1)
+template <int BN, bool SPLIT>
+__global__ void __launch_bounds__(128 + 32 * kEpiWarps, 1)
     fp8_tile_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                     const __grid_constant__ TileParams tp) {
-  using C = TileGeo<BN, EW, SPLIT>;
-  constexpr int A = C::kAccs;
+  using C = TileGeo<BN, SPLIT>;
+  constexpr int A = C::kAccs, EW = kEpiWarps;
   const int S = tp.stages;
   const uint32_t stage_bytes = C::kBBytes + static_cast<uint32_t>(tp.box_rows) * kFp8Block;
   const Fp8Params& p = tp.p;
@@ -750,14 +752,14 @@ int encode_rows(CUtensorMap* map, const void* base, int K, int rows, int64_t row
   return QF_OK;
 }
 
-template <int BN, int EW, bool SPLIT>
+template <int BN, bool SPLIT>
 int launch_tiles(TileParams tp, int dev, int sms, int splits, unsigned flags, cudaStream_t st) {
-  using C = TileGeo<BN, EW, SPLIT>;
+  using C = TileGeo<BN, SPLIT>;
   static bool attr_set[64] = {};
   {
     std::lock_guard<std::mutex> lk(g_dev_mu);
     if (!attr_set[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(fp8_tile_kernel<BN, EW, SPLIT>,
+      const cudaError_t e = cudaFuncSetAttribute(fp8_tile_kernel<BN, SPLIT>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
       if (e != cudaSuccess) return fail(QF_ERR_LAUNCH, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
       attr_set[dev] = true;
@@ -800,7 +802,7 @@ int launch_tiles(TileParams tp, int dev, int sms, int splits, unsigned flags, cu
   }
   cfg.attrs = attr;
   cfg.numAttrs = static_cast<unsigned>(na);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_tile_kernel<BN, EW, SPLIT>, ta, tw, tp);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_tile_kernel<BN, SPLIT>, ta, tw, tp);
   return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
 }
 
@@ -874,7 +876,7 @@ int resident_clusters(int dev, int sms, int split) {
   static int known[64][9] = {};
   std::lock_guard<std::mutex> lk(g_dev_mu);
   if (known[dev][split] == 0) {
-    using C = TileGeo<128, 8, true>;
+    using C = TileGeo<128, true>;
     int n = 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(split * sms));
@@ -887,9 +889,9 @@ int resident_clusters(int dev, int sms, int split) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaFuncSetAttribute(fp8_tile_kernel<128, 8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(fp8_tile_kernel<128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          C::kSmemBytes);
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, fp8_tile_kernel<128, 8, true>, &cfg);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, fp8_tile_kernel<128, true>, &cfg);
     if (e != cudaSuccess) {
       (void)cudaGetLastError();
       n = 0;
@@ -920,13 +922,13 @@ int tiles_any(const TileParams& tp, int dev, int sms, unsigned flags, cudaStream
     }
   }
   if (best_split > 1) {
-    if (best_bn == 64) return launch_tiles<64, 8, true>(tp, dev, sms, best_split, flags, st);
-    if (best_bn == 128) return launch_tiles<128, 8, true>(tp, dev, sms, best_split, flags, st);
-    return launch_tiles<256, 8, true>(tp, dev, sms, best_split, flags, st);
+    if (best_bn == 64) return launch_tiles<64, true>(tp, dev, sms, best_split, flags, st);
+    if (best_bn == 128) return launch_tiles<128, true>(tp, dev, sms, best_split, flags, st);
+    return launch_tiles<256, true>(tp, dev, sms, best_split, flags, st);
   }
-  if (best_bn == 64) return launch_tiles<64, 8, false>(tp, dev, sms, 1, flags, st);
-  if (best_bn == 128) return launch_tiles<128, 8, false>(tp, dev, sms, 1, flags, st);
-  return launch_tiles<256, 8, false>(tp, dev, sms, 1, flags, st);
+  if (best_bn == 64) return launch_tiles<64, false>(tp, dev, sms, 1, flags, st);
+  if (best_bn == 128) return launch_tiles<128, false>(tp, dev, sms, 1, flags, st);
+  return launch_tiles<256, false>(tp, dev, sms, 1, flags, st);
 }
 
 }  // namespace
