@@ -252,9 +252,9 @@ int qf_residual_norm(const void* x, int64_t ldx, const void* residual, int64_t l
                      void* residual_out, int64_t ldro, void* out, int64_t ldo, float* out_scale, int64_t lds, int M,
                      int H, unsigned flags, void* stream);
 
-/* Reads and clears the current device's sticky error flag of qf_residual_norm (synchronises `stream`).  A launch of many rows
- * copies rows ahead and waits for each copy for about 4 s at most; one that did not arrive leaves QF_ERR_TIMEOUT here, and
- * its CTA reads that row and all later ones directly: the result is valid.  Not for the hot path. */
+/* Reads and clears the current device's sticky error flag of qf_residual_norm (synchronises `stream`).  A launch of many
+ * rows copies rows ahead and waits for each copy for about 4 s at most; one that did not arrive leaves QF_ERR_TIMEOUT here,
+ * and the threads that waited read that row and all later ones directly: the result is valid.  Not for the hot path. */
 int qf_residual_norm_status(void* stream, int* status);
 
 /* Reads and clears the workspace's sticky device error flag (synchronises `stream`).  *status receives

@@ -27,18 +27,19 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 
-// 1 / (1 + e^-x) of two values.  e^-x = 2^n * 2^f with n = -x * log2(e) rounded to a whole number and f the rest (log2(e) in two
-// parts); 2^f = 1 + f * g(f), g the polynomial of degree 5 through its values at the six Chebyshev nodes of [-1/2, 1/2]
-// (2^f is then 0.16 * 2^-24 off with the coefficients rounded).  The sum is formed as 2^-64 + 2^(n-64) * 2^f, in one
-// rounding, so that neither it nor its reciprocal leaves the normal range before the last product; the reciprocal is the
-// special-function unit's with one Newton step.  Over all bf16 x, which is what the gates are: within 2 * 2^-24 of the value
-// where that is a normal number (1 / (1 + expf(-x)) 2.3 * 2^-24), within half a step where it is subnormal (expf's form is zero
-// from x = -88.7 on, this one from -104).  Above 40 the result is 1; a NaN stays one.  Some 11 instructions a value (packed
-// fp32 pairs), where expf and an IEEE quotient take some thirty (4096 x 17408 with the gate: 76.7 us against 99.6).
+// 1 / (1 + e^-x) of two values.  e^-x = 2^n * 2^f with n = -x * log2(e) rounded to a whole number and f the rest (log2(e)
+// in two parts); 2^f = 1 + f * g(f), g the polynomial of degree 5 through its values at the six Chebyshev nodes of
+// [-1/2, 1/2] (2^f is then 0.16 * 2^-24 off with the coefficients rounded).  The sum is formed as 2^-64 + 2^(n-64) * 2^f,
+// in one rounding, so that neither it nor its reciprocal leaves the normal range before the last product; the reciprocal
+// is the special-function unit's with one Newton step.
+// Over all bf16 x, which is what the gates are: within 2 * 2^-24 of the value where that is a normal number (2.3 * 2^-24 for
+// 1 / (1 + expf(-x))), within half a step where it is subnormal (zero from x = -104 on, expf's form from -88.7).  Above
+// 40 the result is 1; a NaN stays one.  Some 11 instructions a value (packed fp32 pairs), where expf and an IEEE quotient
+// take some thirty (4096 x 17408 with the gate: 76.7 us through the call, 99.6).
 __device__ __forceinline__ float2 sigmoid2(float a, float b) {
   auto both = [](float v) { return pack_f32x2(v, v); };
   const uint64_t x = pack_f32x2(min_nan(max_nan(a, -105.f), 40.f), min_nan(max_nan(b, -105.f), 40.f));
-  // 1.5 * 2^23 rounds a sum to whole numbers; 63 = 127 - 64 makes its low bits the exponent of 2^(n-64), n from -58 to 151
+  // 1.5 * 2^23 rounds a sum to whole numbers; 63 = 127 - 64 makes its low bits the exponent of 2^(n-64), n -58 to 151
   constexpr float kMagic = 12582912.f + 63.f;
   uint64_t t = both(kMagic);
   fma_f32x2(t, x, both(-1.44269502f));      // log2(e) = 1.44269502 + 1.92596303e-8
@@ -59,7 +60,8 @@ __device__ __forceinline__ float2 sigmoid2(float a, float b) {
   fma_f32x2(p, g, f);
   const float2 tf = unpack_f32x2(t);
   uint64_t d = both(0x1p-64f);
-  fma_f32x2(d, p, pack_f32x2(__uint_as_float(__float_as_uint(tf.x) << 23), __uint_as_float(__float_as_uint(tf.y) << 23)));
+  fma_f32x2(d, p,
+            pack_f32x2(__uint_as_float(__float_as_uint(tf.x) << 23), __uint_as_float(__float_as_uint(tf.y) << 23)));
   const float2 df = unpack_f32x2(d);
   float2 r;  // negative, which saves negating d
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(-df.x));

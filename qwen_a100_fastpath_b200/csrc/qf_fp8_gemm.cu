@@ -9,17 +9,20 @@
 // accumulator per k group; two producer and two issuing warps feed it from a ring of TMA stages (128-byte rows, 128-byte
 // swizzle), eight warps add each finished accumulator, times its scales, to fp32 sums in registers while the next
 // groups are multiplied.  With fewer tiles than SMs a cluster shares a tile's groups and adds its parts over distributed
-// shared memory, in rank order.  What bounds it: shared memory's 128 bytes a clock, which a group's copies and operand
-// reads take twice (2 x (16 KiB + BN * 128)), and L2 (11 TB/s at 2048 x 10240 x 5120).  Measured (us, B200): 72 x 10240 x
-// 5120 18.9; 333 x 2600 x 1160 7.0; 2048 x 5120 x 8192 118; 4096 x 34816 x 5120 777 (1.88 PFLOP/s; 900 under the power
-// cap).
+// shared memory, in rank order.  What bounds it with the operands in L2: a group of 64 / 128 / 256 channels takes a CTA
+// 0.30 / 0.38 / 0.52 us, of which shared memory's 128 bytes a clock (copies in, operands out: 2 x (16 KiB + BN * 128)) are
+// 0.20 / 0.26 / 0.39 and the rest, the same at every width, is about one barrier wait.  With weights from DRAM it is
+// slower.  Measured (us, B200, in a graph): 72 x 10240 x 5120 18.5 (40 tiles x 3 CTAs, 2.9 TB/s);
+// 333 x 2600 x 1160 7.9; 2048 x 5120 x 8192 119 (three rounds of tiles, the last of 24); 4096 x 34816 x 5120 767 (1.90
+// PFLOP/s; 915 in a loop under the power cap).
 //
 // fp8_rows_kernel (up to 16): bound by the weights' bytes.  A CTA takes tiles of 16 or 32 weight rows, a producer copies
 // four or eight k groups of them and of the token rows per stage into a ring (one TMA copy each: a copy costs its issuer
 // and the TMA unit the same whatever it moves), and each of four warps multiplies one or two of the stage's groups with
 // mma.sync m16n8k32 (weights as the 16-row operand, so that 8 token columns are not padded to a tcgen05 tile); the
-// warps' sums are added in shared memory in warp order.  Three CTAs per SM keep some 200 KiB in flight.  Measured (us,
-// B200): 1 x 5120 x 8192 11.3; 5 x 34816 x 5120 28.0 (6.4 TB/s); 1 x 5120 x 17408 19.2; 16 x 10240 x 5120 15.0.
+// warps' sums are added in shared memory in warp order.  Three CTAs per SM hold rings of 144 to 192 KiB together, token rows
+// included.  Measured (us, B200, in a graph): 1 x 5120 x 8192 10.5; 5 x 34816 x 5120 29.9 (6.0 TB/s); 1 x 5120 x 17408
+// 18.7; 16 x 10240 x 5120 14.8.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -217,7 +220,8 @@ __global__ void __launch_bounds__(kRowWarps * 32 + 32, kRowPerSm)
           for (int i = 0; i < 2; ++i) r.sa[j][i] = sa_row[j][i][g * p.sa_g];
       };
       float acc[NT][MT][4] = {};
-      auto add = [&](const uint4 (&lo)[MT][2], const uint4 (&hi)[MT][2], const uint4 (&b)[NT][2], const float (&sc)[NT][2]) {
+      auto add = [&](const uint4 (&lo)[MT][2], const uint4 (&hi)[MT][2], const uint4 (&b)[NT][2],
+                     const float (&sc)[NT][2]) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -243,7 +247,8 @@ __global__ void __launch_bounds__(kRowWarps * 32 + 32, kRowPerSm)
         for (int j = 0; j < NT; ++j) sc[j][0] = r.sw * r.sa[j][0], sc[j][1] = r.sw * r.sa[j][1];
       };
       auto stage = [&](int st, RowScales<NT> (&r)[G]) {
-        // the scales of two stages ahead are on their way before the wait (16 x 10240 x 5120 16.9 us; behind the products 18.4)
+        // the scales of two stages ahead are on their way before the wait (16 x 10240 x 5120 through the linear layer 16.9
+        // us; behind the products 18.4)
         float sc[G][NT][2];
 #pragma unroll
         for (int u = 0; u < G; ++u) {
@@ -257,7 +262,8 @@ __global__ void __launch_bounds__(kRowWarps * 32 + 32, kRowPerSm)
         uint4 lo[G][MT][2], hi[G][MT][2], b[G][NT][2];
 #pragma unroll
         for (int u = 0; u < G; ++u) {
-          const uint32_t w_at = base + static_cast<uint32_t>(s * C::kStage + (u * kRowWarps + warp) * (C::kRows * kFp8Block));
+          const uint32_t w_at =
+              base + static_cast<uint32_t>(s * C::kStage + (u * kRowWarps + warp) * (C::kRows * kFp8Block));
           const uint32_t a_at =
               base + static_cast<uint32_t>(s * C::kStage + C::kWBytes + (u * kRowWarps + warp) * (8 * NT * kFp8Block));
 #pragma unroll
@@ -828,7 +834,8 @@ template <int NT, int MT, int G> int launch_rows(const Fp8Params& p, int dev, in
   {
     std::lock_guard<std::mutex> lk(g_dev_mu);
     if (!attr_set[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(fp8_rows_kernel<NT, MT, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+      const cudaError_t e = cudaFuncSetAttribute(fp8_rows_kernel<NT, MT, G>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
       if (e != cudaSuccess) return fail(QF_ERR_LAUNCH, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
       attr_set[dev] = true;
     }
@@ -846,7 +853,8 @@ template <int NT, int MT, int G> int launch_rows(const Fp8Params& p, int dev, in
   // with one more costs nothing, but a last round for a few would
   const int ntiles = (p.N + C::kRows - 1) / C::kRows;
   const int rounds = (ntiles + sms * kRowPerSm - 1) / (sms * kRowPerSm);
-  cfg.gridDim = dim3(static_cast<unsigned>((ntiles + rounds - 1) / rounds), static_cast<unsigned>((p.M + 8 * NT - 1) / (8 * NT)));
+  cfg.gridDim = dim3(static_cast<unsigned>((ntiles + rounds - 1) / rounds),
+                     static_cast<unsigned>((p.M + 8 * NT - 1) / (8 * NT)));
   cfg.blockDim = dim3(kRowWarps * 32 + 32);
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = st;
@@ -862,7 +870,9 @@ template <int NT, int MT, int G> int launch_rows(const Fp8Params& p, int dev, in
 // Tiles of 32 weight rows halve the token rows copied per weight row and the waits per byte, where there are enough of
 // them for two CTAs on every SM (10240 x 5120, 5 tokens: 10.6 us against 12.4; 34816 x 5120: 28.4 against 29.0); fewer
 // rows are better spread thin (5120 x 17408, one token: 16 rows 19.1 us, 32 rows 25.5).  With 16 rows a warp takes two
-// k groups per stage up to 8 tokens (19.1 us against 20.4); above, a stage of that size would leave a ring of two.
+// k groups per stage up to 8 tokens (two stages of 24 KiB; 5120 x 17408, 8 tokens: 18.3 us against 19.6 with one, 8192: 9.8
+// against 10.3); above, the token rows of two groups do not fit the registers (16 tokens: 36.5 us against 26.1 with one
+// and four stages of 16 KiB).
 int rows_any(const Fp8Params& p, int dev, int sms, unsigned flags, cudaStream_t st) {
   const bool wide = (p.N + 31) / 32 >= 2 * sms;
   if (p.M <= 8) return wide ? launch_rows<1, 2, 1>(p, dev, sms, flags, st) : launch_rows<1, 1, 2>(p, dev, sms, flags, st);
@@ -902,8 +912,9 @@ int resident_clusters(int dev, int sms, int split) {
 }
 
 // Tile width and k split.  Time of a choice in microseconds: whole waves of CTAs, each a start and its groups at the
-// measured rate of one CTA (a group of 64 / 128 / 256 channels takes 0.30 / 0.38 / 0.52 us, shared memory's bandwidth),
-// and for a split the join of the parts.
+// measured rate of one CTA with its operands in L2 (a group of 64 / 128 / 256 channels takes 0.30 / 0.38 / 0.52 us), and
+// for a split the join of the parts.  It ranks the choices; where the weights come from DRAM the time itself is longer
+// (72 x 10240 x 5120: 256 channels in three parts, 10.3 us by this model, 18.5 measured).
 int tiles_any(const TileParams& tp, int dev, int sms, unsigned flags, cudaStream_t st) {
   const Fp8Params& p = tp.p;
   const int mt = (p.M + kTileM - 1) / kTileM;

@@ -8,10 +8,11 @@
 //
 // Bound by memory: 2 (4 with the gate) bytes read and 1 written per element, so one pass with everything in registers.
 // Eight threads share a group (16 elements, 32 contiguous bytes each), its maximum is three shuffles, nothing
-// crosses a warp, and the groups of all rows form one flat index, so one row fills as many SMs as it has work for.  Eight
-// CTAs per SM (six with the gate, whose arithmetic needs the registers; what a thread has loaded stays packed until it is used,
-// which keeps it at 40) keep enough loads in flight: 4096 x 17408 takes 34 us (6.2 TB/s), with the gate 77 us through the call
-// (4.7 TB/s; five CTAs 82; unpacked at once 98); one row of 5120 1.5 us.
+// crosses a warp, and the groups of all rows form one flat index, so one row fills as many SMs as it has work for.
+// Eight CTAs per SM, six with the gate: its arithmetic needs the registers, 40 with what a thread has loaded kept packed
+// until it is used.  4096 x 17408 takes 34 us (6.2 TB/s), with the gate 69 us in a graph, 77 through the call (4.7 TB/s;
+// five CTAs 82; what a thread has in flight between its loads and its stores is not enough for the memory's rate); one
+// row of 5120 1.3 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

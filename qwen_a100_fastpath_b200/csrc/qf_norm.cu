@@ -10,10 +10,12 @@
 //
 // Bound by memory for many rows and by two block-wide sums for one.  A CTA takes a row, a thread C pieces of eight
 // consecutive elements, everything stays in registers between the loads and the stores, and each sum is one
-// shuffle tree and one barrier.  Where there are many rows, CTAs walk over them with the weights kept in registers (packed
-// bf16, which saves reading them from L2 once per row) and the next rows arriving in shared memory.  Sixteen threads hold a group of 128, so the quantizer's maximum is four shuffles.
-// Measured (B200): 8192 x 5120 with fp32 residual, full gate and both norms 95..105 us (5.6..6.2 TB/s); with bf16 residual and
-// quantized output alone 66 us (4.4 TB/s, bound by the barriers of a row); one row 3.5 us.
+// shuffle tree and one barrier.  Where there are many rows, CTAs walk over them with the weights kept in registers
+// (packed bf16, which saves reading them from L2 once per row) and the next rows arriving in shared memory.  Sixteen
+// threads hold a group of 128, so the quantizer's maximum is four shuffles.
+// Measured (B200): 8192 x 5120 with fp32 residual, full gate and both norms 94 us in a graph, 97..102 through the call
+// (5.8..6.2 TB/s); with bf16 residual and quantized output alone 65 us (4.5 TB/s: the phases of a row, load, sum, scale and
+// quantize, follow one another on the few CTAs of an SM); one row 3.3 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -188,7 +190,7 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
   };
   if (MODE == kAhead && threadIdx.x == 0)
     for (int s = 0; s < p.stages; ++s)
-      if (blockIdx.x + static_cast<long long>(s) * gridDim.x < p.M) copy_row(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+      if (const long long m = blockIdx.x + static_cast<long long>(s) * gridDim.x; m < p.M) copy_row(m, s);
   uint32_t wpost[C][4], wpre[C][4];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -209,14 +211,14 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
   for (uint32_t m = blockIdx.x; m < static_cast<uint32_t>(p.M); m += gridDim.x, parity ^= 1) {
     // where this row's operands are: in the ring, or in global memory
     const __nv_bfloat16* x = p.x + static_cast<int64_t>(m) * p.ldx;
-    const uint8_t* res = static_cast<const uint8_t*>(p.residual) + (p.residual ? static_cast<int64_t>(m) * p.ldr * (R32 ? 4 : 2) : 0);
+    const uint8_t* res = static_cast<const uint8_t*>(p.residual);
+    if (p.residual) res += static_cast<int64_t>(m) * p.ldr * (R32 ? 4 : 2);
     const __nv_bfloat16* gate = p.gate + (p.gate ? static_cast<int64_t>(m) * p.gate_sm : 0);
     if (MODE == kAhead && left_at < 0) {
-      // A thread whose wait runs out leaves the ring for good and reads this and all later rows from global memory (no thread
-      // but itself writes the elements it reads): the phases of a barrier that it has not seen complete would no longer tell
-      // it anything.  The others go on: a stage is only filled again by thread 0, after it saw the stage's last copy arrive,
-      // so what they wait for is that copy or one that is never issued.  All this costs 2 % of 8192 x 5120 with fp32 residual
-      // and gate (95.7 -> 97.6 us against a wait that goes on regardless; a flag that tells the others to leave 99).
+      // A thread whose wait runs out leaves the ring for good and reads this and all later rows from global memory (no
+      // thread but itself writes the elements it reads): the phases of a barrier that it has not seen complete would no
+      // longer tell it anything.  The others go on: a stage is only filled again by thread 0, after it saw the stage's last
+      // copy arrive, so what they wait for is that copy or one that is never issued.
       bool have = p.wait_clocks ? mbar_try_wait(&full[stage], phase)   // which may suspend the thread for a while
                                 : mbar_test_wait(&full[stage], phase);
       if (!have)
@@ -304,7 +306,8 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
         if (R32)
           store8_f32<VEC>(static_cast<float*>(p.residual_out) + static_cast<int64_t>(m) * p.ldro + e, p.H - e, v[c]);
         else
-          store8_bf16<VEC>(static_cast<__nv_bfloat16*>(p.residual_out) + static_cast<int64_t>(m) * p.ldro + e, p.H - e, v[c]);
+          store8_bf16<VEC>(static_cast<__nv_bfloat16*>(p.residual_out) + static_cast<int64_t>(m) * p.ldro + e, p.H - e,
+                           v[c]);
       }
     }
     float n = 0.f;
@@ -353,8 +356,8 @@ __global__ void __launch_bounds__(MAX_T, MAX_T == 512 ? 1 : C == 1 ? 3 : 2) resi
     }
   }
   if (MODE == kAhead && threadIdx.x == 0 && left_at >= 0) {
-    // the copies still under way land before the shared memory is given up: those of the rows from left_at on for which there
-    // was a stage
+    // the copies still under way land before the shared memory is given up: those of the rows from left_at on for which
+    // there was a stage
     for (int s = 0; s < p.stages && left_at + static_cast<long long>(s) * gridDim.x < p.M; ++s) {
       const long long t0 = clock64();
       while (!mbar_try_wait(&full[stage], phase) && clock64() - t0 < kRowWaitClocks) {
@@ -379,7 +382,8 @@ cudaError_t launch_norm(NormParams p, bool vec, int threads, int dev, int sms, b
                                            cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            static_cast<int>(norm_ring(1)));
       if (e == cudaSuccess)
-        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&known, residual_norm_kernel<C, MAX_T, kAhead, R32, QUANT>, threads, 0);
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&known, residual_norm_kernel<C, MAX_T, kAhead, R32, QUANT>,
+                                                          threads, 0);
       if (e != cudaSuccess) {
         known = 0;
         return e;
@@ -389,7 +393,8 @@ cudaError_t launch_norm(NormParams p, bool vec, int threads, int dev, int sms, b
     }
     per_sm = known;
   }
-  const long long bytes = static_cast<long long>(p.H) * (2 + (p.residual ? (R32 ? 4 : 2) : 0) + (p.gate && p.gate_sh ? 2 : 0));
+  const int per_element = 2 + (p.residual ? (R32 ? 4 : 2) : 0) + (p.gate && p.gate_sh ? 2 : 0);
+  const long long bytes = static_cast<long long>(p.H) * per_element;
   while (per_sm > 1 && norm_ring(per_sm) / bytes < 2) --per_sm;
   p.stages = static_cast<int>(norm_ring(per_sm) / bytes < kMaxRowStages ? norm_ring(per_sm) / bytes : kMaxRowStages);
   const bool ahead = vec && p.stages >= 2 && p.M > 2 * sms * per_sm;
@@ -491,8 +496,8 @@ extern "C" int qf_residual_norm(const void* x, int64_t ldx, const void* residual
   const bool vec = H % 8 == 0 && rows16(x, ldx) && rows16(residual, ldr) && rows16(residual_out, ldro) &&
                    rows16(out, ldo) && (!gate || gate_sh == 0 || rows16(gate, gate_sm)) && aligned(post_weight, 16) &&
                    aligned(pre_weight, 16);
-  // pieces per thread: the fewest that keep the CTA at 320 threads, so that two are resident and one works while the other
-  // is at a barrier; wider rows, of which shared memory holds too few for two CTAs anyway, take up to 512 threads
+  // pieces per thread: the fewest that keep the CTA at 320 threads, so that two are resident and one works while the
+  // other is at a barrier; wider rows, of which shared memory holds too few for two CTAs anyway, take up to 512 threads
   // (4096 x 8192, fp32 residual and gate: 84 us with two pieces on 512 threads, 116 with four on 256)
   const int pieces = (H + 7) / 8;
   const int C = pieces <= 320 ? 1 : pieces <= 1024 ? 2 : 4;
@@ -510,4 +515,6 @@ extern "C" int qf_residual_norm(const void* x, int64_t ldx, const void* residual
   return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
 }
 
-extern "C" int qf_residual_norm_status(void* stream, int* status) { return read_error_word(&g_norm_err, stream, status); }
+extern "C" int qf_residual_norm_status(void* stream, int* status) {
+  return read_error_word(&g_norm_err, stream, status);
+}

@@ -299,7 +299,8 @@ bool overlap(const at::Tensor& ta, const at::Tensor& tb) {
   }
   // walk both upwards, always on with the row that ends first
   int64_t i = 0, j = 0;
-  if (a.step && b.begin > a.begin + a.width) i = (b.begin - a.begin - a.width) / a.step;  // rows that end before the other begins
+  // rows that end before the other begins
+  if (a.step && b.begin > a.begin + a.width) i = (b.begin - a.begin - a.width) / a.step;
   if (b.step && a.begin > b.begin + b.width) j = (a.begin - b.begin - b.width) / b.step;
   while (i < a.rows && j < b.rows) {
     const int64_t pa = a.begin + i * a.step, pb = b.begin + j * b.step;
@@ -353,8 +354,8 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x2, bool silu
   at::Tensor q = empty_rows(M, K, x2);
   at::Tensor s = empty_on(x2, {M, blocks(K)}, at::kFloat);
   if (M && K)
-    check(qf_fp8_quantize(x2.data_ptr(), x2.stride(0), static_cast<int>(M), static_cast<int>(K), silu_mul, q.data_ptr(), q.stride(0),
-                          s.data_ptr<float>(), s.stride(0), QF_FLAG_PDL, stream_of(x2)),
+    check(qf_fp8_quantize(x2.data_ptr(), x2.stride(0), static_cast<int>(M), static_cast<int>(K), silu_mul, q.data_ptr(),
+                          q.stride(0), s.data_ptr<float>(), s.stride(0), QF_FLAG_PDL, stream_of(x2)),
           "qf_fp8_quantize");
   return {q, s};
 }
@@ -398,8 +399,8 @@ void run_mm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_
         "qf_fp8_block_gemm");
 }
 
-void check_mm(const char* op, const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t, const at::Tensor& w_scale,
-              const OptTensor& bias) {
+void check_mm(const char* op, const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t,
+              const at::Tensor& w_scale, const OptTensor& bias) {
   check_mm_shapes(op, a, a_scale, w_t, w_scale, bias);
   check_input(op, "a", a, a.device());
   check_weight(op, w_t, w_scale, bias, a.device());
@@ -493,11 +494,12 @@ std::tuple<at::Tensor, at::Tensor> run_norm(const at::Tensor& x, const OptTensor
   if (M) {
     auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
     auto ld = [](const at::Tensor& t) { return t.defined() ? t.stride(0) : 0; };
-    check(qf_residual_norm(ptr(x2), ld(x2), ptr(r2), ld(r2), r_out.scalar_type() == at::kFloat ? QF_DTYPE_F32 : QF_DTYPE_BF16,
-                           ptr(g2), gm, gh, static_cast<int>(gate_act), ptr(post), ptr(pre),
-                           static_cast<float>(weight_offset), static_cast<float>(residual_scale), static_cast<float>(eps),
-                           ro2.data_ptr(), ro2.stride(0), ptr(h), ld(h), s.defined() ? s.data_ptr<float>() : nullptr, ld(s),
-                           static_cast<int>(M), static_cast<int>(H), QF_FLAG_PDL, stream_of(x)),
+    check(qf_residual_norm(ptr(x2), ld(x2), ptr(r2), ld(r2),
+                           r_out.scalar_type() == at::kFloat ? QF_DTYPE_F32 : QF_DTYPE_BF16, ptr(g2), gm, gh,
+                           static_cast<int>(gate_act), ptr(post), ptr(pre), static_cast<float>(weight_offset),
+                           static_cast<float>(residual_scale), static_cast<float>(eps), ro2.data_ptr(), ro2.stride(0),
+                           ptr(h), ld(h), s.defined() ? s.data_ptr<float>() : nullptr, ld(s), static_cast<int>(M),
+                           static_cast<int>(H), QF_FLAG_PDL, stream_of(x)),
           "qf_residual_norm");
   }
   if (h.defined()) h = with_leading(h, x);
@@ -580,8 +582,8 @@ std::tuple<at::Tensor, at::Tensor> fp8_quantize_meta(const at::Tensor& x, bool s
   const c10::SymInt K = silu_mul ? x.sym_size(-1) / 2 : x.sym_size(-1);
   return {meta_rows(x, K), meta_like(x, blocks(K), at::kFloat)};
 }
-at::Tensor fp8_block_mm_meta(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t, const at::Tensor& w_scale,
-                             const OptTensor& bias, bool out_f32) {
+at::Tensor fp8_block_mm_meta(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& w_t,
+                             const at::Tensor& w_scale, const OptTensor& bias, bool out_f32) {
   check_mm_shapes("fp8_block_mm", a, a_scale, w_t, w_scale, bias);
   return meta_like(a, w_t.sym_size(1), out_f32 ? at::kFloat : at::kBFloat16);
 }
@@ -591,7 +593,8 @@ void fp8_block_mm_out_meta(const at::Tensor& a, const at::Tensor& a_scale, const
   check_out_shapes("fp8_block_mm", out, a, w_t);
   written(out);
 }
-at::Tensor fp8_block_linear_meta(const at::Tensor& x, const at::Tensor& w_t, const at::Tensor& w_scale, const OptTensor& bias) {
+at::Tensor fp8_block_linear_meta(const at::Tensor& x, const at::Tensor& w_t, const at::Tensor& w_scale,
+                                 const OptTensor& bias) {
   check_linear_shapes("fp8_block_linear", x, w_t, w_scale, bias);
   return meta_like(x, w_t.sym_size(1), at::kBFloat16);
 }

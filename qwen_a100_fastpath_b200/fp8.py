@@ -12,7 +12,8 @@ The weight is read in place: ``w_t`` is the checkpoint's e4m3 ``[N, K]`` row-maj
 
 All tensors must be CUDA tensors on one device; the work goes to that device's current stream and nothing is
 synchronised, so calls can be captured into CUDA graphs.  A call that cannot be taken raises ``ValueError`` before
-anything is launched; there is no CPU path, no backward and no fallback.
+anything is launched; there is no CPU path, no derivative (tensors that require a gradient are refused outside
+``torch.no_grad()``) and no fallback.
 """
 from __future__ import annotations
 
@@ -46,10 +47,10 @@ def fp8_block_mm(a: torch.Tensor, a_scale: torch.Tensor, w_t: torch.Tensor, w_sc
     """``y[m, n] = sum_g a_scale[m, g] * w_scale[n // 128, g] * sum_{k in g} a[m, k] * w[n, k] (+ bias[n])``: exact e4m3
     products, fp32 sums, one rounding to ``out_dtype`` (bf16 or fp32).  ``a`` e4m3 ``[M, K]`` with fp32 ``a_scale
     [M, ceil(K / 128)]`` (any strides) as ``fp8_quantize`` returns them; ``w_t`` e4m3 ``[K, N]`` with stride ``(1, ldw)``,
-    16-byte aligned, ``ldw % 16 == 0``, K and N up to 2^20, M up to 2^31 - 128; ``bias`` bf16 ``[N]``, added in fp32.  Rows of ``a`` that are not 16-byte aligned
-    are copied first.  ``out`` may supply the result (it decides the type then); it must not share memory with an input
-    (refused as ``_lib.QFOverlapError``, a ``ValueError``; bytes between the elements of an input that is not rows of adjacent
-    elements count as its own)."""
+    16-byte aligned, ``ldw % 16 == 0``; ``bias`` bf16 ``[N]``, added in fp32; K and N up to 2^20, M up to 2^31 - 128.  Rows
+    of ``a`` that are not 16-byte aligned are copied first.  ``out`` may supply the result (it decides the type then); it
+    must not share memory with an input (refused as ``_lib.QFOverlapError``, a ``ValueError``; bytes between the elements of
+    an input that is not rows of adjacent elements count as its own)."""
     if out is not None:
         try:
             _mm_out(a, a_scale, w_t, w_scale, bias, out)

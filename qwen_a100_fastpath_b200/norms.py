@@ -55,9 +55,10 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, pre_weight: to
 
 def residual_norm_status(device=None) -> int:
     """Read and clear the device's sticky error flag of ``residual_norm`` (``QF_OK``, or ``QF_ERR_TIMEOUT`` after a bounded
-    wait for a row inside a launch expired; the rows were then read another way and the results are valid); synchronises the
-    device's current stream."""
+    wait for a row inside a launch expired; the rows were then read another way and the results are valid); synchronises
+    the device's current stream."""
     with torch.cuda.device(torch.cuda.current_device() if device is None else device):
         st = ctypes.c_int(0)
-        check("qf_residual_norm_status", LIB.qf_residual_norm_status(torch.cuda.current_stream().cuda_stream, ctypes.byref(st)))
+        stream = torch.cuda.current_stream().cuda_stream
+        check("qf_residual_norm_status", LIB.qf_residual_norm_status(stream, ctypes.byref(st)))
         return st.value

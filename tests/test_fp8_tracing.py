@@ -65,7 +65,8 @@ def test_int8_linear_keeps_the_token_count():
     from qwen_a100_fastpath_b200._lib import load_torch_ops
     op = load_torch_ops()
     w, s = torch.zeros(64, 256, dtype=torch.int8).t(), torch.ones(64)
-    gm = make_fx(lambda x: op(x, w, s, None), tracing_mode="symbolic", _allow_non_fake_inputs=True)(torch.zeros(7, 256, dtype=BF16))
+    trace = make_fx(lambda x: op(x, w, s, None), tracing_mode="symbolic", _allow_non_fake_inputs=True)
+    gm = trace(torch.zeros(7, 256, dtype=BF16))
     out = next(n for n in gm.graph.nodes if "int8_linear" in str(n.target)).meta["val"]
     assert isinstance(out.shape[0], torch.SymInt) and not out.shape[0].node.expr.is_number and out.shape[1] == 64
 

@@ -44,7 +44,8 @@ def test_too_many_rows_are_refused_first(dev):
         with pytest.raises(ValueError, match="too many|more than"):
             f()
     # an output that does not fit is refused before unaligned rows are copied
-    rows = torch.zeros(2 ** 20 * 257 + 1, device=dev, dtype=torch.uint8).view(torch.float8_e4m3fn)[1:].view(2 ** 20, 257)[:, :256]
+    rows = torch.zeros(2 ** 20 * 257 + 1, device=dev, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    rows = rows[1:].view(2 ** 20, 257)[:, :256]
     base = torch.cuda.memory_allocated(dev)
     torch.cuda.reset_peak_memory_stats(dev)
     with pytest.raises(ValueError, match="out must be"):

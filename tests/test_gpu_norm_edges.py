@@ -27,8 +27,8 @@ def test_more_rows_than_2_to_the_30(dev):
 
 def ahead_against_few_rows():
     """Calls of many rows, which arrive ahead in shared memory, against calls of so few that nothing is read ahead: the same
-    bits.  One, two and four pieces a thread, two to four rows in the ring, last rounds that are not full.  Returns whether a wait
-    ran out in any of them."""
+    bits.  One, two and four pieces a thread, two to four rows in the ring, last rounds that are not full.  Returns whether a
+    wait ran out in any of them."""
     import itertools
 
     import torch

@@ -61,8 +61,8 @@ def test_quantizer_keeps_closed_gates(dev, up):
     gg, uu = g.double().cpu().numpy(), u.double().cpu().numpy()
     sg = sigmoid(gg)
     v = gg * sg * uu
-    e_v = (np.where(sg >= TINY, 2.5 * U * sg, 2.0 ** -150) * np.abs(gg) + np.maximum(U * np.abs(gg) * sg, 2.0 ** -150)) * uu * (1 + U) \
-        + U * np.abs(v)
+    e_g = np.where(sg >= TINY, 2.5 * U * sg, 2.0 ** -150) * np.abs(gg) + np.maximum(U * np.abs(gg) * sg, 2.0 ** -150)
+    e_v = e_g * uu * (1 + U) + U * np.abs(v)
     floor = 2.0 ** -60
     top = np.maximum(np.abs(v).max(axis=1), 448 * floor)
     e_top = np.where(np.abs(v).max(axis=1) > 448 * floor, e_v.max(axis=1), 0.0)
