@@ -9,12 +9,12 @@
 // accumulator per k group; two producer and two issuing warps feed it from a ring of TMA stages (128-byte rows, 128-byte
 // swizzle), eight warps add each finished accumulator, times its scales, to fp32 sums in registers while the next
 // groups are multiplied.  With fewer tiles than SMs a cluster shares a tile's groups and adds its parts over distributed
-// shared memory, in rank order.  What bounds it with the operands in L2: a group of 64 / 128 / 256 channels takes a CTA
+// shared memory, in rank order.  What bounds it over many groups: one of 64 / 128 / 256 channels takes a CTA
 // 0.30 / 0.38 / 0.52 us, of which shared memory's 128 bytes a clock (copies in, operands out: 2 x (16 KiB + BN * 128)) are
-// 0.20 / 0.26 / 0.39 and the rest, the same at every width, is about one barrier wait.  With weights from DRAM it is
-// slower.  Measured (us, B200, in a graph): 72 x 10240 x 5120 18.5 (40 tiles x 3 CTAs, 2.9 TB/s);
-// 333 x 2600 x 1160 7.9; 2048 x 5120 x 8192 119 (three rounds of tiles, the last of 24); 4096 x 34816 x 5120 767 (1.90
-// PFLOP/s; 915 in a loop under the power cap).
+// 0.20 / 0.26 / 0.39 and the rest, the same at every width, is about one barrier wait.  A short share of groups costs
+// more (starts and the join of a split).  Measured (us, B200, in a graph): 72 x 10240 x 5120 18.2 (40 tiles x 3 CTAs; 17.8
+// with its weights in L2); 333 x 2600 x 1160 7.9; 2048 x 5120 x 8192 119 (three rounds of tiles, the last of 24); 4096 x
+// 34816 x 5120 767 (1.90 PFLOP/s; 915 in a loop under the power cap).
 //
 // fp8_rows_kernel (up to 16): bound by the weights' bytes.  A CTA takes tiles of 16 or 32 weight rows, a producer copies
 // four or eight k groups of them and of the token rows per stage into a ring (one TMA copy each: a copy costs its issuer
@@ -912,9 +912,9 @@ int resident_clusters(int dev, int sms, int split) {
 }
 
 // Tile width and k split.  Time of a choice in microseconds: whole waves of CTAs, each a start and its groups at the
-// measured rate of one CTA with its operands in L2 (a group of 64 / 128 / 256 channels takes 0.30 / 0.38 / 0.52 us), and
-// for a split the join of the parts.  It ranks the choices; where the weights come from DRAM the time itself is longer
-// (72 x 10240 x 5120: 256 channels in three parts, 10.3 us by this model, 18.5 measured).
+// measured rate of one CTA over many of them (64 / 128 / 256 channels: 0.30 / 0.38 / 0.52 us), and for a split the join of
+// the parts.  It ranks the choices; a split takes longer than it says (72 x 10240 x 5120: 256 channels in three parts, 10.3
+// us by this model, 18.2 measured, 17.8 with the weights in L2).
 int tiles_any(const TileParams& tp, int dev, int sms, unsigned flags, cudaStream_t st) {
   const Fp8Params& p = tp.p;
   const int mt = (p.M + kTileM - 1) / kTileM;

@@ -11,8 +11,7 @@
 // crosses a warp, and the groups of all rows form one flat index, so one row fills as many SMs as it has work for.
 // Eight CTAs per SM, six with the gate: its arithmetic needs the registers, 40 with what a thread has loaded kept packed
 // until it is used.  4096 x 17408 takes 34 us (6.2 TB/s), with the gate 69 us in a graph, 77 through the call (4.7 TB/s;
-// five CTAs 82; what a thread has in flight between its loads and its stores is not enough for the memory's rate); one
-// row of 5120 1.3 us.
+// five CTAs 82; neither DRAM, 56 %, nor issue, 75 %, is at its limit); one row of 5120 1.3 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
