@@ -257,6 +257,82 @@ int qf_residual_norm(const void* x, int64_t ldx, const void* residual, int64_t l
  * and the threads that waited read that row and all later ones directly: the result is valid.  Not for the hot path. */
 int qf_residual_norm_status(void* stream, int* status);
 
+/* ---- the paged cache held in 4 bits -------------------------------------------------------------------------------
+ * No counterpart in the reference, whose cache is bf16 (spec_attn.py).  Keys and values are kept in groups of QF_KV4_GROUP
+ * consecutive dimensions of one head of one token: a nibble n per value (the even dimension in a byte's low half) and for
+ * each group two bf16 numbers, the step s and the offset c:
+ *   lo, hi = least and greatest value;  s = bf16((hi - lo) / 15);  c = bf16(lo - 16 s);
+ *   n = clamp(rint((x - c) / s), 16, 31) - 16, 0 where s = 0 (fp32 operations, nearest even);  n stands for bf16((n + 16) s + c).
+ * A group with a NaN, an infinity or a magnitude of 2^126 or more becomes NaN.  k, v: uint8, element (page, head, slot) at
+ * page * page_stride + head * head_stride + slot * slot_stride bytes, head_size / 2 bytes each; k_scale, v_scale: bf16
+ * [head_size / 64][2] at the scale strides (elements).  head_size 64, 128 or 256; any page size; pointers and strides of the
+ * codes multiples of 16 bytes, those of the scales of head_size / 64 pairs. */
+#define QF_KV4_GROUP 64
+typedef struct qf_kv4_cache {
+  void* k;
+  void* v;
+  void* k_scale;
+  void* v_scale;
+  int64_t page_stride, head_stride, slot_stride;                   /* bytes, of k and v alike */
+  int64_t scale_page_stride, scale_head_stride, scale_slot_stride; /* bf16 elements */
+  int num_pages, page_size, num_heads, head_size;
+} qf_kv4_cache;
+
+/* Keys and values (bf16 [tokens][num_heads][head_size], element strides, unit innermost stride, 16-byte aligned, strides
+ * multiples of 8) into the slots slots[token] (page * page_size + offset).  A token whose slot is negative or behind the cache
+ * is left out.  Slots given twice in one call hold parts of either token afterwards.  tokens * num_heads * head_size / 4
+ * below 2^31. */
+int qf_kv4_write(const void* k, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_t, int64_t sv_h,
+                 const int64_t* slots, int tokens, const qf_kv4_cache* cache, unsigned flags, void* stream);
+/* The bf16 values that the slots stand for, in k and v (as above); zeros for a slot that is none of the cache's. */
+int qf_kv4_read(void* k, int64_t sk_t, int64_t sk_h, void* v, int64_t sv_t, int64_t sv_h, const int64_t* slots,
+                int tokens, const qf_kv4_cache* cache, unsigned flags, void* stream);
+
+/* qf_spec_attn over this cache: num_reqs requests of q_len query tokens each, query qi of request b attends the keys
+ * [0, seq_lens[b] - q_len + qi]; a row with no key gives zeros.  Keys behind max_pages * page_size, and on pages whose entry
+ * is no page of the cache, do not take part; what lies in slots that a row does not attend, NaN included, does not touch it.
+ * q, out: bf16, 16-byte aligned with strides multiples of 8 elements; q_len * num_heads / cache->num_heads <= 64; block_table
+ * int32 (row stride s_bt, max_pages entries each).  The workspace (>= qf_kv4_attn_workspace_bytes() on the current device,
+ * 256-byte aligned) need not be zeroed and holds nothing between calls.  No host synchronisation. */
+size_t qf_kv4_attn_workspace_bytes(int num_reqs, int q_len, int num_heads, int num_kv_heads, int head_size);
+int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_kv4_cache* cache, const int32_t* block_table,
+                int64_t s_bt, int max_pages, const int32_t* seq_lens, void* out, int64_t so_t, int64_t so_h, int num_reqs,
+                int q_len, int num_heads, float scale, void* ws, size_t ws_bytes, unsigned flags, void* stream);
+
+/* ---- norms of queries and keys for each head with the position rotation -------------------------------------------
+ * Per token and head, a row x of head_size values, fp32 inside (the reference plugin leaves both to vLLM):
+ *   y = x, or x * rsqrt(mean(x^2) + eps) * (weight + weight_offset) where the weight (bf16 [head_size]) is given;
+ *   its first `rot` values turn by the angles of the token's position: with cos_i, sin_i = cos_sin[position][i],
+ *   [rot / 2 + i], and (a, b) = (y[i], y[i + rot / 2]), or (y[2 i], y[2 i + 1]) where interleaved:
+ *   (a cos_i - b sin_i, b cos_i + a sin_i);  rounded to bf16 once.
+ * cos_sin: fp32 or bf16 [max_positions][rot], row stride s_cs; a position outside it makes the turned values NaN; rot 0: no
+ * rotation.  q, k, v, q_out, k_out: element strides of token and head, unit innermost stride; an output may be its input
+ * (the same strides), no other overlap.  With a cache the keys are not returned: they (rounded to bf16) and v go to the cache
+ * as qf_kv4_write writes them.  1 <= head_size <= QF_ROPE_MAX_D. */
+#define QF_ROPE_MAX_D 512
+int qf_qk_norm_rope(const void* q, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t, int64_t sk_h,
+                    const void* q_weight, const void* k_weight, float weight_offset, float eps,
+                    const int64_t* positions, const void* cos_sin, int64_t s_cs, int cos_sin_dtype,
+                    int64_t max_positions, int rot, int interleaved, void* q_out, int64_t so_t, int64_t so_h, void* k_out,
+                    int64_t sp_t, int64_t sp_h, const void* v, int64_t sv_t, int64_t sv_h, const int64_t* slots,
+                    const qf_kv4_cache* cache, int tokens, int num_heads, int num_kv_heads, int head_size,
+                    unsigned flags, void* stream);
+
+/* ---- the maps of a step on a paged cache ---------------------------------------------------------------------------
+ * From the lengths of num_reqs requests (query_lens new tokens behind past_lens cached ones, negative counts as zero; sums
+ * stop at 2^31 - 1): query_start [num_reqs + 1] (exclusive prefix sums of query_lens), seq_lens = past + query, and for each
+ * token i of the step its position and its slot, block_table[r][position / page_size] * page_size + position % page_size; -1
+ * where the table (max_pages entries a row) has no page for it.  Entries behind the last token (up to num_tokens) get
+ * position 0 and slot -1.  With free_head (and free_pages [num_free]) each request first grows its row of block_table:
+ * entries ceil(past / page_size) to ceil(seq / page_size) - 1 (within max_pages) receive the next pages of free_pages from
+ * index free_head[0] on, in the requests' order, -1 where the list has run out; free_head_out[0] = free_head[0] + the entries
+ * asked for (beyond num_free: that many pages are missing).  num_reqs <= QF_MAPS_MAX_REQS. */
+#define QF_MAPS_MAX_REQS 16384
+int qf_step_maps(const int32_t* query_lens, const int32_t* past_lens, int num_reqs, int32_t* block_table, int64_t s_bt,
+                 int max_pages, int page_size, const int32_t* free_pages, int num_free, const int32_t* free_head,
+                 int32_t* query_start, int32_t* seq_lens, int64_t* positions, int64_t* slots, int num_tokens,
+                 int32_t* free_head_out, unsigned flags, void* stream);
+
 /* Reads and clears the workspace's sticky device error flag (synchronises `stream`).  *status receives
  * QF_OK or QF_ERR_TIMEOUT.  Not for the hot path. */
 int qf_workspace_status(void* ws, void* stream, int* status);

@@ -27,7 +27,20 @@ QF_NORM_MAX_H = 16384
 QF_GATE_NONE = 0
 QF_GATE_SIGMOID = 1
 QF_GATE_SILU = 2
+QF_KV4_GROUP = 64
+QF_ROPE_MAX_D = 512
+QF_MAPS_MAX_REQS = 16384
 ABI_VERSION = 1
+
+
+class KV4CacheStruct(ctypes.Structure):
+    """``qf_kv4_cache`` of include/qf_b200.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+        [(n, ctypes.c_int64) for n in ("page_stride", "head_stride", "slot_stride", "scale_page_stride",
+                                       "scale_head_stride", "scale_slot_stride")] + \
+        [(n, ctypes.c_int) for n in ("num_pages", "page_size", "num_heads", "head_size")]
+
+
 
 # (name, restype, argtypes) -- one entry per function declared in include/qf_b200.h
 _c = ctypes
@@ -80,6 +93,25 @@ SIGNATURES = [
       _c.c_void_p, _c.c_void_p, _c.c_float, _c.c_float, _c.c_float, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64,
       _c.c_void_p, _c.c_int64, _c.c_int, _c.c_int, _c.c_uint, _c.c_void_p]),
     ("qf_residual_norm_status", _c.c_int, [_c.c_void_p, _c.POINTER(_c.c_int)]),
+    ("qf_kv4_write", _c.c_int,
+     [_c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int,
+      _c.POINTER(KV4CacheStruct), _c.c_uint, _c.c_void_p]),
+    ("qf_kv4_read", _c.c_int,
+     [_c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int,
+      _c.POINTER(KV4CacheStruct), _c.c_uint, _c.c_void_p]),
+    ("qf_kv4_attn_workspace_bytes", _c.c_size_t, [_c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int]),
+    ("qf_kv4_attn", _c.c_int,
+     [_c.c_void_p, _c.c_int64, _c.c_int64, _c.POINTER(KV4CacheStruct), _c.c_void_p, _c.c_int64, _c.c_int, _c.c_void_p,
+      _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int, _c.c_int, _c.c_int, _c.c_float, _c.c_void_p, _c.c_size_t, _c.c_uint,
+      _c.c_void_p]),
+    ("qf_qk_norm_rope", _c.c_int,
+     [_c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_float,
+      _c.c_float, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_int64, _c.c_int, _c.c_int, _c.c_void_p, _c.c_int64,
+      _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p,
+      _c.POINTER(KV4CacheStruct), _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_uint, _c.c_void_p]),
+    ("qf_step_maps", _c.c_int,
+     [_c.c_void_p, _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_int, _c.c_void_p, _c.c_int, _c.c_void_p,
+      _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_uint, _c.c_void_p]),
     ("qf_allreduce_buffer_bytes", _c.c_size_t, [_c.c_int]),
     ("qf_symm_alloc", _c.c_int, [_c.c_size_t, _c.POINTER(_c.c_void_p)]),
     ("qf_symm_free", _c.c_int, [_c.c_void_p]),

@@ -3,7 +3,7 @@
 ``python -m qwen_a100_fastpath_b200.build`` (or ``build_library()``) compiles ``csrc/*.cu`` into
 ``qwen_a100_fastpath_b200/libqf_b200.so`` with the CUDA runtime linked statically, so the library needs no
 toolkit at run time and loads on a machine without a GPU (no CUDA call happens at load).  It then compiles
-``csrc/qf_torch_ops.cpp`` with the host C++ compiler against the installed PyTorch into ``_qf_torch_ops.so``
+``csrc/qf_torch_*.cpp`` with the host C++ compiler against the installed PyTorch into ``_qf_torch_ops.so``
 (``torch.ops.qf_b200.*``), linked to ``libqf_b200.so`` next to it.
 """
 from __future__ import annotations
@@ -19,9 +19,9 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 LIB = PKG / "libqf_b200.so"
 TORCH_OPS = PKG / "_qf_torch_ops.so"
-TORCH_OPS_SOURCE = "qf_torch_ops.cpp"
+TORCH_OPS_SOURCES = ["qf_torch_ops.cpp", "qf_torch_cache_ops.cpp"]
 SOURCES = ["qf_w8a16.cu", "qf_allreduce.cu", "qf_quant.cu", "qf_w8a8.cu", "qf_spec_attn.cu", "qf_fp8_quant.cu",
-           "qf_fp8_gemm.cu", "qf_norm.cu"]
+           "qf_fp8_gemm.cu", "qf_norm.cu", "qf_rope.cu", "qf_kv4.cu", "qf_kv4_attn.cu", "qf_maps.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -41,7 +41,7 @@ def needs_build() -> bool:
     if not LIB.exists() or not TORCH_OPS.exists():
         return True
     t = min(LIB.stat().st_mtime, TORCH_OPS.stat().st_mtime)
-    return any(p.stat().st_mtime > t for p in _inputs() + [CSRC / TORCH_OPS_SOURCE])
+    return any(p.stat().st_mtime > t for p in _inputs() + [CSRC / s for s in TORCH_OPS_SOURCES])
 
 
 def build_library(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
@@ -77,7 +77,7 @@ def build_torch_ops(verbose: bool = False) -> Path:
     # operator layer, and a second copy's locale facets crash where an error message formats a number
     tmp = TORCH_OPS.with_suffix(".so.tmp")
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *incs,
-           str(CSRC / TORCH_OPS_SOURCE), "-o", str(tmp), f"-L{PKG}", "-lqf_b200", f"-L{tdir / 'lib'}", "-lc10",
+           *[str(CSRC / s) for s in TORCH_OPS_SOURCES], "-o", str(tmp), f"-L{PKG}", "-lqf_b200", f"-L{tdir / 'lib'}", "-lc10",
            "-lc10_cuda", "-l:libstdc++.so.6", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)

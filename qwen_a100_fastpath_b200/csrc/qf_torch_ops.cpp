@@ -13,19 +13,13 @@
 // layers (fp8.py and norms.py document them).  They need no workspace: what they make comes from the caching allocator,
 // so calls on several streams, and captured graphs, share nothing.  They refuse a call with a ValueError before anything
 // is launched, and tensors that require a gradient or carry a tangent too: none of them has a derivative.
-#include <ATen/ATen.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/core/AutogradState.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/library.h>
-
-#include <cstdint>
 #include <map>
 #include <mutex>
 #include <tuple>
 
-#include "../../include/qf_b200.h"
+#include "qf_torch.h"
+
+using namespace qf_torch;
 
 namespace {
 
@@ -43,10 +37,6 @@ at::Tensor workspace(const at::Device& dev, cudaStream_t stream, int kind, size_
     return t;
   }
   return it->second;
-}
-
-void check(int rc, const char* fn) {
-  TORCH_CHECK(rc == QF_OK, fn, ": ", qf_strerror(rc), " (", rc, "): ", qf_last_error_detail());
 }
 
 at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& w_q, const at::Tensor& w_s,
@@ -106,54 +96,9 @@ at::Tensor int8_linear_meta(const at::Tensor& x, const at::Tensor& w_q, const at
 }
 
 // ---------------------------------------------------------------------------------------- block-scaled fp8 layers
-#define QF_REFUSE_UNLESS(cond, ...) TORCH_CHECK_VALUE(cond, __VA_ARGS__)
-// Equality of sizes that may be symbolic: tracing goes on with it as a fact and fixes neither side.
-bool same_size(const c10::SymInt& a, const c10::SymInt& b) {
-  if (C10_LIKELY(!a.is_heap_allocated() && !b.is_heap_allocated())) return a.as_int_unchecked() == b.as_int_unchecked();
-  return a.sym_eq(b).expect_true(__FILE__, __LINE__);
-}
-#define QF_REFUSE_UNLESS_EQ(a, b, ...) TORCH_CHECK_VALUE(same_size(a, b), __VA_ARGS__)
-
-using OptTensor = c10::optional<at::Tensor>;
-
 constexpr int64_t kBlock = 128;
 int64_t blocks(int64_t v) { return (v + kBlock - 1) / kBlock; }
 c10::SymInt blocks(const c10::SymInt& v) { return (v + (kBlock - 1)) / kBlock; }
-
-bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
-
-void check_type(const char* op, const char* name, const at::Tensor& t, at::ScalarType type) {
-  QF_REFUSE_UNLESS(t.scalar_type() == type, op, ": ", name, " must be ", type, ", got ", t.scalar_type());
-}
-
-void check_input(const char* op, const char* name, const at::Tensor& t, const at::Device& dev) {
-  QF_REFUSE_UNLESS(t.is_cuda(), op, ": ", name, " must be a CUDA tensor (there is no CPU path)");
-  QF_REFUSE_UNLESS(t.device() == dev, op, ": ", name, " is on ", t.device(), ", the first input on ", dev);
-}
-
-// In the place of torch's fallback for operators without a backward: refuses tensors that want a derivative, outputs among
-// them, and goes on to the operator.  Here the derivatives of torch.func's transformations can be seen too.
-void refuse_derivatives(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
-  const bool backward = at::GradMode::is_enabled();
-  const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
-  const size_t n = op.schema().arguments().size();
-  for (size_t i = 0; i < n; ++i) {
-    const c10::IValue& v = (*stack)[stack->size() - n + i];
-    if (!v.isTensor()) continue;
-    const at::Tensor& t = v.toTensor();
-    if (!t.defined()) continue;
-    QF_REFUSE_UNLESS(!(backward && t.requires_grad()), op.schema().name(), ": ", op.schema().arguments()[i].name(),
-                     " requires a gradient and the operator has no backward (call it under torch.no_grad())");
-    QF_REFUSE_UNLESS(!(forward && t._fw_grad(0).defined()), op.schema().name(), ": ", op.schema().arguments()[i].name(),
-                     " has a forward-mode tangent and the operator has no derivative");
-  }
-  op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
-}
-
-// A tensor was written: autograd tells by its version where a value it kept is no longer there.
-void written(const at::Tensor& t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
 
 // ---- types and shapes, of real calls and of traced ones (whose sizes may be symbolic) ----
 void check_quantize_shapes(const at::Tensor& x, bool silu_mul) {
@@ -251,8 +196,6 @@ void check_norm_shapes(const at::Tensor& x, const OptTensor& residual, const Opt
   QF_REFUSE_UNLESS(eps >= 0 && eps <= 3.4e38, op, ": eps must be finite and >= 0");
 }
 
-cudaStream_t stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
-
 // Rows of [..., K], K >= 1.
 int64_t rows_of(const at::Tensor& x) { return x.dim() == 2 ? x.size(0) : x.numel() / x.size(-1); }
 
@@ -267,63 +210,6 @@ void check_rows(const char* op, int64_t M, int64_t N) {
                    " results are too many");
 }
 
-// The bytes of a tensor as `rows` intervals of `width` bytes, `step` bytes apart.  Exact for rows of adjacent elements; what
-// lies between the elements of other tensors counts as theirs.
-struct Intervals {
-  int64_t begin, width, step, rows;
-  int64_t end() const { return begin + (rows - 1) * step + width; }
-};
-
-Intervals intervals_of(const at::Tensor& t) {
-  // the dimension of the largest stride gives the rows, the others' span their width
-  int64_t rows = 1, step = 0, span = 1;
-  int outer = -1;
-  for (int i = 0; i < t.dim(); ++i)
-    if (t.size(i) > 1 && t.stride(i) > step) step = t.stride(i), rows = t.size(i), outer = i;
-  for (int i = 0; i < t.dim(); ++i)
-    if (i != outer && t.size(i) > 1) span += (t.size(i) - 1) * t.stride(i);
-  const int64_t es = static_cast<int64_t>(t.element_size());
-  Intervals v = {static_cast<int64_t>(reinterpret_cast<uintptr_t>(t.data_ptr())), span * es, step * es, rows};
-  if (v.width >= v.step) v = {v.begin, (v.rows - 1) * v.step + v.width, 0, 1};  // adjacent or overlapping rows: one interval
-  return v;
-}
-
-bool overlap(const at::Tensor& ta, const at::Tensor& tb) {
-  if (ta.numel() == 0 || tb.numel() == 0) return false;
-  Intervals a = intervals_of(ta), b = intervals_of(tb);
-  if (a.end() <= b.begin || b.end() <= a.begin) return false;
-  if (a.rows > 1 && b.rows > 1 && a.step == b.step) {
-    // columns of one larger tensor: the rows' places within a step decide
-    const int64_t at = ((b.begin - a.begin) % a.step + a.step) % a.step;
-    if (at >= a.width && at + b.width <= a.step) return false;
-  }
-  // walk both upwards, always on with the row that ends first
-  int64_t i = 0, j = 0;
-  // rows that end before the other begins
-  if (a.step && b.begin > a.begin + a.width) i = (b.begin - a.begin - a.width) / a.step;
-  if (b.step && a.begin > b.begin + b.width) j = (a.begin - b.begin - b.width) / b.step;
-  while (i < a.rows && j < b.rows) {
-    const int64_t pa = a.begin + i * a.step, pb = b.begin + j * b.step;
-    if (pa < pb + b.width && pb < pa + a.width) return true;
-    if (pa + a.width <= pb) ++i; else ++j;
-  }
-  return false;
-}
-
-// Whether two tensors of one shape and type hold the same elements at the same places.
-bool same_elements(const at::Tensor& a, const at::Tensor& b) {
-  if (a.data_ptr() != b.data_ptr()) return false;
-  for (int i = 0; i < a.dim(); ++i)
-    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
-  return true;
-}
-
-// "single memory location" is what torch's own operators say of such a call.
-void check_no_overlap(const char* op, const char* out_name, const at::Tensor& out, const char* name, const at::Tensor& t) {
-  QF_REFUSE_UNLESS(!overlap(out, t), op, ": ", out_name, " shares memory with ", name,
-                   ": elements of the two refer to a single memory location");
-}
-
 // [..., K] as rows of unit column stride, without a copy where the strides allow it.
 at::Tensor as_rows(const at::Tensor& x) {
   at::Tensor r = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
@@ -336,11 +222,6 @@ at::Tensor as_rows(const at::Tensor& x) {
 at::Tensor with_leading(const at::Tensor& rows, const at::Tensor& x) {
   if (x.dim() == 2) return rows;
   return x.dim() == 1 ? rows.select(0, 0) : rows.unflatten(0, x.sizes().slice(0, x.dim() - 1));
-}
-
-// A new tensor of the caching allocator, without the dispatcher's share of a small call's time.
-at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
-  return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt));
 }
 
 // e4m3 rows of 16-byte stride, as the product's tensor maps take them.

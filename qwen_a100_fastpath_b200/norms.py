@@ -1,9 +1,11 @@
 """The residual update between two blocks of a decoder layer with the norms on both sides of it, in one pass
-(``qf_residual_norm`` in ``libqf_b200``).
+(``qf_residual_norm`` in ``libqf_b200``), and the norms of queries and keys for each head with the position rotation
+(``qf_qk_norm_rope``).
 
 The reference plugin leaves norms to vLLM; ``w8a16.w8a16_mm_rmsnorm`` fuses the plain one into the int8 GEMM.  Here it
 stands alone, with the optional norm after the block, the block's gate and the residual scale, and can hand the next
-block-scaled fp8 product its quantized activations directly.
+block-scaled fp8 product its quantized activations directly.  The norms inside the attention, which come with the rotation,
+can hand the keys and values to the 4-bit cache in the same way.
 """
 from __future__ import annotations
 
@@ -17,6 +19,8 @@ from ._lib import LIB, check, load_torch_ops, refused_out
 load_torch_ops()
 _norm = torch.ops.qf_b200.residual_norm.default
 _norm_out = torch.ops.qf_b200.residual_norm_out.default
+_rope = torch.ops.qf_b200.qk_norm_rope.default
+_rope_kv4 = torch.ops.qf_b200.qk_norm_rope_kv4.default
 
 GATE_ACTS = {"none": _lib.QF_GATE_NONE, "sigmoid": _lib.QF_GATE_SIGMOID, "silu": _lib.QF_GATE_SILU}
 
@@ -51,6 +55,32 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor | None, pre_weight: to
             raise refused_out(e) from None
         r = residual_out
     return ((h, s) if quantize else h), r
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                 positions: torch.Tensor | None, cos_sin: torch.Tensor | None, eps: float = 1e-6,
+                 weight_offset: float = 0.0, interleaved: bool = False, v: torch.Tensor | None = None, cache=None,
+                 slots: torch.Tensor | None = None):
+    """``(q, k)`` bf16 ``[tokens, heads, D]`` (any strides, views of the qkv product's rows; D <= 512) normalised for each
+    head and rotated, in fp32 inside and rounded once:
+
+    * ``y = x``, or with the weight (bf16 ``[D]``) ``y = x * rsqrt(mean(x^2) + eps) * (weight + weight_offset)``;
+    * the first R values of a head turn: with ``cos, sin = cos_sin[position].chunk(2)`` of ``cos_sin`` fp32 or bf16
+      ``[max_positions, R]`` (``None``: no rotation) and ``a, b = y[:R / 2], y[R / 2:R]``, or ``y[0:R:2], y[1:R:2]`` where
+      ``interleaved``: ``a * cos - b * sin`` and ``b * cos + a * sin``.  ``positions`` int64 ``[tokens]``; one outside the
+      table makes the turned values NaN.
+
+    With ``cache`` (a ``kv4.KV4Cache``), ``v`` and ``slots`` the keys, rounded to bf16, and ``v`` go to the cache as
+    ``kv4.kv4_write`` writes them, and the result is ``(q, None)``.  The same rules on devices, streams and errors as in
+    ``kv4``."""
+    if (cache is None) != (v is None) or (cache is None) != (slots is None):
+        raise ValueError("qk_norm_rope: cache, v and slots go together")
+    if cache is None:
+        return _rope(q, k, q_weight, k_weight, positions, cos_sin, weight_offset, eps, interleaved)
+    try:
+        return _rope_kv4(q, k, q_weight, k_weight, positions, cos_sin, weight_offset, eps, interleaved, v, slots, *cache), None
+    except ValueError as e:
+        raise refused_out(e) from None
 
 
 def residual_norm_status(device=None) -> int:
