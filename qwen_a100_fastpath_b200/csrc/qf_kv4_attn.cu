@@ -1,12 +1,33 @@
 // qf_kv4_attn.cu -- attention of uniform decode and verification batches over the paged cache held in 4 bits (qf_kv4.cuh has
 // the format).
 //
-// Mathematics: O = softmax(scale q K^T + mask) V in one pass over the keys with a running maximum and sum in fp32, over the
-// bf16 values that the cache stands for.
+// Mathematics: O = softmax(scale q K^T + mask) V in one pass over the keys, with a running maximum m and sum l for each
+// query row in fp32: a tile's weights are p = 2^(x - m) with x in units of log2, and where m has grown O and l are first
+// scaled by 2^(m_old - m).  Parts of a row's keys that different CTAs hold are joined by their m and l afterwards.
+//
+// Bound by memory for few rows (D / 2 + D / 16 bytes for each key and value), by taking the nibbles apart and the matrix
+// instructions for many.  The R = q_len * group query rows of a key head are one tile, so that its cache is read once.  The
+// tokens are the 16-row operand of mma.sync, the query rows the 8-column one, in both products: S^T = K Q^T and
+// O^T = V^T P^T.  Decoding has 1 to 64 rows, often 6 or 8, and pads them to a multiple of 8 and not of 16 (or of tcgen05's
+// 64 or 128, whose operands would besides have to go through shared memory as bf16, 4 bytes a value written and read for the
+// half byte that came); the operand with 16 rows is the one that is unpacked, straight into registers.
+//
+// A nibble row of a token is both operands as it lies.  For K, ldmatrix gives a thread eight dimensions of token g (and
+// g + 8), and the order of the dimensions within the sum is free as long as the query has the same.  For V, the transposed
+// ldmatrix of 16-bit elements (four dimensions each) gives a thread the same four dimensions of two neighbouring tokens in
+// the two halves of a register, which is what the 16-bit operand wants: token pairs; each of the four nibble places is a
+// tile of 16 dimensions.
+//
+// A CTA of four warps takes 64 tokens at a time: each warp scores 16 of them against all rows, the maxima and then the
+// weights (bf16) are exchanged in shared memory, and each warp adds up 64 of the head's dimensions (over all tokens for
+// D = 256, over half or a quarter of them for 128 and 64).  Codes and scales arrive by cp.async, kStages - 1 tiles ahead;
+// the pages are looked up a tile before that.  The CTAs split all tiles of all requests and heads evenly, whatever the
+// lengths; a CTA's part may begin or end inside a (request, head), and a second kernel joins those.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <mutex>
 #include <string>
 
 #include "../../include/qf_b200.h"
@@ -18,7 +39,11 @@
 namespace qf {
 namespace {
 
-struct Kv4AttnParams {
+constexpr int kTile = 64;       // tokens
+constexpr int kThreads = 128;
+constexpr int kMaxSms = 160;    // the workspace is sized without asking the device
+
+struct AttnParams {
   const __nv_bfloat16* q;
   int64_t qt, qh;
   __nv_bfloat16* out;
@@ -27,76 +52,545 @@ struct Kv4AttnParams {
   const int32_t* table;
   int64_t table_row;
   const int32_t* lens;
-  int max_pages, reqs, q_len, heads, group, D;
+  int64_t width;  // keys that a row of the table can place
+  int reqs, q_len, group, rows;
+  uint32_t div_mul, div_shift;  // by the page size
   float scale_log2;
+  // workspace
+  int32_t* tiles_before;  // [reqs + 1]: tiles of one head before each request
+  float2* part_ml;        // [2 * grid][rows]
+  float* part_o;          // [2 * grid][rows][D]
 };
 
-constexpr int kSimpleThreads = 128;
+template <int D, int NQ> struct Geo {
+  static constexpr int kRow = D / 2;                       // bytes of a token's codes
+  static constexpr int kScale = D / 16;                    // bytes of a token's scales
+  static constexpr int kStageBytes = 2 * kTile * (kRow + kScale);
+  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kCtas = NQ <= 1 ? 4 : NQ <= 4 ? 3 : 2;  // of an SM
+  static constexpr int kPRow = 2 * kTile + 16;             // bytes of a query row's weights, one chunk of padding
+  static constexpr int kQBytes = 4096 * NQ;                // the query's fragments; at a part's end the warps' sums
+  static constexpr int kPBytes = 8 * NQ * kPRow;
+  static constexpr int kOffQ = kStages * kStageBytes;
+  static constexpr int kOffP = kOffQ + kQBytes;
+  static constexpr int kSmem = kOffP + kPBytes;
+  static constexpr int kDimWarps = D / 64, kTokenWarps = 4 / kDimWarps;
+};
 
-// The value of dimension d of the slot at (codes, scale).
-__device__ __forceinline__ float kv4_value(const uint8_t* codes, const __nv_bfloat16* scale, int d) {
-  const float n = static_cast<float>(((codes[d / 2] >> (4 * (d & 1))) & 15) + 16);
-  const float s = __bfloat162float(scale[2 * (d / kKv4Group)]), c = __bfloat162float(scale[2 * (d / kKv4Group) + 1]);
-  return __bfloat162float(__float2bfloat16_rn(fmaf(n, s, c)));
+// ---- small PTX forms ----
+// 16, 8 or 4 bytes from global to shared memory without registers; zeros where !there (nothing is read then).
+template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
+  const int n = there ? N : 0;
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(N) : "memory");
+}
+// Two 8x8 tiles of 16-bit elements into shared memory, transposed: lane l gives the address of row l % 8 of tile l / 8.
+__device__ __forceinline__ void stsm_x2_trans(uint32_t addr, uint32_t r0, uint32_t r1) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1, %2};" ::"r"(addr), "r"(r0), "r"(r1) : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
 }
 
-// One CTA per query token and head; a thread a key of each 128, then two dimensions of the sum.
-__global__ void __launch_bounds__(kSimpleThreads) kv4_attn_simple_kernel(const Kv4AttnParams p) {
-  __shared__ float q[256], w[kSimpleThreads], red[kSimpleThreads / 32];
-  __shared__ int64_t at[kSimpleThreads], sat[kSimpleThreads];
+// Where the 16-byte chunk c of a token's codes lies in its tile: eight neighbouring tokens' chunks c are in different banks.
+template <int ROW> __device__ __forceinline__ uint32_t chunk_at(uint32_t token, uint32_t c) {
+  constexpr int kPerLine = 128 / ROW;  // tokens in 128 bytes
+  return token * ROW + ((c ^ ((token / kPerLine) & (ROW / 16 - 1))) << 4);
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return reinterpret_cast<const uint32_t&>(h);
+}
+
+// Tiles of a request, for each head: at least one, which writes the zeros of a request without keys.
+__device__ __forceinline__ int keys_of(const AttnParams& p, int len) {
+  return static_cast<int>(min(static_cast<int64_t>(max(len, 0)), p.width));
+}
+__device__ __forceinline__ int tiles_of(const AttnParams& p, int len) { return max((keys_of(p, len) - 1) / kTile + 1, 1); }
+
+// A walk over tiles in the order (request, head, tile).
+struct Cursor {
+  int b, h, tile, tiles, len;
+  __device__ __forceinline__ void next(const AttnParams& p) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++h < p.cache.heads) return;
+    h = 0;
+    if (++b < p.reqs) len = p.lens[b], tiles = tiles_of(p, len);
+  }
+};
+
+__device__ __forceinline__ int64_t part_start(int64_t total, int ctas, int i) { return total * i / ctas; }
+
+template <int D, int NQ>
+__global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(const AttnParams p) {
+  using G = Geo<D, NQ>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ int64_t offs[kTile][2];           // of the tile that is copied next: codes (bytes), scales (elements)
+  __shared__ uint32_t there[G::kStages][2];    // a bit for each token of a stage
+  __shared__ float red[4][8 * NQ];
+  __shared__ uint32_t bad[2][4][2];            // tokens whose values' group is not finite, of a tile with masked rows
+  __shared__ int scan[4], found[3];
+  __shared__ uint8_t row_query[8 * NQ];        // qi of a row
   pdl_launch_dependents();
   pdl_wait();
-  const int tid = threadIdx.x, token = blockIdx.x, head = blockIdx.y;
-  const int b = token / p.q_len, qi = token % p.q_len, kv = head / p.group;
-  for (int d = tid; d < p.D; d += kSimpleThreads) q[d] = __bfloat162float(p.q[token * p.qt + head * p.qh + d]);
-  const int64_t keys = min(static_cast<int64_t>(p.lens[b]) - p.q_len + qi + 1,
-                           static_cast<int64_t>(p.max_pages) * p.cache.page_size);
-  float top = -INFINITY, sum = 0.f, acc[2] = {0.f, 0.f};
-  for (int64_t k0 = 0; k0 < keys; k0 += kSimpleThreads) {
-    const int64_t key = k0 + tid;
-    float x = -INFINITY;
-    __syncthreads();  // the last keys have been read
-    at[tid] = -1;
-    if (key < keys) {
-      const int32_t page = p.table[b * p.table_row + key / p.cache.page_size];
-      if (page >= 0 && page < p.cache.num_pages) {
-        const int64_t off = key % p.cache.page_size;
-        at[tid] = page * p.cache.page + kv * p.cache.head + off * p.cache.slot;
-        sat[tid] = page * p.cache.spage + kv * p.cache.shead + off * p.cache.sslot;
-        x = 0.f;
-        for (int d = 0; d < p.D; ++d)
-          x = fmaf(q[d], kv4_value(p.cache.codes[0] + at[tid], p.cache.scale[0] + sat[tid], d), x);
-        x *= p.scale_log2;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const uint32_t sm = smem_u32(smem);
+  for (int r = tid; r < 8 * NQ; r += kThreads) row_query[r] = r < p.rows ? r / p.group : 0;
+
+  // ---- this CTA's part: a scan over the requests, twice (for the sum, then for where the part begins) ----
+  int64_t total = 0;
+  int64_t begin = 0, end = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t base = 0;
+    for (int b0 = 0; b0 < p.reqs; b0 += kThreads) {
+      const int b = b0 + tid;
+      const int n = b < p.reqs ? tiles_of(p, p.lens[b]) : 0;
+      int s = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, s, off);
+        if (lane >= off) s += a;
+      }
+      __syncthreads();
+      if (lane == 31) scan[warp] = s;
+      __syncthreads();
+      int64_t before = base + s - n;
+      for (int w = 0; w < 4; ++w) {
+        if (w < warp) before += scan[w];
+        base += scan[w];
+      }
+      if (pass == 0) {
+        if (blockIdx.x == 0 && b < p.reqs) p.tiles_before[b] = static_cast<int32_t>(before);
+      } else if (n && before * p.cache.heads <= begin && begin < (before + n) * p.cache.heads) {
+        const int64_t in = begin - before * p.cache.heads;
+        found[0] = b, found[1] = static_cast<int>(in / n), found[2] = static_cast<int>(in % n);
       }
     }
-    float m = x;
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, off));
-    __syncthreads();
-    if (tid % 32 == 0) red[tid / 32] = m;
-    __syncthreads();
-    for (int i = 0; i < kSimpleThreads / 32; ++i) m = max_nan(m, red[i]);
-    const float next = max_nan(top, m);
-    if (next == -INFINITY) continue;
-    w[tid] = at[tid] < 0 ? 0.f : exp2f(x - next);
-    __syncthreads();
-    const float old = exp2f(top - next);
-    top = next;
-    sum *= old, acc[0] *= old, acc[1] *= old;
-    const int n = static_cast<int>(min(keys - k0, static_cast<int64_t>(kSimpleThreads)));
-    for (int j = 0; j < n; ++j) {
-      if (at[j] < 0) continue;
-      sum += w[j];
-      for (int i = 0; i < 2; ++i)
-        if (tid + i * kSimpleThreads < p.D)
-          acc[i] = fmaf(w[j], kv4_value(p.cache.codes[1] + at[j], p.cache.scale[1] + sat[j], tid + i * kSimpleThreads),
-                        acc[i]);
+    if (pass == 0) {
+      if (blockIdx.x == 0 && tid == 0) p.tiles_before[p.reqs] = static_cast<int32_t>(base);
+      total = base * p.cache.heads;
+      const int ctas = static_cast<int>(min(total, static_cast<int64_t>(gridDim.x)));
+      if (static_cast<int>(blockIdx.x) >= ctas) return;
+      begin = part_start(total, ctas, blockIdx.x), end = part_start(total, ctas, blockIdx.x + 1);
     }
   }
-  for (int i = 0; i < 2; ++i)
-    if (tid + i * kSimpleThreads < p.D)
-      p.out[token * p.ot + head * p.oh + tid + i * kSimpleThreads] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc[i] / sum);
+  __syncthreads();
+  const int count = static_cast<int>(end - begin);
+  Cursor cur;
+  cur.b = found[0], cur.h = found[1], cur.tile = found[2];
+  cur.len = p.lens[cur.b];
+  cur.tiles = tiles_of(p, cur.len);
+  Cursor ahead = cur;  // of the tile whose pages are looked up next (threads of tokens)
+
+  // ---- copies: threads of tokens look a page up, then all threads copy ----
+  int32_t entry = -1;
+  auto look = [&](int i) {  // tile i's page of this thread's token
+    entry = -1;
+    if (tid >= kTile || i >= count) return;
+    const int pos = ahead.tile * kTile + tid;
+    if (pos < keys_of(p, ahead.len))
+      entry = p.table[ahead.b * p.table_row + ((__umulhi(pos, p.div_mul) + pos) >> p.div_shift)];
+  };
+  auto place = [&](int i) {  // its offsets, and on to the next tile
+    if (tid >= kTile) return;
+    const bool ok = entry >= 0 && entry < p.cache.num_pages;
+    if (ok) {
+      const uint32_t pos = ahead.tile * kTile + tid;
+      const int64_t slot = pos - ((__umulhi(pos, p.div_mul) + pos) >> p.div_shift) * static_cast<uint32_t>(p.cache.page_size);
+      offs[tid][0] = entry * p.cache.page + ahead.h * p.cache.head + slot * p.cache.slot;
+      offs[tid][1] = entry * p.cache.spage + ahead.h * p.cache.shead + slot * p.cache.sslot;
+    } else {
+      offs[tid][0] = -1;
+    }
+    const uint32_t bits = __ballot_sync(0xffffffffu, ok);
+    if (lane == 0) there[i % G::kStages][warp] = bits;
+    if (i + 1 < count) ahead.next(p);
+  };
+  auto copy = [&](int i) {
+    if (i < count) {
+      const uint32_t stage = sm + (i % G::kStages) * G::kStageBytes;
+      constexpr int kChunks = G::kRow / 16;
+#pragma unroll
+      for (int j = 0; j < kTile * kChunks / kThreads; ++j) {
+        const int token = (j * kThreads + tid) / kChunks, c = tid % kChunks;
+        const int64_t o = offs[token][0];
+        const bool ok = o >= 0;
+        const int64_t at = ok ? o + 16 * c : 0;
+        const uint32_t dst = stage + chunk_at<G::kRow>(token, c);
+        copy_async<16>(dst, p.cache.codes[0] + at, ok);
+        copy_async<16>(dst + kTile * G::kRow, p.cache.codes[1] + at, ok);
+      }
+      const int token = tid % kTile, side = tid / kTile;
+      const bool ok = offs[token][0] >= 0;
+      copy_async<G::kScale>(stage + 2 * kTile * G::kRow + (side * kTile + token) * G::kScale,
+                            p.cache.scale[side] + (ok ? offs[token][1] : 0), ok);
+    }
+    cp_async_commit();
+  };
+  look(0);
+  for (int i = 0; i < G::kStages - 1; ++i) {
+    if (i < count) place(i);
+    look(i + 1);
+    __syncthreads();
+    copy(i);
+    __syncthreads();
+  }
+
+  // ---- a part of one (request, head) after the other ----
+  float o[4][NQ][4];  // [nibble place][rows' tile][fragment]: O^T of this warp's 64 dimensions
+  float m[NQ][2], l[NQ][2];
+  const int dim_warp = warp % G::kDimWarps, token_warp = warp / G::kDimWarps;
+  bool fresh = true;
+  int first_tile = 0;
+  for (int i = 0; i < count; ++i) {
+    if (fresh) {
+      // the query's fragments: a thread's eight dimensions of a row in the order in which the nibbles come apart
+      for (int e = tid; e < D / 32 * NQ * 32; e += kThreads) {
+        const int l5 = e & 31, j = (e >> 5) % NQ, c = (e >> 5) / NQ;
+        const int r = 8 * j + (l5 >> 2);
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (r < p.rows) {
+          const int qi = r / p.group, hq = cur.h * p.group + r - qi * p.group;
+          u = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(cur.b) * p.q_len + qi) * p.qt + hq * p.qh + 32 * c +
+                                              8 * (l5 & 3));
+        }
+        reinterpret_cast<uint4*>(smem + G::kOffQ)[e] =
+            make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410),
+                       __byte_perm(u.y, u.w, 0x7632));
+      }
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        m[j][0] = m[j][1] = -INFINITY, l[j][0] = l[j][1] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k][j][0] = o[k][j][1] = o[k][j][2] = o[k][j][3] = 0.f;
+      }
+      first_tile = cur.tile;
+      fresh = false;
+      if (i == 0) cp_async_wait<G::kStages - 2>();
+      __syncthreads();
+    }
+    const uint32_t stage = sm + (i % G::kStages) * G::kStageBytes;
+    const int pos0 = cur.tile * kTile;
+    const bool masked_rows = pos0 + kTile - 1 > cur.len - p.q_len;  // some row does not see some token of the tile
+    const uint64_t ok_bits = static_cast<uint64_t>(there[i % G::kStages][1]) << 32 | there[i % G::kStages][0];
+    if (i + G::kStages - 1 < count) place(i + G::kStages - 1);
+    look(i + G::kStages);
+    if (masked_rows && tid < kTile) {
+      // values that are not finite may be hidden from some rows only: they leave the product (a weight of zero would not
+      // keep them out), and the rows that see one get their NaN afterwards
+#pragma unroll
+      for (int gr = 0; gr < D / 64; ++gr) {
+        const uint32_t at = stage + 2 * kTile * G::kRow + (kTile + tid) * G::kScale + 4 * gr;
+        const uint32_t sc = lds32(at);
+        const float s = bf16_lo(sc), c = bf16_hi(sc);
+        const bool is_bad = !(fabsf(s) < 2.6584559915698317e36f && fabsf(c) < 8.507059173023462e37f);  // 2^121, 2^126
+        if (is_bad) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(0u) : "memory");
+        const uint32_t bits = __ballot_sync(0xffffffffu, is_bad);
+        if (lane == 0) bad[i & 1][gr][warp] = bits;
+      }
+    }
+
+    // ---- scores of this warp's 16 tokens ----
+    float x[NQ][4];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
+    {
+      const uint32_t row = 16 * warp + (lane & 15);          // ldmatrix: lanes 0-15 a chunk's rows, 16-31 the next chunk's
+      const uint32_t scales = stage + 2 * kTile * G::kRow + (16 * warp + g) * G::kScale;
+#pragma unroll
+      for (int gr = 0; gr < D / 64; ++gr) {
+        uint32_t w[4];
+        ldsm_x4(stage + chunk_at<G::kRow>(row, 2 * gr + (lane >> 4)), w[0], w[1], w[2], w[3]);
+        const uint32_t sa = lds32(scales + 4 * gr), sb = lds32(scales + 8 * G::kScale + 4 * gr);
+        const uint32_t ssa = dup_lo(sa), cca = dup_hi(sa), ssb = dup_lo(sb), ccb = dup_hi(sb);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t a0 = kv4_pair<0>(w[2 * h], ssa, cca), a1 = kv4_pair<0>(w[2 * h + 1], ssb, ccb);
+          const uint32_t a2 = kv4_pair<1>(w[2 * h], ssa, cca), a3 = kv4_pair<1>(w[2 * h + 1], ssb, ccb);
+          const uint32_t b0 = kv4_pair<2>(w[2 * h], ssa, cca), b1 = kv4_pair<2>(w[2 * h + 1], ssb, ccb);
+          const uint32_t b2 = kv4_pair<3>(w[2 * h], ssa, cca), b3 = kv4_pair<3>(w[2 * h + 1], ssb, ccb);
+#pragma unroll
+          for (int j = 0; j < NQ; ++j) {
+            const uint4 q = lds128(sm + G::kOffQ + (((2 * gr + h) * NQ + j) * 32 + lane) * 16);
+            mma_bf16_m16n8k16(x[j], a0, a1, a2, a3, q.x, q.y);
+            mma_bf16_m16n8k16(x[j], b0, b1, b2, b3, q.z, q.w);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NQ; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[j][e] *= p.scale_log2;
+    if (masked_rows || ~ok_bits) {
+      const int ta = 16 * warp + g;
+      const bool oka = ok_bits >> ta & 1, okb = ok_bits >> (ta + 8) & 1;
+#pragma unroll
+      for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int last = cur.len - p.q_len + row_query[8 * j + 2 * t + e] - pos0;  // the last token that the row sees
+          if (!(oka && ta <= last)) x[j][e] = -INFINITY;
+          if (!(okb && ta + 8 <= last)) x[j][2 + e] = -INFINITY;
+        }
+    }
+    float top[NQ][2];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v = fmaxf(x[j][e], x[j][2 + e]);
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+        top[j][e] = v;
+      }
+    if (g == 0)
+#pragma unroll
+      for (int j = 0; j < NQ; ++j)
+        *reinterpret_cast<float2*>(&red[warp][8 * j + 2 * t]) = make_float2(top[j][0], top[j][1]);
+    __syncthreads();  // maxima; and all warps have left the last tile, whose stage is filled again now
+    copy(i + G::kStages - 1);
+
+    // ---- weights ----
+    bool grown = false;
+    float scale_o[NQ][2];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float2 v = *reinterpret_cast<const float2*>(&red[w][8 * j + 2 * t]);
+        top[j][0] = fmaxf(top[j][0], v.x), top[j][1] = fmaxf(top[j][1], v.y);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float next = fmaxf(m[j][e], top[j][e]);
+        const float ref = next == -INFINITY ? 0.f : next;  // a row that has seen no key
+        scale_o[j][e] = ex2_approx(m[j][e] - ref);
+        grown |= next > m[j][e];
+        m[j][e] = next;
+        const float pa = ex2_approx(x[j][e] - ref), pb = ex2_approx(x[j][2 + e] - ref);
+        x[j][e] = pa, x[j][2 + e] = pb;
+        l[j][e] = fmaf(l[j][e], scale_o[j][e], pa + pb);
+      }
+      stsm_x2_trans(sm + G::kOffP + (8 * j + (lane & 7)) * G::kPRow + 2 * (16 * warp + (lane & 8)), pack2(x[j][0], x[j][1]),
+                    pack2(x[j][2], x[j][3]));
+    }
+    cp_async_wait<G::kStages - 2>();  // the next tile
+    __syncthreads();                  // weights; and the next tile for all warps
+
+    // ---- O^T += V^T P^T: 64 dimensions of this warp ----
+    if (__any_sync(0xffffffffu, grown))
+#pragma unroll
+      for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[k][j][e] *= scale_o[j][e & 1];
+#pragma unroll
+    for (int kb = 0; kb < 4 / G::kTokenWarps; ++kb) {
+      const int token0 = 16 * (token_warp * (4 / G::kTokenWarps) + kb);
+      uint32_t w[4];
+      ldsm_x4_trans(stage + kTile * G::kRow + chunk_at<G::kRow>(token0 + (lane & 15), 2 * dim_warp + (lane >> 4)), w[0], w[1],
+                    w[2], w[3]);
+      const uint32_t scales = stage + 2 * kTile * G::kRow + (kTile + token0 + 2 * t) * G::kScale + 4 * dim_warp;
+      const uint32_t s0 = lds32(scales), s1 = lds32(scales + G::kScale), s2 = lds32(scales + 8 * G::kScale),
+                     s3 = lds32(scales + 9 * G::kScale);
+      const uint32_t ssa = __byte_perm(s0, s1, 0x5410), cca = __byte_perm(s0, s1, 0x7632);
+      const uint32_t ssb = __byte_perm(s2, s3, 0x5410), ccb = __byte_perm(s2, s3, 0x7632);
+      uint32_t a[4][4];
+      auto take = [&](auto place_k) {
+        constexpr int K = decltype(place_k)::value;
+        a[K][0] = kv4_pair<K>(w[0], ssa, cca), a[K][1] = kv4_pair<K>(w[2], ssa, cca);
+        a[K][2] = kv4_pair<K>(w[1], ssb, ccb), a[K][3] = kv4_pair<K>(w[3], ssb, ccb);
+      };
+      take(std::integral_constant<int, 0>{}), take(std::integral_constant<int, 1>{});
+      take(std::integral_constant<int, 2>{}), take(std::integral_constant<int, 3>{});
+      const uint32_t weights = sm + G::kOffP + g * G::kPRow + 2 * (token0 + 2 * t);
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        const uint32_t b0 = lds32(weights + 8 * j * G::kPRow), b1 = lds32(weights + 8 * j * G::kPRow + 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_bf16_m16n8k16(o[k][j], a[k][0], a[k][1], a[k][2], a[k][3], b0, b1);
+      }
+    }
+    if (masked_rows) {
+      const uint64_t bits = (static_cast<uint64_t>(bad[i & 1][dim_warp][1]) << 32 | bad[i & 1][dim_warp][0]) & ok_bits;
+      if (bits)
+        for (int j = 0; j < NQ; ++j)
+          for (int e = 0; e < 2; ++e) {
+            const int last = cur.len - p.q_len + row_query[8 * j + 2 * t + e] - pos0;
+            if (last >= 0 && (bits & (last >= 63 ? ~0ull : (2ull << last) - 1)))
+              for (int k = 0; k < 4; ++k) o[k][j][e] = o[k][j][2 + e] = __int_as_float(0x7fffffff);
+          }
+    }
+
+    // ---- the end of a (request, head), or of this CTA's share of it ----
+    const bool last_tile = cur.tile + 1 == cur.tiles;
+    if (last_tile || i + 1 == count) {
+#pragma unroll
+      for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], off);
+      if (g == 0)
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+          *reinterpret_cast<float2*>(&red[warp][8 * j + 2 * t]) = make_float2(l[j][0], l[j][1]);
+      // the token warps' sums, in halves
+      float4* sums = reinterpret_cast<float4*>(smem + G::kOffQ);
+#pragma unroll
+      for (int half = G::kTokenWarps / 2; half >= 1; half /= 2) {
+        if (half < G::kTokenWarps / 2) __syncthreads();
+        if (token_warp >= half && token_warp < 2 * half)
+#pragma unroll
+          for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              sums[(((token_warp - half) * G::kDimWarps + dim_warp) * NQ * 4 + j * 4 + k) * 32 + lane] =
+                  make_float4(o[k][j][0], o[k][j][1], o[k][j][2], o[k][j][3]);
+        __syncthreads();
+        if (token_warp < half)
+#pragma unroll
+          for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float4 v = sums[((token_warp * G::kDimWarps + dim_warp) * NQ * 4 + j * 4 + k) * 32 + lane];
+              o[k][j][0] += v.x, o[k][j][1] += v.y, o[k][j][2] += v.z, o[k][j][3] += v.w;
+            }
+      }
+      if (G::kTokenWarps == 1) __syncthreads();  // the sums l
+      if (token_warp == 0) {
+        const bool whole = first_tile == 0 && last_tile;
+        // a share that begins with the CTA's is its first, else its last
+        const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (i + 1 - (cur.tile + 1 - first_tile) == 0 ? 0 : 1);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = 8 * j + 2 * t + e;
+            if (r >= p.rows) continue;
+            const float sum = red[0][r] + red[1][r] + red[2][r] + red[3][r];
+            const int d = 64 * dim_warp + 4 * g;
+            if (whole) {
+              const float n = sum == 0.f ? 0.f : 1.f / sum;  // no key: zeros
+              const int qi = row_query[r], hq = cur.h * p.group + r - qi * p.group;
+              __nv_bfloat16* dst = p.out + (static_cast<int64_t>(cur.b) * p.q_len + qi) * p.ot + hq * p.oh + d;
+              *reinterpret_cast<uint2*>(dst) =
+                  make_uint2(pack2(o[0][j][e] * n, o[1][j][e] * n), pack2(o[2][j][e] * n, o[3][j][e] * n));
+              *reinterpret_cast<uint2*>(dst + 32) = make_uint2(pack2(o[0][j][2 + e] * n, o[1][j][2 + e] * n),
+                                                               pack2(o[2][j][2 + e] * n, o[3][j][2 + e] * n));
+            } else {
+              float* dst = p.part_o + (part * p.rows + r) * D + d;
+              *reinterpret_cast<float4*>(dst) = make_float4(o[0][j][e], o[1][j][e], o[2][j][e], o[3][j][e]);
+              *reinterpret_cast<float4*>(dst + 32) =
+                  make_float4(o[0][j][2 + e], o[1][j][2 + e], o[2][j][2 + e], o[3][j][2 + e]);
+              if (dim_warp == 0 && g == 0) p.part_ml[part * p.rows + r] = make_float2(m[j][e], sum);
+            }
+          }
+      }
+      fresh = true;
+      __syncthreads();  // the query's place and `red` are free again
+    }
+    if (i + 1 < count) cur.next(p);
+  }
 }
+
+// Joins the parts of a (request, head) that several CTAs held: one CTA for each query row, a thread for each two dimensions.
+template <int D> __global__ void __launch_bounds__(D / 2) kv4_join_kernel(const AttnParams p, int grid) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int r = blockIdx.y, b = blockIdx.x / p.cache.heads, h = blockIdx.x % p.cache.heads;
+  const int64_t heads = p.cache.heads;
+  const int before = p.tiles_before[b], after = p.tiles_before[b + 1];
+  const int64_t total = p.tiles_before[p.reqs] * heads;
+  const int ctas = static_cast<int>(min(total, static_cast<int64_t>(grid)));
+  const int64_t first = before * heads + static_cast<int64_t>(h) * (after - before), last = first + (after - before) - 1;
+  // the CTA whose share holds tile x is the last i with total * i / ctas <= x
+  const int i0 = static_cast<int>(((first + 1) * ctas - 1) / total), i1 = static_cast<int>(((last + 1) * ctas - 1) / total);
+  if (i0 == i1) return;
+  auto part_of = [&](int i) {
+    return 2 * static_cast<int64_t>(i) + (i == i0 && part_start(total, ctas, i) != first ? 1 : 0);
+  };
+  float m = -INFINITY;
+  for (int i = i0; i <= i1; ++i) m = fmaxf(m, p.part_ml[part_of(i) * p.rows + r].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float sum = 0.f;
+  float2 acc = make_float2(0.f, 0.f);
+  for (int i = i0; i <= i1; ++i) {
+    const int64_t at = part_of(i) * p.rows + r;
+    const float2 ml = p.part_ml[at];
+    const float w = ex2_approx(ml.x - ref);
+    const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * D + 2 * threadIdx.x);
+    sum = fmaf(ml.y, w, sum);
+    acc.x = fmaf(v.x, w, acc.x), acc.y = fmaf(v.y, w, acc.y);
+  }
+  const float n = sum == 0.f ? 0.f : 1.f / sum;
+  const int qi = r / p.group, hq = h * p.group + r - qi * p.group;
+  *reinterpret_cast<uint32_t*>(p.out + (static_cast<int64_t>(b) * p.q_len + qi) * p.ot + hq * p.oh + 2 * threadIdx.x) =
+      pack2(acc.x * n, acc.y * n);
+}
+
+int tiles_of_rows(int rows) {
+  const int n = (rows + 7) / 8;
+  return n == 5 ? 6 : n == 7 ? 8 : n;
+}
+
+// CTAs of an SM (Geo::kCtas).
+int ctas_per_sm(int rows) {
+  const int n = tiles_of_rows(rows);
+  return n <= 1 ? 4 : n <= 4 ? 3 : 2;
+}
+
+template <int D, int NQ> cudaError_t launch(const AttnParams& p, int grid, int dev, bool pdl, cudaStream_t st) {
+  using G = Geo<D, NQ>;
+  static std::mutex mu;
+  static bool set[64] = {};
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (!set[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(kv4_attn_kernel<D, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
+      if (e != cudaSuccess) return e;
+      set[dev] = true;
+    }
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = G::kSmem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attn_kernel<D, NQ>, p);
+  if (e != cudaSuccess) return e;
+  cfg.gridDim = dim3(static_cast<unsigned>(p.reqs) * p.cache.heads, static_cast<unsigned>(p.rows));
+  cfg.blockDim = dim3(D / 2);
+  cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, p, grid);
+}
+
+template <int D> cudaError_t launch(const AttnParams& p, int grid, int dev, bool pdl, cudaStream_t st) {
+  switch (tiles_of_rows(p.rows)) {
+    case 1: return launch<D, 1>(p, grid, dev, pdl, st);
+    case 2: return launch<D, 2>(p, grid, dev, pdl, st);
+    case 3: return launch<D, 3>(p, grid, dev, pdl, st);
+    case 4: return launch<D, 4>(p, grid, dev, pdl, st);
+    case 6: return launch<D, 6>(p, grid, dev, pdl, st);
+    default: return launch<D, 8>(p, grid, dev, pdl, st);
+  }
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace qf
@@ -104,22 +598,25 @@ __global__ void __launch_bounds__(kSimpleThreads) kv4_attn_simple_kernel(const K
 using namespace qf;
 
 extern "C" size_t qf_kv4_attn_workspace_bytes(int num_reqs, int q_len, int num_heads, int num_kv_heads, int head_size) {
-  (void)num_reqs, (void)q_len, (void)num_heads, (void)num_kv_heads, (void)head_size;
-  return 256;
+  if (num_reqs <= 0 || q_len <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0) return 256;
+  const int64_t rows = static_cast<int64_t>(q_len) * (num_heads / num_kv_heads);
+  const size_t parts = 2 * static_cast<size_t>(kMaxSms) * ctas_per_sm(static_cast<int>(rows < 64 ? rows : 64));
+  return up256((static_cast<size_t>(num_reqs) + 1) * 4) + up256(parts * rows * 8) + parts * rows * head_size * 4;
 }
 
 extern "C" int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_kv4_cache* cache,
                            const int32_t* block_table, int64_t s_bt, int max_pages, const int32_t* seq_lens, void* out,
                            int64_t so_t, int64_t so_h, int num_reqs, int q_len, int num_heads, float scale, void* ws,
                            size_t ws_bytes, unsigned flags, void* stream) {
-  Kv4AttnParams p = {};
+  AttnParams p = {};
   int rc = kv4_view(cache, &p.cache);
   if (rc) return rc;
   if (num_reqs < 0 || q_len < 1 || num_heads < 0 || max_pages < 0) return fail(QF_ERR_SHAPE, "sizes");
   if (num_heads % cache->num_heads) return fail(QF_ERR_SHAPE, "query heads must be a multiple of the cache's heads");
   if (static_cast<int64_t>(q_len) * (num_heads / cache->num_heads) > 64)
     return fail(QF_ERR_SHAPE, "more than 64 query rows for a key head");
-  if (static_cast<int64_t>(num_reqs) * q_len > INT32_MAX / 64 || num_heads > 65535)
+  if (static_cast<int64_t>(num_reqs) * q_len > INT32_MAX / 64 || num_heads > 65535 ||
+      static_cast<int64_t>(num_reqs) * cache->num_heads > INT32_MAX)
     return fail(QF_ERR_SHAPE, "too many query rows");
   if (!(scale > -3.4e38f && scale < 3.4e38f)) return fail(QF_ERR_INVALID, "scale must be finite");
   if (num_reqs == 0 || num_heads == 0) return QF_OK;
@@ -131,24 +628,33 @@ extern "C" int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_k
     return fail(QF_ERR_ALIGN, "query and out 16-byte aligned with strides multiples of eight, workspace 256-byte aligned");
   if (!ws || ws_bytes < qf_kv4_attn_workspace_bytes(num_reqs, q_len, num_heads, cache->num_heads, cache->head_size))
     return fail(QF_ERR_WORKSPACE, "workspace missing or too small");
-  rc = require_b200(nullptr, nullptr);
+  int dev = 0, sms = 0;
+  rc = require_b200(&dev, &sms);
   if (rc) return rc;
   p.q = static_cast<const __nv_bfloat16*>(q), p.qt = sq_t, p.qh = sq_h;
   p.out = static_cast<__nv_bfloat16*>(out), p.ot = so_t, p.oh = so_h;
-  p.table = block_table, p.table_row = s_bt, p.max_pages = max_pages;
+  p.table = block_table, p.table_row = s_bt;
+  p.width = static_cast<int64_t>(max_pages) * cache->page_size;
+  if (p.width > INT32_MAX - 4 * kTile) p.width = INT32_MAX - 4 * kTile;  // positions stay 32-bit numbers
   p.lens = seq_lens;
-  p.reqs = num_reqs, p.q_len = q_len, p.heads = num_heads, p.group = num_heads / cache->num_heads;
-  p.D = cache->head_size;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(num_reqs * q_len), static_cast<unsigned>(num_heads));
-  cfg.blockDim = dim3(kSimpleThreads);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = (flags & QF_FLAG_PDL) ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attn_simple_kernel, p);
+  p.reqs = num_reqs, p.q_len = q_len, p.group = num_heads / cache->num_heads, p.rows = q_len * p.group;
+  p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+  // n / page_size = (umulhi(n, mul) + n) >> shift for n below 2^31 (Granlund and Montgomery, PLDI 1994)
+  while ((1ull << p.div_shift) < static_cast<uint64_t>(cache->page_size)) ++p.div_shift;
+  p.div_mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << p.div_shift) - cache->page_size)) / cache->page_size + 1);
+  if (sms > kMaxSms) sms = kMaxSms;
+  const int grid = sms * ctas_per_sm(p.rows);
+  const size_t parts = 2 * static_cast<size_t>(kMaxSms) * ctas_per_sm(p.rows);
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  p.tiles_before = reinterpret_cast<int32_t*>(w);
+  w += up256((static_cast<size_t>(num_reqs) + 1) * 4);
+  p.part_ml = reinterpret_cast<float2*>(w);
+  w += up256(parts * p.rows * 8);
+  p.part_o = reinterpret_cast<float*>(w);
+  const bool pdl = (flags & QF_FLAG_PDL) != 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = cache->head_size == 64    ? launch<64>(p, grid, dev, pdl, st)
+                        : cache->head_size == 128 ? launch<128>(p, grid, dev, pdl, st)
+                                                  : launch<256>(p, grid, dev, pdl, st);
   return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
 }
