@@ -18,11 +18,15 @@
 // the two halves of a register, which is what the 16-bit operand wants: token pairs; each of the four nibble places is a
 // tile of 16 dimensions.
 //
-// A CTA of four warps takes 64 tokens at a time: each warp scores 16 of them against all rows, the maxima and then the
-// weights (bf16) are exchanged in shared memory, and each warp adds up 64 of the head's dimensions (over all tokens for
-// D = 256, over half or a quarter of them for 128 and 64).  Codes and scales arrive by cp.async, kStages - 1 tiles ahead;
-// the pages are looked up a tile before that.  The CTAs split all tiles of all requests and heads evenly, whatever the
-// lengths; a CTA's part may begin or end inside a (request, head), and a second kernel joins those.
+// A CTA of four warps takes 64 tokens at a time: each warp scores 16 of them against all rows, the weights (bf16) are
+// exchanged in shared memory, and each warp adds up 64 of the head's dimensions (over all tokens for D = 256, over half or a
+// quarter of them for 128 and 64).  The weights are relative to a reference, not to the maximum itself: bf16 and fp32 have
+// the same range of exponents, so that any reference within 2^16 of the maximum gives the same relative precision.  It is
+// set by the first tile and raised, with the exchange that this needs, only where a score exceeds it by more than 16.
+//
+// Codes and scales arrive by cp.async, kAhead tiles ahead; the pages are looked up a tile before that.  The CTAs split all
+// tiles of all requests and heads evenly, whatever the lengths; a CTA's part may begin or end inside a (request, head), and
+// a second kernel joins those.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -57,21 +61,23 @@ struct AttnParams {
   uint32_t div_mul, div_shift;  // by the page size
   float scale_log2;
   // workspace
-  int32_t* tiles_before;  // [reqs + 1]: tiles of one head before each request
-  float2* part_ml;        // [2 * grid][rows]
-  float* part_o;          // [2 * grid][rows][D]
+  int4* joins;      // [grid]: the (request, head) that begins in a CTA's share and ends in a later one's
+  float2* part_ml;  // [2 * grid][rows]: reference and sum
+  float* part_o;    // [2 * grid][rows][D]
 };
 
 template <int D, int NQ> struct Geo {
   static constexpr int kRow = D / 2;                       // bytes of a token's codes
   static constexpr int kScale = D / 16;                    // bytes of a token's scales
-  static constexpr int kStageBytes = 2 * kTile * (kRow + kScale);
-  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kSide = kTile * (kRow + kScale);    // bytes of a tile's keys, or values
+  // A tile's keys are done with when its weights are exchanged, its values a tile later.
+  static constexpr int kAhead = D == 64 ? 3 : 2, kKeyStages = kAhead, kValueStages = kAhead + 1;
   static constexpr int kCtas = NQ <= 1 ? 4 : NQ <= 4 ? 3 : 2;  // of an SM
   static constexpr int kPRow = 2 * kTile + 16;             // bytes of a query row's weights, one chunk of padding
   static constexpr int kQBytes = 4096 * NQ;                // the query's fragments; at a part's end the warps' sums
   static constexpr int kPBytes = 8 * NQ * kPRow;
-  static constexpr int kOffQ = kStages * kStageBytes;
+  static constexpr int kOffV = kKeyStages * kSide;
+  static constexpr int kOffQ = kOffV + kValueStages * kSide;
   static constexpr int kOffP = kOffQ + kQBytes;
   static constexpr int kSmem = kOffP + kPBytes;
   static constexpr int kDimWarps = D / 64, kTokenWarps = 4 / kDimWarps;
@@ -125,6 +131,9 @@ struct Cursor {
   }
 };
 
+constexpr float kNoRef = -3e38f;  // stands for the reference of a row that has seen no key, in a part that is joined
+constexpr float kSlack = 16.f;
+
 __device__ __forceinline__ int64_t part_start(int64_t total, int ctas, int i) { return total * i / ctas; }
 
 template <int D, int NQ>
@@ -132,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
   using G = Geo<D, NQ>;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t offs[kTile][2];           // of the tile that is copied next: codes (bytes), scales (elements)
-  __shared__ uint32_t there[G::kStages][2];    // a bit for each token of a stage
+  __shared__ uint32_t there[G::kAhead + 1][2];  // a bit for each token of a tile
   __shared__ float red[4][8 * NQ];
   __shared__ uint32_t bad[2][4][2];            // tokens whose values' group is not finite, of a tile with masked rows
   __shared__ int scan[4], found[3];
@@ -146,6 +155,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
   // ---- this CTA's part: a scan over the requests, twice (for the sum, then for where the part begins) ----
   int64_t total = 0;
   int64_t begin = 0, end = 0;
+  int ctas = 0;
   for (int pass = 0; pass < 2; ++pass) {
     int64_t base = 0;
     for (int b0 = 0; b0 < p.reqs; b0 += kThreads) {
@@ -165,18 +175,18 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
         if (w < warp) before += scan[w];
         base += scan[w];
       }
-      if (pass == 0) {
-        if (blockIdx.x == 0 && b < p.reqs) p.tiles_before[b] = static_cast<int32_t>(before);
-      } else if (n && before * p.cache.heads <= begin && begin < (before + n) * p.cache.heads) {
+      if (pass == 1 && n && before * p.cache.heads <= begin && begin < (before + n) * p.cache.heads) {
         const int64_t in = begin - before * p.cache.heads;
         found[0] = b, found[1] = static_cast<int>(in / n), found[2] = static_cast<int>(in % n);
       }
     }
     if (pass == 0) {
-      if (blockIdx.x == 0 && tid == 0) p.tiles_before[p.reqs] = static_cast<int32_t>(base);
       total = base * p.cache.heads;
-      const int ctas = static_cast<int>(min(total, static_cast<int64_t>(gridDim.x)));
-      if (static_cast<int>(blockIdx.x) >= ctas) return;
+      ctas = static_cast<int>(min(total, static_cast<int64_t>(gridDim.x)));
+      if (static_cast<int>(blockIdx.x) >= ctas) {
+        if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        return;
+      }
       begin = part_start(total, ctas, blockIdx.x), end = part_start(total, ctas, blockIdx.x + 1);
     }
   }
@@ -209,12 +219,12 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
       offs[tid][0] = -1;
     }
     const uint32_t bits = __ballot_sync(0xffffffffu, ok);
-    if (lane == 0) there[i % G::kStages][warp] = bits;
+    if (lane == 0) there[i % (G::kAhead + 1)][warp] = bits;
     if (i + 1 < count) ahead.next(p);
   };
   auto copy = [&](int i) {
     if (i < count) {
-      const uint32_t stage = sm + (i % G::kStages) * G::kStageBytes;
+      const uint32_t keys = sm + (i % G::kKeyStages) * G::kSide, vals = sm + G::kOffV + (i % G::kValueStages) * G::kSide;
       constexpr int kChunks = G::kRow / 16;
 #pragma unroll
       for (int j = 0; j < kTile * kChunks / kThreads; ++j) {
@@ -222,19 +232,19 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
         const int64_t o = offs[token][0];
         const bool ok = o >= 0;
         const int64_t at = ok ? o + 16 * c : 0;
-        const uint32_t dst = stage + chunk_at<G::kRow>(token, c);
-        copy_async<16>(dst, p.cache.codes[0] + at, ok);
-        copy_async<16>(dst + kTile * G::kRow, p.cache.codes[1] + at, ok);
+        const uint32_t dst = chunk_at<G::kRow>(token, c);
+        copy_async<16>(keys + dst, p.cache.codes[0] + at, ok);
+        copy_async<16>(vals + dst, p.cache.codes[1] + at, ok);
       }
       const int token = tid % kTile, side = tid / kTile;
       const bool ok = offs[token][0] >= 0;
-      copy_async<G::kScale>(stage + 2 * kTile * G::kRow + (side * kTile + token) * G::kScale,
+      copy_async<G::kScale>((side ? vals : keys) + kTile * G::kRow + token * G::kScale,
                             p.cache.scale[side] + (ok ? offs[token][1] : 0), ok);
     }
     cp_async_commit();
   };
   look(0);
-  for (int i = 0; i < G::kStages - 1; ++i) {
+  for (int i = 0; i < G::kAhead; ++i) {
     if (i < count) place(i);
     look(i + 1);
     __syncthreads();
@@ -244,8 +254,9 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
 
   // ---- a part of one (request, head) after the other ----
   float o[4][NQ][4];  // [nibble place][rows' tile][fragment]: O^T of this warp's 64 dimensions
-  float m[NQ][2], l[NQ][2];
+  float ref[NQ][2], l[NQ][2];
   const int dim_warp = warp % G::kDimWarps, token_warp = warp / G::kDimWarps;
+  uint32_t unset = 0;  // a bit for each ref of a row that has seen no key (its ref is 0)
   bool fresh = true;
   int first_tile = 0;
   for (int i = 0; i < count; ++i) {
@@ -266,27 +277,29 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
       }
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
-        m[j][0] = m[j][1] = -INFINITY, l[j][0] = l[j][1] = 0.f;
+        ref[j][0] = ref[j][1] = l[j][0] = l[j][1] = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k][j][0] = o[k][j][1] = o[k][j][2] = o[k][j][3] = 0.f;
       }
+      unset = (1u << 2 * NQ) - 1;
       first_tile = cur.tile;
       fresh = false;
-      if (i == 0) cp_async_wait<G::kStages - 2>();
+      if (i == 0) cp_async_wait<G::kAhead - 1>();
       __syncthreads();
     }
-    const uint32_t stage = sm + (i % G::kStages) * G::kStageBytes;
+    const uint32_t keys = sm + (i % G::kKeyStages) * G::kSide, vals = sm + G::kOffV + (i % G::kValueStages) * G::kSide;
     const int pos0 = cur.tile * kTile;
     const bool masked_rows = pos0 + kTile - 1 > cur.len - p.q_len;  // some row does not see some token of the tile
-    const uint64_t ok_bits = static_cast<uint64_t>(there[i % G::kStages][1]) << 32 | there[i % G::kStages][0];
-    if (i + G::kStages - 1 < count) place(i + G::kStages - 1);
-    look(i + G::kStages);
+    const uint64_t ok_bits =
+        static_cast<uint64_t>(there[i % (G::kAhead + 1)][1]) << 32 | there[i % (G::kAhead + 1)][0];
+    if (i + G::kAhead < count) place(i + G::kAhead);
+    look(i + G::kAhead + 1);
     if (masked_rows && tid < kTile) {
       // values that are not finite may be hidden from some rows only: they leave the product (a weight of zero would not
       // keep them out), and the rows that see one get their NaN afterwards
 #pragma unroll
       for (int gr = 0; gr < D / 64; ++gr) {
-        const uint32_t at = stage + 2 * kTile * G::kRow + (kTile + tid) * G::kScale + 4 * gr;
+        const uint32_t at = vals + kTile * G::kRow + tid * G::kScale + 4 * gr;
         const uint32_t sc = lds32(at);
         const float s = bf16_lo(sc), c = bf16_hi(sc);
         const bool is_bad = !(fabsf(s) < 2.6584559915698317e36f && fabsf(c) < 8.507059173023462e37f);  // 2^121, 2^126
@@ -298,15 +311,19 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
 
     // ---- scores of this warp's 16 tokens ----
     float x[NQ][4];
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
     {
+      constexpr int kChains = NQ <= 2 ? 2 : 1;  // sums of their own for every second group where there are few to take turns
+      float y[kChains][NQ][4];
+#pragma unroll
+      for (int c = 0; c < kChains; ++c)
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) y[c][j][0] = y[c][j][1] = y[c][j][2] = y[c][j][3] = 0.f;
       const uint32_t row = 16 * warp + (lane & 15);          // ldmatrix: lanes 0-15 a chunk's rows, 16-31 the next chunk's
-      const uint32_t scales = stage + 2 * kTile * G::kRow + (16 * warp + g) * G::kScale;
+      const uint32_t scales = keys + kTile * G::kRow + (16 * warp + g) * G::kScale;
 #pragma unroll
       for (int gr = 0; gr < D / 64; ++gr) {
         uint32_t w[4];
-        ldsm_x4(stage + chunk_at<G::kRow>(row, 2 * gr + (lane >> 4)), w[0], w[1], w[2], w[3]);
+        ldsm_x4(keys + chunk_at<G::kRow>(row, 2 * gr + (lane >> 4)), w[0], w[1], w[2], w[3]);
         const uint32_t sa = lds32(scales + 4 * gr), sb = lds32(scales + 8 * G::kScale + 4 * gr);
         const uint32_t ssa = dup_lo(sa), cca = dup_hi(sa), ssb = dup_lo(sb), ccb = dup_hi(sb);
 #pragma unroll
@@ -318,16 +335,21 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
 #pragma unroll
           for (int j = 0; j < NQ; ++j) {
             const uint4 q = lds128(sm + G::kOffQ + (((2 * gr + h) * NQ + j) * 32 + lane) * 16);
-            mma_bf16_m16n8k16(x[j], a0, a1, a2, a3, q.x, q.y);
-            mma_bf16_m16n8k16(x[j], b0, b1, b2, b3, q.z, q.w);
+            mma_bf16_m16n8k16(y[h % kChains][j], a0, a1, a2, a3, q.x, q.y);
+            mma_bf16_m16n8k16(y[h % kChains][j], b0, b1, b2, b3, q.z, q.w);
           }
         }
       }
+#pragma unroll
+      for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[j][e] = kChains == 2 ? y[0][j][e] + y[kChains - 1][j][e] : y[0][j][e];
     }
+    // distances to the reference: the weights are 2^x from here on
 #pragma unroll
     for (int j = 0; j < NQ; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[j][e] *= p.scale_log2;
+      for (int e = 0; e < 4; ++e) x[j][e] = fmaf(x[j][e], p.scale_log2, -ref[j][e & 1]);
     if (masked_rows || ~ok_bits) {
       const int ta = 16 * warp + g;
       const bool oka = ok_bits >> ta & 1, okb = ok_bits >> (ta + 8) & 1;
@@ -340,52 +362,66 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
           if (!(okb && ta + 8 <= last)) x[j][2 + e] = -INFINITY;
         }
     }
-    float top[NQ][2];
+    float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < NQ; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float v = fmaxf(x[j][e], x[j][2 + e]);
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-        top[j][e] = v;
-      }
-    if (g == 0)
+    for (int j = 0; j < NQ; ++j) top = fmaxf(top, fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])));
+    if (unset)
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
-        *reinterpret_cast<float2*>(&red[warp][8 * j + 2 * t]) = make_float2(top[j][0], top[j][1]);
-    __syncthreads();  // maxima; and all warps have left the last tile, whose stage is filled again now
-    copy(i + G::kStages - 1);
-
-    // ---- weights ----
-    bool grown = false;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (unset >> (2 * j + e) & 1 && fmaxf(x[j][e], x[j][2 + e]) > -INFINITY) top = INFINITY;
+    // (all warps have read this tile's keys and the last one's values, whose stages are filled again now)
+    const bool raise = __syncthreads_or(top > kSlack);
+    copy(i + G::kAhead);
     float scale_o[NQ][2];
+    if (raise) {
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        float v[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          v[e] = fmaxf(x[j][e], x[j][2 + e]);
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) v[e] = fmaxf(v[e], __shfl_xor_sync(0xffffffffu, v[e], off));
+        }
+        if (g == 0) *reinterpret_cast<float2*>(&red[warp][8 * j + 2 * t]) = make_float2(v[0], v[1]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        float v[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 r = *reinterpret_cast<const float2*>(&red[k][8 * j + 2 * t]);
+          v[0] = fmaxf(v[0], r.x), v[1] = fmaxf(v[1], r.y);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t bit = 1u << (2 * j + e);
+          // a row's first reference is its maximum so far, whatever its sign; later ones only rise
+          const float rise = !(unset & bit) ? fmaxf(v[e], 0.f) : v[e] == -INFINITY ? 0.f : v[e];
+          scale_o[j][e] = unset & bit ? 1.f : ex2_approx(-rise);  // (sums of an unset row are zero, or NaN for good)
+          if (v[e] > -INFINITY) unset &= ~bit;
+          l[j][e] *= scale_o[j][e];
+          ref[j][e] += rise;
+          x[j][e] -= rise, x[j][2 + e] -= rise;
+        }
+      }
+    }
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float2 v = *reinterpret_cast<const float2*>(&red[w][8 * j + 2 * t]);
-        top[j][0] = fmaxf(top[j][0], v.x), top[j][1] = fmaxf(top[j][1], v.y);
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float next = fmaxf(m[j][e], top[j][e]);
-        const float ref = next == -INFINITY ? 0.f : next;  // a row that has seen no key
-        scale_o[j][e] = ex2_approx(m[j][e] - ref);
-        grown |= next > m[j][e];
-        m[j][e] = next;
-        const float pa = ex2_approx(x[j][e] - ref), pb = ex2_approx(x[j][2 + e] - ref);
-        x[j][e] = pa, x[j][2 + e] = pb;
-        l[j][e] = fmaf(l[j][e], scale_o[j][e], pa + pb);
-      }
+      for (int e = 0; e < 4; ++e) x[j][e] = ex2_approx(x[j][e]);
+      l[j][0] += x[j][0] + x[j][2], l[j][1] += x[j][1] + x[j][3];
       stsm_x2_trans(sm + G::kOffP + (8 * j + (lane & 7)) * G::kPRow + 2 * (16 * warp + (lane & 8)), pack2(x[j][0], x[j][1]),
                     pack2(x[j][2], x[j][3]));
     }
-    cp_async_wait<G::kStages - 2>();  // the next tile
-    __syncthreads();                  // weights; and the next tile for all warps
+    cp_async_wait<G::kAhead - 1>();  // the next tile
+    __syncthreads();                 // weights; and the next tile for all warps
 
     // ---- O^T += V^T P^T: 64 dimensions of this warp ----
-    if (__any_sync(0xffffffffu, grown))
+    if (raise)
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -396,9 +432,9 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
     for (int kb = 0; kb < 4 / G::kTokenWarps; ++kb) {
       const int token0 = 16 * (token_warp * (4 / G::kTokenWarps) + kb);
       uint32_t w[4];
-      ldsm_x4_trans(stage + kTile * G::kRow + chunk_at<G::kRow>(token0 + (lane & 15), 2 * dim_warp + (lane >> 4)), w[0], w[1],
+      ldsm_x4_trans(vals + chunk_at<G::kRow>(token0 + (lane & 15), 2 * dim_warp + (lane >> 4)), w[0], w[1],
                     w[2], w[3]);
-      const uint32_t scales = stage + 2 * kTile * G::kRow + (kTile + token0 + 2 * t) * G::kScale + 4 * dim_warp;
+      const uint32_t scales = vals + kTile * G::kRow + (token0 + 2 * t) * G::kScale + 4 * dim_warp;
       const uint32_t s0 = lds32(scales), s1 = lds32(scales + G::kScale), s2 = lds32(scales + 8 * G::kScale),
                      s3 = lds32(scales + 9 * G::kScale);
       const uint32_t ssa = __byte_perm(s0, s1, 0x5410), cca = __byte_perm(s0, s1, 0x7632);
@@ -491,9 +527,16 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
               *reinterpret_cast<float4*>(dst) = make_float4(o[0][j][e], o[1][j][e], o[2][j][e], o[3][j][e]);
               *reinterpret_cast<float4*>(dst + 32) =
                   make_float4(o[0][j][2 + e], o[1][j][2 + e], o[2][j][2 + e], o[3][j][2 + e]);
-              if (dim_warp == 0 && g == 0) p.part_ml[part * p.rows + r] = make_float2(m[j][e], sum);
+              if (dim_warp == 0 && g == 0) p.part_ml[part * p.rows + r] = make_float2(unset >> (2 * j + e) & 1 ? kNoRef : ref[j][e], sum);
             }
           }
+      }
+      if (i + 1 == count && tid == 0) {
+        // the CTA that begins a (request, head) which others end names it for the join
+        const bool open = first_tile == 0 && !last_tile;
+        const int64_t end_tile = end - 1 + (cur.tiles - 1 - cur.tile);  // its last tile; the CTA that holds it: the last
+        const int to = static_cast<int>(((end_tile + 1) * ctas - 1) / total);  // one whose share begins at or before it
+        p.joins[blockIdx.x] = open ? make_int4(cur.b, cur.h, to, cur.tile + 1 == count ? 0 : 1) : make_int4(-1, 0, 0, 0);
       }
       fresh = true;
       __syncthreads();  // the query's place and `red` are free again
@@ -502,39 +545,93 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
   }
 }
 
-// Joins the parts of a (request, head) that several CTAs held: one CTA for each query row, a thread for each two dimensions.
-template <int D> __global__ void __launch_bounds__(D / 2) kv4_join_kernel(const AttnParams p, int grid) {
+// Joins the parts of each (request, head) that several CTAs held.  Work is a (join, row, 64 dimensions): 16 threads a part,
+// four dimensions each.
+constexpr int kJoinThreads = 256, kJoinDims = 64, kJoinGroups = kJoinThreads / (kJoinDims / 4), kJoinEarly = 8;
+constexpr int kMaxCtas = 4;  // of an SM
+
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const AttnParams p, int grid, int D) {
+  __shared__ int list[kMaxSms * kMaxCtas];
+  __shared__ float weight[kMaxSms * kMaxCtas];
+  __shared__ float warp_val[kJoinThreads / 32];
+  __shared__ int warp_count[kJoinThreads / 32];
+  __shared__ float4 sums[kJoinGroups][kJoinDims / 4];
   pdl_launch_dependents();
   pdl_wait();
-  const int r = blockIdx.y, b = blockIdx.x / p.cache.heads, h = blockIdx.x % p.cache.heads;
-  const int64_t heads = p.cache.heads;
-  const int before = p.tiles_before[b], after = p.tiles_before[b + 1];
-  const int64_t total = p.tiles_before[p.reqs] * heads;
-  const int ctas = static_cast<int>(min(total, static_cast<int64_t>(grid)));
-  const int64_t first = before * heads + static_cast<int64_t>(h) * (after - before), last = first + (after - before) - 1;
-  // the CTA whose share holds tile x is the last i with total * i / ctas <= x
-  const int i0 = static_cast<int>(((first + 1) * ctas - 1) / total), i1 = static_cast<int>(((last + 1) * ctas - 1) / total);
-  if (i0 == i1) return;
-  auto part_of = [&](int i) {
-    return 2 * static_cast<int64_t>(i) + (i == i0 && part_start(total, ctas, i) != first ? 1 : 0);
-  };
-  float m = -INFINITY;
-  for (int i = i0; i <= i1; ++i) m = fmaxf(m, p.part_ml[part_of(i) * p.rows + r].x);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float sum = 0.f;
-  float2 acc = make_float2(0.f, 0.f);
-  for (int i = i0; i <= i1; ++i) {
-    const int64_t at = part_of(i) * p.rows + r;
-    const float2 ml = p.part_ml[at];
-    const float w = ex2_approx(ml.x - ref);
-    const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * D + 2 * threadIdx.x);
-    sum = fmaf(ml.y, w, sum);
-    acc.x = fmaf(v.x, w, acc.x), acc.y = fmaf(v.y, w, acc.y);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int n = 0;
+  for (int i0 = 0; i0 < grid; i0 += kJoinThreads) {
+    const bool named = i0 + tid < grid && p.joins[i0 + tid].x >= 0;
+    const uint32_t bits = __ballot_sync(0xffffffffu, named);
+    if (lane == 0) warp_count[warp] = __popc(bits);
+    __syncthreads();
+    int at = n;
+    for (int w = 0; w < kJoinThreads / 32; ++w) {
+      if (w < warp) at += warp_count[w];
+      n += warp_count[w];
+    }
+    if (named) list[at + __popc(bits & ((1u << lane) - 1))] = i0 + tid;
+    __syncthreads();
   }
-  const float n = sum == 0.f ? 0.f : 1.f / sum;
-  const int qi = r / p.group, hq = h * p.group + r - qi * p.group;
-  *reinterpret_cast<uint32_t*>(p.out + (static_cast<int64_t>(b) * p.q_len + qi) * p.ot + hq * p.oh + 2 * threadIdx.x) =
-      pack2(acc.x * n, acc.y * n);
+  const int pieces = D / kJoinDims, items = n * p.rows * pieces;
+  const int col = tid % (kJoinDims / 4), group = tid / (kJoinDims / 4);
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    const int piece = item % pieces, r = item / pieces % p.rows, from = list[item / pieces / p.rows];
+    const int4 join = p.joins[from];
+    const int parts = join.z - from + 1;
+    // part k is CTA from + k's first, or its last where the (request, head) begins inside its share
+    auto row_of = [&](int k) { return (2 * static_cast<int64_t>(from + k) + (k == 0 ? join.w : 0)) * p.rows + r; };
+    auto load = [&](int k) {
+      return *reinterpret_cast<const float4*>(p.part_o + row_of(k) * D + kJoinDims * piece + 4 * col);
+    };
+    float4 early[kJoinEarly];  // on their way while the weights are made
+#pragma unroll
+    for (int e = 0; e < kJoinEarly; ++e) {
+      early[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (group + e * kJoinGroups < parts) early[e] = load(group + e * kJoinGroups);
+    }
+    float top = kNoRef;
+    for (int k = tid; k < parts; k += kJoinThreads) top = fmaxf(top, p.part_ml[row_of(k)].x);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if (lane == 0) warp_val[warp] = top;
+    __syncthreads();
+    for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, warp_val[w]);
+    __syncthreads();
+    float sum = 0.f;
+    for (int k = tid; k < parts; k += kJoinThreads) {
+      const float2 ml = p.part_ml[row_of(k)];
+      const float w = ex2_approx(ml.x - top);
+      weight[k] = w;
+      sum = fmaf(ml.y, w, sum);
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane == 0) warp_val[warp] = sum;
+    __syncthreads();
+    sum = 0.f;
+    for (int w = 0; w < kJoinThreads / 32; ++w) sum += warp_val[w];
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float4& v, float w) {
+      acc.x = fmaf(v.x, w, acc.x), acc.y = fmaf(v.y, w, acc.y), acc.z = fmaf(v.z, w, acc.z), acc.w = fmaf(v.w, w, acc.w);
+    };
+#pragma unroll
+    for (int e = 0; e < kJoinEarly; ++e)
+      if (group + e * kJoinGroups < parts) add(early[e], weight[group + e * kJoinGroups]);
+#pragma unroll 4
+    for (int k = group + kJoinEarly * kJoinGroups; k < parts; k += kJoinGroups) add(load(k), weight[k]);
+    sums[group][col] = acc;
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int k = 1; k < kJoinGroups; ++k) add(sums[k][col], 1.f);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int qi = r / p.group, hq = join.y * p.group + r - qi * p.group;
+      __nv_bfloat16* dst = p.out + (static_cast<int64_t>(join.x) * p.q_len + qi) * p.ot + hq * p.oh + kJoinDims * piece + 4 * col;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
+    }
+    __syncthreads();
+  }
 }
 
 int tiles_of_rows(int rows) {
@@ -548,7 +645,7 @@ int ctas_per_sm(int rows) {
   return n <= 1 ? 4 : n <= 4 ? 3 : 2;
 }
 
-template <int D, int NQ> cudaError_t launch(const AttnParams& p, int grid, int dev, bool pdl, cudaStream_t st) {
+template <int D, int NQ> cudaError_t launch(const AttnParams& p, int grid, int dev, int sms, bool pdl, cudaStream_t st) {
   using G = Geo<D, NQ>;
   static std::mutex mu;
   static bool set[64] = {};
@@ -572,21 +669,21 @@ template <int D, int NQ> cudaError_t launch(const AttnParams& p, int grid, int d
   cfg.numAttrs = pdl ? 1 : 0;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attn_kernel<D, NQ>, p);
   if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3(static_cast<unsigned>(p.reqs) * p.cache.heads, static_cast<unsigned>(p.rows));
-  cfg.blockDim = dim3(D / 2);
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * sms));
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, p, grid);
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel, p, grid, D);
 }
 
-template <int D> cudaError_t launch(const AttnParams& p, int grid, int dev, bool pdl, cudaStream_t st) {
+template <int D> cudaError_t launch(const AttnParams& p, int grid, int dev, int sms, bool pdl, cudaStream_t st) {
   switch (tiles_of_rows(p.rows)) {
-    case 1: return launch<D, 1>(p, grid, dev, pdl, st);
-    case 2: return launch<D, 2>(p, grid, dev, pdl, st);
-    case 3: return launch<D, 3>(p, grid, dev, pdl, st);
-    case 4: return launch<D, 4>(p, grid, dev, pdl, st);
-    case 6: return launch<D, 6>(p, grid, dev, pdl, st);
-    default: return launch<D, 8>(p, grid, dev, pdl, st);
+    case 1: return launch<D, 1>(p, grid, dev, sms, pdl, st);
+    case 2: return launch<D, 2>(p, grid, dev, sms, pdl, st);
+    case 3: return launch<D, 3>(p, grid, dev, sms, pdl, st);
+    case 4: return launch<D, 4>(p, grid, dev, sms, pdl, st);
+    case 6: return launch<D, 6>(p, grid, dev, sms, pdl, st);
+    default: return launch<D, 8>(p, grid, dev, sms, pdl, st);
   }
 }
 
@@ -601,7 +698,7 @@ extern "C" size_t qf_kv4_attn_workspace_bytes(int num_reqs, int q_len, int num_h
   if (num_reqs <= 0 || q_len <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0) return 256;
   const int64_t rows = static_cast<int64_t>(q_len) * (num_heads / num_kv_heads);
   const size_t parts = 2 * static_cast<size_t>(kMaxSms) * ctas_per_sm(static_cast<int>(rows < 64 ? rows : 64));
-  return up256((static_cast<size_t>(num_reqs) + 1) * 4) + up256(parts * rows * 8) + parts * rows * head_size * 4;
+  return up256(parts / 2 * sizeof(int4)) + up256(parts * rows * 8) + parts * rows * head_size * 4;
 }
 
 extern "C" int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_kv4_cache* cache,
@@ -646,15 +743,15 @@ extern "C" int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_k
   const int grid = sms * ctas_per_sm(p.rows);
   const size_t parts = 2 * static_cast<size_t>(kMaxSms) * ctas_per_sm(p.rows);
   uint8_t* w = static_cast<uint8_t*>(ws);
-  p.tiles_before = reinterpret_cast<int32_t*>(w);
-  w += up256((static_cast<size_t>(num_reqs) + 1) * 4);
+  p.joins = reinterpret_cast<int4*>(w);
+  w += up256(parts / 2 * sizeof(int4));
   p.part_ml = reinterpret_cast<float2*>(w);
   w += up256(parts * p.rows * 8);
   p.part_o = reinterpret_cast<float*>(w);
   const bool pdl = (flags & QF_FLAG_PDL) != 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = cache->head_size == 64    ? launch<64>(p, grid, dev, pdl, st)
-                        : cache->head_size == 128 ? launch<128>(p, grid, dev, pdl, st)
-                                                  : launch<256>(p, grid, dev, pdl, st);
+  const cudaError_t e = cache->head_size == 64    ? launch<64>(p, grid, dev, sms, pdl, st)
+                        : cache->head_size == 128 ? launch<128>(p, grid, dev, sms, pdl, st)
+                                                  : launch<256>(p, grid, dev, sms, pdl, st);
   return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
 }
