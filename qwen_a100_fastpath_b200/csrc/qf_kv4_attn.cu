@@ -92,6 +92,13 @@ template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const 
   else
     asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(N) : "memory");
 }
+// As mma_bf16_m16n8k16, free to be moved among other instructions.
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 // Two 8x8 tiles of 16-bit elements into shared memory, transposed: lane l gives the address of row l % 8 of tile l / 8.
 __device__ __forceinline__ void stsm_x2_trans(uint32_t addr, uint32_t r0, uint32_t r1) {
   asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1, %2};" ::"r"(addr), "r"(r0), "r"(r1) : "memory");
@@ -119,6 +126,10 @@ __device__ __forceinline__ int keys_of(const AttnParams& p, int len) {
 }
 __device__ __forceinline__ int tiles_of(const AttnParams& p, int len) { return max((keys_of(p, len) - 1) / kTile + 1, 1); }
 
+// What a (request, head) costs besides its tiles, in tiles: the query, the first reference, the output.  The CTAs' shares are
+// even in these units: positions v below kStart in front of a (request, head)'s first tile, tile v - kStart behind.
+constexpr int kStart = 2;
+
 // A walk over tiles in the order (request, head, tile).
 struct Cursor {
   int b, h, tile, tiles, len;
@@ -145,6 +156,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
   __shared__ float red[4][8 * NQ];
   __shared__ uint32_t bad[2][4][2];            // tokens whose values' group is not finite, of a tile with masked rows
   __shared__ int scan[4], found[3];
+  __shared__ int64_t bounds[2];
   __shared__ uint8_t row_query[8 * NQ];        // qi of a row
   pdl_launch_dependents();
   pdl_wait();
@@ -152,33 +164,44 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
   const uint32_t sm = smem_u32(smem);
   for (int r = tid; r < 8 * NQ; r += kThreads) row_query[r] = r < p.rows ? r / p.group : 0;
 
-  // ---- this CTA's part: a scan over the requests, twice (for the sum, then for where the part begins) ----
-  int64_t total = 0;
-  int64_t begin = 0, end = 0;
-  int ctas = 0;
+  // ---- this CTA's part: a scan over the requests, twice (for the sum, then for where the part begins and ends) ----
+  int64_t total = 0, begin = 0, end = 0;
+  int ctas = 0, n = 0;
   for (int pass = 0; pass < 2; ++pass) {
     int64_t base = 0;
     for (int b0 = 0; b0 < p.reqs; b0 += kThreads) {
       const int b = b0 + tid;
-      const int n = b < p.reqs ? tiles_of(p, p.lens[b]) : 0;
-      int s = n;
+      if (pass == 0 || p.reqs > kThreads) n = b < p.reqs ? tiles_of(p, p.lens[b]) + kStart : 0;
+      int sum = n;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, s, off);
-        if (lane >= off) s += a;
+        const int a = __shfl_up_sync(0xffffffffu, sum, off);
+        if (lane >= off) sum += a;
       }
       __syncthreads();
-      if (lane == 31) scan[warp] = s;
+      if (lane == 31) scan[warp] = sum;
       __syncthreads();
-      int64_t before = base + s - n;
+      int64_t before = base + sum - n;
       for (int w = 0; w < 4; ++w) {
         if (w < warp) before += scan[w];
         base += scan[w];
       }
-      if (pass == 1 && n && before * p.cache.heads <= begin && begin < (before + n) * p.cache.heads) {
-        const int64_t in = begin - before * p.cache.heads;
-        found[0] = b, found[1] = static_cast<int>(in / n), found[2] = static_cast<int>(in % n);
+      if (pass == 0 || !n) continue;
+      before *= p.cache.heads;
+      const int64_t after = before + static_cast<int64_t>(n) * p.cache.heads;
+      // tiles before a position: all those before the request, those of its heads before, those before it
+      auto tiles_before = [&](int64_t v) {
+        const int in = static_cast<int>((v - before) / n), rest = static_cast<int>((v - before) % n);
+        return before - static_cast<int64_t>(kStart) * p.cache.heads * b + static_cast<int64_t>(in) * (n - kStart) +
+               max(rest - kStart, 0);
+      };
+      if (before <= begin && begin < after) {
+        found[0] = b, found[1] = static_cast<int>((begin - before) / n);
+        found[2] = max(static_cast<int>((begin - before) % n) - kStart, 0);
+        bounds[0] = tiles_before(begin);
       }
+      if (before < end && end <= after)
+        bounds[1] = end == after ? after - static_cast<int64_t>(kStart) * p.cache.heads * (b + 1) : tiles_before(end);
     }
     if (pass == 0) {
       total = base * p.cache.heads;
@@ -191,12 +214,33 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
     }
   }
   __syncthreads();
-  const int count = static_cast<int>(end - begin);
+  const int count = static_cast<int>(bounds[1] - bounds[0]);
+  if (count == 0) {
+    if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    return;
+  }
   Cursor cur;
   cur.b = found[0], cur.h = found[1], cur.tile = found[2];
   cur.len = p.lens[cur.b];
   cur.tiles = tiles_of(p, cur.len);
   Cursor ahead = cur;  // of the tile whose pages are looked up next (threads of tokens)
+
+  // the query's fragments: a thread's eight dimensions of a row in the order in which the nibbles come apart
+  auto query = [&] {
+    for (int e = tid; e < D / 32 * NQ * 32; e += kThreads) {
+      const int l5 = e & 31, j = (e >> 5) % NQ, c = (e >> 5) / NQ;
+      const int r = 8 * j + (l5 >> 2);
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (r < p.rows) {
+        const int qi = row_query[r], hq = cur.h * p.group + r - qi * p.group;
+        u = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(cur.b) * p.q_len + qi) * p.qt + hq * p.qh + 32 * c +
+                                            8 * (l5 & 3));
+      }
+      reinterpret_cast<uint4*>(smem + G::kOffQ)[e] =
+          make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410),
+                     __byte_perm(u.y, u.w, 0x7632));
+    }
+  };
 
   // ---- copies: threads of tokens look a page up, then all threads copy ----
   int32_t entry = -1;
@@ -207,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
     if (pos < keys_of(p, ahead.len))
       entry = p.table[ahead.b * p.table_row + ((__umulhi(pos, p.div_mul) + pos) >> p.div_shift)];
   };
-  auto place = [&](int i) {  // its offsets, and on to the next tile
+  auto place = [&](int i, int value_slot) {  // its offsets, and on to the next tile
     if (tid >= kTile) return;
     const bool ok = entry >= 0 && entry < p.cache.num_pages;
     if (ok) {
@@ -219,12 +263,12 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
       offs[tid][0] = -1;
     }
     const uint32_t bits = __ballot_sync(0xffffffffu, ok);
-    if (lane == 0) there[i % (G::kAhead + 1)][warp] = bits;
+    if (lane == 0) there[value_slot][warp] = bits;
     if (i + 1 < count) ahead.next(p);
   };
-  auto copy = [&](int i) {
+  auto copy = [&](int i, int key_slot, int value_slot) {
     if (i < count) {
-      const uint32_t keys = sm + (i % G::kKeyStages) * G::kSide, vals = sm + G::kOffV + (i % G::kValueStages) * G::kSide;
+      const uint32_t keys = sm + key_slot * G::kSide, vals = sm + G::kOffV + value_slot * G::kSide;
       constexpr int kChunks = G::kRow / 16;
 #pragma unroll
       for (int j = 0; j < kTile * kChunks / kThreads; ++j) {
@@ -244,11 +288,12 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
     cp_async_commit();
   };
   look(0);
+  query();
   for (int i = 0; i < G::kAhead; ++i) {
-    if (i < count) place(i);
+    if (i < count) place(i, i);
     look(i + 1);
     __syncthreads();
-    copy(i);
+    copy(i, i, i);
     __syncthreads();
   }
 
@@ -259,22 +304,10 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
   uint32_t unset = 0;  // a bit for each ref of a row that has seen no key (its ref is 0)
   bool fresh = true;
   int first_tile = 0;
+  int key_stage = 0, value_stage = 0;   // of tile i
   for (int i = 0; i < count; ++i) {
     if (fresh) {
-      // the query's fragments: a thread's eight dimensions of a row in the order in which the nibbles come apart
-      for (int e = tid; e < D / 32 * NQ * 32; e += kThreads) {
-        const int l5 = e & 31, j = (e >> 5) % NQ, c = (e >> 5) / NQ;
-        const int r = 8 * j + (l5 >> 2);
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (r < p.rows) {
-          const int qi = r / p.group, hq = cur.h * p.group + r - qi * p.group;
-          u = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(cur.b) * p.q_len + qi) * p.qt + hq * p.qh + 32 * c +
-                                              8 * (l5 & 3));
-        }
-        reinterpret_cast<uint4*>(smem + G::kOffQ)[e] =
-            make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410),
-                       __byte_perm(u.y, u.w, 0x7632));
-      }
+      if (i > 0) query();
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
         ref[j][0] = ref[j][1] = l[j][0] = l[j][1] = 0.f;
@@ -287,12 +320,13 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
       if (i == 0) cp_async_wait<G::kAhead - 1>();
       __syncthreads();
     }
-    const uint32_t keys = sm + (i % G::kKeyStages) * G::kSide, vals = sm + G::kOffV + (i % G::kValueStages) * G::kSide;
+    const uint32_t keys = sm + key_stage * G::kSide, vals = sm + G::kOffV + value_stage * G::kSide;
     const int pos0 = cur.tile * kTile;
     const bool masked_rows = pos0 + kTile - 1 > cur.len - p.q_len;  // some row does not see some token of the tile
     const uint64_t ok_bits =
-        static_cast<uint64_t>(there[i % (G::kAhead + 1)][1]) << 32 | there[i % (G::kAhead + 1)][0];
-    if (i + G::kAhead < count) place(i + G::kAhead);
+        static_cast<uint64_t>(there[value_stage][1]) << 32 | there[value_stage][0];
+    const int value_free = value_stage == 0 ? G::kValueStages - 1 : value_stage - 1;  // the last tile's
+    if (i + G::kAhead < count) place(i + G::kAhead, value_free);
     look(i + G::kAhead + 1);
     if (masked_rows && tid < kTile) {
       // values that are not finite may be hidden from some rows only: they leave the product (a weight of zero would not
@@ -328,16 +362,17 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
         const uint32_t ssa = dup_lo(sa), cca = dup_hi(sa), ssb = dup_lo(sb), ccb = dup_hi(sb);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          uint4 q[NQ];
+#pragma unroll
+          for (int j = 0; j < NQ; ++j) q[j] = reinterpret_cast<const uint4*>(smem + G::kOffQ)[((2 * gr + h) * NQ + j) * 32 + lane];
           const uint32_t a0 = kv4_pair<0>(w[2 * h], ssa, cca), a1 = kv4_pair<0>(w[2 * h + 1], ssb, ccb);
           const uint32_t a2 = kv4_pair<1>(w[2 * h], ssa, cca), a3 = kv4_pair<1>(w[2 * h + 1], ssb, ccb);
           const uint32_t b0 = kv4_pair<2>(w[2 * h], ssa, cca), b1 = kv4_pair<2>(w[2 * h + 1], ssb, ccb);
           const uint32_t b2 = kv4_pair<3>(w[2 * h], ssa, cca), b3 = kv4_pair<3>(w[2 * h + 1], ssb, ccb);
 #pragma unroll
-          for (int j = 0; j < NQ; ++j) {
-            const uint4 q = lds128(sm + G::kOffQ + (((2 * gr + h) * NQ + j) * 32 + lane) * 16);
-            mma_bf16_m16n8k16(y[h % kChains][j], a0, a1, a2, a3, q.x, q.y);
-            mma_bf16_m16n8k16(y[h % kChains][j], b0, b1, b2, b3, q.z, q.w);
-          }
+          for (int j = 0; j < NQ; ++j) mma(y[0][j], a0, a1, a2, a3, q[j].x, q[j].y);
+#pragma unroll
+          for (int j = 0; j < NQ; ++j) mma(y[kChains - 1][j], b0, b1, b2, b3, q[j].z, q[j].w);
         }
       }
 #pragma unroll
@@ -373,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
           if (unset >> (2 * j + e) & 1 && fmaxf(x[j][e], x[j][2 + e]) > -INFINITY) top = INFINITY;
     // (all warps have read this tile's keys and the last one's values, whose stages are filled again now)
     const bool raise = __syncthreads_or(top > kSlack);
-    copy(i + G::kAhead);
+    copy(i + G::kAhead, key_stage, value_free);
     float scale_o[NQ][2];
     if (raise) {
 #pragma unroll
@@ -439,21 +474,22 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
                      s3 = lds32(scales + 9 * G::kScale);
       const uint32_t ssa = __byte_perm(s0, s1, 0x5410), cca = __byte_perm(s0, s1, 0x7632);
       const uint32_t ssb = __byte_perm(s2, s3, 0x5410), ccb = __byte_perm(s2, s3, 0x7632);
-      uint32_t a[4][4];
-      auto take = [&](auto place_k) {
-        constexpr int K = decltype(place_k)::value;
-        a[K][0] = kv4_pair<K>(w[0], ssa, cca), a[K][1] = kv4_pair<K>(w[2], ssa, cca);
-        a[K][2] = kv4_pair<K>(w[1], ssb, ccb), a[K][3] = kv4_pair<K>(w[3], ssb, ccb);
-      };
-      take(std::integral_constant<int, 0>{}), take(std::integral_constant<int, 1>{});
-      take(std::integral_constant<int, 2>{}), take(std::integral_constant<int, 3>{});
-      const uint32_t weights = sm + G::kOffP + g * G::kPRow + 2 * (token0 + 2 * t);
+      const uint8_t* weights = smem + G::kOffP + g * G::kPRow + 2 * (token0 + 2 * t);
+      uint32_t pb[NQ][2];
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
-        const uint32_t b0 = lds32(weights + 8 * j * G::kPRow), b1 = lds32(weights + 8 * j * G::kPRow + 16);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mma_bf16_m16n8k16(o[k][j], a[k][0], a[k][1], a[k][2], a[k][3], b0, b1);
+        pb[j][0] = *reinterpret_cast<const uint32_t*>(weights + 8 * j * G::kPRow);
+        pb[j][1] = *reinterpret_cast<const uint32_t*>(weights + 8 * j * G::kPRow + 16);
       }
+      auto times = [&](auto place_k) {
+        constexpr int K = decltype(place_k)::value;
+        const uint32_t a0 = kv4_pair<K>(w[0], ssa, cca), a1 = kv4_pair<K>(w[2], ssa, cca);
+        const uint32_t a2 = kv4_pair<K>(w[1], ssb, ccb), a3 = kv4_pair<K>(w[3], ssb, ccb);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) mma(o[K][j], a0, a1, a2, a3, pb[j][0], pb[j][1]);
+      };
+      times(std::integral_constant<int, 0>{}), times(std::integral_constant<int, 1>{});
+      times(std::integral_constant<int, 2>{}), times(std::integral_constant<int, 3>{});
     }
     if (masked_rows) {
       const uint64_t bits = (static_cast<uint64_t>(bad[i & 1][dim_warp][1]) << 32 | bad[i & 1][dim_warp][0]) & ok_bits;
@@ -542,6 +578,8 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
       __syncthreads();  // the query's place and `red` are free again
     }
     if (i + 1 < count) cur.next(p);
+    if (++key_stage == G::kKeyStages) key_stage = 0;
+    if (++value_stage == G::kValueStages) value_stage = 0;
   }
 }
 
