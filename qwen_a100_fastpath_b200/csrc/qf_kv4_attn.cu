@@ -43,7 +43,6 @@
 namespace qf {
 namespace {
 
-constexpr int kTile = 64;       // tokens
 constexpr int kThreads = 128;
 constexpr int kMaxSms = 160;    // the workspace is sized without asking the device
 
@@ -66,13 +65,19 @@ struct AttnParams {
   float* part_o;    // [2 * grid][rows][D]
 };
 
+// Blocks of 16 tokens of a warp in a tile, and CTAs of an SM.
+constexpr int token_blocks(int d, int nq) { return (d == 128 && nq <= 2) || (d == 64 && nq == 1) ? 2 : 1; }
+constexpr int ctas_per_sm(int d, int nq) { return nq == 1 ? 4 : nq <= 4 ? 3 : 2; }
+
 template <int D, int NQ> struct Geo {
+  static constexpr int kBlocks = token_blocks(D, NQ), kTile = 64 * kBlocks;  // tokens
+  static constexpr int kWords = kTile / 32;                // of a bit for each token
   static constexpr int kRow = D / 2;                       // bytes of a token's codes
   static constexpr int kScale = D / 16;                    // bytes of a token's scales
   static constexpr int kSide = kTile * (kRow + kScale);    // bytes of a tile's keys, or values
   // A tile's keys are done with when its weights are exchanged, its values a tile later.
-  static constexpr int kAhead = D == 64 ? 3 : 2, kKeyStages = kAhead, kValueStages = kAhead + 1;
-  static constexpr int kCtas = NQ <= 1 ? 4 : NQ <= 4 ? 3 : 2;  // of an SM
+  static constexpr int kAhead = D == 64 && kBlocks == 1 ? 3 : 2, kKeyStages = kAhead, kValueStages = kAhead + 1;
+  static constexpr int kCtas = ctas_per_sm(D, NQ);
   static constexpr int kPRow = 2 * kTile + 16;             // bytes of a query row's weights, one chunk of padding
   static constexpr int kQBytes = 4096 * NQ;                // the query's fragments; at a part's end the warps' sums
   static constexpr int kPBytes = 8 * NQ * kPRow;
@@ -124,21 +129,23 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 __device__ __forceinline__ int keys_of(const AttnParams& p, int len) {
   return static_cast<int>(min(static_cast<int64_t>(max(len, 0)), p.width));
 }
-__device__ __forceinline__ int tiles_of(const AttnParams& p, int len) { return max((keys_of(p, len) - 1) / kTile + 1, 1); }
+template <int TILE> __device__ __forceinline__ int tiles_of(const AttnParams& p, int len) {
+  return max((keys_of(p, len) - 1) / TILE + 1, 1);
+}
 
 // What a (request, head) costs besides its tiles, in tiles: the query, the first reference, the output.  The CTAs' shares are
 // even in these units: positions v below kStart in front of a (request, head)'s first tile, tile v - kStart behind.
 constexpr int kStart = 2;
 
 // A walk over tiles in the order (request, head, tile).
-struct Cursor {
+template <int TILE> struct Cursor {
   int b, h, tile, tiles, len;
   __device__ __forceinline__ void next(const AttnParams& p) {
     if (++tile < tiles) return;
     tile = 0;
     if (++h < p.cache.heads) return;
     h = 0;
-    if (++b < p.reqs) len = p.lens[b], tiles = tiles_of(p, len);
+    if (++b < p.reqs) len = p.lens[b], tiles = tiles_of<TILE>(p, len);
   }
 };
 
@@ -150,11 +157,12 @@ __device__ __forceinline__ int64_t part_start(int64_t total, int ctas, int i) { 
 template <int D, int NQ>
 __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(const AttnParams p) {
   using G = Geo<D, NQ>;
+  constexpr int kTile = G::kTile, kBlocks = G::kBlocks, kWords = G::kWords;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t offs[kTile][2];           // of the tile that is copied next: codes (bytes), scales (elements)
-  __shared__ uint32_t there[G::kAhead + 1][2];  // a bit for each token of a tile
+  __shared__ uint32_t there[G::kAhead + 1][kWords];  // a bit for each token of a tile
   __shared__ float red[4][8 * NQ];
-  __shared__ uint32_t bad[2][4][2];            // tokens whose values' group is not finite, of a tile with masked rows
+  __shared__ uint32_t bad[2][4][kWords];       // tokens whose values' group is not finite, of a tile with masked rows
   __shared__ int scan[4], found[3];
   __shared__ int64_t bounds[2];
   __shared__ uint8_t row_query[8 * NQ];        // qi of a row
@@ -171,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
     int64_t base = 0;
     for (int b0 = 0; b0 < p.reqs; b0 += kThreads) {
       const int b = b0 + tid;
-      if (pass == 0 || p.reqs > kThreads) n = b < p.reqs ? tiles_of(p, p.lens[b]) + kStart : 0;
+      if (pass == 0 || p.reqs > kThreads) n = b < p.reqs ? tiles_of<kTile>(p, p.lens[b]) + kStart : 0;
       int sum = n;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -219,11 +227,11 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
     if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
-  Cursor cur;
+  Cursor<kTile> cur;
   cur.b = found[0], cur.h = found[1], cur.tile = found[2];
   cur.len = p.lens[cur.b];
-  cur.tiles = tiles_of(p, cur.len);
-  Cursor ahead = cur;  // of the tile whose pages are looked up next (threads of tokens)
+  cur.tiles = tiles_of<kTile>(p, cur.len);
+  Cursor<kTile> ahead = cur;  // of the tile whose pages are looked up next (threads of tokens)
 
   // the query's fragments: a thread's eight dimensions of a row in the order in which the nibbles come apart
   auto query = [&] {
@@ -280,10 +288,13 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
         copy_async<16>(keys + dst, p.cache.codes[0] + at, ok);
         copy_async<16>(vals + dst, p.cache.codes[1] + at, ok);
       }
-      const int token = tid % kTile, side = tid / kTile;
-      const bool ok = offs[token][0] >= 0;
-      copy_async<G::kScale>((side ? vals : keys) + kTile * G::kRow + token * G::kScale,
-                            p.cache.scale[side] + (ok ? offs[token][1] : 0), ok);
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) {
+        const int token = (j * kThreads + tid) % kTile, side = (j * kThreads + tid) / kTile;
+        const bool ok = offs[token][0] >= 0;
+        copy_async<G::kScale>((side ? vals : keys) + kTile * G::kRow + token * G::kScale,
+                              p.cache.scale[side] + (ok ? offs[token][1] : 0), ok);
+      }
     }
     cp_async_commit();
   };
@@ -323,8 +334,10 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
     const uint32_t keys = sm + key_stage * G::kSide, vals = sm + G::kOffV + value_stage * G::kSide;
     const int pos0 = cur.tile * kTile;
     const bool masked_rows = pos0 + kTile - 1 > cur.len - p.q_len;  // some row does not see some token of the tile
-    const uint64_t ok_bits =
-        static_cast<uint64_t>(there[value_stage][1]) << 32 | there[value_stage][0];
+    uint32_t all_there = ~0u;
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) all_there &= there[value_stage][k];
+    const uint32_t ok_bits = there[value_stage][kBlocks * warp / 2] >> (16 * (kBlocks * warp % 2));  // this warp's tokens
     const int value_free = value_stage == 0 ? G::kValueStages - 1 : value_stage - 1;  // the last tile's
     if (i + G::kAhead < count) place(i + G::kAhead, value_free);
     look(i + G::kAhead + 1);
@@ -343,21 +356,24 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
       }
     }
 
-    // ---- scores of this warp's 16 tokens ----
-    float x[NQ][4];
-    {
-      constexpr int kChains = NQ <= 2 ? 2 : 1;  // sums of their own for every second group where there are few to take turns
+    // ---- scores of this warp's tokens ----
+    float x[kBlocks][NQ][4];
+#pragma unroll
+    for (int blk = 0; blk < kBlocks; ++blk) {
+      // sums of their own for every second half group where there are few to take turns
+      constexpr int kChains = NQ <= 2 ? 2 : 1;
       float y[kChains][NQ][4];
 #pragma unroll
       for (int c = 0; c < kChains; ++c)
 #pragma unroll
         for (int j = 0; j < NQ; ++j) y[c][j][0] = y[c][j][1] = y[c][j][2] = y[c][j][3] = 0.f;
-      const uint32_t row = 16 * warp + (lane & 15);          // ldmatrix: lanes 0-15 a chunk's rows, 16-31 the next chunk's
-      const uint32_t scales = keys + kTile * G::kRow + (16 * warp + g) * G::kScale;
+      const uint32_t token0 = 16 * (kBlocks * warp + blk);
+      const uint32_t scales = keys + kTile * G::kRow + (token0 + g) * G::kScale;
 #pragma unroll
       for (int gr = 0; gr < D / 64; ++gr) {
         uint32_t w[4];
-        ldsm_x4(keys + chunk_at<G::kRow>(row, 2 * gr + (lane >> 4)), w[0], w[1], w[2], w[3]);
+        // ldmatrix: lanes 0-15 a chunk's rows, 16-31 the next chunk's
+        ldsm_x4(keys + chunk_at<G::kRow>(token0 + (lane & 15), 2 * gr + (lane >> 4)), w[0], w[1], w[2], w[3]);
         const uint32_t sa = lds32(scales + 4 * gr), sb = lds32(scales + 8 * G::kScale + 4 * gr);
         const uint32_t ssa = dup_lo(sa), cca = dup_hi(sa), ssb = dup_lo(sb), ccb = dup_hi(sb);
 #pragma unroll
@@ -375,37 +391,44 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
           for (int j = 0; j < NQ; ++j) mma(y[kChains - 1][j], b0, b1, b2, b3, q[j].z, q[j].w);
         }
       }
+      // distances to the reference: the weights are 2^x from here on
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[j][e] = kChains == 2 ? y[0][j][e] + y[kChains - 1][j][e] : y[0][j][e];
+        for (int e = 0; e < 4; ++e)
+          x[blk][j][e] = fmaf(kChains == 2 ? y[0][j][e] + y[kChains - 1][j][e] : y[0][j][e], p.scale_log2, -ref[j][e & 1]);
     }
-    // distances to the reference: the weights are 2^x from here on
+    if (masked_rows || ~all_there) {
 #pragma unroll
-    for (int j = 0; j < NQ; ++j)
+      for (int blk = 0; blk < kBlocks; ++blk) {
+        const int ta = 16 * (kBlocks * warp + blk) + g;
+        const bool oka = ok_bits >> (16 * blk + g) & 1, okb = ok_bits >> (16 * blk + g + 8) & 1;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[j][e] = fmaf(x[j][e], p.scale_log2, -ref[j][e & 1]);
-    if (masked_rows || ~ok_bits) {
-      const int ta = 16 * warp + g;
-      const bool oka = ok_bits >> ta & 1, okb = ok_bits >> (ta + 8) & 1;
+        for (int j = 0; j < NQ; ++j)
 #pragma unroll
-      for (int j = 0; j < NQ; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int last = cur.len - p.q_len + row_query[8 * j + 2 * t + e] - pos0;  // the last token that the row sees
-          if (!(oka && ta <= last)) x[j][e] = -INFINITY;
-          if (!(okb && ta + 8 <= last)) x[j][2 + e] = -INFINITY;
-        }
+          for (int e = 0; e < 2; ++e) {
+            const int last = cur.len - p.q_len + row_query[8 * j + 2 * t + e] - pos0;  // the last token that the row sees
+            if (!(oka && ta <= last)) x[blk][j][e] = -INFINITY;
+            if (!(okb && ta + 8 <= last)) x[blk][j][2 + e] = -INFINITY;
+          }
+      }
     }
+    // the largest of a row's distances in this thread
+    auto highest = [&](int j, int e) {
+      float v = fmaxf(x[0][j][e], x[0][j][2 + e]);
+#pragma unroll
+      for (int blk = 1; blk < kBlocks; ++blk) v = fmaxf(v, fmaxf(x[blk][j][e], x[blk][j][2 + e]));
+      return v;
+    };
     float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < NQ; ++j) top = fmaxf(top, fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])));
+    for (int j = 0; j < NQ; ++j) top = fmaxf(top, fmaxf(highest(j, 0), highest(j, 1)));
     if (unset)
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          if (unset >> (2 * j + e) & 1 && fmaxf(x[j][e], x[j][2 + e]) > -INFINITY) top = INFINITY;
+          if (unset >> (2 * j + e) & 1 && highest(j, e) > -INFINITY) top = INFINITY;
     // (all warps have read this tile's keys and the last one's values, whose stages are filled again now)
     const bool raise = __syncthreads_or(top > kSlack);
     copy(i + G::kAhead, key_stage, value_free);
@@ -416,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
         float v[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          v[e] = fmaxf(x[j][e], x[j][2 + e]);
+          v[e] = highest(j, e);
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) v[e] = fmaxf(v[e], __shfl_xor_sync(0xffffffffu, v[e], off));
         }
@@ -440,18 +463,22 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
           if (v[e] > -INFINITY) unset &= ~bit;
           l[j][e] *= scale_o[j][e];
           ref[j][e] += rise;
-          x[j][e] -= rise, x[j][2 + e] -= rise;
+#pragma unroll
+          for (int blk = 0; blk < kBlocks; ++blk) x[blk][j][e] -= rise, x[blk][j][2 + e] -= rise;
         }
       }
     }
 #pragma unroll
-    for (int j = 0; j < NQ; ++j) {
+    for (int blk = 0; blk < kBlocks; ++blk)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[j][e] = ex2_approx(x[j][e]);
-      l[j][0] += x[j][0] + x[j][2], l[j][1] += x[j][1] + x[j][3];
-      stsm_x2_trans(sm + G::kOffP + (8 * j + (lane & 7)) * G::kPRow + 2 * (16 * warp + (lane & 8)), pack2(x[j][0], x[j][1]),
-                    pack2(x[j][2], x[j][3]));
-    }
+      for (int j = 0; j < NQ; ++j) {
+        float(&w)[4] = x[blk][j];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = ex2_approx(w[e]);
+        l[j][0] += w[0] + w[2], l[j][1] += w[1] + w[3];
+        stsm_x2_trans(sm + G::kOffP + (8 * j + (lane & 7)) * G::kPRow + 2 * (16 * (kBlocks * warp + blk) + (lane & 8)),
+                      pack2(w[0], w[1]), pack2(w[2], w[3]));
+      }
     cp_async_wait<G::kAhead - 1>();  // the next tile
     __syncthreads();                 // weights; and the next tile for all warps
 
@@ -463,9 +490,11 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
         for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[k][j][e] *= scale_o[j][e & 1];
+    constexpr int kValueBlocks = kTile / 16 / G::kTokenWarps;
+    uint32_t pb[NQ][4];
 #pragma unroll
-    for (int kb = 0; kb < 4 / G::kTokenWarps; ++kb) {
-      const int token0 = 16 * (token_warp * (4 / G::kTokenWarps) + kb);
+    for (int kb = 0; kb < kValueBlocks; ++kb) {
+      const int token0 = 16 * (token_warp * kValueBlocks + kb);
       uint32_t w[4];
       ldsm_x4_trans(vals + chunk_at<G::kRow>(token0 + (lane & 15), 2 * dim_warp + (lane >> 4)), w[0], w[1],
                     w[2], w[3]);
@@ -474,32 +503,40 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
                      s3 = lds32(scales + 9 * G::kScale);
       const uint32_t ssa = __byte_perm(s0, s1, 0x5410), cca = __byte_perm(s0, s1, 0x7632);
       const uint32_t ssb = __byte_perm(s2, s3, 0x5410), ccb = __byte_perm(s2, s3, 0x7632);
-      const uint8_t* weights = smem + G::kOffP + g * G::kPRow + 2 * (token0 + 2 * t);
-      uint32_t pb[NQ][2];
+      if constexpr (kValueBlocks > 1) {
+        if (kb % 2 == 0)  // this block's weights and the next one's
 #pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        pb[j][0] = *reinterpret_cast<const uint32_t*>(weights + 8 * j * G::kPRow);
-        pb[j][1] = *reinterpret_cast<const uint32_t*>(weights + 8 * j * G::kPRow + 16);
+          for (int j = 0; j < NQ; ++j)
+            ldsm_x4(sm + G::kOffP + (8 * j + (lane & 7)) * G::kPRow + 2 * (token0 + (lane & 24)), pb[j][0], pb[j][1], pb[j][2],
+                    pb[j][3]);
+      } else {
+        const uint8_t* weights = smem + G::kOffP + g * G::kPRow + 2 * (token0 + 2 * t);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+          pb[j][0] = *reinterpret_cast<const uint32_t*>(weights + 8 * j * G::kPRow);
+          pb[j][1] = *reinterpret_cast<const uint32_t*>(weights + 8 * j * G::kPRow + 16);
+        }
       }
       auto times = [&](auto place_k) {
         constexpr int K = decltype(place_k)::value;
         const uint32_t a0 = kv4_pair<K>(w[0], ssa, cca), a1 = kv4_pair<K>(w[2], ssa, cca);
         const uint32_t a2 = kv4_pair<K>(w[1], ssb, ccb), a3 = kv4_pair<K>(w[3], ssb, ccb);
 #pragma unroll
-        for (int j = 0; j < NQ; ++j) mma(o[K][j], a0, a1, a2, a3, pb[j][0], pb[j][1]);
+        for (int j = 0; j < NQ; ++j) mma(o[K][j], a0, a1, a2, a3, pb[j][2 * (kb % 2)], pb[j][2 * (kb % 2) + 1]);
       };
       times(std::integral_constant<int, 0>{}), times(std::integral_constant<int, 1>{});
       times(std::integral_constant<int, 2>{}), times(std::integral_constant<int, 3>{});
     }
     if (masked_rows) {
-      const uint64_t bits = (static_cast<uint64_t>(bad[i & 1][dim_warp][1]) << 32 | bad[i & 1][dim_warp][0]) & ok_bits;
-      if (bits)
-        for (int j = 0; j < NQ; ++j)
-          for (int e = 0; e < 2; ++e) {
-            const int last = cur.len - p.q_len + row_query[8 * j + 2 * t + e] - pos0;
-            if (last >= 0 && (bits & (last >= 63 ? ~0ull : (2ull << last) - 1)))
-              for (int k = 0; k < 4; ++k) o[k][j][e] = o[k][j][2 + e] = __int_as_float(0x7fffffff);
-          }
+#pragma unroll
+      for (int k = 0; k < kWords; ++k)
+        if (const uint32_t bits = bad[i & 1][dim_warp][k])
+          for (int j = 0; j < NQ; ++j)
+            for (int e = 0; e < 2; ++e) {
+              const int last = cur.len - p.q_len + row_query[8 * j + 2 * t + e] - pos0 - 32 * k;
+              if (last >= 0 && (bits & (last >= 31 ? ~0u : (2u << last) - 1)))
+                for (int m = 0; m < 4; ++m) o[m][j][e] = o[m][j][2 + e] = __int_as_float(0x7fffffff);
+            }
     }
 
     // ---- the end of a (request, head), or of this CTA's share of it ----
@@ -583,104 +620,139 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
   }
 }
 
-// Joins the parts of each (request, head) that several CTAs held.  Work is a (join, row, 64 dimensions): 16 threads a part,
-// four dimensions each.
+// Joins the parts of each (request, head) that several CTAs held.  Work is a (join, row, 64 dimensions), 16 threads with four
+// dimensions each; several such groups share the parts of one where there are many (a long context), or take one each where
+// there are few (a batch).  A CTA takes a round of work of one join at a time.
 constexpr int kJoinThreads = 256, kJoinDims = 64, kJoinGroups = kJoinThreads / (kJoinDims / 4), kJoinEarly = 8;
 constexpr int kMaxCtas = 4;  // of an SM
 
+// Groups that share a piece of work.
+__device__ __forceinline__ int join_share(int parts) {
+  int n = 1;
+  while (n < kJoinGroups && n * 4 < parts) n *= 2;
+  return n;
+}
+
 __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const AttnParams p, int grid, int D) {
-  __shared__ int list[kMaxSms * kMaxCtas];
-  __shared__ float weight[kMaxSms * kMaxCtas];
-  __shared__ float warp_val[kJoinThreads / 32];
-  __shared__ int warp_count[kJoinThreads / 32];
+  __shared__ int4 list[kMaxSms * kMaxCtas];
+  __shared__ int rounds[kMaxSms * kMaxCtas + 1];  // before each join
+  __shared__ int2 warp_sum[kJoinThreads / 32];
+  __shared__ float weight[kJoinGroups][kMaxSms * kMaxCtas / 4];
   __shared__ float4 sums[kJoinGroups][kJoinDims / 4];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int n = 0;
+  const int pieces = D / kJoinDims, work = p.rows * pieces;
+  int n = 0, total = 0;
   for (int i0 = 0; i0 < grid; i0 += kJoinThreads) {
-    const bool named = i0 + tid < grid && p.joins[i0 + tid].x >= 0;
-    const uint32_t bits = __ballot_sync(0xffffffffu, named);
-    if (lane == 0) warp_count[warp] = __popc(bits);
-    __syncthreads();
-    int at = n;
-    for (int w = 0; w < kJoinThreads / 32; ++w) {
-      if (w < warp) at += warp_count[w];
-      n += warp_count[w];
+    const int from = i0 + tid;
+    int4 join = make_int4(-1, 0, 0, 0);
+    if (from < grid) join = p.joins[from];
+    const bool named = join.x >= 0;
+    const int share = join_share(join.z - from + 1);
+    int2 sum = make_int2(named, named ? (work * share + kJoinGroups - 1) / kJoinGroups : 0);
+    const int2 own = sum;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, sum.x, off), c = __shfl_up_sync(0xffffffffu, sum.y, off);
+      if (lane >= off) sum.x += a, sum.y += c;
     }
-    if (named) list[at + __popc(bits & ((1u << lane) - 1))] = i0 + tid;
+    if (lane == 31) warp_sum[warp] = sum;
+    __syncthreads();
+    int at = n + sum.x - own.x, before = total + sum.y - own.y;
+    for (int w = 0; w < kJoinThreads / 32; ++w) {
+      const int2 v = warp_sum[w];
+      if (w < warp) at += v.x, before += v.y;
+      n += v.x, total += v.y;
+    }
+    if (named) {
+      // (request and head, the CTA that begins it, the last one, whether its part is the first's last share)
+      list[at] = make_int4(join.x * p.cache.heads + join.y, from, join.z, join.w);
+      rounds[at] = before;
+    }
     __syncthreads();
   }
-  const int pieces = D / kJoinDims, items = n * p.rows * pieces;
   const int col = tid % (kJoinDims / 4), group = tid / (kJoinDims / 4);
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const int piece = item % pieces, r = item / pieces % p.rows, from = list[item / pieces / p.rows];
-    const int4 join = p.joins[from];
-    const int parts = join.z - from + 1;
-    // part k is CTA from + k's first, or its last where the (request, head) begins inside its share
-    auto row_of = [&](int k) { return (2 * static_cast<int64_t>(from + k) + (k == 0 ? join.w : 0)) * p.rows + r; };
+  for (int round = blockIdx.x; round < total; round += gridDim.x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (rounds[mid] <= round) lo = mid; else hi = mid - 1;
+    }
+    const int4 join = list[lo];
+    const int parts = join.z - join.y + 1, share = join_share(parts);
+    const int item = (round - rounds[lo]) * (kJoinGroups / share) + group / share, sub = group % share;
+    const bool active = item < work;
+    const int piece = item % pieces, r = active ? item / pieces : 0;
+    // part k is CTA join.y + k's first, or its last where the (request, head) begins inside its share
+    auto row_of = [&](int k) { return (2 * static_cast<int64_t>(join.y + k) + (k == 0 ? join.w : 0)) * p.rows + r; };
     auto load = [&](int k) {
       return *reinterpret_cast<const float4*>(p.part_o + row_of(k) * D + kJoinDims * piece + 4 * col);
     };
-    float4 early[kJoinEarly];  // on their way while the weights are made
+    float4 early[kJoinEarly];  // this group's parts sub, sub + share, ..., on their way while the weights are made
 #pragma unroll
     for (int e = 0; e < kJoinEarly; ++e) {
       early[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (group + e * kJoinGroups < parts) early[e] = load(group + e * kJoinGroups);
+      if (active && sub + e * share < parts) early[e] = load(sub + e * share);
     }
-    float top = kNoRef;
-    for (int k = tid; k < parts; k += kJoinThreads) top = fmaxf(top, p.part_ml[row_of(k)].x);
+    // the weights of the row (every group that shares it makes them all, and keeps its own)
+    float top = kNoRef, sum = 0.f;
+    float2 ml[kJoinEarly];
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    if (lane == 0) warp_val[warp] = top;
-    __syncthreads();
-    for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, warp_val[w]);
-    __syncthreads();
-    float sum = 0.f;
-    for (int k = tid; k < parts; k += kJoinThreads) {
-      const float2 ml = p.part_ml[row_of(k)];
-      const float w = ex2_approx(ml.x - top);
-      weight[k] = w;
-      sum = fmaf(ml.y, w, sum);
+    for (int e = 0; e < kJoinEarly; ++e) {
+      const int k = col + e * (kJoinDims / 4);
+      ml[e] = make_float2(kNoRef, 0.f);
+      if (k < parts) ml[e] = p.part_ml[row_of(k)];
     }
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (lane == 0) warp_val[warp] = sum;
-    __syncthreads();
-    sum = 0.f;
-    for (int w = 0; w < kJoinThreads / 32; ++w) sum += warp_val[w];
+    for (int e = 0; e < kJoinEarly; ++e) top = fmaxf(top, ml[e].x);
+    for (int k = col + kJoinEarly * (kJoinDims / 4); k < parts; k += kJoinDims / 4) top = fmaxf(top, p.part_ml[row_of(k)].x);
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    auto weigh = [&](int k, const float2& v) {
+      const float w = ex2_approx(v.x - top);
+      if (k % share == sub) weight[group][k / share] = w;
+      sum = fmaf(v.y, w, sum);
+    };
+#pragma unroll
+    for (int e = 0; e < kJoinEarly; ++e)
+      if (const int k = col + e * (kJoinDims / 4); k < parts) weigh(k, ml[e]);
+    for (int k = col + kJoinEarly * (kJoinDims / 4); k < parts; k += kJoinDims / 4) weigh(k, p.part_ml[row_of(k)]);
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    __syncwarp();
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](const float4& v, float w) {
       acc.x = fmaf(v.x, w, acc.x), acc.y = fmaf(v.y, w, acc.y), acc.z = fmaf(v.z, w, acc.z), acc.w = fmaf(v.w, w, acc.w);
     };
+    if (active) {
 #pragma unroll
-    for (int e = 0; e < kJoinEarly; ++e)
-      if (group + e * kJoinGroups < parts) add(early[e], weight[group + e * kJoinGroups]);
+      for (int e = 0; e < kJoinEarly; ++e)
+        if (sub + e * share < parts) add(early[e], weight[group][e]);
 #pragma unroll 4
-    for (int k = group + kJoinEarly * kJoinGroups; k < parts; k += kJoinGroups) add(load(k), weight[k]);
-    sums[group][col] = acc;
-    __syncthreads();
-    if (group == 0) {
-#pragma unroll
-      for (int k = 1; k < kJoinGroups; ++k) add(sums[k][col], 1.f);
+      for (int k = sub + kJoinEarly * share; k < parts; k += share) add(load(k), weight[group][k / share]);
+    }
+    if (share > 1) {
+      sums[group][col] = acc;
+      __syncthreads();
+      if (sub == 0)
+        for (int k = 1; k < share; ++k) add(sums[group + k][col], 1.f);
+      __syncthreads();
+    }
+    if (active && sub == 0) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const int qi = r / p.group, hq = join.y * p.group + r - qi * p.group;
-      __nv_bfloat16* dst = p.out + (static_cast<int64_t>(join.x) * p.q_len + qi) * p.ot + hq * p.oh + kJoinDims * piece + 4 * col;
+      const int b = join.x / p.cache.heads, h = join.x - b * p.cache.heads;
+      const int qi = r / p.group, hq = h * p.group + r - qi * p.group;
+      __nv_bfloat16* dst = p.out + (static_cast<int64_t>(b) * p.q_len + qi) * p.ot + hq * p.oh + kJoinDims * piece + 4 * col;
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
     }
-    __syncthreads();
+    __syncwarp();
   }
 }
 
 int tiles_of_rows(int rows) {
   const int n = (rows + 7) / 8;
   return n == 5 ? 6 : n == 7 ? 8 : n;
-}
-
-// CTAs of an SM (Geo::kCtas).
-int ctas_per_sm(int rows) {
-  const int n = tiles_of_rows(rows);
-  return n <= 1 ? 4 : n <= 4 ? 3 : 2;
 }
 
 template <int D, int NQ> cudaError_t launch(const AttnParams& p, int grid, int dev, int sms, bool pdl, cudaStream_t st) {
@@ -735,7 +807,7 @@ using namespace qf;
 extern "C" size_t qf_kv4_attn_workspace_bytes(int num_reqs, int q_len, int num_heads, int num_kv_heads, int head_size) {
   if (num_reqs <= 0 || q_len <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_size <= 0) return 256;
   const int64_t rows = static_cast<int64_t>(q_len) * (num_heads / num_kv_heads);
-  const size_t parts = 2 * static_cast<size_t>(kMaxSms) * ctas_per_sm(static_cast<int>(rows < 64 ? rows : 64));
+  const size_t parts = 2 * static_cast<size_t>(kMaxSms) * ctas_per_sm(head_size, tiles_of_rows(static_cast<int>(rows < 64 ? rows : 64)));
   return up256(parts / 2 * sizeof(int4)) + up256(parts * rows * 8) + parts * rows * head_size * 4;
 }
 
@@ -770,7 +842,7 @@ extern "C" int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_k
   p.out = static_cast<__nv_bfloat16*>(out), p.ot = so_t, p.oh = so_h;
   p.table = block_table, p.table_row = s_bt;
   p.width = static_cast<int64_t>(max_pages) * cache->page_size;
-  if (p.width > INT32_MAX - 4 * kTile) p.width = INT32_MAX - 4 * kTile;  // positions stay 32-bit numbers
+  if (p.width > INT32_MAX - 1024) p.width = INT32_MAX - 1024;  // positions stay 32-bit numbers
   p.lens = seq_lens;
   p.reqs = num_reqs, p.q_len = q_len, p.group = num_heads / cache->num_heads, p.rows = q_len * p.group;
   p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
@@ -778,8 +850,8 @@ extern "C" int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_k
   while ((1ull << p.div_shift) < static_cast<uint64_t>(cache->page_size)) ++p.div_shift;
   p.div_mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << p.div_shift) - cache->page_size)) / cache->page_size + 1);
   if (sms > kMaxSms) sms = kMaxSms;
-  const int grid = sms * ctas_per_sm(p.rows);
-  const size_t parts = 2 * static_cast<size_t>(kMaxSms) * ctas_per_sm(p.rows);
+  const int grid = sms * ctas_per_sm(cache->head_size, tiles_of_rows(p.rows));
+  const size_t parts = 2 * static_cast<size_t>(kMaxSms) * ctas_per_sm(cache->head_size, tiles_of_rows(p.rows));
   uint8_t* w = static_cast<uint8_t*>(ws);
   p.joins = reinterpret_cast<int4*>(w);
   w += up256(parts / 2 * sizeof(int4));
