@@ -292,7 +292,8 @@ int qf_kv4_read(void* k, int64_t sk_t, int64_t sk_h, void* v, int64_t sv_t, int6
  * [0, seq_lens[b] - q_len + qi]; a row with no key gives zeros.  Keys behind max_pages * page_size, and on pages whose entry
  * is no page of the cache, do not take part; what lies in slots that a row does not attend, NaN included, does not touch it.
  * q, out: bf16, 16-byte aligned with strides multiples of 8 elements; q_len * num_heads / cache->num_heads <= 64; block_table
- * int32 (row stride s_bt, max_pages entries each).  The workspace (>= qf_kv4_attn_workspace_bytes() on the current device,
+ * int32 (row stride s_bt, max_pages entries each);
+ * num_reqs * heads * (max_pages * page_size / 64 + 4) below 2^31, page and slot strides below 2^32 bytes.  The workspace (>= qf_kv4_attn_workspace_bytes() on the current device,
  * 256-byte aligned) need not be zeroed and holds nothing between calls.  No host synchronisation. */
 size_t qf_kv4_attn_workspace_bytes(int num_reqs, int q_len, int num_heads, int num_kv_heads, int head_size);
 int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_kv4_cache* cache, const int32_t* block_table,

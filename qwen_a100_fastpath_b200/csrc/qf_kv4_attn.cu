@@ -51,7 +51,11 @@ struct AttnParams {
   int64_t qt, qh;
   __nv_bfloat16* out;
   int64_t ot, oh;
-  Kv4View cache;
+  // the cache: keys' codes and scales, and how many bytes further the values' are; strides in bytes
+  const uint8_t *codes, *scales;
+  int64_t value_codes, value_scales, head, shead;
+  uint32_t page, slot, spage, sslot;
+  int num_pages, page_size, heads;
   const int32_t* table;
   int64_t table_row;
   const int32_t* lens;
@@ -143,7 +147,7 @@ template <int TILE> struct Cursor {
   __device__ __forceinline__ void next(const AttnParams& p) {
     if (++tile < tiles) return;
     tile = 0;
-    if (++h < p.cache.heads) return;
+    if (++h < p.heads) return;
     h = 0;
     if (++b < p.reqs) len = p.lens[b], tiles = tiles_of<TILE>(p, len);
   }
@@ -152,19 +156,33 @@ template <int TILE> struct Cursor {
 constexpr float kNoRef = -3e38f;  // stands for the reference of a row that has seen no key, in a part that is joined
 constexpr float kSlack = 16.f;
 
-__device__ __forceinline__ int64_t part_start(int64_t total, int ctas, int i) { return total * i / ctas; }
+// Positions 0 to total - 1 split evenly: CTA i begins at start(i), position v is in CTA holder(v)'s share.
+struct Shares {
+  uint32_t each, more;  // the first `more` CTAs have one more than `each`
+  __device__ __forceinline__ Shares(uint32_t total, uint32_t ctas) : each(total / ctas), more(total - each * ctas) {}
+  __device__ __forceinline__ uint32_t start(uint32_t i) const { return each * i + min(i, more); }
+  __device__ __forceinline__ uint32_t holder(uint32_t v) const {
+    const uint32_t big = (each + 1) * more;
+    return v < big ? v / (each + 1) : more + (v - big) / each;
+  }
+};
+
+// Where a token's keys are.
+struct __align__(16) Place {
+  const uint8_t *codes, *scales;
+};
 
 template <int D, int NQ>
 __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(const AttnParams p) {
   using G = Geo<D, NQ>;
   constexpr int kTile = G::kTile, kBlocks = G::kBlocks, kWords = G::kWords;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ int64_t offs[kTile][2];           // of the tile that is copied next: codes (bytes), scales (elements)
-  __shared__ uint32_t there[G::kAhead + 1][kWords];  // a bit for each token of a tile
+  __shared__ Place places[kTile];               // of the tile that is copied next
+  __shared__ __align__(16) uint32_t there[G::kAhead + 1][kWords];  // a bit for each token of a tile
   __shared__ float red[4][8 * NQ];
   __shared__ uint32_t bad[2][4][kWords];       // tokens whose values' group is not finite, of a tile with masked rows
-  __shared__ int scan[4], found[3];
-  __shared__ int64_t bounds[2];
+  __shared__ uint32_t scan[4], bounds[2];
+  __shared__ int found[4];
   __shared__ uint8_t row_query[8 * NQ];        // qi of a row
   pdl_launch_dependents();
   pdl_wait();
@@ -173,52 +191,57 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
   for (int r = tid; r < 8 * NQ; r += kThreads) row_query[r] = r < p.rows ? r / p.group : 0;
 
   // ---- this CTA's part: a scan over the requests, twice (for the sum, then for where the part begins and ends) ----
-  int64_t total = 0, begin = 0, end = 0;
-  int ctas = 0, n = 0;
+  uint32_t total = 0, begin = 0, end = 0, n = 0;
+  uint32_t ctas = 1;
+  int len = 0;
   for (int pass = 0; pass < 2; ++pass) {
-    int64_t base = 0;
+    uint32_t base = 0;
     for (int b0 = 0; b0 < p.reqs; b0 += kThreads) {
       const int b = b0 + tid;
-      if (pass == 0 || p.reqs > kThreads) n = b < p.reqs ? tiles_of<kTile>(p, p.lens[b]) + kStart : 0;
-      int sum = n;
+      if (pass == 0 || p.reqs > kThreads) {
+        if (b < p.reqs) len = p.lens[b];
+        n = b < p.reqs ? tiles_of<kTile>(p, len) + kStart : 0;
+      }
+      uint32_t sum = n;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, sum, off);
+        const uint32_t a = __shfl_up_sync(0xffffffffu, sum, off);
         if (lane >= off) sum += a;
       }
       __syncthreads();
       if (lane == 31) scan[warp] = sum;
       __syncthreads();
-      int64_t before = base + sum - n;
+      uint32_t before = base + sum - n;
+#pragma unroll
       for (int w = 0; w < 4; ++w) {
         if (w < warp) before += scan[w];
         base += scan[w];
       }
       if (pass == 0 || !n) continue;
-      before *= p.cache.heads;
-      const int64_t after = before + static_cast<int64_t>(n) * p.cache.heads;
+      before *= p.heads;
+      const uint32_t after = before + n * p.heads;
       // tiles before a position: all those before the request, those of its heads before, those before it
-      auto tiles_before = [&](int64_t v) {
-        const int in = static_cast<int>((v - before) / n), rest = static_cast<int>((v - before) % n);
-        return before - static_cast<int64_t>(kStart) * p.cache.heads * b + static_cast<int64_t>(in) * (n - kStart) +
-               max(rest - kStart, 0);
-      };
+      const uint32_t tiles = before - kStart * p.heads * b;
       if (before <= begin && begin < after) {
-        found[0] = b, found[1] = static_cast<int>((begin - before) / n);
-        found[2] = max(static_cast<int>((begin - before) % n) - kStart, 0);
-        bounds[0] = tiles_before(begin);
+        const uint32_t h = (begin - before) / n, rest = begin - before - h * n;
+        const uint32_t tile = rest > kStart ? rest - kStart : 0;
+        found[0] = b, found[1] = h, found[2] = tile, found[3] = len;
+        bounds[0] = tiles + h * (n - kStart) + tile;
       }
-      if (before < end && end <= after)
-        bounds[1] = end == after ? after - static_cast<int64_t>(kStart) * p.cache.heads * (b + 1) : tiles_before(end);
+      if (before < end && end <= after) {
+        const uint32_t h = (end - before) / n, rest = end - before - h * n;
+        bounds[1] = tiles + h * (n - kStart) + (rest > kStart ? rest - kStart : 0);
+      }
     }
     if (pass == 0) {
-      total = base * p.cache.heads;
-      ctas = static_cast<int>(min(total, static_cast<int64_t>(gridDim.x)));
-      if (static_cast<int>(blockIdx.x) >= ctas) {
+      total = base * p.heads;
+      ctas = min(total, gridDim.x);
+      if (blockIdx.x >= ctas) {
         if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
         return;
       }
-      begin = part_start(total, ctas, blockIdx.x), end = part_start(total, ctas, blockIdx.x + 1);
+      const Shares shares(total, ctas);
+      begin = shares.start(blockIdx.x), end = shares.start(blockIdx.x + 1);
     }
   }
   __syncthreads();
@@ -228,84 +251,115 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
     return;
   }
   Cursor<kTile> cur;
-  cur.b = found[0], cur.h = found[1], cur.tile = found[2];
-  cur.len = p.lens[cur.b];
+  cur.b = found[0], cur.h = found[1], cur.tile = found[2], cur.len = found[3];
   cur.tiles = tiles_of<kTile>(p, cur.len);
-  Cursor<kTile> ahead = cur;  // of the tile whose pages are looked up next (threads of tokens)
 
   // the query's fragments: a thread's eight dimensions of a row in the order in which the nibbles come apart
   auto query = [&] {
-    for (int e = tid; e < D / 32 * NQ * 32; e += kThreads) {
-      const int l5 = e & 31, j = (e >> 5) % NQ, c = (e >> 5) / NQ;
-      const int r = 8 * j + (l5 >> 2);
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (r < p.rows) {
-        const int qi = row_query[r], hq = cur.h * p.group + r - qi * p.group;
-        u = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(cur.b) * p.q_len + qi) * p.qt + hq * p.qh + 32 * c +
-                                            8 * (l5 & 3));
+    constexpr int kAll = D / 32 * NQ * 32, kBatch = 4;
+    for (int e0 = tid; e0 < kAll; e0 += kBatch * kThreads) {
+      uint4 u[kBatch];  // on their way together
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int e = e0 + k * kThreads, l5 = e & 31, j = (e >> 5) % NQ, c = (e >> 5) / NQ;
+        const int r = 8 * j + (l5 >> 2);
+        u[k] = make_uint4(0, 0, 0, 0);
+        if (e < kAll && r < p.rows) {
+          const int qi = row_query[r], hq = cur.h * p.group + r - qi * p.group;
+          u[k] = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(cur.b) * p.q_len + qi) * p.qt + hq * p.qh +
+                                                 32 * c + 8 * (l5 & 3));
+        }
       }
-      reinterpret_cast<uint4*>(smem + G::kOffQ)[e] =
-          make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410),
-                     __byte_perm(u.y, u.w, 0x7632));
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+        if (e0 + k * kThreads < kAll)
+          reinterpret_cast<uint4*>(smem + G::kOffQ)[e0 + k * kThreads] =
+              make_uint4(__byte_perm(u[k].x, u[k].z, 0x5410), __byte_perm(u[k].x, u[k].z, 0x7632),
+                         __byte_perm(u[k].y, u[k].w, 0x5410), __byte_perm(u[k].y, u[k].w, 0x7632));
     }
   };
 
-  // ---- copies: threads of tokens look a page up, then all threads copy ----
-  int32_t entry = -1;
-  auto look = [&](int i) {  // tile i's page of this thread's token
-    entry = -1;
-    if (tid >= kTile || i >= count) return;
-    const int pos = ahead.tile * kTile + tid;
-    if (pos < keys_of(p, ahead.len))
-      entry = p.table[ahead.b * p.table_row + ((__umulhi(pos, p.div_mul) + pos) >> p.div_shift)];
+  // ---- copies: the threads of tokens look pages up, then all threads copy ----
+  Cursor<kTile> ahead = cur;  // of the tile whose pages are looked up next
+  struct Look {
+    int32_t entry;
+    uint32_t off;  // in the page
+    int h;
   };
-  auto place = [&](int i, int value_slot) {  // its offsets, and on to the next tile
-    if (tid >= kTile) return;
-    const bool ok = entry >= 0 && entry < p.cache.num_pages;
-    if (ok) {
-      const uint32_t pos = ahead.tile * kTile + tid;
-      const int64_t slot = pos - ((__umulhi(pos, p.div_mul) + pos) >> p.div_shift) * static_cast<uint32_t>(p.cache.page_size);
-      offs[tid][0] = entry * p.cache.page + ahead.h * p.cache.head + slot * p.cache.slot;
-      offs[tid][1] = entry * p.cache.spage + ahead.h * p.cache.shead + slot * p.cache.sslot;
-    } else {
-      offs[tid][0] = -1;
+  auto look = [&](int i) {  // tile i's page of this thread's token; and on to the next tile
+    Look r = {-1, 0, 0};
+    if (tid >= kTile || i >= count) return r;
+    const uint32_t pos = ahead.tile * kTile + tid;
+    if (static_cast<int>(pos) < keys_of(p, ahead.len)) {
+      const uint32_t col = (__umulhi(pos, p.div_mul) + pos) >> p.div_shift;
+      r.entry = p.table[ahead.b * p.table_row + col];
+      r.off = pos - col * p.page_size;
     }
+    r.h = ahead.h;
+    if (i + 1 < count) ahead.next(p);
+    return r;
+  };
+  auto place = [&](const Look& r, Place* to, int value_slot) {
+    if (tid >= kTile) return;
+    const bool ok = static_cast<uint32_t>(r.entry) < static_cast<uint32_t>(p.num_pages);
+    const uint32_t e = ok ? r.entry : 0, off = ok ? r.off : 0;  // (a place that is not read, all the same within the cache)
+    to[tid].codes = p.codes + r.h * p.head + static_cast<uint64_t>(e) * p.page + static_cast<uint64_t>(off) * p.slot;
+    to[tid].scales = p.scales + r.h * p.shead + static_cast<uint64_t>(e) * p.spage + static_cast<uint64_t>(off) * p.sslot;
     const uint32_t bits = __ballot_sync(0xffffffffu, ok);
     if (lane == 0) there[value_slot][warp] = bits;
-    if (i + 1 < count) ahead.next(p);
   };
-  auto copy = [&](int i, int key_slot, int value_slot) {
+  constexpr int kChunks = G::kRow / 16, kRows = kThreads / kChunks;
+  static_assert(kRows / (128 / G::kRow) % (G::kRow / 16) == 0, "a thread's rows have their chunks in the same places");
+  const int copy_row = tid / kChunks, copy_chunk = tid % kChunks;
+  const uint32_t copy_at = chunk_at<G::kRow>(copy_row, copy_chunk);
+  auto copy = [&](int i, const Place* from, int key_slot, int value_slot) {
     if (i < count) {
       const uint32_t keys = sm + key_slot * G::kSide, vals = sm + G::kOffV + value_slot * G::kSide;
-      constexpr int kChunks = G::kRow / 16;
+      // everything that is read from shared memory first
+      const uint8_t* codes[kTile / kRows];
+      const uint8_t* scales[kBlocks];
+      uint32_t words[kWords];
 #pragma unroll
-      for (int j = 0; j < kTile * kChunks / kThreads; ++j) {
-        const int token = (j * kThreads + tid) / kChunks, c = tid % kChunks;
-        const int64_t o = offs[token][0];
-        const bool ok = o >= 0;
-        const int64_t at = ok ? o + 16 * c : 0;
-        const uint32_t dst = chunk_at<G::kRow>(token, c);
-        copy_async<16>(keys + dst, p.cache.codes[0] + at, ok);
-        copy_async<16>(vals + dst, p.cache.codes[1] + at, ok);
+      for (int j = 0; j < kTile / kRows; ++j) codes[j] = from[j * kRows + copy_row].codes + 16 * copy_chunk;
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) scales[j] = from[(j * kThreads + tid) % kTile].scales;
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) words[k] = there[value_slot][k];
+#pragma unroll
+      for (int j = 0; j < kTile / kRows; ++j) {
+        const int token = j * kRows + copy_row;
+        const uint32_t word = kRows <= 32 ? words[j * kRows / 32] : copy_row < 32 ? words[2 * j] : words[(2 * j + 1) % kWords];
+        const bool ok = word >> (token % 32) & 1;
+        copy_async<16>(keys + copy_at + j * kRows * G::kRow, codes[j], ok);
+        copy_async<16>(vals + copy_at + j * kRows * G::kRow, codes[j] + p.value_codes, ok);
       }
 #pragma unroll
       for (int j = 0; j < kBlocks; ++j) {
         const int token = (j * kThreads + tid) % kTile, side = (j * kThreads + tid) / kTile;
-        const bool ok = offs[token][0] >= 0;
+        uint32_t word = words[0];
+#pragma unroll
+        for (int k = 1; k < kWords; ++k) word = warp % kWords == k ? words[k] : word;  // a warp's tokens are those of a word
         copy_async<G::kScale>((side ? vals : keys) + kTile * G::kRow + token * G::kScale,
-                              p.cache.scale[side] + (ok ? offs[token][1] : 0), ok);
+                              scales[j] + (side ? p.value_scales : 0), word >> lane & 1);
       }
     }
     cp_async_commit();
   };
-  look(0);
-  query();
-  for (int i = 0; i < G::kAhead; ++i) {
-    if (i < count) place(i, i);
-    look(i + 1);
+  Look next;  // of the tile kAhead tiles ahead
+  {
+    // (the later ones' where the weights will be)
+    static_assert((G::kAhead - 1) * kTile * sizeof(Place) <= G::kPBytes, "places fit where the weights will be");
+    auto places_of = [&](int i) { return i == 0 ? places : reinterpret_cast<Place*>(smem + G::kOffP) + (i - 1) * kTile; };
+    Look first[G::kAhead];  // all on their way at once, with the query
+#pragma unroll
+    for (int i = 0; i < G::kAhead; ++i) first[i] = look(i);
+    next = look(G::kAhead);
+    query();
+#pragma unroll
+    for (int i = 0; i < G::kAhead; ++i) place(first[i], places_of(i), i);
     __syncthreads();
-    copy(i, i, i);
-    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < G::kAhead; ++i) copy(i, places_of(i), i, i);
   }
 
   // ---- a part of one (request, head) after the other ----
@@ -317,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
   int first_tile = 0;
   int key_stage = 0, value_stage = 0;   // of tile i
   for (int i = 0; i < count; ++i) {
-    if (fresh) {
+    if (__builtin_expect(fresh, 0)) {
       if (i > 0) query();
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
@@ -334,14 +388,17 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
     const uint32_t keys = sm + key_stage * G::kSide, vals = sm + G::kOffV + value_stage * G::kSide;
     const int pos0 = cur.tile * kTile;
     const bool masked_rows = pos0 + kTile - 1 > cur.len - p.q_len;  // some row does not see some token of the tile
-    uint32_t all_there = ~0u;
+    uint32_t words[kWords];
 #pragma unroll
-    for (int k = 0; k < kWords; ++k) all_there &= there[value_stage][k];
-    const uint32_t ok_bits = there[value_stage][kBlocks * warp / 2] >> (16 * (kBlocks * warp % 2));  // this warp's tokens
+    for (int k = 0; k < kWords; ++k) words[k] = there[value_stage][k];
+    uint32_t all_there = words[0], ok_bits = words[0];
+#pragma unroll
+    for (int k = 1; k < kWords; ++k) all_there &= words[k], ok_bits = kBlocks * warp / 2 == k ? words[k] : ok_bits;
+    ok_bits >>= 16 * (kBlocks * warp % 2);  // this warp's tokens
     const int value_free = value_stage == 0 ? G::kValueStages - 1 : value_stage - 1;  // the last tile's
-    if (i + G::kAhead < count) place(i + G::kAhead, value_free);
-    look(i + G::kAhead + 1);
-    if (masked_rows && tid < kTile) {
+    if (i + G::kAhead < count) place(next, places, value_free);
+    next = look(i + G::kAhead + 1);
+    if (__builtin_expect(masked_rows, 0) && tid < kTile) {
       // values that are not finite may be hidden from some rows only: they leave the product (a weight of zero would not
       // keep them out), and the rows that see one get their NaN afterwards
 #pragma unroll
@@ -398,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
         for (int e = 0; e < 4; ++e)
           x[blk][j][e] = fmaf(kChains == 2 ? y[0][j][e] + y[kChains - 1][j][e] : y[0][j][e], p.scale_log2, -ref[j][e & 1]);
     }
-    if (masked_rows || ~all_there) {
+    if (__builtin_expect(masked_rows || ~all_there, 0)) {
 #pragma unroll
       for (int blk = 0; blk < kBlocks; ++blk) {
         const int ta = 16 * (kBlocks * warp + blk) + g;
@@ -423,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
     float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NQ; ++j) top = fmaxf(top, fmaxf(highest(j, 0), highest(j, 1)));
-    if (unset)
+    if (__builtin_expect(unset != 0, 0))
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -431,9 +488,9 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
           if (unset >> (2 * j + e) & 1 && highest(j, e) > -INFINITY) top = INFINITY;
     // (all warps have read this tile's keys and the last one's values, whose stages are filled again now)
     const bool raise = __syncthreads_or(top > kSlack);
-    copy(i + G::kAhead, key_stage, value_free);
+    copy(i + G::kAhead, places, key_stage, value_free);
     float scale_o[NQ][2];
-    if (raise) {
+    if (__builtin_expect(raise, 0)) {
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
         float v[2];
@@ -483,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
     __syncthreads();                 // weights; and the next tile for all warps
 
     // ---- O^T += V^T P^T: 64 dimensions of this warp ----
-    if (raise)
+    if (__builtin_expect(raise, 0))
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -527,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
       times(std::integral_constant<int, 0>{}), times(std::integral_constant<int, 1>{});
       times(std::integral_constant<int, 2>{}), times(std::integral_constant<int, 3>{});
     }
-    if (masked_rows) {
+    if (__builtin_expect(masked_rows, 0)) {
 #pragma unroll
       for (int k = 0; k < kWords; ++k)
         if (const uint32_t bits = bad[i & 1][dim_warp][k])
@@ -541,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
 
     // ---- the end of a (request, head), or of this CTA's share of it ----
     const bool last_tile = cur.tile + 1 == cur.tiles;
-    if (last_tile || i + 1 == count) {
+    if (__builtin_expect(last_tile || i + 1 == count, 0)) {
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -607,9 +664,9 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
       if (i + 1 == count && tid == 0) {
         // the CTA that begins a (request, head) which others end names it for the join
         const bool open = first_tile == 0 && !last_tile;
-        const int64_t end_tile = end - 1 + (cur.tiles - 1 - cur.tile);  // its last tile; the CTA that holds it: the last
-        const int to = static_cast<int>(((end_tile + 1) * ctas - 1) / total);  // one whose share begins at or before it
-        p.joins[blockIdx.x] = open ? make_int4(cur.b, cur.h, to, cur.tile + 1 == count ? 0 : 1) : make_int4(-1, 0, 0, 0);
+        const uint32_t last = end - 1 + (cur.tiles - 1 - cur.tile);  // the position of its last tile
+        p.joins[blockIdx.x] = open ? make_int4(cur.b, cur.h, Shares(total, ctas).holder(last), cur.tile + 1 == count ? 0 : 1)
+                                   : make_int4(-1, 0, 0, 0);
       }
       fresh = true;
       __syncthreads();  // the query's place and `red` are free again
@@ -667,7 +724,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const AttnParams
     }
     if (named) {
       // (request and head, the CTA that begins it, the last one, whether its part is the first's last share)
-      list[at] = make_int4(join.x * p.cache.heads + join.y, from, join.z, join.w);
+      list[at] = make_int4(join.x * p.heads + join.y, from, join.z, join.w);
       rounds[at] = before;
     }
     __syncthreads();
@@ -741,7 +798,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const AttnParams
     }
     if (active && sub == 0) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const int b = join.x / p.cache.heads, h = join.x - b * p.cache.heads;
+      const int b = join.x / p.heads, h = join.x - b * p.heads;
       const int qi = r / p.group, hq = h * p.group + r - qi * p.group;
       __nv_bfloat16* dst = p.out + (static_cast<int64_t>(b) * p.q_len + qi) * p.ot + hq * p.oh + kJoinDims * piece + 4 * col;
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
@@ -816,7 +873,8 @@ extern "C" int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_k
                            int64_t so_t, int64_t so_h, int num_reqs, int q_len, int num_heads, float scale, void* ws,
                            size_t ws_bytes, unsigned flags, void* stream) {
   AttnParams p = {};
-  int rc = kv4_view(cache, &p.cache);
+  Kv4View c;
+  int rc = kv4_view(cache, &c);
   if (rc) return rc;
   if (num_reqs < 0 || q_len < 1 || num_heads < 0 || max_pages < 0) return fail(QF_ERR_SHAPE, "sizes");
   if (num_heads % cache->num_heads) return fail(QF_ERR_SHAPE, "query heads must be a multiple of the cache's heads");
@@ -825,6 +883,11 @@ extern "C" int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_k
   if (static_cast<int64_t>(num_reqs) * q_len > INT32_MAX / 64 || num_heads > 65535 ||
       static_cast<int64_t>(num_reqs) * cache->num_heads > INT32_MAX)
     return fail(QF_ERR_SHAPE, "too many query rows");
+  const int64_t tiles = static_cast<int64_t>(max_pages) * cache->page_size / 64 + 4;
+  if (static_cast<int64_t>(num_reqs) * cache->num_heads > INT32_MAX / (tiles < INT32_MAX ? tiles : INT32_MAX))
+    return fail(QF_ERR_SHAPE, "more keys than 2^31 tiles of 64 (requests, heads and the table's width together)");
+  if (c.page > UINT32_MAX || c.slot > UINT32_MAX || 2 * c.spage > UINT32_MAX || 2 * c.sslot > UINT32_MAX)
+    return fail(QF_ERR_STRIDE, "page and slot strides must be below 2^32 bytes");
   if (!(scale > -3.4e38f && scale < 3.4e38f)) return fail(QF_ERR_INVALID, "scale must be finite");
   if (num_reqs == 0 || num_heads == 0) return QF_OK;
   if (!q || !out || !seq_lens || (max_pages && !block_table)) return fail(QF_ERR_INVALID, "null pointer");
@@ -843,6 +906,17 @@ extern "C" int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_k
   p.table = block_table, p.table_row = s_bt;
   p.width = static_cast<int64_t>(max_pages) * cache->page_size;
   if (p.width > INT32_MAX - 1024) p.width = INT32_MAX - 1024;  // positions stay 32-bit numbers
+  p.codes = c.codes[0], p.scales = reinterpret_cast<const uint8_t*>(c.scale[0]);
+  p.value_codes = c.codes[1] - c.codes[0];
+  p.value_scales = reinterpret_cast<const uint8_t*>(c.scale[1]) - p.scales;
+  p.head = c.head, p.shead = 2 * c.shead;
+  p.page = static_cast<uint32_t>(c.page), p.slot = static_cast<uint32_t>(c.slot);
+  p.spage = static_cast<uint32_t>(2 * c.spage), p.sslot = static_cast<uint32_t>(2 * c.sslot);
+  if (c.num_pages == 0) {  // nothing is read, but addresses are formed
+    p.codes = p.scales = static_cast<const uint8_t*>(q);
+    p.value_codes = p.value_scales = 0;
+  }
+  p.num_pages = c.num_pages, p.page_size = c.page_size, p.heads = c.heads;
   p.lens = seq_lens;
   p.reqs = num_reqs, p.q_len = q_len, p.group = num_heads / cache->num_heads, p.rows = q_len * p.group;
   p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);

@@ -292,7 +292,15 @@ qf_kv4_cache check_attention(const char* op, const at::Tensor& query, const Cach
   check_input(op, "block_table", block_table, query.device());
   QF_REFUSE_UNLESS(query.size(0) <= INT32_MAX / 64 && query.size(1) <= 65535 && block_table.size(1) <= INT32_MAX, op,
                    ": too many query rows or pages for one call");
-  return check_cache(op, c, query.device(), false);
+  const qf_kv4_cache cache = check_cache(op, c, query.device(), false);
+  const int64_t tiles = block_table.size(1) * cache.page_size / 64 + 4;  // of a request and head
+  QF_REFUSE_UNLESS(tiles <= INT32_MAX && seq_lens.size(0) * cache.num_heads <= INT32_MAX / tiles, op, ": ",
+                   seq_lens.size(0), " requests of up to ", block_table.size(1) * cache.page_size, " keys in ",
+                   cache.num_heads, " heads are too many for one call");
+  for (int i : {0, 2})
+    QF_REFUSE_UNLESS(stride_of(c.k, i) <= UINT32_MAX && stride_of(c.k_scale, i) <= UINT32_MAX / 2, op,
+                     ": a cache's pages and slots must lie less than 2^32 bytes apart");
+  return cache;
 }
 
 at::Tensor kv4_attention(const at::Tensor& query, const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& cks,
