@@ -266,7 +266,7 @@ int qf_residual_norm_status(void* stream, int* status);
  * A group with a NaN, an infinity or a magnitude of 2^126 or more becomes NaN.  k, v: uint8, element (page, head, slot) at
  * page * page_stride + head * head_stride + slot * slot_stride bytes, head_size / 2 bytes each; k_scale, v_scale: bf16
  * [head_size / 64][2] at the scale strides (elements).  head_size 64, 128 or 256; any page size; pointers and strides of the
- * codes multiples of 16 bytes, those of the scales of head_size / 64 pairs. */
+ * codes multiples of 16 bytes, those of the scales of head_size / 64 pairs, page and slot strides below 2^32 bytes. */
 #define QF_KV4_GROUP 64
 typedef struct qf_kv4_cache {
   void* k;
@@ -293,7 +293,7 @@ int qf_kv4_read(void* k, int64_t sk_t, int64_t sk_h, void* v, int64_t sv_t, int6
  * is no page of the cache, do not take part; what lies in slots that a row does not attend, NaN included, does not touch it.
  * q, out: bf16, 16-byte aligned with strides multiples of 8 elements; q_len * num_heads / cache->num_heads <= 64; block_table
  * int32 (row stride s_bt, max_pages entries each);
- * num_reqs * heads * (max_pages * page_size / 64 + 4) below 2^31, page and slot strides below 2^32 bytes.  The workspace (>= qf_kv4_attn_workspace_bytes() on the current device,
+ * num_reqs * heads * (max_pages * page_size / 64 + 4) below 2^31.  The workspace (>= qf_kv4_attn_workspace_bytes() on the current device,
  * 256-byte aligned) need not be zeroed and holds nothing between calls.  No host synchronisation. */
 size_t qf_kv4_attn_workspace_bytes(int num_reqs, int q_len, int num_heads, int num_kv_heads, int head_size);
 int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_kv4_cache* cache, const int32_t* block_table,

@@ -1,7 +1,8 @@
 // qf_kv4.cu -- writes keys and values into a paged cache held in 4 bits, and reads them back (qf_kv4.cuh has the format).
 //
 // Both are bound by memory: a token and head of D values is 2 D bytes on one side and D / 2 + D / 16 on the other.  A thread
-// takes eight values (16 bytes of bf16, one word of nibbles), eight threads a group, whose extremes are three shuffles.
+// takes eight values (16 bytes of bf16, one word of nibbles) of several tokens, eight threads a group, whose extremes are
+// three shuffles.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -35,12 +36,15 @@ int kv4_view(const qf_kv4_cache* c, Kv4View* v) {
   for (int i = 0; i < 2; ++i)
     if (reinterpret_cast<uintptr_t>(codes[i]) % 16 || reinterpret_cast<uintptr_t>(scales[i]) % (2 * pair))
       return fail(QF_ERR_ALIGN, "cache pointers");
+  if (st[0] > UINT32_MAX || st[2] > UINT32_MAX || ss[0] > UINT32_MAX / 2 || ss[2] > UINT32_MAX / 2)
+    return fail(QF_ERR_STRIDE, "a cache's pages and slots must lie less than 2^32 bytes apart");
   v->codes[0] = static_cast<uint8_t*>(c->k);
   v->codes[1] = static_cast<uint8_t*>(c->v);
-  v->scale[0] = static_cast<__nv_bfloat16*>(c->k_scale);
-  v->scale[1] = static_cast<__nv_bfloat16*>(c->v_scale);
-  v->page = st[0], v->head = st[1], v->slot = st[2];
-  v->spage = ss[0], v->shead = ss[1], v->sslot = ss[2];
+  v->scale[0] = static_cast<uint8_t*>(c->k_scale);
+  v->scale[1] = static_cast<uint8_t*>(c->v_scale);
+  v->page = static_cast<uint32_t>(st[0]), v->head = st[1], v->slot = static_cast<uint32_t>(st[2]);
+  v->spage = static_cast<uint32_t>(2 * ss[0]), v->shead = 2 * ss[1], v->sslot = static_cast<uint32_t>(2 * ss[2]);
+  kv4_divisor(c->page_size, &v->div_mul, &v->div_shift);
   v->num_pages = c->num_pages, v->page_size = c->page_size, v->heads = c->num_heads;
   return QF_OK;
 }
@@ -52,85 +56,99 @@ struct Kv4IoParams {
   __nv_bfloat16* x[2];  // keys and values: read, or written by the reader
   int64_t xt[2], xh[2];
   const int64_t* slots;
-  uint32_t items;       // pieces of eight values
-  int pieces;           // of a head
+  int tokens;
+  int items;            // pieces of eight values of a token: (keys or values, head, piece), the piece innermost
+  int per_pass;         // tokens that a CTA takes at a time
+  int passes;           // up to kIoTokens
 };
 
-// Where a slot is: false if it is none of the cache's.
-__device__ __forceinline__ bool place(const Kv4View& c, int64_t slot, int64_t& page, int64_t& off) {
-  if (slot < 0) return false;
-  page = slot / c.page_size;
-  off = slot - page * c.page_size;
-  return page < c.num_pages;
-}
-
 constexpr int kIoThreads = 256;
+constexpr int kIoTokens = 4;
 
-// Items: (token, keys or values, head, piece), the piece innermost; eight in a row share a group and a warp.
-__global__ void __launch_bounds__(kIoThreads) kv4_write_kernel(const Kv4IoParams p) {
+// A CTA takes passes * per_pass tokens, a thread the same piece of `passes` of them: which piece that is, and of which head,
+// is found out once, and the passes' loads are under way together.  Eight threads in a row share a group and a warp.
+template <int D, bool WRITE> __global__ void __launch_bounds__(kIoThreads) kv4_io_kernel(const Kv4IoParams p) {
+  constexpr int kPieces = D / 8;
   pdl_launch_dependents();
   pdl_wait();
-  const uint32_t i = blockIdx.x * kIoThreads + threadIdx.x;
-  const uint32_t at = i < p.items ? i : p.items - 1;
-  const int piece = at % p.pieces;
-  uint32_t rest = at / p.pieces;
-  const int head = rest % p.cache.heads;
-  rest /= p.cache.heads;
-  const int side = rest & 1;
-  const int64_t token = rest >> 1;
-  const uint4 u = *reinterpret_cast<const uint4*>(p.x[side] + token * p.xt[side] + head * p.xh[side] + 8 * piece);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-  float x[8];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) x[2 * j] = bf16_lo(w[j]), x[2 * j + 1] = bf16_hi(w[j]);
-  float hi = x[0], lo = -x[0];
-#pragma unroll
-  for (int j = 1; j < 8; ++j) hi = max_nan(hi, x[j]), lo = max_nan(lo, -x[j]);
-#pragma unroll
-  for (int off = 1; off < 8; off <<= 1) {
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-    lo = max_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-  }
-  float s, c;
-  kv4_scale(-lo, hi, s, c);
-  uint32_t code = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) code |= kv4_code(x[j], s, c) << (4 * j);
-  int64_t page, off;
-  if (i >= p.items || !place(p.cache, p.slots[token], page, off)) return;
   const Kv4View& v = p.cache;
-  reinterpret_cast<uint32_t*>(v.codes[side] + page * v.page + head * v.head + off * v.slot)[piece] = code;
-  if (piece % 8 == 0)
-    reinterpret_cast<__nv_bfloat162*>(v.scale[side] + page * v.spage + head * v.shead + off * v.sslot)[piece / 8] =
-        __floats2bfloat162_rn(s, c);
+  const int local = p.items >= kIoThreads ? 0 : threadIdx.x / p.items;
+  if (local >= p.per_pass) return;  // (whole groups of eight)
+  const uint32_t group = 0xffu << (threadIdx.x & 24);
+  for (int item = threadIdx.x - local * p.items; item < p.items; item += kIoThreads) {
+    const int piece = item % kPieces, hh = item / kPieces, side = hh >= v.heads, head = hh - side * v.heads;
+    __nv_bfloat16* const x = p.x[side] + head * p.xh[side] + 8 * piece;
+    uint8_t* const codes = v.codes[side] + head * v.head + 4 * piece;
+    uint8_t* const scale = v.scale[side] + head * v.shead + 4 * (piece / 8);
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (p.passes * p.per_pass) + local;
+    int64_t slot[kIoTokens];
+    uint4 u[kIoTokens];
+#pragma unroll
+    for (int i = 0; i < kIoTokens; ++i) {
+      const int64_t token = first + i * p.per_pass;
+      slot[i] = -1;
+      if (i < p.passes && token < p.tokens) {
+        slot[i] = p.slots[token];
+        if (WRITE) u[i] = *reinterpret_cast<const uint4*>(x + token * p.xt[side]);
+      }
+    }
+    uint32_t page[kIoTokens], off[kIoTokens];
+    bool ok[kIoTokens];
+#pragma unroll
+    for (int i = 0; i < kIoTokens; ++i) ok[i] = v.place(slot[i], page[i], off[i]);
+    if (WRITE) {
+#pragma unroll
+      for (int i = 0; i < kIoTokens; ++i) {
+        if (!ok[i]) continue;  // (the same for the eight threads of a group)
+        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[2 * j] = bf16_lo(w[j]), f[2 * j + 1] = bf16_hi(w[j]);
+        float hi = f[0], lo = -f[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) hi = max_nan(hi, f[j]), lo = max_nan(lo, -f[j]);
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) {
+          hi = max_nan(hi, __shfl_xor_sync(group, hi, d));
+          lo = max_nan(lo, __shfl_xor_sync(group, lo, d));
+        }
+        float s, c;
+        kv4_scale(-lo, hi, s, c);
+        *reinterpret_cast<uint32_t*>(codes + v.codes_at(page[i], off[i])) = kv4_codes(f, s, c);
+        if (piece % 8 == 0)
+          *reinterpret_cast<__nv_bfloat162*>(scale + v.scale_at(page[i], off[i])) = __floats2bfloat162_rn(s, c);
+      }
+    } else {
+      uint32_t w[kIoTokens], sc[kIoTokens];
+#pragma unroll
+      for (int i = 0; i < kIoTokens; ++i)
+        if (ok[i]) {
+          w[i] = *reinterpret_cast<const uint32_t*>(codes + v.codes_at(page[i], off[i]));
+          sc[i] = *reinterpret_cast<const uint32_t*>(scale + v.scale_at(page[i], off[i]));
+        }
+#pragma unroll
+      for (int i = 0; i < kIoTokens; ++i) {
+        const int64_t token = first + i * p.per_pass;
+        if (i >= p.passes || token >= p.tokens) continue;
+        uint4 r = make_uint4(0, 0, 0, 0);
+        if (ok[i]) {
+          const uint32_t ss = dup_lo(sc[i]), cc = dup_hi(sc[i]);
+          // pairs of nibbles (k, k + 4) -> values in order
+          const uint32_t a = kv4_pair<0>(w[i], ss, cc), b = kv4_pair<1>(w[i], ss, cc), c = kv4_pair<2>(w[i], ss, cc),
+                         d = kv4_pair<3>(w[i], ss, cc);
+          r = make_uint4(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), __byte_perm(a, b, 0x7632),
+                         __byte_perm(c, d, 0x7632));
+        }
+        *reinterpret_cast<uint4*>(x + token * p.xt[side]) = r;
+      }
+    }
+  }
 }
 
-__global__ void __launch_bounds__(kIoThreads) kv4_read_kernel(const Kv4IoParams p) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const uint32_t i = blockIdx.x * kIoThreads + threadIdx.x;
-  if (i >= p.items) return;
-  const int piece = i % p.pieces;
-  uint32_t rest = i / p.pieces;
-  const int head = rest % p.cache.heads;
-  rest /= p.cache.heads;
-  const int side = rest & 1;
-  const int64_t token = rest >> 1;
-  uint4 r = make_uint4(0, 0, 0, 0);
-  int64_t page, off;
-  if (place(p.cache, p.slots[token], page, off)) {
-    const Kv4View& v = p.cache;
-    const uint32_t w = reinterpret_cast<const uint32_t*>(v.codes[side] + page * v.page + head * v.head + off * v.slot)[piece];
-    const uint32_t sc = reinterpret_cast<const uint32_t*>(v.scale[side] + page * v.spage + head * v.shead +
-                                                          off * v.sslot)[piece / 8];
-    const uint32_t ss = dup_lo(sc), cc = dup_hi(sc);
-    // pairs of nibbles (k, k + 4) -> values in order
-    const uint32_t a = kv4_pair<0>(w, ss, cc), b = kv4_pair<1>(w, ss, cc), c = kv4_pair<2>(w, ss, cc),
-                   d = kv4_pair<3>(w, ss, cc);
-    r = make_uint4(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), __byte_perm(a, b, 0x7632),
-                   __byte_perm(c, d, 0x7632));
-  }
-  *reinterpret_cast<uint4*>(p.x[side] + token * p.xt[side] + head * p.xh[side] + 8 * piece) = r;
+template <bool WRITE> cudaError_t launch_io(const cudaLaunchConfig_t& cfg, const Kv4IoParams& p, int head_size) {
+  return head_size == 64    ? cudaLaunchKernelEx(&cfg, kv4_io_kernel<64, WRITE>, p)
+         : head_size == 128 ? cudaLaunchKernelEx(&cfg, kv4_io_kernel<128, WRITE>, p)
+                            : cudaLaunchKernelEx(&cfg, kv4_io_kernel<256, WRITE>, p);
 }
 
 int kv4_io(const void* k, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_t, int64_t sv_h, const int64_t* slots,
@@ -141,9 +159,8 @@ int kv4_io(const void* k, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_
   if (tokens < 0) return fail(QF_ERR_SHAPE, "negative size");
   if (tokens == 0) return QF_OK;
   if (!k || !v || !slots) return fail(QF_ERR_INVALID, "null pointer");
-  p.pieces = cache->head_size / 8;
-  const int64_t items = 2ll * tokens * cache->num_heads * p.pieces;
-  if (items > INT32_MAX) return fail(QF_ERR_SHAPE, "more than 2^31 - 1 pieces of eight values");
+  const int64_t items = 2ll * cache->num_heads * (cache->head_size / 8);
+  if (items * tokens > INT32_MAX) return fail(QF_ERR_SHAPE, "more than 2^31 - 1 pieces of eight values");
   const int64_t st[] = {sk_t, sk_h, sv_t, sv_h};
   for (int64_t s : st) {
     if (s < 0) return fail(QF_ERR_STRIDE, "negative stride");
@@ -158,9 +175,14 @@ int kv4_io(const void* k, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_
   p.x[1] = static_cast<__nv_bfloat16*>(const_cast<void*>(v));
   p.xt[0] = sk_t, p.xh[0] = sk_h, p.xt[1] = sv_t, p.xh[1] = sv_h;
   p.slots = slots;
-  p.items = static_cast<uint32_t>(items);
+  p.tokens = tokens;
+  p.items = static_cast<int>(items);
+  p.per_pass = items >= kIoThreads ? 1 : static_cast<int>(kIoThreads / items);
+  // several passes where there are CTAs enough for the SMs all the same
+  p.passes = tokens / p.per_pass >= 4 * kIoTokens * 148 ? kIoTokens : 1;
+  const int per_cta = p.passes * p.per_pass;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((items + kIoThreads - 1) / kIoThreads));
+  cfg.gridDim = dim3(static_cast<unsigned>((tokens + static_cast<int64_t>(per_cta) - 1) / per_cta));
   cfg.blockDim = dim3(kIoThreads);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
@@ -168,7 +190,7 @@ int kv4_io(const void* k, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = (flags & QF_FLAG_PDL) ? 1 : 0;
-  const cudaError_t e = write ? cudaLaunchKernelEx(&cfg, kv4_write_kernel, p) : cudaLaunchKernelEx(&cfg, kv4_read_kernel, p);
+  const cudaError_t e = write ? launch_io<true>(cfg, p, cache->head_size) : launch_io<false>(cfg, p, cache->head_size);
   return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
 }
 

@@ -19,17 +19,44 @@ namespace qf {
 
 constexpr int kKv4Group = QF_KV4_GROUP;
 
-// Device copy of qf_kv4_cache with typed pointers; strides of codes in bytes, of scales in bf16 elements.
+// Device copy of qf_kv4_cache; strides in bytes.
 struct Kv4View {
   uint8_t* codes[2];
-  __nv_bfloat16* scale[2];
-  int64_t page, head, slot;
-  int64_t spage, shead, sslot;
+  uint8_t* scale[2];
+  int64_t head, shead;
+  uint32_t page, slot, spage, sslot;
   int num_pages, page_size, heads;
+  uint32_t div_mul, div_shift;  // by the page size
+  __device__ __forceinline__ int64_t codes_at(uint32_t pg, uint32_t off) const {
+    return static_cast<int64_t>(static_cast<uint64_t>(pg) * page + static_cast<uint64_t>(off) * slot);
+  }
+  __device__ __forceinline__ int64_t scale_at(uint32_t pg, uint32_t off) const {
+    return static_cast<int64_t>(static_cast<uint64_t>(pg) * spage + static_cast<uint64_t>(off) * sslot);
+  }
+  // Where a slot is: false if it is none of the cache's.
+  __device__ __forceinline__ bool place(int64_t s, uint32_t& pg, uint32_t& off) const {
+    if (static_cast<uint64_t>(s) < 0x80000000u) {
+      pg = (__umulhi(static_cast<uint32_t>(s), div_mul) + static_cast<uint32_t>(s)) >> div_shift;
+      off = static_cast<uint32_t>(s) - pg * static_cast<uint32_t>(page_size);
+      return pg < static_cast<uint32_t>(num_pages);
+    }
+    pg = off = 0;
+    if (s < 0 || s >= static_cast<int64_t>(num_pages) * page_size) return false;
+    pg = static_cast<uint32_t>(s / page_size);
+    off = static_cast<uint32_t>(s - static_cast<int64_t>(pg) * page_size);
+    return true;
+  }
 };
 
 // Checks of a caller's cache that need no device; fills the view.  QF_OK or the code recorded by fail().
 int kv4_view(const qf_kv4_cache* cache, Kv4View* view);
+
+// n / d = (umulhi(n, mul) + n) >> shift for n below 2^31 (Granlund and Montgomery, PLDI 1994).
+inline void kv4_divisor(int d, uint32_t* mul, uint32_t* shift) {
+  *shift = 0;
+  while ((1ull << *shift) < static_cast<uint64_t>(d)) ++*shift;
+  *mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << *shift) - static_cast<uint64_t>(d))) / static_cast<uint64_t>(d) + 1);
+}
 
 // Step and offset of a group from its least and greatest value (any NaN among them makes both NaN).
 __device__ __forceinline__ void kv4_scale(float lo, float hi, float& s, float& c) {
@@ -40,10 +67,32 @@ __device__ __forceinline__ void kv4_scale(float lo, float hi, float& s, float& c
   if (!(fabsf(lo) < kMax && fabsf(hi) < kMax)) s = c = __int_as_float(0x7fffffff);
 }
 
-// The nibble of a value.  NaN groups keep nibble 0.
-__device__ __forceinline__ uint32_t kv4_code(float x, float s, float c) {
-  const float q = rintf(__fdiv_rn(x - c, s));
-  return s > 0.f ? static_cast<uint32_t>(fminf(fmaxf(q, 16.f), 31.f)) - 16u : 0u;
+// The nibbles of a group's values.  Quotients are below 128 (the step is at least 2^-13 of the largest magnitude, and c's
+// rounding moves them by less than a hundred), so that one by the reciprocal, two roundings, is at most 2^-16 off; only where
+// it comes within 2^-14 of a border between two nibbles, where that might decide, is it made by a division.
+struct Kv4Coder {
+  float s, c, inv;
+  __device__ __forceinline__ Kv4Coder(float step, float offset) {
+    s = step, c = offset;
+    // a step of zero, and steps so small that their reciprocal is no normal number, take the division
+    inv = s > 1e-37f ? __frcp_rn(s) : __int_as_float(0x7fffffff);
+  }
+  __device__ __forceinline__ uint32_t operator()(float x) const {
+    const float d = x - c, q = d * inv;
+    constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers, ties to even
+    float n = (q + kWhole) - kWhole;
+    if (!(fabsf(q - n) < 0.5f - 6.1035156e-5f)) n = s > 0.f ? rintf(__fdiv_rn(d, s)) : 16.f;
+    return static_cast<uint32_t>(__float_as_int(fminf(fmaxf(n, 16.f), 31.f) + kWhole)) & 15u;  // (31 - 16 = 15, 16 = 0)
+  }
+};
+
+// The word of eight values' nibbles.
+__device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], float s, float c) {
+  const Kv4Coder code(s, c);
+  uint32_t r = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r |= code(x[j]) << (4 * j);
+  return r;
 }
 
 // The two values of the nibbles at bits 4 k and 16 + 4 k of w, as the low and the high half of a bf16 pair.

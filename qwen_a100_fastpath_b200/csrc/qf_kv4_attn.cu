@@ -886,8 +886,6 @@ extern "C" int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_k
   const int64_t tiles = static_cast<int64_t>(max_pages) * cache->page_size / 64 + 4;
   if (static_cast<int64_t>(num_reqs) * cache->num_heads > INT32_MAX / (tiles < INT32_MAX ? tiles : INT32_MAX))
     return fail(QF_ERR_SHAPE, "more keys than 2^31 tiles of 64 (requests, heads and the table's width together)");
-  if (c.page > UINT32_MAX || c.slot > UINT32_MAX || 2 * c.spage > UINT32_MAX || 2 * c.sslot > UINT32_MAX)
-    return fail(QF_ERR_STRIDE, "page and slot strides must be below 2^32 bytes");
   if (!(scale > -3.4e38f && scale < 3.4e38f)) return fail(QF_ERR_INVALID, "scale must be finite");
   if (num_reqs == 0 || num_heads == 0) return QF_OK;
   if (!q || !out || !seq_lens || (max_pages && !block_table)) return fail(QF_ERR_INVALID, "null pointer");
@@ -906,12 +904,11 @@ extern "C" int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_k
   p.table = block_table, p.table_row = s_bt;
   p.width = static_cast<int64_t>(max_pages) * cache->page_size;
   if (p.width > INT32_MAX - 1024) p.width = INT32_MAX - 1024;  // positions stay 32-bit numbers
-  p.codes = c.codes[0], p.scales = reinterpret_cast<const uint8_t*>(c.scale[0]);
-  p.value_codes = c.codes[1] - c.codes[0];
-  p.value_scales = reinterpret_cast<const uint8_t*>(c.scale[1]) - p.scales;
-  p.head = c.head, p.shead = 2 * c.shead;
-  p.page = static_cast<uint32_t>(c.page), p.slot = static_cast<uint32_t>(c.slot);
-  p.spage = static_cast<uint32_t>(2 * c.spage), p.sslot = static_cast<uint32_t>(2 * c.sslot);
+  p.codes = c.codes[0], p.scales = c.scale[0];
+  p.value_codes = c.codes[1] - c.codes[0], p.value_scales = c.scale[1] - c.scale[0];
+  p.head = c.head, p.shead = c.shead;
+  p.page = c.page, p.slot = c.slot, p.spage = c.spage, p.sslot = c.sslot;
+  p.div_mul = c.div_mul, p.div_shift = c.div_shift;
   if (c.num_pages == 0) {  // nothing is read, but addresses are formed
     p.codes = p.scales = static_cast<const uint8_t*>(q);
     p.value_codes = p.value_scales = 0;
@@ -920,9 +917,6 @@ extern "C" int qf_kv4_attn(const void* q, int64_t sq_t, int64_t sq_h, const qf_k
   p.lens = seq_lens;
   p.reqs = num_reqs, p.q_len = q_len, p.group = num_heads / cache->num_heads, p.rows = q_len * p.group;
   p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
-  // n / page_size = (umulhi(n, mul) + n) >> shift for n below 2^31 (Granlund and Montgomery, PLDI 1994)
-  while ((1ull << p.div_shift) < static_cast<uint64_t>(cache->page_size)) ++p.div_shift;
-  p.div_mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << p.div_shift) - cache->page_size)) / cache->page_size + 1);
   if (sms > kMaxSms) sms = kMaxSms;
   const int grid = sms * ctas_per_sm(cache->head_size, tiles_of_rows(p.rows));
   const size_t parts = 2 * static_cast<size_t>(kMaxSms) * ctas_per_sm(cache->head_size, tiles_of_rows(p.rows));

@@ -36,12 +36,171 @@ struct RopeParams {
   float offset, eps, inv_d;
   int heads[2];
   int D, rot;
-  int rows;       // of a token
-  uint32_t total;  // rows of all tokens
+  int rows;        // of a token; kWide: groups of rows
+  uint32_t total;  // of all tokens
+  int groups[2];   // kWide: of the queries and of the keys
   int cs_f32, interleaved;
 };
 
 constexpr int kRopeWarps = 4;
+
+// How rows are read: kAny takes any size, stride and alignment, element by element with the row in shared memory; kWide rows
+// whose pointers and strides are multiples of 16 bytes, with heads of up to 256 (a multiple of eight) and a rotated part that
+// is a multiple of 16 (of eight where interleaved).  8192 tokens of 24 + 4 heads of 256, 64 of them rotated: 99 us with kAny.
+
+// kWide: L lanes take a row, a lane eight consecutive values in one 16-byte load.  A group of L lanes takes ROWS heads of one
+// side of one token, so that the token's angles and the weight are loaded once for them and ROWS loads are under way.  The
+// other half of a turned pair is L's other lanes' (a shuffle of the raw bf16 words; its weight is loaded beside the lane's
+// own), or the neighbour in the lane's own registers where interleaved.
+template <int L, int ROWS>
+__global__ void __launch_bounds__(kRopeWarps * 32) rope_wide_kernel(const RopeParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x % L;
+  const uint32_t item = blockIdx.x * (kRopeWarps * 32 / L) + threadIdx.x / L;
+  // (groups past the end go on with the last one's work, without storing: the shuffles name whole warps)
+  const uint32_t at = item < p.total ? item : p.total - 1;
+  const uint32_t token = at / p.rows;
+  int part = at - token * p.rows, side = 0;
+  if (part >= p.groups[0]) part -= p.groups[0], side = 1;
+  if (side == 1 && part >= p.groups[1]) part -= p.groups[1], side = 2;
+  const int heads = side == 0 ? p.heads[0] : p.heads[1], head0 = part * ROWS;
+  const int e = 8 * lane;
+  const bool in = e < p.D;
+  const __nv_bfloat16* x = p.x[side] + static_cast<int64_t>(token) * p.xt[side] + head0 * p.xh[side] + e;
+  uint4 u[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    u[i] = make_uint4(0, 0, 0, 0);
+    if (in && head0 + i < heads) u[i] = *reinterpret_cast<const uint4*>(x + i * p.xh[side]);
+  }
+  const bool normed = side < 2 && p.weight[side], turned = side < 2 && p.cos_sin && e < p.rot;
+  const int half = p.rot / 2;
+  const int swap = half / 8;  // lanes between the halves of a pair
+  const bool upper = !p.interleaved && e >= half;
+  float cs[8], sn[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f;
+  if (turned) {
+    const int64_t pos = p.positions[token];
+    const int n = p.interleaved ? 4 : 8, i0 = p.interleaved ? e / 2 : upper ? e - half : e;
+    if (pos >= 0 && pos < p.max_pos) {
+      const int64_t row = pos * p.cs_row + i0;
+      if (p.cs_f32) {
+        const float* t = static_cast<const float*>(p.cos_sin) + row;
+        for (int k = 0; k < n; k += 4) {
+          const float4 a = *reinterpret_cast<const float4*>(t + k), b = *reinterpret_cast<const float4*>(t + half + k);
+          cs[k] = a.x, cs[k + 1] = a.y, cs[k + 2] = a.z, cs[k + 3] = a.w;
+          sn[k] = b.x, sn[k + 1] = b.y, sn[k + 2] = b.z, sn[k + 3] = b.w;
+        }
+      } else {
+        const __nv_bfloat16* t = static_cast<const __nv_bfloat16*>(p.cos_sin) + row;
+        for (int k = 0; k < n; k += 4) {
+          const uint2 a = *reinterpret_cast<const uint2*>(t + k), b = *reinterpret_cast<const uint2*>(t + half + k);
+          cs[k] = bf16_lo(a.x), cs[k + 1] = bf16_hi(a.x), cs[k + 2] = bf16_lo(a.y), cs[k + 3] = bf16_hi(a.y);
+          sn[k] = bf16_lo(b.x), sn[k + 1] = bf16_hi(b.x), sn[k + 2] = bf16_lo(b.y), sn[k + 3] = bf16_hi(b.y);
+        }
+      }
+    } else {
+      for (int k = 0; k < 8; ++k) cs[k] = sn[k] = __int_as_float(0x7fffffff);
+    }
+    if (p.interleaved)
+#pragma unroll
+      for (int k = 3; k >= 0; --k) cs[2 * k] = cs[2 * k + 1] = cs[k], sn[2 * k] = -sn[k], sn[2 * k + 1] = -sn[2 * k];
+    else if (!upper)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sn[k] = -sn[k];
+  }
+  // y = n (x w cos + x' w' sin), x' the other of the pair, the sign of the sine taken in above: two coefficients an element
+  const int other = turned && !p.interleaved ? (upper ? lane - swap : lane + swap) : lane;
+  uint64_t ca[4], cb[4];
+  {
+    float w[8], w2[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = w2[i] = 1.f;
+    if (normed && in) {
+      const uint4 a = *reinterpret_cast<const uint4*>(p.weight[side] + e);
+      const uint4 b = *reinterpret_cast<const uint4*>(p.weight[side] + 8 * other);
+      const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        w[2 * k] = bf16_lo(wa[k]) + p.offset, w[2 * k + 1] = bf16_hi(wa[k]) + p.offset;
+        w2[2 * k] = bf16_lo(wb[k]) + p.offset, w2[2 * k + 1] = bf16_hi(wb[k]) + p.offset;
+        if (p.interleaved) {
+          const float t = w2[2 * k];
+          w2[2 * k] = w2[2 * k + 1], w2[2 * k + 1] = t;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      ca[k] = pack_f32x2(w[2 * k] * cs[2 * k], w[2 * k + 1] * cs[2 * k + 1]);
+      cb[k] = pack_f32x2(w2[2 * k] * sn[2 * k], w2[2 * k + 1] * sn[2 * k + 1]);
+    }
+  }
+  uint32_t page = 0, off = 0;
+  const bool cached = side > 0 && !p.out[1] && p.cache.place(p.slots[token], page, off);
+  const uint32_t keep = turned ? ~0u : 0u;  // values that do not turn have no other (an infinity times zero would be NaN)
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const uint32_t raw[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+    uint64_t v2[4], sums = pack_f32x2(0.f, 0.f);
+    uint32_t r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t a = pack_f32x2(bf16_lo(raw[k]), bf16_hi(raw[k]));
+      fma_f32x2(sums, a, a);
+      // the other half of a turned pair: another lane's words, or this one's with its halves exchanged
+      const uint32_t x2 = keep & (p.interleaved ? __byte_perm(raw[k], raw[k], 0x1032)
+                                                : __shfl_sync(0xffffffffu, raw[k], other, L));
+      v2[k] = mul_f32x2(pack_f32x2(bf16_lo(x2), bf16_hi(x2)), cb[k]);
+      fma_f32x2(v2[k], a, ca[k]);
+    }
+    const float2 both = unpack_f32x2(sums);
+    float n = 1.f;
+    if (p.weight[0] || p.weight[1]) {
+      float sum = both.x + both.y;
+#pragma unroll
+      for (int d = L / 2; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (normed) n = rsqrtf(fmaf(sum, p.inv_d, p.eps));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 y = unpack_f32x2(mul_f32x2(v2[k], pack_f32x2(n, n)));
+      const __nv_bfloat162 h = __floats2bfloat162_rn(y.x, y.y);
+      r[k] = reinterpret_cast<const uint32_t&>(h);
+    }
+    const bool store = in && item < p.total && head0 + i < heads;
+    if (side < 2 && p.out[side]) {
+      if (store)
+        *reinterpret_cast<uint4*>(p.out[side] + static_cast<int64_t>(token) * p.ot[side] + (head0 + i) * p.oh[side] + e) =
+            make_uint4(r[0], r[1], r[2], r[3]);
+    }
+    if (p.out[1]) continue;
+    // into the cache, from the rounded values (all lanes go along: a warp may hold groups of queries too)
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[2 * k] = bf16_lo(r[k]), v[2 * k + 1] = bf16_hi(r[k]);
+    float hi = v[0], lo = -v[0];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) hi = max_nan(hi, v[k]), lo = max_nan(lo, -v[k]);
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) {
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+      lo = max_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+    }
+    if (!cached || !store) continue;
+    float s, c;
+    kv4_scale(-lo, hi, s, c);
+    const Kv4View& view = p.cache;
+    const int kv = side - 1, head = head0 + i;
+    *reinterpret_cast<uint32_t*>(view.codes[kv] + head * view.head + view.codes_at(page, off) + e / 2) =
+        kv4_codes(v, s, c);
+    if (lane % 8 == 0)
+      reinterpret_cast<__nv_bfloat162*>(view.scale[kv] + head * view.shead + view.scale_at(page, off))[lane / 8] =
+          __floats2bfloat162_rn(s, c);
+  }
+}
 
 __global__ void __launch_bounds__(kRopeWarps * 32) rope_any_kernel(const RopeParams p) {
   __shared__ float row_buf[kRopeWarps][QF_ROPE_MAX_D];
@@ -96,14 +255,12 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_any_kernel(const RopePar
     for (int e = lane; e < p.D; e += 32) o[e] = __float2bfloat16_rn(buf[e]);
     return;
   }
-  const int64_t slot = p.slots[token];
-  if (slot < 0) return;
-  const int64_t page = slot / p.cache.page_size, off = slot % p.cache.page_size;
-  if (page >= p.cache.num_pages) return;
+  uint32_t page, off;
   const Kv4View& v = p.cache;
+  if (!v.place(p.slots[token], page, off)) return;
   const int kv = side - 1;
-  uint8_t* codes = v.codes[kv] + page * v.page + head * v.head + off * v.slot;
-  __nv_bfloat16* scale = v.scale[kv] + page * v.spage + head * v.shead + off * v.sslot;
+  uint8_t* codes = v.codes[kv] + head * v.head + v.codes_at(page, off);
+  uint8_t* scale = v.scale[kv] + head * v.shead + v.scale_at(page, off);
   for (int g = 0; g < p.D / kKv4Group; ++g) {
     const float a = __bfloat162float(__float2bfloat16_rn(buf[g * kKv4Group + 2 * lane]));
     const float b = __bfloat162float(__float2bfloat16_rn(buf[g * kKv4Group + 2 * lane + 1]));
@@ -115,7 +272,8 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_any_kernel(const RopePar
     }
     float s, c;
     kv4_scale(-lo, hi, s, c);
-    codes[g * (kKv4Group / 2) + lane] = static_cast<uint8_t>(kv4_code(a, s, c) | kv4_code(b, s, c) << 4);
+    const Kv4Coder code(s, c);
+    codes[g * (kKv4Group / 2) + lane] = static_cast<uint8_t>(code(a) | code(b) << 4);
     if (lane == 0) reinterpret_cast<__nv_bfloat162*>(scale)[g] = __floats2bfloat162_rn(s, c);
   }
 }
@@ -186,8 +344,25 @@ extern "C" int qf_qk_norm_rope(const void* q, int64_t sq_t, int64_t sq_h, const 
   p.D = head_size;
   p.rows = static_cast<int>(rows);
   p.total = static_cast<uint32_t>(rows * tokens);
+  auto wide_rows = [](const void* ptr, int64_t st_t, int64_t st_h) {
+    return !ptr || (aligned(ptr, 16) && st_t % 8 == 0 && st_h % 8 == 0);
+  };
+  const bool wide = head_size % 8 == 0 && head_size <= 256 && rot % (interleaved ? 8 : 16) == 0 &&
+                    wide_rows(q, sq_t, sq_h) && wide_rows(k, sk_t, sk_h) && wide_rows(q_out, so_t, so_h) &&
+                    wide_rows(k_out, sp_t, sp_h) && wide_rows(v, sv_t, sv_h) && aligned(q_weight, 16) &&
+                    aligned(k_weight, 16) && (!p.cos_sin || (aligned(cos_sin, 16) && s_cs % 8 == 0));
+  const int lanes = head_size <= 64 ? 8 : head_size <= 128 ? 16 : 32;
+  // four heads at a time where there are enough to fill the SMs with them (a few thousand groups)
+  const int per_group = wide && p.total / 4 * lanes >= 1u << 17 ? 4 : 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.total + kRopeWarps - 1) / kRopeWarps);
+  if (wide) {
+    const auto groups = [&](int heads) { return (heads + per_group - 1) / per_group; };
+    p.groups[0] = groups(num_heads), p.groups[1] = groups(num_kv_heads);
+    p.rows = p.groups[0] + p.groups[1] * (cache ? 2 : 1);
+    p.total = static_cast<uint32_t>(p.rows) * static_cast<uint32_t>(tokens);
+  }
+  const uint32_t per_cta = wide ? kRopeWarps * 32 / lanes : kRopeWarps;
+  cfg.gridDim = dim3((p.total + per_cta - 1) / per_cta);
   cfg.blockDim = dim3(kRopeWarps * 32);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
@@ -195,6 +370,16 @@ extern "C" int qf_qk_norm_rope(const void* q, int64_t sq_t, int64_t sq_h, const 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = (flags & QF_FLAG_PDL) ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, rope_any_kernel, p);
+  cudaError_t e;
+  if (!wide)
+    e = cudaLaunchKernelEx(&cfg, rope_any_kernel, p);
+  else if (per_group == 4)
+    e = lanes == 8    ? cudaLaunchKernelEx(&cfg, rope_wide_kernel<8, 4>, p)
+        : lanes == 16 ? cudaLaunchKernelEx(&cfg, rope_wide_kernel<16, 4>, p)
+                      : cudaLaunchKernelEx(&cfg, rope_wide_kernel<32, 4>, p);
+  else
+    e = lanes == 8    ? cudaLaunchKernelEx(&cfg, rope_wide_kernel<8, 1>, p)
+        : lanes == 16 ? cudaLaunchKernelEx(&cfg, rope_wide_kernel<16, 1>, p)
+                      : cudaLaunchKernelEx(&cfg, rope_wide_kernel<32, 1>, p);
   return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
 }

@@ -185,6 +185,9 @@ qf_kv4_cache check_cache(const char* op, const CacheArgs& c, const at::Device& d
     QF_REFUSE_UNLESS(stride_of(c.k, i) % 16 == 0 && stride_of(c.k_scale, i) % (2 * G) == 0, op,
                      ": a cache's strides must be multiples of 16 bytes, its scales' of ", 2 * G, " elements");
   }
+  for (int i : {0, 2})
+    QF_REFUSE_UNLESS(stride_of(c.k, i) <= UINT32_MAX && stride_of(c.k_scale, i) <= UINT32_MAX / 2, op,
+                     ": a cache's pages and slots must lie less than 2^32 bytes apart");
   for (const auto& [name, t] : all) {
     const bool scale = t->dim() == 5;
     QF_REFUSE_UNLESS(t->numel() == 0 || (scale ? t->stride(4) == 1 && (G == 1 || t->stride(3) == 2) : t->stride(3) == 1), op,
@@ -297,9 +300,6 @@ qf_kv4_cache check_attention(const char* op, const at::Tensor& query, const Cach
   QF_REFUSE_UNLESS(tiles <= INT32_MAX && seq_lens.size(0) * cache.num_heads <= INT32_MAX / tiles, op, ": ",
                    seq_lens.size(0), " requests of up to ", block_table.size(1) * cache.page_size, " keys in ",
                    cache.num_heads, " heads are too many for one call");
-  for (int i : {0, 2})
-    QF_REFUSE_UNLESS(stride_of(c.k, i) <= UINT32_MAX && stride_of(c.k_scale, i) <= UINT32_MAX / 2, op,
-                     ": a cache's pages and slots must lie less than 2^32 bytes apart");
   return cache;
 }
 
