@@ -116,6 +116,20 @@ inline bool same_elements(const at::Tensor& a, const at::Tensor& b) {
   return true;
 }
 
+// The bytes from a tensor's first element to the end of its last: where two tensors' do not meet, neither do they.
+struct Extent {
+  uintptr_t begin, end;
+};
+inline Extent extent_of(const at::Tensor& t) {
+  if (t.numel() == 0) return {0, 0};
+  int64_t last = 0;
+  const auto sizes = t.sizes(), strides = t.strides();
+  for (size_t i = 0; i < sizes.size(); ++i) last += (sizes[i] - 1) * strides[i];
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(t.data_ptr());
+  return {begin, begin + (last + 1) * t.element_size()};
+}
+inline bool meet(const Extent& a, const Extent& b) { return a.begin < b.end && b.begin < a.end; }
+
 // "single memory location" is what torch's own operators say of such a call.
 inline void check_no_overlap(const char* op, const char* out_name, const at::Tensor& out, const char* name, const at::Tensor& t) {
   QF_REFUSE_UNLESS(!overlap(out, t), op, ": ", out_name, " shares memory with ", name,

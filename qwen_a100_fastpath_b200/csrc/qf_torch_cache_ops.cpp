@@ -5,7 +5,6 @@
 // As the operators of qf_torch_ops.cpp: what they make, the attention's partial sums among it, comes from the caching
 // allocator, so that calls on several streams, and captured graphs, share nothing.  A call that cannot be taken raises a
 // ValueError before anything is launched, tensors that require a gradient or carry a tangent too.
-#include <algorithm>
 #include <array>
 #include <tuple>
 #include <vector>
@@ -25,6 +24,7 @@ void check_dims(const char* op, const char* name, const at::Tensor& t, at::Scala
 
 struct CacheArgs {
   const at::Tensor &k, &v, &k_scale, &v_scale;
+  const at::Tensor& operator[](int i) const { return i == 0 ? k : i == 1 ? v : i == 2 ? k_scale : v_scale; }
   c10::SymInt heads() const { return k.sym_size(1); }
   c10::SymInt head_size() const { return k.sym_size(3) * 2; }
 };
@@ -148,18 +148,21 @@ int64_t stride_of(const at::Tensor& t, int i) { return t.size(i) > 1 ? t.stride(
 
 bool at16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
-// No two elements of a tensor that is written at one place.
+// No two elements of a tensor that is written at one place (up to eight dimensions: taken from the smallest stride on, each
+// steps over what the ones before span).
 bool distinct(const at::Tensor& t) {
-  std::vector<std::pair<int64_t, int64_t>> d;
-  for (int i = 0; i < t.dim(); ++i)
-    if (t.size(i) > 1) d.emplace_back(t.stride(i), t.size(i));
-  std::sort(d.begin(), d.end());
+  const auto sizes = t.sizes(), strides = t.strides();
+  bool done[8] = {};
   int64_t extent = 1;
-  for (const auto& [stride, size] : d) {
-    if (stride < extent) return false;
-    extent += stride * (size - 1);
+  for (;;) {
+    int next = -1;
+    for (int i = 0; i < static_cast<int>(sizes.size()); ++i)
+      if (!done[i] && sizes[i] > 1 && (next < 0 || strides[i] < strides[next])) next = i;
+    if (next < 0) return true;
+    if (strides[next] < extent) return false;
+    extent += strides[next] * (sizes[next] - 1);
+    done[next] = true;
   }
-  return true;
 }
 
 // [tokens, heads, D] as the kernels read it (unit innermost stride; with `wide` 16-byte aligned heads), copied where it is not.
@@ -198,7 +201,9 @@ qf_kv4_cache check_cache(const char* op, const CacheArgs& c, const at::Device& d
   }
   if (written_to)
     for (size_t i = 0; i < all.size(); ++i)
-      for (size_t j = 0; j < i; ++j) check_no_overlap(op, all[i].first, *all[i].second, all[j].first, *all[j].second);
+      for (size_t j = 0; j < i; ++j)
+        if (meet(extent_of(*all[i].second), extent_of(*all[j].second)))
+          check_no_overlap(op, all[i].first, *all[i].second, all[j].first, *all[j].second);
   qf_kv4_cache r = {};
   r.k = c.k.data_ptr(), r.v = c.v.data_ptr();
   r.k_scale = c.k_scale.data_ptr(), r.v_scale = c.v_scale.data_ptr();
@@ -210,12 +215,19 @@ qf_kv4_cache check_cache(const char* op, const CacheArgs& c, const at::Device& d
   return r;
 }
 
-void check_cache_apart(const char* op, const CacheArgs& c, const char* name, const at::Tensor& t) {
-  check_no_overlap(op, "cache.k", c.k, name, t);
-  check_no_overlap(op, "cache.v", c.v, name, t);
-  check_no_overlap(op, "cache.k_scale", c.k_scale, name, t);
-  check_no_overlap(op, "cache.v_scale", c.v_scale, name, t);
-}
+// Nothing that a call reads lies in a cache that it writes, nor the other way round.
+struct CacheExtents {
+  const CacheArgs& c;
+  Extent e[4];
+  explicit CacheExtents(const CacheArgs& args) : c(args), e{extent_of(c.k), extent_of(c.v), extent_of(c.k_scale),
+                                                             extent_of(c.v_scale)} {}
+  void apart(const char* op, const char* name, const at::Tensor& t) const {
+    static const char* const names[] = {"cache.k", "cache.v", "cache.k_scale", "cache.v_scale"};
+    const Extent x = extent_of(t);
+    for (int i = 0; i < 4; ++i)
+      if (C10_UNLIKELY(meet(e[i], x))) check_no_overlap(op, names[i], c[i], name, t);
+  }
+};
 
 void cache_written(const CacheArgs& c) {
   for (const at::Tensor* t : {&c.k, &c.v, &c.k_scale, &c.v_scale}) written(*t);
@@ -237,9 +249,10 @@ void kv4_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots
   check_input(op, "slots", slots, k.device());
   const qf_kv4_cache cache = check_cache(op, c, k.device(), true);
   check_pieces(op, k.size(0), k.size(1), k.size(2));
-  check_cache_apart(op, c, "k", k);
-  check_cache_apart(op, c, "v", v);
-  check_cache_apart(op, c, "slots", slots);
+  const CacheExtents extents(c);
+  extents.apart(op, "k", k);
+  extents.apart(op, "v", v);
+  extents.apart(op, "slots", slots);
   if (k.size(0) == 0) return;
   c10::cuda::CUDAGuard guard(k.device());
   const at::Tensor k3 = as_heads(k, true), v3 = as_heads(v, true), s = slots.contiguous();
@@ -333,7 +346,7 @@ void kv4_attention_out(const at::Tensor& query, const at::Tensor& ck, const at::
                                         stride_of(out, 1) % 8 == 0 && distinct(out)),
                    op, ": out must have unit stride within a head, 16-byte aligned heads and no two elements at one place");
   check_no_overlap(op, "out", out, "query", query);
-  check_cache_apart(op, c, "out", out);
+  CacheExtents(c).apart(op, "out", out);
   check_no_overlap(op, "out", out, "seq_lens", seq_lens);
   check_no_overlap(op, "out", out, "block_table", block_table);
   c10::cuda::CUDAGuard guard(query.device());
@@ -416,12 +429,13 @@ at::Tensor qk_norm_rope_kv4(const at::Tensor& q, const at::Tensor& k, const OptT
   check_input(op, "v", v, q.device());
   check_input(op, "slots", slots, q.device());
   const qf_kv4_cache cache = check_cache(op, c, q.device(), true);
+  const CacheExtents extents(c);
   for (const auto& [name, t] : {std::make_pair("q", &q), std::make_pair("k", &k), std::make_pair("v", &v),
                                 std::make_pair("slots", &slots)})
-    check_cache_apart(op, c, name, *t);
+    extents.apart(op, name, *t);
   for (const auto& [name, t] : {std::make_pair("q_weight", &q_weight), std::make_pair("k_weight", &k_weight),
                                 std::make_pair("positions", &positions), std::make_pair("cos_sin", &cos_sin)})
-    if (given(*t)) check_cache_apart(op, c, name, **t);
+    if (given(*t)) extents.apart(op, name, **t);
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor q_out = empty_on(q, q.sizes(), at::kBFloat16);
   run_rope(r, q_out, nullptr, &v, &slots, &cache);
@@ -430,6 +444,14 @@ at::Tensor qk_norm_rope_kv4(const at::Tensor& q, const at::Tensor& k, const OptT
 }
 
 // ---- the maps of a step ----
+// `n` elements of a buffer as a tensor of their own.  (Results that share a buffer share none of its elements.)
+at::Tensor piece_of(const at::Tensor& buffer, int64_t offset, int64_t n) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), buffer.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 using Maps = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
 
 void check_maps(const char* op, const at::Tensor& query_lens, const at::Tensor& past_lens, const at::Tensor& block_table,
@@ -448,12 +470,15 @@ Maps run_maps(const at::Tensor& query_lens, const at::Tensor& past_lens, const a
   const int64_t B = query_lens.size(0);
   c10::cuda::CUDAGuard guard(query_lens.device());
   const at::Tensor q = query_lens.contiguous(), past = past_lens.contiguous();
-  at::Tensor start = empty_on(q, {B + 1}, at::kInt), seq = empty_on(q, {B}, at::kInt);
-  at::Tensor pos = empty_on(q, {num_tokens}, at::kLong), slots = empty_on(q, {num_tokens}, at::kLong);
+  // an allocation for each type (64 32-bit numbers are 256 bytes: every result is aligned as one of its own)
+  const int64_t row = (B + 1 + 63) / 64 * 64, col = (num_tokens + 31) / 32 * 32;
+  const at::Tensor ints = empty_on(q, {2 * row + 1}, at::kInt), longs = empty_on(q, {2 * col}, at::kLong);
+  at::Tensor start = piece_of(ints, 0, B + 1), seq = piece_of(ints, row, B);
+  at::Tensor pos = piece_of(longs, 0, num_tokens), slots = piece_of(longs, col, num_tokens);
   at::Tensor free;
   if (free_pages) {
     free = free_pages->contiguous();
-    *head_out = empty_on(q, {1}, at::kInt);
+    *head_out = piece_of(ints, 2 * row, 1);
   }
   check(qf_step_maps(q.data_ptr<int32_t>(), past.data_ptr<int32_t>(), static_cast<int>(B), table.data_ptr<int32_t>(),
                      B > 1 ? table.stride(0) : table.size(1), static_cast<int>(table.size(1)), static_cast<int>(page_size),
@@ -488,10 +513,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> step_maps
   QF_REFUSE_UNLESS((W <= 1 || block_table.stride(1) == 1) && (B <= 1 || block_table.stride(0) >= W), op,
                    ": a block_table that grows must have rows of adjacent entries that do not overlap");
   QF_REFUSE_UNLESS(free_pages.size(0) <= INT32_MAX, op, ": too many free pages");
-  check_no_overlap(op, "block_table", block_table, "query_lens", query_lens);
-  check_no_overlap(op, "block_table", block_table, "past_lens", past_lens);
-  check_no_overlap(op, "block_table", block_table, "free_pages", free_pages);
-  check_no_overlap(op, "block_table", block_table, "free_head", free_head);
+  const Extent table = extent_of(block_table);
+  for (const auto& [name, t] : {std::make_pair("query_lens", &query_lens), std::make_pair("past_lens", &past_lens),
+                                std::make_pair("free_pages", &free_pages), std::make_pair("free_head", &free_head)})
+    if (C10_UNLIKELY(meet(table, extent_of(*t)))) check_no_overlap(op, "block_table", block_table, name, *t);
   at::Tensor head;
   auto [start, seq, pos, slots] =
       run_maps(query_lens, past_lens, block_table, page_size, num_tokens, &free_pages, &free_head, &head);
