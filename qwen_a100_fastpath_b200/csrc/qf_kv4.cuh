@@ -14,6 +14,7 @@
 #include <cstdint>
 
 #include "../../include/qf_b200.h"
+#include "qf_ptx.cuh"
 
 namespace qf {
 
@@ -67,31 +68,57 @@ __device__ __forceinline__ void kv4_scale(float lo, float hi, float& s, float& c
   if (!(fabsf(lo) < kMax && fabsf(hi) < kMax)) s = c = __int_as_float(0x7fffffff);
 }
 
-// The nibbles of a group's values.  Quotients are below 128 (the step is at least 2^-13 of the largest magnitude, and c's
-// rounding moves them by less than a hundred), so that one by the reciprocal, two roundings, is at most 2^-16 off; only where
-// it comes within 2^-14 of a border between two nibbles, where that might decide, is it made by a division.
+// The nibbles of two of a group's values, without a division: n is the whole number next to (x - c) / s by the reciprocal,
+// at most one off and that only next to a border between two nibbles, and the exact remainder d - n s, d = x - c, tells on
+// which side of the border d lies.  On the border itself, and where the rounding of the quotient to fp32 would put it there
+// (within 2^-20 of it, half a step for quotients from 16 to 32), the even one is taken.  (Quotients are below 128: the step is
+// at least 2^-13 of the largest magnitude, and c's rounding moves them by less than a hundred.)  A step of zero or NaN gives 0.
 struct Kv4Coder {
-  float s, c, inv;
+  uint64_t c2, s2, inv2;  // -c, -s and 1 / s, twice each
+  float s, tol;
+  bool plain;
   __device__ __forceinline__ Kv4Coder(float step, float offset) {
-    s = step, c = offset;
-    // a step of zero, and steps so small that their reciprocal is no normal number, take the division
-    inv = s > 1e-37f ? __frcp_rn(s) : __int_as_float(0x7fffffff);
+    s = step, tol = step * 1.9073486328125e-06f;  // 2^-19
+    plain = step > 1e-30f;  // reciprocal, remainders and tolerance are normal numbers
+    const float inv = plain ? __frcp_rn(step) : 0.f;
+    c2 = pack_f32x2(-offset, -offset), s2 = pack_f32x2(-step, -step), inv2 = pack_f32x2(inv, inv);
   }
-  __device__ __forceinline__ uint32_t operator()(float x) const {
-    const float d = x - c, q = d * inv;
-    constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers, ties to even
-    float n = (q + kWhole) - kWhole;
-    if (!(fabsf(q - n) < 0.5f - 6.1035156e-5f)) n = s > 0.f ? rintf(__fdiv_rn(d, s)) : 16.f;
-    return static_cast<uint32_t>(__float_as_int(fminf(fmaxf(n, 16.f), 31.f) + kWhole)) & 15u;  // (31 - 16 = 15, 16 = 0)
+  __device__ __forceinline__ float settle(float n, float m, float r) const {
+    const float a = fmaf(2.f, fabsf(r), -s);  // > 0: nearer to the next whole number
+    if (a >= -tol && (a > tol || (__float_as_int(m) & 1))) n += r < 0.f ? -1.f : 1.f;
+    return n;
   }
+  __device__ __forceinline__ uint32_t bits(float n) const {
+    return static_cast<uint32_t>(__float_as_int(fminf(fmaxf(n, 16.f), 31.f) + kWhole)) & 15u;  // 16 -> 0, 31 -> 15
+  }
+  __device__ __forceinline__ uint32_t slow(float x, float offset) const {
+    return s > 0.f ? bits(rintf(__fdiv_rn(x - offset, s))) : 0u;
+  }
+  // lo's nibble in bits 0 to 3, hi's in bits 4 to 7
+  __device__ __forceinline__ uint32_t operator()(float lo, float hi) const {
+    if (!plain) {
+      const float offset = -unpack_f32x2(c2).x;
+      return slow(lo, offset) | slow(hi, offset) << 4;
+    }
+    const uint64_t one = pack_f32x2(1.f, 1.f);
+    uint64_t d = c2, m = pack_f32x2(kWhole, kWhole), n = pack_f32x2(-kWhole, -kWhole);
+    fma_f32x2(d, pack_f32x2(lo, hi), one);
+    fma_f32x2(m, d, inv2);
+    fma_f32x2(n, m, one);
+    uint64_t r = d;
+    fma_f32x2(r, n, s2);
+    const float2 nn = unpack_f32x2(n), mm = unpack_f32x2(m), rr = unpack_f32x2(r);
+    return bits(settle(nn.x, mm.x, rr.x)) + 16u * bits(settle(nn.y, mm.y, rr.y));
+  }
+  static constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers, ties to even
 };
 
 // The word of eight values' nibbles.
 __device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], float s, float c) {
   const Kv4Coder code(s, c);
-  uint32_t r = 0;
+  uint32_t r = code(x[6], x[7]);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) r |= code(x[j]) << (4 * j);
+  for (int j = 4; j >= 0; j -= 2) r = 256u * r + code(x[j], x[j + 1]);
   return r;
 }
 

@@ -39,6 +39,7 @@ struct RopeParams {
   int rows;        // of a token; kWide: groups of rows
   uint32_t total;  // of all tokens
   int groups[2];   // kWide: of the queries and of the keys
+  int chunk;       // kWide: heads of a group
   int cs_f32, interleaved;
 };
 
@@ -48,11 +49,12 @@ constexpr int kRopeWarps = 4;
 // whose pointers and strides are multiples of 16 bytes, with heads of up to 256 (a multiple of eight) and a rotated part that
 // is a multiple of 16 (of eight where interleaved).  8192 tokens of 24 + 4 heads of 256, 64 of them rotated: 99 us with kAny.
 
-// kWide: L lanes take a row, a lane eight consecutive values in one 16-byte load.  A group of L lanes takes ROWS heads of one
-// side of one token, so that the token's angles and the weight are loaded once for them and ROWS loads are under way.  The
+// kWide: L lanes take a row, a lane eight consecutive values in one 16-byte load.  A group of L lanes takes p.chunk heads of
+// one side of one token, ROWS at a time, so that the token's angles and the weight are loaded and multiplied once for them
+// and ROWS loads are under way.  The
 // other half of a turned pair is L's other lanes' (a shuffle of the raw bf16 words; its weight is loaded beside the lane's
-// own), or the neighbour in the lane's own registers where interleaved.
-template <int L, int ROWS>
+// own), or the neighbour in the lane's own registers where interleaved (INTER).
+template <int L, int ROWS, bool INTER>
 __global__ void __launch_bounds__(kRopeWarps * 32) rope_wide_kernel(const RopeParams p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -64,55 +66,59 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_wide_kernel(const RopePa
   int part = at - token * p.rows, side = 0;
   if (part >= p.groups[0]) part -= p.groups[0], side = 1;
   if (side == 1 && part >= p.groups[1]) part -= p.groups[1], side = 2;
-  const int heads = side == 0 ? p.heads[0] : p.heads[1], head0 = part * ROWS;
+  const int all = side == 0 ? p.heads[0] : p.heads[1], chunk0 = part * p.chunk;
   const int e = 8 * lane;
   const bool in = e < p.D;
-  const __nv_bfloat16* x = p.x[side] + static_cast<int64_t>(token) * p.xt[side] + head0 * p.xh[side] + e;
+  const int heads = min(all, chunk0 + p.chunk);
+  const __nv_bfloat16* const x = p.x[side] + static_cast<int64_t>(token) * p.xt[side] + e;
+  const int64_t xh = p.xh[side];
   uint4 u[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     u[i] = make_uint4(0, 0, 0, 0);
-    if (in && head0 + i < heads) u[i] = *reinterpret_cast<const uint4*>(x + i * p.xh[side]);
+    if (in && chunk0 + i < heads) u[i] = *reinterpret_cast<const uint4*>(x + (chunk0 + i) * xh);
   }
   const bool normed = side < 2 && p.weight[side], turned = side < 2 && p.cos_sin && e < p.rot;
   const int half = p.rot / 2;
   const int swap = half / 8;  // lanes between the halves of a pair
-  const bool upper = !p.interleaved && e >= half;
+  const bool upper = !INTER && e >= half;
+  constexpr int kAngles = INTER ? 4 : 8;  // of a lane
   float cs[8], sn[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f;
   if (turned) {
     const int64_t pos = p.positions[token];
-    const int n = p.interleaved ? 4 : 8, i0 = p.interleaved ? e / 2 : upper ? e - half : e;
     if (pos >= 0 && pos < p.max_pos) {
-      const int64_t row = pos * p.cs_row + i0;
-      if (p.cs_f32) {
-        const float* t = static_cast<const float*>(p.cos_sin) + row;
-        for (int k = 0; k < n; k += 4) {
-          const float4 a = *reinterpret_cast<const float4*>(t + k), b = *reinterpret_cast<const float4*>(t + half + k);
-          cs[k] = a.x, cs[k + 1] = a.y, cs[k + 2] = a.z, cs[k + 3] = a.w;
-          sn[k] = b.x, sn[k + 1] = b.y, sn[k + 2] = b.z, sn[k + 3] = b.w;
+      const int64_t row = pos * p.cs_row + (INTER ? e / 2 : upper ? e - half : e);
+#pragma unroll
+      for (int k = 0; k < kAngles; k += 4) {
+        float4 a, b;
+        if (p.cs_f32) {
+          const float* t = static_cast<const float*>(p.cos_sin) + row + k;
+          a = *reinterpret_cast<const float4*>(t), b = *reinterpret_cast<const float4*>(t + half);
+        } else {
+          const __nv_bfloat16* t = static_cast<const __nv_bfloat16*>(p.cos_sin) + row + k;
+          const uint2 c = *reinterpret_cast<const uint2*>(t), d = *reinterpret_cast<const uint2*>(t + half);
+          a = make_float4(bf16_lo(c.x), bf16_hi(c.x), bf16_lo(c.y), bf16_hi(c.y));
+          b = make_float4(bf16_lo(d.x), bf16_hi(d.x), bf16_lo(d.y), bf16_hi(d.y));
         }
-      } else {
-        const __nv_bfloat16* t = static_cast<const __nv_bfloat16*>(p.cos_sin) + row;
-        for (int k = 0; k < n; k += 4) {
-          const uint2 a = *reinterpret_cast<const uint2*>(t + k), b = *reinterpret_cast<const uint2*>(t + half + k);
-          cs[k] = bf16_lo(a.x), cs[k + 1] = bf16_hi(a.x), cs[k + 2] = bf16_lo(a.y), cs[k + 3] = bf16_hi(a.y);
-          sn[k] = bf16_lo(b.x), sn[k + 1] = bf16_hi(b.x), sn[k + 2] = bf16_lo(b.y), sn[k + 3] = bf16_hi(b.y);
-        }
+        cs[k] = a.x, cs[k + 1] = a.y, cs[k + 2] = a.z, cs[k + 3] = a.w;
+        sn[k] = b.x, sn[k + 1] = b.y, sn[k + 2] = b.z, sn[k + 3] = b.w;
       }
     } else {
+#pragma unroll
       for (int k = 0; k < 8; ++k) cs[k] = sn[k] = __int_as_float(0x7fffffff);
     }
-    if (p.interleaved)
+    if (INTER) {
 #pragma unroll
       for (int k = 3; k >= 0; --k) cs[2 * k] = cs[2 * k + 1] = cs[k], sn[2 * k] = -sn[k], sn[2 * k + 1] = -sn[2 * k];
-    else if (!upper)
+    } else if (!upper) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) sn[k] = -sn[k];
+    }
   }
   // y = n (x w cos + x' w' sin), x' the other of the pair, the sign of the sine taken in above: two coefficients an element
-  const int other = turned && !p.interleaved ? (upper ? lane - swap : lane + swap) : lane;
+  const int other = turned && !INTER ? (upper ? lane - swap : lane + swap) : lane;
   uint64_t ca[4], cb[4];
   {
     float w[8], w2[8];
@@ -126,7 +132,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_wide_kernel(const RopePa
       for (int k = 0; k < 4; ++k) {
         w[2 * k] = bf16_lo(wa[k]) + p.offset, w[2 * k + 1] = bf16_hi(wa[k]) + p.offset;
         w2[2 * k] = bf16_lo(wb[k]) + p.offset, w2[2 * k + 1] = bf16_hi(wb[k]) + p.offset;
-        if (p.interleaved) {
+        if (INTER) {
           const float t = w2[2 * k];
           w2[2 * k] = w2[2 * k + 1], w2[2 * k + 1] = t;
         }
@@ -141,64 +147,71 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_wide_kernel(const RopePa
   uint32_t page = 0, off = 0;
   const bool cached = side > 0 && !p.out[1] && p.cache.place(p.slots[token], page, off);
   const uint32_t keep = turned ? ~0u : 0u;  // values that do not turn have no other (an infinity times zero would be NaN)
+  __nv_bfloat16* const out = side < 2 && p.out[side] ? p.out[side] + static_cast<int64_t>(token) * p.ot[side] + e : nullptr;
+  const int64_t oh = side < 2 ? p.oh[side] : 0;
+  const bool sums_needed = p.weight[0] || p.weight[1], to_cache = !p.out[1], stores = in && item < p.total;
+  // (the same number of turns for all lanes of a warp: its groups may be of different sides)
+  for (int turn = 0; turn < p.chunk; turn += ROWS) {
+    const int head0 = chunk0 + turn;
+    if (turn > 0)
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const uint32_t raw[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-    uint64_t v2[4], sums = pack_f32x2(0.f, 0.f);
-    uint32_t r[4];
+      for (int i = 0; i < ROWS; ++i)
+        if (in && head0 + i < heads) u[i] = *reinterpret_cast<const uint4*>(x + (head0 + i) * xh);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint64_t a = pack_f32x2(bf16_lo(raw[k]), bf16_hi(raw[k]));
-      fma_f32x2(sums, a, a);
-      // the other half of a turned pair: another lane's words, or this one's with its halves exchanged
-      const uint32_t x2 = keep & (p.interleaved ? __byte_perm(raw[k], raw[k], 0x1032)
-                                                : __shfl_sync(0xffffffffu, raw[k], other, L));
-      v2[k] = mul_f32x2(pack_f32x2(bf16_lo(x2), bf16_hi(x2)), cb[k]);
-      fma_f32x2(v2[k], a, ca[k]);
+    for (int i = 0; i < ROWS; ++i) {
+      const uint32_t raw[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+      uint64_t v2[4], sums = pack_f32x2(0.f, 0.f);
+      uint32_t r[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint64_t a = pack_f32x2(bf16_lo(raw[k]), bf16_hi(raw[k]));
+        fma_f32x2(sums, a, a);
+        // the other half of a turned pair: another lane's words, or this one's with its halves exchanged
+        const uint32_t x2 = keep & (INTER ? __byte_perm(raw[k], raw[k], 0x1032)
+                                          : __shfl_sync(0xffffffffu, raw[k], other, L));
+        v2[k] = mul_f32x2(pack_f32x2(bf16_lo(x2), bf16_hi(x2)), cb[k]);
+        fma_f32x2(v2[k], a, ca[k]);
+      }
+      const float2 both = unpack_f32x2(sums);
+      float n = 1.f;
+      if (sums_needed) {
+        float sum = both.x + both.y;
+#pragma unroll
+        for (int d = L / 2; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (normed) n = rsqrtf(fmaf(sum, p.inv_d, p.eps));
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 y = unpack_f32x2(mul_f32x2(v2[k], pack_f32x2(n, n)));
+        const __nv_bfloat162 h = __floats2bfloat162_rn(y.x, y.y);
+        r[k] = reinterpret_cast<const uint32_t&>(h);
+      }
+      const bool store = stores && head0 + i < heads;
+      if (out && store) *reinterpret_cast<uint4*>(out + (head0 + i) * oh) = make_uint4(r[0], r[1], r[2], r[3]);
+      if (!to_cache) continue;
+      // into the cache, from the rounded values (all lanes go along: a warp may hold groups of queries too)
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[2 * k] = bf16_lo(r[k]), v[2 * k + 1] = bf16_hi(r[k]);
+      float hi = v[0], lo = -v[0];
+#pragma unroll
+      for (int k = 1; k < 8; ++k) hi = max_nan(hi, v[k]), lo = max_nan(lo, -v[k]);
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) {
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+        lo = max_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+      }
+      if (!cached || !store) continue;
+      float s, c;
+      kv4_scale(-lo, hi, s, c);
+      const Kv4View& view = p.cache;
+      const int kv = side - 1, head = head0 + i;
+      *reinterpret_cast<uint32_t*>(view.codes[kv] + head * view.head + view.codes_at(page, off) + e / 2) =
+          kv4_codes(v, s, c);
+      if (lane % 8 == 0)
+        reinterpret_cast<__nv_bfloat162*>(view.scale[kv] + head * view.shead + view.scale_at(page, off))[lane / 8] =
+            __floats2bfloat162_rn(s, c);
     }
-    const float2 both = unpack_f32x2(sums);
-    float n = 1.f;
-    if (p.weight[0] || p.weight[1]) {
-      float sum = both.x + both.y;
-#pragma unroll
-      for (int d = L / 2; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (normed) n = rsqrtf(fmaf(sum, p.inv_d, p.eps));
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 y = unpack_f32x2(mul_f32x2(v2[k], pack_f32x2(n, n)));
-      const __nv_bfloat162 h = __floats2bfloat162_rn(y.x, y.y);
-      r[k] = reinterpret_cast<const uint32_t&>(h);
-    }
-    const bool store = in && item < p.total && head0 + i < heads;
-    if (side < 2 && p.out[side]) {
-      if (store)
-        *reinterpret_cast<uint4*>(p.out[side] + static_cast<int64_t>(token) * p.ot[side] + (head0 + i) * p.oh[side] + e) =
-            make_uint4(r[0], r[1], r[2], r[3]);
-    }
-    if (p.out[1]) continue;
-    // into the cache, from the rounded values (all lanes go along: a warp may hold groups of queries too)
-    float v[8];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[2 * k] = bf16_lo(r[k]), v[2 * k + 1] = bf16_hi(r[k]);
-    float hi = v[0], lo = -v[0];
-#pragma unroll
-    for (int k = 1; k < 8; ++k) hi = max_nan(hi, v[k]), lo = max_nan(lo, -v[k]);
-#pragma unroll
-    for (int d = 1; d < 8; d <<= 1) {
-      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-      lo = max_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-    }
-    if (!cached || !store) continue;
-    float s, c;
-    kv4_scale(-lo, hi, s, c);
-    const Kv4View& view = p.cache;
-    const int kv = side - 1, head = head0 + i;
-    *reinterpret_cast<uint32_t*>(view.codes[kv] + head * view.head + view.codes_at(page, off) + e / 2) =
-        kv4_codes(v, s, c);
-    if (lane % 8 == 0)
-      reinterpret_cast<__nv_bfloat162*>(view.scale[kv] + head * view.shead + view.scale_at(page, off))[lane / 8] =
-          __floats2bfloat162_rn(s, c);
   }
 }
 
@@ -272,10 +285,19 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_any_kernel(const RopePar
     }
     float s, c;
     kv4_scale(-lo, hi, s, c);
-    const Kv4Coder code(s, c);
-    codes[g * (kKv4Group / 2) + lane] = static_cast<uint8_t>(code(a) | code(b) << 4);
+    codes[g * (kKv4Group / 2) + lane] = static_cast<uint8_t>(Kv4Coder(s, c)(a, b));
     if (lane == 0) reinterpret_cast<__nv_bfloat162*>(scale)[g] = __floats2bfloat162_rn(s, c);
   }
+}
+
+template <bool INTER> cudaError_t launch_wide(const cudaLaunchConfig_t& cfg, const RopeParams& p, int lanes, bool many) {
+  if (many)
+    return lanes == 8    ? cudaLaunchKernelEx(&cfg, rope_wide_kernel<8, 4, INTER>, p)
+           : lanes == 16 ? cudaLaunchKernelEx(&cfg, rope_wide_kernel<16, 4, INTER>, p)
+                         : cudaLaunchKernelEx(&cfg, rope_wide_kernel<32, 4, INTER>, p);
+  return lanes == 8    ? cudaLaunchKernelEx(&cfg, rope_wide_kernel<8, 1, INTER>, p)
+         : lanes == 16 ? cudaLaunchKernelEx(&cfg, rope_wide_kernel<16, 1, INTER>, p)
+                       : cudaLaunchKernelEx(&cfg, rope_wide_kernel<32, 1, INTER>, p);
 }
 
 bool aligned(const void* ptr, size_t n) { return reinterpret_cast<uintptr_t>(ptr) % n == 0; }
@@ -352,11 +374,12 @@ extern "C" int qf_qk_norm_rope(const void* q, int64_t sq_t, int64_t sq_h, const 
                     wide_rows(k_out, sp_t, sp_h) && wide_rows(v, sv_t, sv_h) && aligned(q_weight, 16) &&
                     aligned(k_weight, 16) && (!p.cos_sin || (aligned(cos_sin, 16) && s_cs % 8 == 0));
   const int lanes = head_size <= 64 ? 8 : head_size <= 128 ? 16 : 32;
-  // four heads at a time where there are enough to fill the SMs with them (a few thousand groups)
-  const int per_group = wide && p.total / 4 * lanes >= 1u << 17 ? 4 : 1;
+  // eight heads to a group, four at a time, where that leaves groups enough for the SMs
+  const bool many = wide && p.total / 8 * lanes >= 1u << 17;
+  p.chunk = many ? 8 : 1;
   cudaLaunchConfig_t cfg = {};
   if (wide) {
-    const auto groups = [&](int heads) { return (heads + per_group - 1) / per_group; };
+    const auto groups = [&](int heads) { return (heads + p.chunk - 1) / p.chunk; };
     p.groups[0] = groups(num_heads), p.groups[1] = groups(num_kv_heads);
     p.rows = p.groups[0] + p.groups[1] * (cache ? 2 : 1);
     p.total = static_cast<uint32_t>(p.rows) * static_cast<uint32_t>(tokens);
@@ -373,13 +396,9 @@ extern "C" int qf_qk_norm_rope(const void* q, int64_t sq_t, int64_t sq_h, const 
   cudaError_t e;
   if (!wide)
     e = cudaLaunchKernelEx(&cfg, rope_any_kernel, p);
-  else if (per_group == 4)
-    e = lanes == 8    ? cudaLaunchKernelEx(&cfg, rope_wide_kernel<8, 4>, p)
-        : lanes == 16 ? cudaLaunchKernelEx(&cfg, rope_wide_kernel<16, 4>, p)
-                      : cudaLaunchKernelEx(&cfg, rope_wide_kernel<32, 4>, p);
+  else if (interleaved)
+    e = launch_wide<true>(cfg, p, lanes, many);
   else
-    e = lanes == 8    ? cudaLaunchKernelEx(&cfg, rope_wide_kernel<8, 1>, p)
-        : lanes == 16 ? cudaLaunchKernelEx(&cfg, rope_wide_kernel<16, 1>, p)
-                      : cudaLaunchKernelEx(&cfg, rope_wide_kernel<32, 1>, p);
+    e = launch_wide<false>(cfg, p, lanes, many);
   return e == cudaSuccess ? QF_OK : fail(QF_ERR_LAUNCH, std::string("launch: ") + cudaGetErrorString(e));
 }
