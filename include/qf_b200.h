@@ -261,8 +261,9 @@ int qf_residual_norm_status(void* stream, int* status);
  * No counterpart in the reference, whose cache is bf16 (spec_attn.py).  Keys and values are kept in groups of QF_KV4_GROUP
  * consecutive dimensions of one head of one token: a nibble n per value (the even dimension in a byte's low half) and for
  * each group two bf16 numbers, the step s and the offset c:
- *   lo, hi = least and greatest value;  s = bf16((hi - lo) / 15);  c = bf16(lo - 16 s);
- *   n = clamp(rint((x - c) / s), 16, 31) - 16, 0 where s = 0 (fp32 operations, nearest even);  n stands for bf16((n + 16) s + c).
+ *   lo, hi = least and greatest value;  s = bf16((hi - lo) * (1 / 15));  c = bf16(lo - 16 s);
+ *   n = clamp(rint((x - c) / s), 16, 31) - 16, 0 where s = 0;  n stands for bf16((n + 16) s + c)
+ * (fp32 operations, 1 / 15 as an fp32 number, nearest even).
  * A group with a NaN, an infinity or a magnitude of 2^126 or more becomes NaN.  k, v: uint8, element (page, head, slot) at
  * page * page_stride + head * head_stride + slot * slot_stride bytes, head_size / 2 bytes each; k_scale, v_scale: bf16
  * [head_size / 64][2] at the scale strides (elements).  head_size 64, 128 or 256; any page size; pointers and strides of the

@@ -27,7 +27,7 @@ def quantize(x: np.ndarray):
     g = np.asarray(x, np.float32).reshape(*x.shape[:-1], x.shape[-1] // GROUP, GROUP)
     with np.errstate(all="ignore"):
         lo, hi = g.min(-1), g.max(-1)
-        s = round_bf16(((hi - lo) / np.float32(15)).astype(np.float32)).astype(np.float32)
+        s = round_bf16(((hi - lo) * (np.float32(1) / np.float32(15))).astype(np.float32)).astype(np.float32)
         c = round_bf16((lo - np.float32(16) * s).astype(np.float32)).astype(np.float32)
         bad = ~((np.abs(lo) < 2.0 ** 126) & (np.abs(hi) < 2.0 ** 126))
         q = np.rint(((g - c[..., None]).astype(np.float32) / s[..., None]).astype(np.float32))

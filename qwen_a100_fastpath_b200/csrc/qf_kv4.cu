@@ -67,7 +67,7 @@ constexpr int kIoTokens = 4;
 
 // A CTA takes passes * per_pass tokens, a thread the same piece of `passes` of them: which piece that is, and of which head,
 // is found out once, and the passes' loads are under way together.  Eight threads in a row share a group and a warp.
-template <int D, bool WRITE> __global__ void __launch_bounds__(kIoThreads) kv4_io_kernel(const Kv4IoParams p) {
+template <int D, bool WRITE> __global__ void __launch_bounds__(kIoThreads, 4) kv4_io_kernel(const Kv4IoParams p) {
   constexpr int kPieces = D / 8;
   pdl_launch_dependents();
   pdl_wait();
@@ -104,16 +104,9 @@ template <int D, bool WRITE> __global__ void __launch_bounds__(kIoThreads) kv4_i
         float f[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[2 * j] = bf16_lo(w[j]), f[2 * j + 1] = bf16_hi(w[j]);
-        float hi = f[0], lo = -f[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) hi = max_nan(hi, f[j]), lo = max_nan(lo, -f[j]);
-#pragma unroll
-        for (int d = 1; d < 8; d <<= 1) {
-          hi = max_nan(hi, __shfl_xor_sync(group, hi, d));
-          lo = max_nan(lo, __shfl_xor_sync(group, lo, d));
-        }
+        const uint32_t ends = kv4_extremes(w[0], w[1], w[2], w[3], group);
         float s, c;
-        kv4_scale(-lo, hi, s, c);
+        kv4_scale(-bf16_hi(ends), bf16_lo(ends), s, c);
         *reinterpret_cast<uint32_t*>(codes + v.codes_at(page[i], off[i])) = kv4_codes(f, s, c);
         if (piece % 8 == 0)
           *reinterpret_cast<__nv_bfloat162*>(scale + v.scale_at(page[i], off[i])) = __floats2bfloat162_rn(s, c);

@@ -1,8 +1,8 @@
 // qf_kv4.cuh -- the 4-bit cache format shared by the kernels that write, read and attend it.
 //
 // A group is 64 consecutive dimensions of one head of one token.  With lo and hi its least and greatest value,
-//   s = bf16((hi - lo) / 15),   c = bf16(lo - 16 s),   n = clamp(rint((x - c) / s), 16, 31) - 16  (0 where s = 0)
-// (fp32 operations, round to nearest even) and the nibble n stands for bf16((n + 16) s + c).  The 16 in front is what makes
+//   s = bf16((hi - lo) * (1 / 15)),   c = bf16(lo - 16 s),   n = clamp(rint((x - c) / s), 16, 31) - 16  (0 where s = 0)
+// (fp32 operations, 1 / 15 as an fp32 number, round to nearest even) and the nibble n stands for bf16((n + 16) s + c).  The 16 in front is what makes
 // it cheap to take apart: a nibble put into the four upper mantissa bits of the bf16 number 16 is the bf16 number n + 16, so
 // that two values cost a shift, one logical operation and one packed multiply-add.  (s, c) and not (s, lo): c carries
 // that 16, at the price of c's own rounding, 2^-8 |lo - 16 s|, at most s / 16 + 2^-8 |lo| beside the s / 2 of the nibble.
@@ -61,64 +61,81 @@ inline void kv4_divisor(int d, uint32_t* mul, uint32_t* shift) {
 
 // Step and offset of a group from its least and greatest value (any NaN among them makes both NaN).
 __device__ __forceinline__ void kv4_scale(float lo, float hi, float& s, float& c) {
-  const float s32 = __fdiv_rn(hi - lo, 15.f);
-  s = __bfloat162float(__float2bfloat16_rn(s32));
+  s = __bfloat162float(__float2bfloat16_rn((hi - lo) * (1.f / 15.f)));
   c = __bfloat162float(__float2bfloat16_rn(fmaf(-16.f, s, lo)));
   constexpr float kMax = 8.507059173023462e37f;  // 2^126
   if (!(fabsf(lo) < kMax && fabsf(hi) < kMax)) s = c = __int_as_float(0x7fffffff);
 }
 
-// The nibbles of two of a group's values, without a division: n is the whole number next to (x - c) / s by the reciprocal,
-// at most one off and that only next to a border between two nibbles, and the exact remainder d - n s, d = x - c, tells on
-// which side of the border d lies.  On the border itself, and where the rounding of the quotient to fp32 would put it there
-// (within 2^-20 of it, half a step for quotients from 16 to 32), the even one is taken.  (Quotients are below 128: the step is
-// at least 2^-13 of the largest magnitude, and c's rounding moves them by less than a hundred.)  A step of zero or NaN gives 0.
+// The nibbles of a group's values.  The quotient (x - c) / s is the correctly rounded fp32 one of the definition, by
+// Markstein's theorem (IBM J. Res. Dev. 34, 1990): with y the correctly rounded 1 / s and q = d y, the sum q + (d - q s) y in
+// two fused operations rounds to d / s.  On packed pairs that is 1.5 instructions a value (a call of the division some ten).
+// It needs a step whose remainders are normal numbers; smaller ones (and zero and NaN, which give 0) take the division.
 struct Kv4Coder {
-  uint64_t c2, s2, inv2;  // -c, -s and 1 / s, twice each
-  float s, tol;
+  float s, c, inv;
   bool plain;
   __device__ __forceinline__ Kv4Coder(float step, float offset) {
-    s = step, tol = step * 1.9073486328125e-06f;  // 2^-19
-    plain = step > 1e-30f;  // reciprocal, remainders and tolerance are normal numbers
-    const float inv = plain ? __frcp_rn(step) : 0.f;
-    c2 = pack_f32x2(-offset, -offset), s2 = pack_f32x2(-step, -step), inv2 = pack_f32x2(inv, inv);
+    s = step, c = offset;
+    plain = step > 1e-25f;
+    inv = plain ? __frcp_rn(step) : 0.f;
   }
-  __device__ __forceinline__ float settle(float n, float m, float r) const {
-    const float a = fmaf(2.f, fabsf(r), -s);  // > 0: nearer to the next whole number
-    if (a >= -tol && (a > tol || (__float_as_int(m) & 1))) n += r < 0.f ? -1.f : 1.f;
-    return n;
+  // Bits of 1.5 * 2^23 + the whole number next to the quotient (the sum rounds to whole numbers, ties to even), from 16 to 31.
+  static constexpr float kWhole = 12582912.f;
+  static constexpr int kBits = 0x4b400000;
+  __device__ __forceinline__ static uint32_t clamp(float m) {
+    return static_cast<uint32_t>(min(max(__float_as_int(m), kBits + 16), kBits + 31));
   }
-  __device__ __forceinline__ uint32_t bits(float n) const {
-    return static_cast<uint32_t>(__float_as_int(fminf(fmaxf(n, 16.f), 31.f) + kWhole)) & 15u;  // 16 -> 0, 31 -> 15
+  __device__ __forceinline__ uint32_t slow(float x) const {
+    return clamp(s > 0.f ? rintf(__fdiv_rn(x - c, s)) + kWhole : kWhole);
   }
-  __device__ __forceinline__ uint32_t slow(float x, float offset) const {
-    return s > 0.f ? bits(rintf(__fdiv_rn(x - offset, s))) : 0u;
+  __device__ __forceinline__ void pair(float x0, float x1, uint32_t& n0, uint32_t& n1) const {
+    const uint64_t one = pack_f32x2(1.f, 1.f), y = pack_f32x2(inv, inv);
+    uint64_t d = pack_f32x2(-c, -c), m = pack_f32x2(kWhole, kWhole);
+    fma_f32x2(d, pack_f32x2(x0, x1), one);
+    uint64_t q = mul_f32x2(d, y), r = d;
+    fma_f32x2(r, q, pack_f32x2(-s, -s));
+    fma_f32x2(q, r, y);
+    fma_f32x2(m, q, one);
+    const float2 mm = unpack_f32x2(m);
+    n0 = clamp(mm.x), n1 = clamp(mm.y);
   }
-  // lo's nibble in bits 0 to 3, hi's in bits 4 to 7
-  __device__ __forceinline__ uint32_t operator()(float lo, float hi) const {
-    if (!plain) {
-      const float offset = -unpack_f32x2(c2).x;
-      return slow(lo, offset) | slow(hi, offset) << 4;
-    }
-    const uint64_t one = pack_f32x2(1.f, 1.f);
-    uint64_t d = c2, m = pack_f32x2(kWhole, kWhole), n = pack_f32x2(-kWhole, -kWhole);
-    fma_f32x2(d, pack_f32x2(lo, hi), one);
-    fma_f32x2(m, d, inv2);
-    fma_f32x2(n, m, one);
-    uint64_t r = d;
-    fma_f32x2(r, n, s2);
-    const float2 nn = unpack_f32x2(n), mm = unpack_f32x2(m), rr = unpack_f32x2(r);
-    return bits(settle(nn.x, mm.x, rr.x)) + 16u * bits(settle(nn.y, mm.y, rr.y));
-  }
-  static constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers, ties to even
 };
 
 // The word of eight values' nibbles.
 __device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], float s, float c) {
   const Kv4Coder code(s, c);
-  uint32_t r = code(x[6], x[7]);
+  uint32_t n[8];
+  if (__builtin_expect(code.plain, 1)) {
 #pragma unroll
-  for (int j = 4; j >= 0; j -= 2) r = 256u * r + code(x[j], x[j + 1]);
+    for (int j = 0; j < 8; j += 2) code.pair(x[j], x[j + 1], n[j], n[j + 1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) n[j] = code.slow(x[j]);
+  }
+  uint32_t r = n[7];
+#pragma unroll
+  for (int j = 6; j >= 0; --j) r = 16u * r + n[j];
+  // (each term has kBits + 16 more than its nibble; sums of 32-bit numbers lose nothing that a difference wants back)
+  return r - 0x11111111u * static_cast<uint32_t>(Kv4Coder::kBits + 16);
+}
+
+// The greatest value, and the greatest of the negated ones, of eight bf16 values in four words and of the seven neighbouring
+// threads' (the lanes of `mask`, which differ in the lowest three bits): the low and the high half of one word, NaN if any is.
+__device__ __forceinline__ uint32_t kv4_extremes(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t mask) {
+  auto max2 = [](uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  };
+  auto min2 = [](uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  };
+  const uint32_t hi = max2(max2(w0, w1), max2(w2, w3)), lo = min2(min2(w0, w1), min2(w2, w3)) ^ 0x80008000u;
+  uint32_t r = max2(__byte_perm(hi, lo, 0x5410), __byte_perm(hi, lo, 0x7632));
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) r = max2(r, __shfl_xor_sync(mask, r, d));
   return r;
 }
 

@@ -55,7 +55,7 @@ constexpr int kRopeWarps = 4;
 // other half of a turned pair is L's other lanes' (a shuffle of the raw bf16 words; its weight is loaded beside the lane's
 // own), or the neighbour in the lane's own registers where interleaved (INTER).
 template <int L, int ROWS, bool INTER>
-__global__ void __launch_bounds__(kRopeWarps * 32) rope_wide_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRopeWarps * 32, ROWS == 1 ? 1 : 8) rope_wide_kernel(const RopeParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x % L;
@@ -193,17 +193,10 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_wide_kernel(const RopePa
       float v[8];
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[2 * k] = bf16_lo(r[k]), v[2 * k + 1] = bf16_hi(r[k]);
-      float hi = v[0], lo = -v[0];
-#pragma unroll
-      for (int k = 1; k < 8; ++k) hi = max_nan(hi, v[k]), lo = max_nan(lo, -v[k]);
-#pragma unroll
-      for (int d = 1; d < 8; d <<= 1) {
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-        lo = max_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-      }
+      const uint32_t ends = kv4_extremes(r[0], r[1], r[2], r[3], 0xffffffffu);
       if (!cached || !store) continue;
       float s, c;
-      kv4_scale(-lo, hi, s, c);
+      kv4_scale(-bf16_hi(ends), bf16_lo(ends), s, c);
       const Kv4View& view = p.cache;
       const int kv = side - 1, head = head0 + i;
       *reinterpret_cast<uint32_t*>(view.codes[kv] + head * view.head + view.codes_at(page, off) + e / 2) =
@@ -285,7 +278,9 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_any_kernel(const RopePar
     }
     float s, c;
     kv4_scale(-lo, hi, s, c);
-    codes[g * (kKv4Group / 2) + lane] = static_cast<uint8_t>(Kv4Coder(s, c)(a, b));
+    const Kv4Coder code(s, c);
+    const uint32_t n0 = code.slow(a) & 15u, n1 = code.slow(b) & 15u;
+    codes[g * (kKv4Group / 2) + lane] = static_cast<uint8_t>(n0 | n1 << 4);
     if (lane == 0) reinterpret_cast<__nv_bfloat162*>(scale)[g] = __floats2bfloat162_rn(s, c);
   }
 }
@@ -353,7 +348,8 @@ extern "C" int qf_qk_norm_rope(const void* q, int64_t sq_t, int64_t sq_h, const 
   p.out[1] = static_cast<__nv_bfloat16*>(k_out), p.ot[1] = sp_t, p.oh[1] = sp_h;
   p.positions = positions;
   p.rot = rot;
-  p.cos_sin = rot ? cos_sin : nullptr;
+  // (a table of no positions is never read, but it still turns: every position is outside it)
+  p.cos_sin = !rot ? nullptr : max_positions ? cos_sin : static_cast<const void*>(positions);
   p.cs_row = s_cs;
   p.max_pos = max_positions;
   p.cs_f32 = cos_sin_dtype == QF_DTYPE_F32;

@@ -61,8 +61,8 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: KV4C
     """Quantizes ``k`` and ``v`` bf16 ``[tokens, heads, D]`` (any strides) into the slots ``slots`` int64 ``[tokens]``, slot
     ``page * page_size + offset``.  Tokens whose slot is negative (padding) or behind the cache are left out; the slots of a
     call must differ (one that is given twice holds parts of either token afterwards).  For each group of 64 values with
-    ``lo`` and ``hi`` the least and the greatest: ``s = bf16((hi - lo) / 15)``, ``c = bf16(lo - 16 s)``,
-    ``n = clamp(rint((x - c) / s), 16, 31) - 16`` (0 where ``s`` is 0); ``n`` stands for ``bf16((n + 16) s + c)``, which is
+    ``lo`` and ``hi`` the least and the greatest: ``s = bf16((hi - lo) * (1 / 15))``, ``c = bf16(lo - 16 s)``,
+    ``n = clamp(rint((x - c) / s), 16, 31) - 16`` (0 where ``s`` is 0), fp32 operations; ``n`` stands for ``bf16((n + 16) s + c)``, which is
     within ``s / 2 + s / 8 + |lo| / 256`` of ``x`` before its own rounding to bf16.  A group with a NaN, an infinity or a magnitude of
     2^126 or more becomes NaN."""
     try:

@@ -114,6 +114,41 @@ def test_attention_large_scores(dev):
     run_case(dev, 8, [700, 1500], 2, 6, 2, 128, 16, q_scale=30.0)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.07, 1e-30])
+def test_attention_scales(dev, scale):
+    """Of either sign, and zero: the mean of the values."""
+    from qwen_a100_fastpath_b200.kv4 import kv4_attention
+    gen = torch.Generator(device=dev).manual_seed(14)
+    lens = [300, 65, 2]
+    table, pages = table_for(gen, lens, 16)
+    cache = random_cache(gen, pages, 16, 2, 128)
+    query = torch.randn(9, 10, 128, device=dev, generator=gen).to(BF16)
+    out = kv4_attention(query, cache, torch.tensor(lens, dtype=torch.int32, device=dev), table, 3, scale)
+    check_attention(out, query, cache, lens, table, 3, scale)
+
+
+def test_attention_query_rows_are_apart(dev):
+    """A row of NaN, of infinities or of very large values leaves the other rows as they are."""
+    from qwen_a100_fastpath_b200.kv4 import kv4_attention
+    gen = torch.Generator(device=dev).manual_seed(15)
+    lens = [400, 90]
+    table, pages = table_for(gen, lens, 16)
+    cache = random_cache(gen, pages, 16, 2, 256)
+    query = torch.randn(4, 12, 256, device=dev, generator=gen).to(BF16)
+    seq = torch.tensor(lens, dtype=torch.int32, device=dev)
+    clean = kv4_attention(query, cache, seq, table, 2, 0.06)
+    query[0, 3], query[1, 7], query[2, 0, 5], query[3, 11] = float("nan"), float("inf"), 3e38, 1e30
+    out = kv4_attention(query, cache, seq, table, 2, 0.06)
+    other = torch.ones(4, 12, dtype=torch.bool, device=dev)
+    other[0, 3] = other[1, 7] = other[2, 0] = other[3, 11] = False
+    assert out[0, 3].isnan().all() and out[1, 7].isnan().all()
+    # another row may have the references raised at another tile: the weights' roundings (2^-8 of them, on both sides) and the
+    # result's may differ, no more
+    _, spread, _ = orc.attention(host(query.nan_to_num(0.0, 0.0, 0.0)), [host(t) for t in cache], lens, host(table), 2, 0.06)
+    bound = torch.from_numpy(2 * 2.0 ** -8 * spread).to(dev) + 2 * 2.0 ** -8 * clean.double().abs() + 2.0 ** -16
+    assert ((out.double() - clean.double()).abs() <= bound)[other].all()
+
+
 def test_attention_one_key_rows_are_its_values(dev):
     """With one key the weight is exactly 1."""
     from qwen_a100_fastpath_b200.kv4 import kv4_attention, kv4_read

@@ -113,8 +113,17 @@ def test_strides_and_edges(dev):
     assert not a[0].any() and a[3].isnan().all()
 
 
+def test_a_table_of_no_positions(dev):
+    """Every position is outside it."""
+    from qwen_a100_fastpath_b200.norms import qk_norm_rope
+    x = torch.ones(3, 2, 128, device=dev, dtype=BF16)
+    a, b = qk_norm_rope(x, x, None, None, torch.arange(3, device=dev), torch.empty(0, 64, device=dev))
+    for t in (a, b):
+        assert t[..., :64].isnan().all() and torch.equal(t[..., 64:], x[..., 64:])
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("T,h,hkv,rot,interleaved", [(1, 4, 1, 64, False), (5, 24, 4, 32, False), (133, 3, 3, 20, True),
+@pytest.mark.parametrize("T,h,hkv,rot,interleaved", [(3000, 16, 2, 64, False), (1, 4, 1, 64, False), (5, 24, 4, 32, False), (133, 3, 3, 20, True),
                                                      (40, 0, 2, 64, False), (64, 8, 8, 0, False)])
 def test_into_the_cache(dev, d, T, h, hkv, rot, interleaved):
     """The same bits as the two calls that it replaces."""
@@ -122,16 +131,17 @@ def test_into_the_cache(dev, d, T, h, hkv, rot, interleaved):
     from qwen_a100_fastpath_b200.norms import qk_norm_rope
     gen = torch.Generator(device=dev).manual_seed(T + d)
     page = 16
-    cache = random_cache(gen, 20, page, hkv, d)
+    pages = max(20, T // page + 1)
+    cache = random_cache(gen, pages, page, hkv, d)
     before = KV4Cache(*(t.clone() for t in cache))
     qkv = torch.randn(T, h + 2 * hkv, d, device=dev, generator=gen).to(BF16)
     q, k, v = qkv[:, :h], qkv[:, h:h + hkv], qkv[:, h + hkv:]
     kw = (1 + 0.3 * torch.randn(d, device=dev, generator=gen)).to(BF16)
     pos = torch.randint(0, 100, (T,), device=dev, generator=gen)
     cs = table(dev, 100, rot) if rot else None
-    slots = torch.randperm(20 * page, generator=gen, device=dev)[:T]
+    slots = torch.randperm(pages * page, generator=gen, device=dev)[:T]
     if T > 3:
-        slots[2], slots[3], pos[1] = -1, 20 * page, 100
+        slots[2], slots[3], pos[1] = -1, pages * page, 100
     a, none = qk_norm_rope(q, k, kw, kw, pos, cs, interleaved=interleaved, v=v, cache=cache, slots=slots)
     b, kr = qk_norm_rope(q, k, kw, kw, pos, cs, interleaved=interleaved)
     assert none is None and torch.equal(a.nan_to_num(7), b.nan_to_num(7))

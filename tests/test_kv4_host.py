@@ -60,7 +60,8 @@ def io(fn=LIB.qf_kv4_write, cache=None, **kw):
 
 BAD_CACHES = [(dict(num_pages=-1), -2), (dict(page_size=0), -2), (dict(num_heads=0), -2), (dict(head_size=96), -2),
               (dict(k=None), -1), (dict(v_scale=None), -1), (dict(slot_stride=-128), -3), (dict(page_stride=8200), -4),
-              (dict(scale_slot_stride=4), -4), (dict(v=FAKE + 8), -4), (dict(k_scale=FAKE + 8), -4)]
+              (dict(scale_slot_stride=4), -4), (dict(page_stride=1 << 33), -3), (dict(slot_stride=1 << 32), -3),
+              (dict(scale_page_stride=1 << 32), -3), (dict(v=FAKE + 8), -4), (dict(k_scale=FAKE + 8), -4)]
 
 
 @pytest.mark.parametrize("fn", ["write", "read"])
@@ -89,7 +90,7 @@ def attn(**kw):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(reqs=-1), -2), (dict(q_len=0), -2), (dict(heads=25), -2), (dict(q_len=11), -2), (dict(max_pages=-1), -2),
-    (dict(heads=65536 * 4), -2), (dict(reqs=1 << 30), -2), (dict(scale=float("inf")), -1), (dict(scale=float("nan")), -1),
+    (dict(heads=65536 * 4), -2), (dict(reqs=1 << 30), -2), (dict(max_pages=1 << 30), -2), (dict(scale=float("inf")), -1), (dict(scale=float("nan")), -1),
     (dict(q=None), -1), (dict(out=None), -1), (dict(lens=None), -1), (dict(table=None), -1), (dict(s_bt=-1), -3),
     (dict(sq_t=-8), -3), (dict(sq_h=100), -4), (dict(out=FAKE + 8), -4), (dict(lens=FAKE + 2), -4), (dict(ws=FAKE + 8), -4),
     (dict(ws=None), -6), (dict(ws_bytes=0), -6)])
