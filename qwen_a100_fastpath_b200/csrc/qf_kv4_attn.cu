@@ -27,6 +27,17 @@
 // Codes and scales arrive by cp.async, kAhead tiles ahead; the pages are looked up a tile before that.  The CTAs split all
 // tiles of all requests and heads evenly, whatever the lengths; a CTA's part may begin or end inside a (request, head), and
 // a second kernel joins those.
+//
+// Measured (in a graph, the cache from DRAM): 100000 keys x 2 requests, 4 heads of 256, 30 rows 116 us (2.0 TB/s, 212 TFLOP/s;
+// floor 35), 38400 keys, 18 rows 31 us (floor 6.8), 64 requests of 1 to 8192 keys, 8 heads of 128, 8 rows 36 us (floor 12),
+// 700 keys 10.3 us.  What bounds it: neither DRAM (a third) nor the tensor pipe (48 %) nor issue (IPC 1.9 of 4), but how few
+// warps (12 an SM with 30 rows, 168 registers each) have to cover the latencies of a tile's phases.  At the first size without
+// the matrix instructions 121 us, without the unpacking 104, without the copies 111, without the first two 100.  Of a tile's
+// 5300 to 6000 clocks the scores take 1600 to 1900, the values 1400 to 1900, its copies 600 to 700, the bookkeeping before it 500
+// to 900, the weights 350.
+// Not kept, at the four sizes or the first: scores of the next tile beside this one's values in one block of code 120; the
+// loops over groups rolled 121; five or six CTAs an SM with one row tile 54 (50 then); pages of a tile or more by every thread
+// itself, without places in shared memory 121.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -69,7 +80,9 @@ struct AttnParams {
   float* part_o;    // [2 * grid][rows][D]
 };
 
-// Blocks of 16 tokens of a warp in a tile, and CTAs of an SM.
+// Blocks of 16 tokens of a warp in a tile, and CTAs of an SM.  Two blocks halve a tile's fixed share of time, where registers
+// and shared memory allow it: D = 128 with 8 rows 43.6 -> 38.6 us (the ragged batch above, then), with 16 rows 97 -> 74 (16
+// requests of 8192 keys), D = 64 with 8 rows 76 -> 66; with 16 rows D = 64 loses, 53 -> 65 (64 requests of 4096 keys).
 constexpr int token_blocks(int d, int nq) { return (d == 128 && nq <= 2) || (d == 64 && nq == 1) ? 2 : 1; }
 constexpr int ctas_per_sm(int d, int nq) { return nq == 1 ? 4 : nq <= 4 ? 3 : 2; }
 
@@ -138,7 +151,8 @@ template <int TILE> __device__ __forceinline__ int tiles_of(const AttnParams& p,
 }
 
 // What a (request, head) costs besides its tiles, in tiles: the query, the first reference, the output.  The CTAs' shares are
-// even in these units: positions v below kStart in front of a (request, head)'s first tile, tile v - kStart behind.
+// even in these units: positions v below kStart in front of a (request, head)'s first tile, tile v - kStart behind.  (Ragged
+// batch above, then: 69 us without, 51.8 with 1, 50.4 with 2, 52.9 with 4.)
 constexpr int kStart = 2;
 
 // A walk over tiles in the order (request, head, tile).

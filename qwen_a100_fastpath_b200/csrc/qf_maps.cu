@@ -10,7 +10,8 @@
 // The work is a scan over the requests (two sums) and 16 bytes for each token, so that the call is bound by latency: a
 // launch, one round trip for the lengths, the scan, a search, one round trip for a table entry.  Every CTA makes the scan on
 // its own in shared memory instead of waiting for one that does; a token on a new page computes its entry from the scan,
-// so that no CTA reads what another writes.
+// so that no CTA reads what another writes.  Measured: 2.1 us for one request, 5.0 for 256 requests and 8192 tokens, 7.8 for
+// 1024 requests and 131072 tokens (in a graph; the call's host time is 7.9).
 #include <cuda_runtime.h>
 
 #include <cstdint>

@@ -6,6 +6,10 @@
 //   the first R values turn by the token's angles: with (cos_i, sin_i) = the table's row of the token's position,
 //   a = y[i], b = y[i + R / 2] (or y[2 i], y[2 i + 1]):  a' = a cos_i - b sin_i,  b' = b cos_i + a sin_i
 //   the result is rounded to bf16 once; a key that goes into the cache is quantized from those bf16 values.
+//
+// Bound by memory on paper (a row is read and written once); in fact by the instructions around the 16 bytes of a lane and by
+// the loads in flight: 8192 tokens of 24 + 4 heads of 256 with 64 turned values 49 us in a graph (4.8 TB/s; floor 36), IPC 2.8 of
+// 4, half of the logic pipe; 5 tokens into the cache and back 4.2 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -47,13 +51,16 @@ constexpr int kRopeWarps = 4;
 
 // How rows are read: kAny takes any size, stride and alignment, element by element with the row in shared memory; kWide rows
 // whose pointers and strides are multiples of 16 bytes, with heads of up to 256 (a multiple of eight) and a rotated part that
-// is a multiple of 16 (of eight where interleaved).  8192 tokens of 24 + 4 heads of 256, 64 of them rotated: 99 us with kAny.
+// is a multiple of 16 (of eight where interleaved).  8192 tokens of 24 + 4 heads of 256, 64 of them rotated: 99 us with kAny, 49
+// with kWide.
 
 // kWide: L lanes take a row, a lane eight consecutive values in one 16-byte load.  A group of L lanes takes p.chunk heads of
 // one side of one token, ROWS at a time, so that the token's angles and the weight are loaded and multiplied once for them
-// and ROWS loads are under way.  The
-// other half of a turned pair is L's other lanes' (a shuffle of the raw bf16 words; its weight is loaded beside the lane's
-// own), or the neighbour in the lane's own registers where interleaved (INTER).
+// and ROWS loads are under way.  The other half of a turned pair is another of the L lanes' (a shuffle of the raw bf16 words;
+// its weight is loaded beside the lane's own), or the neighbour in the lane's own registers where interleaved (INTER).
+// Measured at the size above: four heads to a group and separate products with weight, cosine and sine 75 us; one coefficient
+// each for the value and the other one, on packed pairs, 59; eight heads to a group 54; 64 registers, so that eight CTAs
+// share an SM, 49 (ten CTAs, with spills, 72; eight rows at a time 53, two 56).
 template <int L, int ROWS, bool INTER>
 __global__ void __launch_bounds__(kRopeWarps * 32, ROWS == 1 ? 1 : 8) rope_wide_kernel(const RopeParams p) {
   pdl_launch_dependents();
@@ -370,7 +377,8 @@ extern "C" int qf_qk_norm_rope(const void* q, int64_t sq_t, int64_t sq_h, const 
                     wide_rows(k_out, sp_t, sp_h) && wide_rows(v, sv_t, sv_h) && aligned(q_weight, 16) &&
                     aligned(k_weight, 16) && (!p.cos_sin || (aligned(cos_sin, 16) && s_cs % 8 == 0));
   const int lanes = head_size <= 64 ? 8 : head_size <= 128 ? 16 : 32;
-  // eight heads to a group, four at a time, where that leaves groups enough for the SMs
+  // eight heads to a group, four at a time, where that leaves groups enough for the SMs (about 900 threads each); a head to a
+  // group below, where the first load's latency counts and not the angles' share
   const bool many = wide && p.total / 8 * lanes >= 1u << 17;
   p.chunk = many ? 8 : 1;
   cudaLaunchConfig_t cfg = {};
