@@ -1,4 +1,4 @@
-"""CPU definition of the 4-bit paged cache and of what a step does around it: the checker of ``kv4.py``, ``paged.py`` and
+"""CPU definition of the 4-bit paged cache and of what a step does around it: the oracle of ``kv4.py``, ``paged.py`` and
 ``norms.qk_norm_rope``.
 
 The quantizer is defined in fp32 operations (include/qf_b200.h), so that ``quantize`` and ``values`` are exact; everything

@@ -714,11 +714,18 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const AttnParams
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int pieces = D / kJoinDims, work = p.rows * pieces;
+  constexpr int kLists = (kMaxSms * kMaxCtas + kJoinThreads - 1) / kJoinThreads;
+  int4 joins[kLists];  // all on their way at once
+#pragma unroll
+  for (int i = 0; i < kLists; ++i) {
+    joins[i] = make_int4(-1, 0, 0, 0);
+    if (i * kJoinThreads + tid < grid) joins[i] = p.joins[i * kJoinThreads + tid];
+  }
   int n = 0, total = 0;
-  for (int i0 = 0; i0 < grid; i0 += kJoinThreads) {
-    const int from = i0 + tid;
-    int4 join = make_int4(-1, 0, 0, 0);
-    if (from < grid) join = p.joins[from];
+#pragma unroll
+  for (int i = 0; i < kLists; ++i) {
+    const int from = i * kJoinThreads + tid;
+    const int4 join = joins[i];
     const bool named = join.x >= 0;
     const int share = join_share(join.z - from + 1);
     int2 sum = make_int2(named, named ? (work * share + kJoinGroups - 1) / kJoinGroups : 0);
