@@ -1,9 +1,9 @@
 // qf_kv4_attn.cu -- attention of uniform decode and verification batches over the paged cache held in 4 bits (qf_kv4.cuh has
 // the format).
 //
-// Mathematics: O = softmax(scale q K^T + mask) V in one pass over the keys, with a running maximum m and sum l for each
-// query row in fp32: a tile's weights are p = 2^(x - m) with x in units of log2, and where m has grown O and l are first
-// scaled by 2^(m_old - m).  Parts of a row's keys that different CTAs hold are joined by their m and l afterwards.
+// Mathematics: O = softmax(scale q K^T + mask) V in one pass over the keys, with a reference m and a sum l for each query row
+// in fp32: a tile's weights are p = 2^(x - m) with x in units of log2, and where m has to rise O and l are first scaled by
+// 2^(m_old - m).  Parts of a row's keys that different CTAs hold are joined by their m and l afterwards.
 //
 // Bound by memory for few rows (D / 2 + D / 16 bytes for each key and value), by taking the nibbles apart and the matrix
 // instructions for many.  The R = q_len * group query rows of a key head are one tile, so that its cache is read once.  The
@@ -20,9 +20,12 @@
 //
 // A CTA of four warps takes 64 tokens at a time: each warp scores 16 of them against all rows, the weights (bf16) are
 // exchanged in shared memory, and each warp adds up 64 of the head's dimensions (over all tokens for D = 256, over half or a
-// quarter of them for 128 and 64).  The weights are relative to a reference, not to the maximum itself: bf16 and fp32 have
-// the same range of exponents, so that any reference within 2^16 of the maximum gives the same relative precision.  It is
-// set by the first tile and raised, with the exchange that this needs, only where a score exceeds it by more than 16.
+// quarter of them for 128 and 64).  The weights are relative to a reference, not to the running maximum: bf16 and fp32 have
+// the same range of exponents, so that the precision of a weight does not depend on where the reference lies.  It is set 32
+// above the first tile's maximum, and set anew, with the exchange that this needs, only where a score has come within 16 of
+// it.  So weights are at most 2^-16, and the sums over 2^18 keys of the largest values that the cache keeps (2^126) stay below
+// 2^128; the row's largest weight is at least 2^-32, so that means of values down to 2^-90 lose nothing to fp32's range either.
+// (Set at the first maximum itself, the weights reached 2^16, and sums of values from 2^112 on could become infinite.)
 //
 // Codes and scales arrive by cp.async, kAhead tiles ahead; the pages are looked up a tile before that.  The CTAs split all
 // tiles of all requests and heads evenly, whatever the lengths; a CTA's part may begin or end inside a (request, head), and
@@ -168,7 +171,8 @@ template <int TILE> struct Cursor {
 };
 
 constexpr float kNoRef = -3e38f;  // stands for the reference of a row that has seen no key, in a part that is joined
-constexpr float kSlack = 16.f;
+constexpr float kAbove = 32.f;    // of the maximum, where a reference is set
+constexpr float kNear = -16.f;    // a score that comes nearer has it set anew
 
 // Positions 0 to total - 1 split evenly: CTA i begins at start(i), position v is in CTA holder(v)'s share.
 struct Shares {
@@ -501,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
         for (int e = 0; e < 2; ++e)
           if (unset >> (2 * j + e) & 1 && highest(j, e) > -INFINITY) top = INFINITY;
     // (all warps have read this tile's keys and the last one's values, whose stages are filled again now)
-    const bool raise = __syncthreads_or(top > kSlack);
+    const bool raise = __syncthreads_or(top > kNear);
     copy(i + G::kAhead, places, key_stage, value_free);
     float scale_o[NQ][2];
     if (__builtin_expect(raise, 0)) {
@@ -528,8 +532,8 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t bit = 1u << (2 * j + e);
-          // a row's first reference is its maximum so far, whatever its sign; later ones only rise
-          const float rise = !(unset & bit) ? fmaxf(v[e], 0.f) : v[e] == -INFINITY ? 0.f : v[e];
+          // a row's first reference goes by its maximum so far, whatever its sign; later ones only rise
+          const float rise = !(unset & bit) ? fmaxf(v[e] + kAbove, 0.f) : v[e] == -INFINITY ? 0.f : v[e] + kAbove;
           scale_o[j][e] = unset & bit ? 1.f : ex2_approx(-rise);  // (sums of an unset row are zero, or NaN for good)
           if (v[e] > -INFINITY) unset &= ~bit;
           l[j][e] *= scale_o[j][e];

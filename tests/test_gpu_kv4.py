@@ -290,6 +290,31 @@ def test_attention_same_bits_every_time(dev):
     check_attention(caught, query, cache, small, table, 2, 0.1)
 
 
+@pytest.mark.parametrize("size", [2.0 ** 113, 2.0 ** 125.9, 2.0 ** -90])
+@pytest.mark.parametrize("d,g,hkv", [(64, 1, 1), (128, 4, 2), (256, 6, 2)])
+def test_attention_sums_of_large_and_small_values(dev, d, g, hkv, size):
+    """A row's result is a mean of its values: their weighted sums stay within fp32 on the way, with scores that rise along
+    the keys by nearly the 2^16 up to which a row's reference stays, in one share and over many CTAs.  (The reference lies 16 to
+    32 above a row's maximum, so that the distances to it are off by 2^-19 for their rounding, twice in a mean: 2 ln 2 2^-19 of
+    A, within the 2^-18 above.)"""
+    from qwen_a100_fastpath_b200.kv4 import kv4_attention, kv4_cache, kv4_read, kv4_write
+    gen = torch.Generator(device=dev).manual_seed(d)
+    lens, q_len, page = [30, 700, 6000], 2, 16
+    table, pages = table_for(gen, lens, page)
+    cache = kv4_cache(pages, page, hkv, d, dev)
+    n = sum(lens)
+    slots = torch.cat([table[b, :-(-m // page)].long().repeat_interleave(page)[:m] * page +
+                       torch.arange(m, device=dev) % page for b, m in enumerate(lens)])
+    k = 0.1 * torch.randn(n, hkv, d, device=dev, generator=gen)
+    k += torch.cat([torch.linspace(0, 1, m, device=dev) for m in lens])[:, None, None]
+    v = size * (0.5 + 0.5 * torch.rand(n, hkv, d, device=dev, generator=gen))
+    kv4_write(k.to(BF16), v.to(BF16), slots, cache)
+    query = (1 + 0.1 * torch.randn(len(lens) * q_len, hkv * g, d, device=dev, generator=gen)).to(BF16)
+    out = kv4_attention(query, cache, torch.tensor(lens, dtype=torch.int32, device=dev), table, q_len, 10.0 / d)
+    assert out.isfinite().all() and out.min() > 0.4 * size and out.max() < 1.1 * size
+    check_attention(out, query, cache, lens, table, q_len, 10.0 / d)
+
+
 # ---- writer and reader --------------------------------------------------------------------------------------------
 def tokens(gen, t, hkv, d):
     x = torch.randn(t, hkv, d, device=gen.device, generator=gen) * torch.exp(
