@@ -418,13 +418,16 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NQ>::kCtas) kv4_attn_kernel(c
     next = look(i + G::kAhead + 1);
     if (__builtin_expect(masked_rows, 0) && tid < kTile) {
       // values that are not finite may be hidden from some rows only: they leave the product (a weight of zero would not
-      // keep them out), and the rows that see one get their NaN afterwards
+      // keep them out), and the rows that see one get their NaN afterwards.  A group's values are finite if those of its least
+      // and its greatest nibble are.  (The writer makes no others but NaN; in a group from elsewhere that could hold an infinity
+      // every value counts as NaN here.)
 #pragma unroll
       for (int gr = 0; gr < D / 64; ++gr) {
         const uint32_t at = vals + kTile * G::kRow + tid * G::kScale + 4 * gr;
         const uint32_t sc = lds32(at);
         const float s = bf16_lo(sc), c = bf16_hi(sc);
-        const bool is_bad = !(fabsf(s) < 2.6584559915698317e36f && fabsf(c) < 8.507059173023462e37f);  // 2^121, 2^126
+        constexpr float kEnd = 3.39617752923046e38f;  // 2^128 - 2^119, from which on a sum rounds to an infinite bf16 number
+        const bool is_bad = !(fabsf(fmaf(16.f, s, c)) < kEnd && fabsf(fmaf(31.f, s, c)) < kEnd);
         if (is_bad) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(0u) : "memory");
         const uint32_t bits = __ballot_sync(0xffffffffu, is_bad);
         if (lane == 0) bad[i & 1][gr][warp] = bits;

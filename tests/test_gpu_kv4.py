@@ -315,6 +315,29 @@ def test_attention_sums_of_large_and_small_values(dev, d, g, hkv, size):
     check_attention(out, query, cache, lens, table, q_len, 10.0 / d)
 
 
+@pytest.mark.parametrize("size", [2.0 ** 118, 2.0 ** 122, 2.0 ** 124, 2.0 ** 125.9])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_values_at_the_end_of_the_range(dev, d, size):
+    """Groups that the writer keeps as numbers are numbers wherever they lie: in a tile that some rows do not see whole, in
+    one that all rows do, in the last token, and hidden from the first rows of a request."""
+    from qwen_a100_fastpath_b200.kv4 import kv4_attention, kv4_read, kv4_write
+    gen = torch.Generator(device=dev).manual_seed(d)
+    lens, q_len, g, hkv, page = [40, 300, 2], 2, 3, 2, 16
+    table, pages = table_for(gen, lens, page)
+    cache = random_cache(gen, pages, page, hkv, d)
+    places = [(0, 7), (0, 39), (1, 20), (1, 290), (2, 1)]
+    slots = torch.tensor([table[b, p // page].item() * page + p % page for b, p in places], device=dev)
+    k, _ = kv4_read(cache, slots)
+    v = (size * (2 * torch.rand(len(places), hkv, d, device=dev, generator=gen) - 1)).to(BF16)
+    v[..., 0], v[..., 1] = size, -size
+    kv4_write(k, v, slots, cache)
+    assert kv4_read(cache, slots)[1].isfinite().all()
+    query = torch.randn(len(lens) * q_len, hkv * g, d, device=dev, generator=gen).to(BF16)
+    out = kv4_attention(query, cache, torch.tensor(lens, dtype=torch.int32, device=dev), table, q_len, d ** -0.5)
+    assert out.isfinite().all()
+    check_attention(out, query, cache, lens, table, q_len, d ** -0.5)
+
+
 # ---- writer and reader --------------------------------------------------------------------------------------------
 def tokens(gen, t, hkv, d):
     x = torch.randn(t, hkv, d, device=gen.device, generator=gen) * torch.exp(
