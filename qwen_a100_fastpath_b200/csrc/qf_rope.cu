@@ -148,7 +148,8 @@ __global__ void __launch_bounds__(kRopeWarps * 32, ROWS == 1 ? 1 : 8) rope_wide_
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       ca[k] = pack_f32x2(w[2 * k] * cs[2 * k], w[2 * k + 1] * cs[2 * k + 1]);
-      cb[k] = pack_f32x2(w2[2 * k] * sn[2 * k], w2[2 * k + 1] * sn[2 * k + 1]);
+      // (an infinite weight times the zero that stands for the other of a value that does not turn would be NaN)
+      cb[k] = turned ? pack_f32x2(w2[2 * k] * sn[2 * k], w2[2 * k + 1] * sn[2 * k + 1]) : pack_f32x2(0.f, 0.f);
     }
   }
   uint32_t page = 0, off = 0;

@@ -113,6 +113,26 @@ def test_strides_and_edges(dev):
     assert not a[0].any() and a[3].isnan().all()
 
 
+@pytest.mark.parametrize("d,rot", [(128, 64), (256, 64), (64, 0), (96, 20)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_an_infinite_weight_of_values_that_do_not_turn(dev, d, rot, interleaved):
+    """It makes them infinite, in every form of the kernel, and leaves the others as they are."""
+    from qwen_a100_fastpath_b200.norms import qk_norm_rope
+    gen = torch.Generator(device=dev).manual_seed(d)
+    q = (2 + torch.rand(9, 6, d, device=dev, generator=gen)).to(BF16) * torch.tensor([1, -1] * 3, device=dev)[:, None]
+    q = q.to(BF16)
+    w = (1 + 0.3 * torch.randn(d, device=dev, generator=gen)).to(BF16)
+    pos, cs = torch.arange(9, device=dev), table(dev, 9, rot) if rot else None
+    a, b = qk_norm_rope(q, q, w, w, pos, cs, interleaved=interleaved)
+    at = torch.zeros(d, dtype=torch.bool, device=dev)
+    at[[rot + 3, d - 1]] = True
+    w[at] = float("inf")
+    x, y = qk_norm_rope(q, q, w, w, pos, cs, interleaved=interleaved)
+    for got, ref in ((x, a), (y, b)):
+        assert torch.equal(got[..., ~at], ref[..., ~at])
+        assert torch.equal(got[..., at].float(), torch.sign(q[..., at].float()) * float("inf"))
+
+
 def test_a_table_of_no_positions(dev):
     """Every position is outside it."""
     from qwen_a100_fastpath_b200.norms import qk_norm_rope
