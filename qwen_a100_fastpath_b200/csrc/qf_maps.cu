@@ -36,6 +36,7 @@ struct MapsParams {
 };
 
 constexpr int kMapThreads = 256;
+constexpr size_t kMapStatic = 1024;  // no less than the kernel's static shared memory
 constexpr uint32_t kMapMax = 0x7fffffffu;
 
 __device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, kMapMax); }
@@ -46,6 +47,7 @@ __global__ void __launch_bounds__(kMapThreads) maps_kernel(const MapsParams p) {
   uint32_t* first = start + p.reqs + 1;      // pages taken before request r
   uint32_t* past = first + p.reqs;
   __shared__ uint2 warp_sum[kMapThreads / 32];
+  static_assert(sizeof(warp_sum) <= kMapStatic, "counted with the dynamic part against the default limit");
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -158,7 +160,7 @@ extern "C" int qf_step_maps(const int32_t* query_lens, const int32_t* past_lens,
                   query_start, seq_lens, free_head_out, positions, slots, num_reqs, max_pages, page_size, num_free,
                   num_tokens, free_head != nullptr};
   const size_t smem = (3 * static_cast<size_t>(num_reqs) + 1) * 4;
-  if (smem > 48 * 1024) {
+  if (smem + kMapStatic > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (3 * QF_MAPS_MAX_REQS + 1) * 4);
     if (e != cudaSuccess) return fail(QF_ERR_LAUNCH, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));

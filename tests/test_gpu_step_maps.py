@@ -2,6 +2,9 @@
 from __future__ import annotations
 
 import random
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -71,6 +74,21 @@ def test_many_requests(dev):
     b = 16384
     q = [rng.randrange(3) for _ in range(b)]
     run(dev, q, [rng.randrange(20) for _ in range(b)], 3, 8, sum(q) + 1, list(range(b)), 0)
+
+
+def test_request_counts_around_48_kilobytes_of_scan(dev):
+    """In a process of its own: no earlier call with more requests has asked for the larger shared memory."""
+    code = """
+import random, torch
+from tests.test_gpu_step_maps import run
+rng = random.Random(6)
+for b in (4088, 4090, 4091, 4093, 4095, 4096, 4097):
+    q = [rng.randrange(3) for _ in range(b)]
+    run(torch.device("cuda", 0), q, [rng.randrange(20) for _ in range(b)], 3, 8, sum(q) + 1, list(range(b)), 0)
+"""
+    got = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True,
+                         timeout=600)
+    assert got.returncode == 0, got.stderr[-2000:]
 
 
 def test_one_long_prompt_among_others(dev):
