@@ -170,7 +170,7 @@ at::Tensor as_heads(const at::Tensor& t, bool wide) {
   if (t.numel() == 0) return t;
   const bool fits = (t.size(2) == 1 || t.stride(2) == 1) &&
                     (!wide || (at16(t) && stride_of(t, 0) % 8 == 0 && stride_of(t, 1) % 8 == 0));
-  return fits ? t : t.contiguous();
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);  // (contiguous() returns contiguous heads at an odd address as they are)
 }
 
 qf_kv4_cache check_cache(const char* op, const CacheArgs& c, const at::Device& dev, bool written_to) {

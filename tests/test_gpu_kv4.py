@@ -441,6 +441,38 @@ def test_write_strided(dev):
         check_written(cache, before, k, v, slots)
 
 
+def at_odd_address(x):
+    """The same values, contiguous, two bytes behind a 16-byte boundary."""
+    buf = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)
+    buf[1:] = x.reshape(-1)
+    return buf[1:].view(x.shape)
+
+
+@pytest.mark.parametrize("t,hkv,d", [(1, 1, 64), (1, 2, 256), (9, 1, 128), (40, 2, 128)])
+def test_contiguous_heads_at_odd_addresses(dev, t, hkv, d):
+    """They are copied like other heads that are not aligned: keys, values and the query, each alone and together; a slice of
+    a single token and head counts as contiguous whatever its strides."""
+    from qwen_a100_fastpath_b200.kv4 import KV4Cache, kv4_attention, kv4_write
+    gen = torch.Generator(device=dev).manual_seed(t)
+    cache = random_cache(gen, 9, 16, hkv, d)
+    k, v = tokens(gen, t, hkv, d), tokens(gen, t, hkv, d)
+    for a, b in ((at_odd_address(k), v), (k, at_odd_address(v)), (at_odd_address(k), at_odd_address(v)),
+                 (tokens(gen, t, hkv, d + 1)[..., 1:], v)):
+        before = KV4Cache(*(x.clone() for x in cache))
+        slots = torch.randperm(144, generator=gen, device=dev)[:t]
+        kv4_write(a, b, slots, cache)
+        check_written(cache, before, a, b, slots)
+    lens = [30] * t
+    table, pages = table_for(gen, lens, 16)
+    cache = random_cache(gen, pages, 16, hkv, d)
+    seq = torch.tensor(lens, dtype=torch.int32, device=dev)
+    for query in (at_odd_address(tokens(gen, t, hkv, d)), torch.randn(t, hkv, d + 1, device=dev, generator=gen).to(BF16)[..., 1:]):
+        got = kv4_attention(query, cache, seq, table, 1, 0.05)
+        check_attention(got, query, cache, lens, table, 1, 0.05)
+        out = torch.empty(query.shape, dtype=BF16, device=dev)
+        assert torch.equal(kv4_attention(query, cache, seq, table, 1, 0.05, out=out), got)
+
+
 def test_write_far_pages(dev):
     from qwen_a100_fastpath_b200.kv4 import KV4Cache, kv4_read, kv4_write
     gen = torch.Generator(device=dev).manual_seed(3)
