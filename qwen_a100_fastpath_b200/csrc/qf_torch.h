@@ -66,7 +66,7 @@ inline void written(const at::Tensor& t) {
 inline cudaStream_t stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
 // The bytes of a tensor as `rows` intervals of `width` bytes, `step` bytes apart.  Exact for rows of adjacent elements; what
-// lies between the elements of other tensors counts as theirs.
+// lies between the elements of other tensors counts as theirs (`overlap` looks closer where these intervals meet).
 struct Intervals {
   int64_t begin, width, step, rows;
   int64_t end() const { return begin + (rows - 1) * step + width; }
@@ -86,7 +86,7 @@ inline Intervals intervals_of(const at::Tensor& t) {
   return v;
 }
 
-inline bool overlap(const at::Tensor& ta, const at::Tensor& tb) {
+inline bool spans_overlap(const at::Tensor& ta, const at::Tensor& tb) {
   if (ta.numel() == 0 || tb.numel() == 0) return false;
   Intervals a = intervals_of(ta), b = intervals_of(tb);
   if (a.end() <= b.begin || b.end() <= a.begin) return false;
@@ -106,6 +106,65 @@ inline bool overlap(const at::Tensor& ta, const at::Tensor& tb) {
     if (pa + a.width <= pb) ++i; else ++j;
   }
   return false;
+}
+
+// The bytes of a tensor as runs of span[n] adjacent bytes, repeated at nested strides, the largest first; level l and those
+// inside it reach over span[l] bytes.  For up to kLevels strides.
+struct Runs {
+  static constexpr int kLevels = 8;
+  int64_t begin = 0, stride[kLevels], size[kLevels], span[kLevels + 1];
+  int n = 0;
+  bool fits = true;
+  explicit Runs(const at::Tensor& t) : begin(static_cast<int64_t>(reinterpret_cast<uintptr_t>(t.data_ptr()))) {
+    const int64_t es = static_cast<int64_t>(t.element_size());
+    for (int i = 0; i < t.dim(); ++i) {
+      if (t.size(i) == 1 || t.stride(i) == 0) continue;
+      if (n == kLevels) {
+        fits = false;
+        return;
+      }
+      int at = n++;
+      for (; at > 0 && stride[at - 1] < t.stride(i) * es; --at) stride[at] = stride[at - 1], size[at] = size[at - 1];
+      stride[at] = t.stride(i) * es, size[at] = t.size(i);
+    }
+    int64_t run = es;
+    while (n > 0 && stride[n - 1] == run) run *= size[--n];
+    for (int i = n - 1; i > 0; --i)
+      if (stride[i - 1] == stride[i] * size[i]) {  // rows of rows without a gap between: one level
+        stride[i - 1] = stride[i], size[i - 1] *= size[i];
+        for (int j = i; j + 1 < n; ++j) stride[j] = stride[j + 1], size[j] = size[j + 1];
+        --n;
+      }
+    span[n] = run;
+    for (int i = n - 1; i >= 0; --i) span[i] = (size[i] - 1) * stride[i] + span[i + 1];
+  }
+};
+
+inline int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+
+// Whether bytes of a's levels from la on and of b's from lb on, d bytes further, are the same; exact within `budget` steps,
+// true beyond it.  Levels of one stride are taken together: only rows whose distance brings them within reach of one another
+// are looked at, two or three of any number.
+inline bool runs_meet(const Runs& a, int la, const Runs& b, int lb, int64_t d, int* budget) {
+  if (d >= a.span[la] || -d >= b.span[lb]) return false;
+  if (la == a.n && lb == b.n) return true;
+  if (--*budget < 0) return true;
+  const int64_t sa = la < a.n ? a.stride[la] : 0, sb = lb < b.n ? b.stride[lb] : 0;
+  const int ia = la + (sa >= sb), ib = lb + (sb >= sa);
+  // rows i of a and j of b lie d + m s apart, m = j - i (of the one that steps, where only one does)
+  const int64_t s = sa > sb ? sa : sb, ra = sa >= sb ? a.size[la] - 1 : 0, rb = sb >= sa ? b.size[lb] - 1 : 0;
+  const int64_t lo = floor_div(-b.span[ib] - d, s) + 1, hi = floor_div(a.span[ia] - d - 1, s);
+  for (int64_t m = lo > -ra ? lo : -ra; m <= (hi < rb ? hi : rb); ++m)
+    if (runs_meet(a, ia, b, ib, d + m * s, budget)) return true;
+  return false;
+}
+
+inline bool overlap(const at::Tensor& ta, const at::Tensor& tb) {
+  if (!spans_overlap(ta, tb)) return false;
+  // views side by side within a row (keys and values of a slot, for instance)
+  const Runs a(ta), b(tb);
+  int budget = 4096;
+  return !a.fits || !b.fits || runs_meet(a, 0, b, 0, b.begin - a.begin, &budget);
 }
 
 // Whether two tensors of one shape and type hold the same elements at the same places.

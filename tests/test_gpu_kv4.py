@@ -487,6 +487,59 @@ def test_write_far_pages(dev):
         assert np.array_equal(host(r), orc.values(orc.pack(nib), sc))
 
 
+def side_by_side(dev, pages, hkv, page, d, how):
+    """Keys and values, and their scales, as views of shared buffers without a common byte."""
+    from qwen_a100_fastpath_b200.kv4 import KV4Cache
+    half, g = d // 2, d // 64
+    if how == "slot":
+        codes = torch.zeros(pages, hkv, page, 2, half, dtype=torch.uint8, device=dev)
+        scale = torch.zeros(pages, hkv, page, 2, g, 2, dtype=BF16, device=dev)
+        return KV4Cache(codes[:, :, :, 0], codes[:, :, :, 1], scale[:, :, :, 0], scale[:, :, :, 1])
+    if how == "head":
+        codes = torch.zeros(pages, hkv, 2, page, half, dtype=torch.uint8, device=dev)
+        scale = torch.zeros(pages, hkv, 2, page, g, 2, dtype=BF16, device=dev)
+        return KV4Cache(codes[:, :, 0], codes[:, :, 1], scale[:, :, 0], scale[:, :, 1])
+    if how == "slots_first":
+        codes = torch.zeros(pages, page, hkv, 2, half, dtype=torch.uint8, device=dev).transpose(1, 2)
+        scale = torch.zeros(pages, page, 2, hkv, g, 2, dtype=BF16, device=dev).transpose(1, 3)
+        return KV4Cache(codes[:, :, :, 0], codes[:, :, :, 1], scale[:, :, 0], scale[:, :, 1])
+    # all four in one record for each head and slot
+    record = 2 * half + 8 * g + (-8 * g) % 16
+    raw = torch.zeros(pages, hkv, page, record, dtype=torch.uint8, device=dev)
+    parts = [raw[..., 2 * half + 4 * g * i:2 * half + 4 * g * (i + 1)].view(BF16).unflatten(-1, (g, 2)) for i in range(2)]
+    return KV4Cache(raw[..., :half], raw[..., half:2 * half], *parts)
+
+
+@pytest.mark.parametrize("how", ["slot", "head", "slots_first", "record"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_keys_and_values_side_by_side(dev, d, how):
+    """Written (both ways), read and attended like a cache of four buffers."""
+    from qwen_a100_fastpath_b200.kv4 import KV4Cache, kv4_attention, kv4_read, kv4_write
+    from qwen_a100_fastpath_b200.norms import qk_norm_rope
+    gen = torch.Generator(device=dev).manual_seed(d)
+    pages, hkv, page, g, t = 7, 3, 5, 2, 30
+    cache = side_by_side(dev, pages, hkv, page, d, how)
+    plain = KV4Cache(*(x.clone(memory_format=torch.contiguous_format) for x in cache))
+    k, v = tokens(gen, t, hkv, d), tokens(gen, t, hkv, d)
+    slots = torch.randperm(pages * page, generator=gen, device=dev)[:t]
+    before = KV4Cache(*(x.clone() for x in cache))
+    for c in (cache, plain):
+        kv4_write(k, v, slots, c)
+    check_written(cache, before, k, v, slots)
+    query = tokens(gen, t, hkv * g, d)
+    before = KV4Cache(*(x.clone() for x in cache))
+    qk_norm_rope(query, v, None, None, None, None, v=k, cache=cache, slots=slots)
+    check_written(cache, before, v, k, slots)
+    for c in (cache, plain):
+        kv4_write(k, v, slots, c)
+    table = torch.randperm(pages, generator=gen, device=dev).to(torch.int32)[None]
+    lens = torch.tensor([33], dtype=torch.int32, device=dev)
+    a, b = (kv4_attention(query, c, lens, table, 1, 0.1) for c in (cache, plain))
+    assert torch.equal(a, b)
+    for x, y in zip(kv4_read(cache, slots), kv4_read(plain, slots)):
+        assert torch.equal(x, y)
+
+
 # ---- a step as it is used ------------------------------------------------------------------------------------------
 def test_step_of_a_layer(dev):
     """Maps from lengths, norms and rotation into the cache, attention: several steps of growing requests, eagerly and as

@@ -50,6 +50,36 @@ def test_cache_memory(dev):
     kv4_read(KV4Cache(c.k, c.k, c.k_scale, c.k_scale), slots)             # reading one side twice is fine
 
 
+@pytest.mark.parametrize("shift", [16, 48, 64, 80, 112])
+def test_caches_whose_rows_meet(dev, shift):
+    """Values that begin inside the keys' rows, or whose rows reach into the next keys: side by side only at the row's end.
+    (Ones are a step of 0, an offset of 1 and nibbles of 0: what a call wrote is seen in the offsets.)"""
+    from qwen_a100_fastpath_b200.kv4 import KV4Cache, kv4_cache, kv4_write
+    c = kv4_cache(3, 4, 2, 128, dev)
+    k = torch.ones(5, 2, 128, dtype=BF16, device=dev)
+    slots = torch.arange(5, device=dev)
+    for lead in ((3, 2, 4), (3, 4, 2)):
+        raw = torch.zeros(3 * 2 * 4 * 128 + 128, dtype=torch.uint8, device=dev)
+        rows = [raw[at:at + 3072].view(*lead, 128)[..., :64] for at in (0, shift)]
+        if lead[1] == 4:
+            rows = [r.transpose(1, 2) for r in rows]
+        cache = KV4Cache(rows[0], rows[1], c.k_scale, c.v_scale)
+        if shift == 64:
+            kv4_write(k, k, slots, cache)
+            assert (c.k_scale[0, :, :, :, 1] == 1).all() and torch.equal(c.v_scale, c.k_scale)
+            c.k_scale.zero_(), c.v_scale.zero_()
+        else:
+            refused(lambda: kv4_write(k, k, slots, cache))
+            assert not c.k_scale.any() and not c.v_scale.any()
+    # the same on the level of heads: the values' page of heads begins one head late
+    raw = torch.zeros(3 * 2 * 2 * 4 * 64 + 1024, dtype=torch.uint8, device=dev)
+    rows = [raw[at:at + 3072].view(3, 2, 2, 4, 64)[:, :, 0] for at in (0, 512, 256)]
+    refused(lambda: kv4_write(k, k, slots, KV4Cache(rows[0], rows[1], c.k_scale, c.v_scale)))
+    assert not c.k_scale.any() and not c.v_scale.any()
+    kv4_write(k, k, slots, KV4Cache(rows[0], rows[2], c.k_scale, c.v_scale))
+    assert (c.k_scale[0, :, :, :, 1] == 1).all()
+
+
 def test_attention_memory(dev):
     from qwen_a100_fastpath_b200.kv4 import kv4_attention, kv4_cache
     c = kv4_cache(4, 16, 2, 128, dev)
