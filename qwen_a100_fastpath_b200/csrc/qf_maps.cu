@@ -10,8 +10,10 @@
 // The work is a scan over the requests (two sums) and 16 bytes for each token, so that the call is bound by latency: a
 // launch, one round trip for the lengths, the scan, a search, one round trip for a table entry.  Every CTA makes the scan on
 // its own in shared memory instead of waiting for one that does; a token on a new page computes its entry from the scan,
-// so that no CTA reads what another writes.  Measured: 2.1 us for one request, 5.0 for 256 requests and 8192 tokens, 7.8 for
-// 1024 requests and 131072 tokens (in a graph; the call's host time is 7.9).
+// so that no CTA reads what another writes.  The entries themselves are written page by page, whatever the number of tokens
+// and of places for them: 64 contexts of 100000 tokens, opened without a place for any, are 400000 entries and 31 us (a token
+// at a time it was 25000 turns of one CTA).  Measured: 2.1 us for one request, 3.5 for 256 requests and 8192 tokens, 8.0 for
+// 1024 requests and 131072 tokens (in a graph; with the entries written by the tokens 5.1 and 7.8; the call's host time is 7.9).
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -44,8 +46,8 @@ __device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min
 __global__ void __launch_bounds__(kMapThreads) maps_kernel(const MapsParams p) {
   extern __shared__ uint32_t sm[];
   uint32_t* start = sm;                      // [reqs + 1]
-  uint32_t* first = start + p.reqs + 1;      // pages taken before request r
-  uint32_t* past = first + p.reqs;
+  uint32_t* first = start + p.reqs + 1;      // [reqs + 1]: pages taken before request r
+  uint32_t* past = first + p.reqs + 1;
   __shared__ uint2 warp_sum[kMapThreads / 32];
   static_assert(sizeof(warp_sum) <= kMapStatic, "counted with the dynamic part against the default limit");
   pdl_launch_dependents();
@@ -78,7 +80,7 @@ __global__ void __launch_bounds__(kMapThreads) maps_kernel(const MapsParams p) {
     sq = sat_add(sq, wq), sp = sat_add(sp, wp);
     if (r < p.reqs) {
       start[r + 1] = sq;
-      first[r] = sp;  // inclusive so far
+      first[r + 1] = sp;
       past[r] = before;
       if (blockIdx.x == 0) {
         p.query_start[r + 1] = static_cast<int32_t>(sq);
@@ -87,46 +89,50 @@ __global__ void __launch_bounds__(kMapThreads) maps_kernel(const MapsParams p) {
     }
     __syncthreads();
   }
-  if (tid == 0) start[0] = 0;
+  if (tid == 0) start[0] = first[0] = 0;
   const uint32_t head = p.free_head ? max(p.free_head[0], 0) : 0;
   if (blockIdx.x == 0 && tid == 0) {
     p.query_start[0] = 0;
     if (p.free_head_out) p.free_head_out[0] = static_cast<int32_t>(sat_add(head, base_p));
   }
   __syncthreads();
-  const uint32_t total = base_q;
-  // tokens behind the map's end still open their pages
-  const uint32_t end = p.grow && total > static_cast<uint32_t>(p.tokens) ? total : static_cast<uint32_t>(p.tokens);
-  for (uint64_t j = blockIdx.x * static_cast<uint64_t>(kMapThreads) + tid; j < end;
-       j += static_cast<uint64_t>(gridDim.x) * kMapThreads) {
+  // the last request whose tokens (or pages) begin at or before v
+  auto holder = [&](const uint32_t* begin, uint32_t v) {
+    int lo = 0, hi = p.reqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (begin[mid] <= v) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+  };
+  // the new page `taken` places behind the list's head
+  auto new_page = [&](uint32_t taken) {
+    const uint64_t from = static_cast<uint64_t>(head) + taken;
+    return from < static_cast<uint64_t>(p.num_free) ? p.free_pages[from] : -1;
+  };
+  const uint64_t self = blockIdx.x * static_cast<uint64_t>(kMapThreads) + tid, threads = static_cast<uint64_t>(gridDim.x) * kMapThreads;
+  const uint32_t total = base_q, opened = p.grow ? base_p : 0;
+  for (uint64_t j = self; j < static_cast<uint32_t>(p.tokens); j += threads) {
     const uint32_t i = static_cast<uint32_t>(j);
     int64_t pos = 0, slot = -1;
     if (i < total) {
-      int lo = 0, hi = p.reqs - 1;  // the last request whose tokens begin at or before i
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (start[mid] <= i) lo = mid; else hi = mid - 1;
-      }
-      const uint32_t before = past[lo], q = start[lo + 1] - start[lo];
-      pos = static_cast<int64_t>(before) + (i - start[lo]);
+      const int r = holder(start, i);
+      pos = static_cast<int64_t>(past[r]) + (i - start[r]);
       const uint32_t at = static_cast<uint32_t>(min(pos, static_cast<int64_t>(kMapMax)));
       const uint32_t col = at / p.page, off = at - col * p.page;
       if (col < static_cast<uint32_t>(p.width)) {
-        int32_t* entry = p.table + lo * p.table_row + col;
-        const uint32_t old = pages(before);
-        int32_t page;
-        if (p.grow && col >= old) {
-          const uint32_t taken = pages(sat_add(before, q)) - old;
-          const uint64_t from = static_cast<uint64_t>(head) + (first[lo] - taken) + (col - old);
-          page = from < static_cast<uint64_t>(p.num_free) ? p.free_pages[from] : -1;
-          if (off == 0) *entry = page;
-        } else {
-          page = *entry;
-        }
+        const uint32_t old = pages(past[r]);
+        const int32_t page = p.grow && col >= old ? new_page(first[r] + (col - old)) : p.table[r * p.table_row + col];
         if (page >= 0) slot = static_cast<int64_t>(page) * p.page + off;
       }
     }
-    if (i < static_cast<uint32_t>(p.tokens)) p.positions[i] = pos, p.slots[i] = slot;
+    p.positions[i] = pos, p.slots[i] = slot;
+  }
+  // (from the last thread on: the first ones have had a token more where those do not come out even)
+  for (uint64_t j = threads - 1 - self; j < opened; j += threads) {
+    const uint32_t i = static_cast<uint32_t>(j);
+    const int r = holder(first, i);
+    p.table[r * p.table_row + pages(past[r]) + (i - first[r])] = new_page(i);
   }
 }
 
@@ -159,13 +165,17 @@ extern "C" int qf_step_maps(const int32_t* query_lens, const int32_t* past_lens,
   MapsParams p = {query_lens, past_lens, block_table, s_bt, free_pages, free_head,
                   query_start, seq_lens, free_head_out, positions, slots, num_reqs, max_pages, page_size, num_free,
                   num_tokens, free_head != nullptr};
-  const size_t smem = (3 * static_cast<size_t>(num_reqs) + 1) * 4;
+  const size_t smem = (3 * static_cast<size_t>(num_reqs) + 2) * 4;
   if (smem + kMapStatic > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (3 * QF_MAPS_MAX_REQS + 1) * 4);
+                                               (3 * QF_MAPS_MAX_REQS + 2) * 4);
     if (e != cudaSuccess) return fail(QF_ERR_LAUNCH, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
   }
-  const int64_t ctas = (static_cast<int64_t>(num_tokens) + 4 * kMapThreads - 1) / (4 * kMapThreads);
+  // four tokens a thread; how many pages open is known on the device only: at most 64 entries a thread, until all SMs are in use
+  const int64_t entries = p.grow ? static_cast<int64_t>(num_reqs) * max_pages : 0;
+  const int64_t for_tokens = (static_cast<int64_t>(num_tokens) + 4 * kMapThreads - 1) / (4 * kMapThreads);
+  const int64_t for_pages = (entries + 64 * kMapThreads - 1) / (64 * kMapThreads);
+  const int64_t ctas = for_tokens > for_pages ? for_tokens : for_pages;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas < 1 ? 1 : ctas > sms ? sms : ctas));
   cfg.blockDim = dim3(kMapThreads);
