@@ -215,6 +215,32 @@ def test_attention_pages_that_are_none(dev):
     assert none.shape == query.shape and not none.any()
 
 
+def test_attention_lengths_of_any_value(dev):
+    """Lengths at the ends of 32 bits: what the table can place takes part, or nothing."""
+    from qwen_a100_fastpath_b200.kv4 import kv4_attention
+    gen = torch.Generator(device=dev).manual_seed(10)
+    lens = [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 64, 1 - 2 ** 31, 70]
+    table = torch.randperm(30, generator=gen, device=dev).to(torch.int32).view(5, 6)
+    query = torch.randn(15, 8, 128, device=dev, generator=gen).to(BF16)
+    cache = random_cache(gen, 30, 16, 2, 128)
+    out = kv4_attention(query, cache, torch.tensor(lens, dtype=torch.int32, device=dev), table, 3, 0.09)
+    check_attention(out, query, cache, lens, table, 3, 0.09)
+    assert not out[3:6].any() and not out[9:12].any()
+
+
+def test_a_cache_of_no_pages(dev):
+    """Nothing is written, zeros are read, rows without keys are zeros."""
+    from qwen_a100_fastpath_b200.kv4 import kv4_attention, kv4_cache, kv4_read, kv4_write
+    cache = kv4_cache(0, 16, 2, 128, dev)
+    x, slots = torch.ones(3, 2, 128, dtype=BF16, device=dev), torch.tensor([0, -1, 5], device=dev)
+    kv4_write(x, x, slots, cache)
+    k, v = kv4_read(cache, slots)
+    assert k.shape == x.shape and not k.any() and not v.any()
+    lens, table = torch.tensor([5, 0, 40], dtype=torch.int32, device=dev), torch.zeros(3, 2, dtype=torch.int32, device=dev)
+    out = kv4_attention(x.repeat(1, 3, 1), cache, lens, table, 1, 0.1)
+    assert out.shape == (3, 6, 128) and not out.any()
+
+
 def test_attention_strided_query_and_out(dev):
     """Views of a larger buffer, rows behind the last request left as they were, the version raised."""
     from qwen_a100_fastpath_b200.kv4 import kv4_attention
@@ -390,6 +416,30 @@ def test_write_and_read(dev, d, t, hkv, page, layout):
         lo = np.repeat(host(x).reshape(t, hkv, -1, 64).min(-1), 64, -1)
         err = np.abs(want - host(x))[kept]
         assert (err <= (0.625 * s + np.abs(lo) / 256 + np.abs(want) / 256)[kept] * (1 + 1e-6)).all()
+
+
+@pytest.mark.parametrize("hkv,d", [(1, 64), (4, 64), (3, 128), (3, 256), (8, 256)])
+def test_write_and_read_many_tokens(dev, hkv, d):
+    """On both sides of the number of tokens from which a CTA takes several times as many, none a multiple of what it takes."""
+    from qwen_a100_fastpath_b200.kv4 import KV4Cache, kv4_read, kv4_write
+    gen = torch.Generator(device=dev).manual_seed(hkv * d)
+    page, per_pass = 16, max(1, 256 // (hkv * d // 4))
+    edge = 4 * 4 * 148 * per_pass
+    for t in (edge - 1, edge, edge + 2 * per_pass + 1):
+        pages = t // page + 2
+        cache = random_cache(gen, pages, page, hkv, d)
+        before = KV4Cache(*(x.clone() for x in cache))
+        k, v = tokens(gen, t, hkv, d), tokens(gen, t, hkv, d)
+        slots = torch.randperm(pages * page, generator=gen, device=dev)[:t]
+        slots[7], slots[t - 1] = -5, pages * page
+        kv4_write(k, v, slots, cache)
+        check_written(cache, before, k, v, slots)
+        kept = ((slots >= 0) & (slots < pages * page)).cpu().numpy()
+        for x, r in zip((k, v), kv4_read(cache, slots)):
+            nib, sc = orc.quantize(host(x))
+            want = orc.values(orc.pack(nib), sc)
+            want[~kept] = 0
+            assert np.array_equal(host(r), want)
 
 
 def test_write_edges(dev):

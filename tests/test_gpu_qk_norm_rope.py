@@ -168,6 +168,37 @@ def test_into_the_cache(dev, d, T, h, hkv, rot, interleaved):
     check_written(cache, before, kr, v, slots)
 
 
+@pytest.mark.parametrize("d,rot", [(64, 64), (64, 16), (80, 80), (128, 128), (192, 64), (256, 64)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_many_rows(dev, d, rot, interleaved):
+    """On both sides of the number of rows from which several heads share a group of lanes, with head counts that do not fill
+    the last group, against float64; and the same bits into the cache."""
+    from qwen_a100_fastpath_b200.kv4 import KV4Cache
+    from qwen_a100_fastpath_b200.norms import qk_norm_rope
+    gen = torch.Generator(device=dev).manual_seed(d + rot)
+    h, hkv, page = 12, 3, 16
+    lanes = 8 if d <= 64 else 16 if d <= 128 else 32
+    rows = (1 << 17) // lanes * 8
+    qw, kw = (0.3 * torch.randn(2, d, device=dev, generator=gen)).to(BF16)
+    cs = table(dev, 500, rot)
+    for T in (rows // (h + hkv) - 1, rows // (h + hkv) + 3):
+        qkv = torch.randn(T, h + 2 * hkv, d, device=dev, generator=gen).to(BF16)
+        q, k, v = qkv[:, :h], qkv[:, h:h + hkv], qkv[:, h + hkv:]
+        pos = torch.randint(0, 500, (T,), device=dev, generator=gen)
+        a, b = qk_norm_rope(q, k, qw, kw, pos, cs, weight_offset=1.0, interleaved=interleaved)
+        check(a, q, qw, pos, cs, 1e-6, 1.0, interleaved)
+        check(b, k, kw, pos, cs, 1e-6, 1.0, interleaved)
+    if d in (64, 128, 256):
+        pages = T // page + 1
+        cache = random_cache(gen, pages, page, hkv, d)
+        before = KV4Cache(*(t.clone() for t in cache))
+        slots = torch.randperm(pages * page, generator=gen, device=dev)[:T]
+        slots[5], slots[T - 2] = -1, pages * page
+        c, _ = qk_norm_rope(q, k, qw, kw, pos, cs, weight_offset=1.0, interleaved=interleaved, v=v, cache=cache, slots=slots)
+        assert torch.equal(c, a)
+        check_written(cache, before, b, v, slots)
+
+
 def test_two_streams_and_a_graph(dev):
     from qwen_a100_fastpath_b200.norms import qk_norm_rope
     gen = torch.Generator(device=dev).manual_seed(8)
