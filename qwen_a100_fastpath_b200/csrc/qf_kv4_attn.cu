@@ -33,7 +33,7 @@
 //
 // Measured (in a graph, the cache from DRAM): 100000 keys x 2 requests, 4 heads of 256, 30 rows 116 us (2.0 TB/s, 212 TFLOP/s;
 // floor 35), 38400 keys, 18 rows 31 us (floor 6.8), 64 requests of 1 to 8192 keys, 8 heads of 128, 8 rows 36 us (floor 12),
-// 700 keys 10.3 us.  What bounds it: neither DRAM (a third) nor the tensor pipe (48 %) nor issue (IPC 1.9 of 4), but how few
+// 700 keys 9.8 us.  What bounds it: neither DRAM (a third) nor the tensor pipe (48 %) nor issue (IPC 1.9 of 4), but how few
 // warps (12 an SM with 30 rows, 168 registers each) have to cover the latencies of a tile's phases.  At the first size without
 // the matrix instructions 121 us, without the unpacking 104, without the copies 111, without the first two 100.  Of a tile's
 // 5300 to 6000 clocks the scores take 1600 to 1900, the values 1400 to 1900, its copies 600 to 700, the bookkeeping before it 500

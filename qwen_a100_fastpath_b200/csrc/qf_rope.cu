@@ -52,7 +52,8 @@ constexpr int kRopeWarps = 4;
 // How rows are read: kAny takes any size, stride and alignment, element by element with the row in shared memory; kWide rows
 // whose pointers and strides are multiples of 16 bytes, with heads of up to 256 (a multiple of eight) and a rotated part that
 // is a multiple of 16 (of eight where interleaved).  8192 tokens of 24 + 4 heads of 256, 64 of them rotated: 99 us with kAny, 49
-// with kWide.
+// with kWide.  One operand at an odd address takes all to kAny: copying it for kWide costs more (queries at the sizes above, 333
+// tokens of 40 + 8 heads of 128 and 5 tokens of 24 + 4 of 256: 99, 7.9 and 2.7 us, with a copy 118, 14.4 and 4.0).
 
 // kWide: L lanes take a row, a lane eight consecutive values in one 16-byte load.  A group of L lanes takes p.chunk heads of
 // one side of one token, ROWS at a time, so that the token's angles and the weight are loaded and multiplied once for them

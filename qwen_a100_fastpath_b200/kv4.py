@@ -37,7 +37,8 @@ class KV4Cache(NamedTuple):
     ``v_scale``: bf16 ``[pages, heads, slots, D / 64, 2]``, the step and the offset of each group.  D is 64, 128 or 256, a
     page may have any number of slots.  Views are fine where k and v (and their scales) have the same strides, the last
     dimensions are adjacent, and addresses and the other strides are multiples of 16 bytes (of ``D / 64`` pairs for the
-    scales)."""
+    scales): of one buffer that holds keys and values (and their scales) side by side for each page, head or slot, for
+    instance."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor

@@ -21,7 +21,8 @@ _maps_grow = torch.ops.qf_b200.step_maps_grow.default
 class StepMaps(NamedTuple):
     """``query_start`` int32 ``[B + 1]``: where each request's tokens begin in the step, and their number; ``seq_lens`` int32
     ``[B]``: the lengths after the step; ``positions``, ``slots`` int64 ``[num_tokens]``; ``free_head`` int32 ``[1]``: the first
-    page of the free list that is left, ``None`` where none was given."""
+    page of the free list that is left, ``None`` where none was given.  Results of one type are pieces of one allocation
+    without a common element: one that is kept (or saved) keeps the others' memory, a ``clone()`` does not."""
     query_start: torch.Tensor
     seq_lens: torch.Tensor
     positions: torch.Tensor
