@@ -292,7 +292,7 @@ int qf_kv4_read(void* k, int64_t sk_t, int64_t sk_h, void* v, int64_t sv_t, int6
 /* qf_spec_attn over this cache: num_reqs requests of q_len query tokens each, query qi of request b attends the keys
  * [0, seq_lens[b] - q_len + qi]; a row with no key gives zeros.  Keys behind max_pages * page_size, and on pages whose entry
  * is no page of the cache, do not take part; what lies in slots that a row does not attend, NaN included, does not touch it.
- * The weighted sums of a row stay finite for up to 2^18 keys of the largest values that the cache keeps.  (In a cache that is
+ * The weighted sums of a row stay finite for up to 2^17 keys of the largest values that the cache keeps.  (In a cache that is
  * filled by other means, a group of values whose n = 0 or n = 15 would stand for an infinity may count as NaN.)
  * q, out: bf16, 16-byte aligned with strides multiples of 8 elements; q_len * num_heads / cache->num_heads <= 64; block_table
  * int32 (row stride s_bt, max_pages entries each);

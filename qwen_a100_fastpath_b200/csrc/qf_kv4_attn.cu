@@ -23,7 +23,7 @@
 // quarter of them for 128 and 64).  The weights are relative to a reference, not to the running maximum: bf16 and fp32 have
 // the same range of exponents, so that the precision of a weight does not depend on where the reference lies.  It is set 32
 // above the first tile's maximum, and set anew, with the exchange that this needs, only where a score has come within 16 of
-// it.  So weights are at most 2^-16, and the sums over 2^18 keys of the largest values that the cache keeps (2^126) stay below
+// it.  So weights are at most 2^-16, and the sums over 2^17 keys of the largest values that the cache keeps (2^126) stay below
 // 2^128; the row's largest weight is at least 2^-32, so that means of values down to 2^-90 lose nothing to fp32's range either.
 // (Set at the first maximum itself, the weights reached 2^16, and sums of values from 2^112 on could become infinite.)
 //

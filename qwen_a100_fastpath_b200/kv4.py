@@ -89,7 +89,7 @@ def kv4_attention(query: torch.Tensor, cache: KV4Cache, seq_lens: torch.Tensor, 
     no page of the cache (-1, for instance), do not take part.  What lies in slots that a row does not attend does not touch
     it, NaN included.  Scores, references, sums and outputs are held in fp32; the weights (relative to a reference 16 to 32
     powers of two above the row's largest score so far) are rounded to bf16 for the product with the values, while their sum
-    takes them unrounded.  The sums hold up to 2^18 keys of the largest values that the cache keeps.
+    takes them unrounded.  The sums hold up to 2^17 keys of the largest values that the cache keeps.
 
     Returns bf16 ``[B * q_len, H, D]``, or ``out`` (the query's shape) with its first ``B * q_len`` tokens written and the
     others left as they were; ``out`` must share no memory with an input."""
